@@ -359,6 +359,59 @@ int kvflux_write_paged_kv_tail(void* key_cache, void* value_cache, uint64_t num_
                                const uint64_t* seq_lens, uint64_t num_rows, void* stream);
 
 /* ---------------------------------------------------------------------------
+ * From the projection's output to the attention's inputs, one launch: RMS norm
+ * of every query and key head, position rotation, queries as the FP32 rows the
+ * attention takes, K and V into their pages. No counterpart in the reference,
+ * whose path starts at finished K/V rows (src/v2/paged_kv_write.cu:101-139);
+ * the writes are those of kvflux_write_paged_kv and kvflux_write_paged_kv_tail.
+ *
+ * Inputs of `input_dtype` (any of the three, whatever the cache's `dtype`):
+ *   query_in [num_tokens][query_heads][head_size], key_in and value_in
+ *   [num_tokens][num_kv_heads][head_size], with query_stride, key_stride and
+ *   value_stride elements from one token to the next (at least a token's
+ *   heads), so the three may lie side by side in one projection's output.
+ *   They are only read; query_out must not overlap them.
+ * For a query or key row x and position t:
+ *   n = x / sqrt(mean(x^2) + eps) * w     (w = query_norm or key_norm, device
+ *       float [head_size]; NULL: n = x), eps >= 0
+ *   over the first rotary_dim dims (even, at most head_size; 0: no rotation),
+ *   angle_j = t * inv_freq[j], inv_freq device double [rotary_dim / 2]:
+ *     y_a = n_a cos - n_b sin, y_b = n_b cos + n_a sin for the pairs (a, b) =
+ *     (j, j + rotary_dim / 2), or (2j, 2j + 1) with interleaved != 0.
+ *   The arithmetic is FP32, the angle FP64. Queries go to query_out, device
+ *   float [num_tokens][query_heads][head_size]; keys are rounded once to the
+ *   cache's type; values are cast to it (the same type: a bit copy).
+ *
+ * kvflux_norm_rope_write: token n at positions[n] (device uint64, below 2^53)
+ *   and slots[n] (device uint64, page * block_size + offset). A slot >=
+ *   num_blocks * block_size is skipped: that token's query is still written.
+ *   Duplicate slots are the caller's to avoid.
+ * kvflux_norm_rope_write_tail: one token for each row of a decode batch, at
+ *   position seq_lens[r] - 1 of table row r (as kvflux_write_paged_kv_tail).
+ *   Of rows with a zero length nothing is written, query_out included; a block
+ *   index >= table_width or a page id >= num_blocks skips K and V only.
+ * Any head_size up to 512 (larger: KVFLUX_ERR_UNSUPPORTED, as are
+ * num_tokens * (query_heads + 2 * num_kv_heads) of 2^26 and more). Buffers
+ * need the alignment of their elements; with 16 bytes, and rows that keep them,
+ * the fast kernel runs. Safe under graph capture; no workspace.
+ * ------------------------------------------------------------------------- */
+int kvflux_norm_rope_write(void* key_cache, void* value_cache, uint64_t num_blocks, uint64_t num_kv_heads,
+                           uint64_t block_size, uint64_t head_size, int dtype, const void* query_in,
+                           const void* key_in, const void* value_in, int input_dtype, uint64_t query_stride,
+                           uint64_t key_stride, uint64_t value_stride, uint64_t query_heads,
+                           const float* query_norm, const float* key_norm, float eps, const double* inv_freq,
+                           uint64_t rotary_dim, int interleaved, const uint64_t* positions,
+                           const uint64_t* slots, uint64_t num_tokens, float* query_out, void* stream);
+int kvflux_norm_rope_write_tail(void* key_cache, void* value_cache, uint64_t num_blocks, uint64_t num_kv_heads,
+                                uint64_t block_size, uint64_t head_size, int dtype, const void* query_in,
+                                const void* key_in, const void* value_in, int input_dtype, uint64_t query_stride,
+                                uint64_t key_stride, uint64_t value_stride, uint64_t query_heads,
+                                const float* query_norm, const float* key_norm, float eps, const double* inv_freq,
+                                uint64_t rotary_dim, int interleaved, const uint64_t* block_table,
+                                uint64_t table_width, const uint64_t* seq_lens, uint64_t num_rows,
+                                float* query_out, void* stream);
+
+/* ---------------------------------------------------------------------------
  * GPU <-> CPU chunk transfer (KV offload).
  *
  * kvflux_copy_chunks: for every pair i of `pairs` (device uint64

@@ -77,6 +77,11 @@ SIGNATURES = {
     "kvflux_table_apply": (_i32, [_vp, _u64, _vp, _u64, _vp, _u64, _vp]),
     "kvflux_write_paged_kv_tail": (_i32, [_vp, _vp, _u64, _u64, _u64, _u64, _i32, _vp, _vp, _vp,
                                           _u64, _vp, _u64, _vp]),
+    "kvflux_norm_rope_write": (_i32, [_vp, _vp, _u64, _u64, _u64, _u64, _i32, _vp, _vp, _vp, _i32, _u64, _u64, _u64,
+                                      _u64, _vp, _vp, C.c_float, _vp, _u64, _i32, _vp, _vp, _u64, _vp, _vp]),
+    "kvflux_norm_rope_write_tail": (_i32, [_vp, _vp, _u64, _u64, _u64, _u64, _i32, _vp, _vp, _vp, _i32, _u64, _u64,
+                                           _u64, _u64, _vp, _vp, C.c_float, _vp, _u64, _i32, _vp, _u64, _vp, _u64,
+                                           _vp, _vp]),
     "kvflux_copy_chunks": (_i32, [_vp, _u64, _u64, _vp]),
     "kvflux_copy_page_list": (_i32, [_vp, _vp, _u64, _u64, _vp, _u64, _vp]),
     "kvflux_bandwidth_probe": (_i32, [_i32, _vp, _vp, _u64, C.c_uint32, C.c_uint32, C.c_uint32, _i32, _vp]),

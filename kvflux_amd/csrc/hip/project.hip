@@ -1,0 +1,318 @@
+// From the projection's output to the attention's inputs in one pass: the RMS
+// norm of every query and key head, the position rotation, queries as the FP32
+// rows the attention takes, keys and values into their pages.
+//
+// For a row x of D values (one head of one token) with weight w:
+//   n = x / sqrt(mean(x^2) + eps) * w          (w null: n = x)
+// and over the first R of the D dims, with angle_j = position * inv_freq[j]:
+//   (y_a, y_b) = (n_a cos - n_b sin, n_b cos + n_a sin)
+// for the pairs (a, b) = (j, j + R/2), or (2j, 2j + 1) when interleaved. Values
+// are neither normed nor rotated. All arithmetic is FP32, the angle FP64 (in
+// turns, reduced exactly): at position 131071 an FP32 angle is off by 2^-8.
+// Keys are rounded once, to the cache's type; values with the cache's type are
+// copied bit by bit.
+#include "common.h"
+
+#include <cmath>
+#include <type_traits>
+
+namespace kvflux_hip {
+namespace {
+
+constexpr std::uint64_t kMaxHead = 512;
+
+struct Bf16 { using Storage = std::uint16_t; };
+struct F16 { using Storage = std::uint16_t; };
+struct F32 { using Storage = std::uint32_t; };
+
+template <typename E>
+__device__ inline float to_float(typename E::Storage x) {
+    if constexpr (std::is_same<E, F32>::value) return __uint_as_float(x);
+    if constexpr (std::is_same<E, F16>::value) return static_cast<float>(__builtin_bit_cast(_Float16, x));
+    return __uint_as_float(static_cast<std::uint32_t>(x) << 16);
+}
+// Rounded to nearest even (the only rounding a key meets after the FP32 steps).
+template <typename E>
+__device__ inline typename E::Storage from_float(float x) {
+    if constexpr (std::is_same<E, F32>::value) return __float_as_uint(x);
+    else if constexpr (std::is_same<E, F16>::value) return __builtin_bit_cast(std::uint16_t, static_cast<_Float16>(x));
+    else return __builtin_bit_cast(std::uint16_t, static_cast<__bf16>(x));
+}
+
+struct Params {
+    const void* query_in;
+    const void* key_in;
+    const void* value_in;
+    std::uint64_t query_stride, key_stride, value_stride;  // elements from a token to the next
+    void* key_cache;
+    void* value_cache;
+    std::uint64_t slot_count;
+    FastDiv block_size;       // slots below 2^32; wide: 64-bit divisions
+    bool wide;
+    std::uint32_t kv_heads, query_heads, head_dim;
+    FastDiv token_rows;       // query_heads + 2 * kv_heads: rows of a token, queries, keys, values
+    std::uint32_t rows;       // num_tokens * token_rows
+    std::uint32_t tokens;
+    const float* query_norm;  // null: no norm
+    const float* key_norm;
+    float eps;
+    const double* inv_freq;   // [rotary / 2]
+    std::uint32_t rotary;
+    bool interleaved;
+    float* query_out;
+};
+
+// Where a token's position and slot come from: arrays, or the place just
+// appended to a sequence, read from a device batch block table (position
+// len - 1 of row n). No slot: ~0. A token without a place at all (an empty row)
+// is not `live`: nothing of it is written.
+struct Listed {
+    const std::uint64_t* positions;
+    const std::uint64_t* slots;
+    __device__ bool live(std::uint32_t) const { return true; }
+    __device__ std::uint64_t position(std::uint32_t n) const { return positions[n]; }
+    __device__ std::uint64_t slot(std::uint32_t n) const { return slots[n]; }
+};
+struct Tail {
+    const std::uint64_t* table;
+    std::uint64_t width;
+    const std::uint64_t* lens;
+    std::uint64_t block_size, num_blocks;
+    __device__ bool live(std::uint32_t n) const { return lens[n] != 0; }
+    __device__ std::uint64_t position(std::uint32_t n) const { return lens[n] - 1; }
+    __device__ std::uint64_t slot(std::uint32_t n) const {
+        const std::uint64_t len = lens[n];
+        if (len == 0) return ~0ULL;
+        const std::uint64_t b = (len - 1) / block_size;
+        if (b >= width) return ~0ULL;
+        const std::uint64_t page = table[static_cast<std::uint64_t>(n) * width + b];
+        return page < num_blocks ? page * block_size + (len - 1) % block_size : ~0ULL;
+    }
+};
+
+// cos and sin of position * inv_freq. In turns the reduction is exact: the
+// quarter turn nearest is taken off in FP64, so FP32 sees at most an eighth of
+// a turn (its rounding is 2^-27 turns), and the quarters swap and negate.
+__device__ inline void rotation(std::uint64_t position, double inv_freq, float* c, float* s) {
+    const double quarters = static_cast<double>(position) * (inv_freq * 0.63661977236758134308);  // 2 / pi
+    const double nearest = rint(quarters);
+    float sn, cs;
+    sincospif(static_cast<float>(0.5 * (quarters - nearest)), &sn, &cs);
+    const int k = static_cast<int>(nearest - 4.0 * floor(0.25 * nearest));  // nearest mod 4 (NaN for an angle past FP64: garbage in)
+    *c = k == 0 ? cs : k == 1 ? -sn : k == 2 ? -cs : sn;
+    *s = k == 0 ? sn : k == 1 ? cs : k == 2 ? -sn : -cs;
+}
+
+// Start of row `head` of `slot` in a cache, in elements.
+__device__ inline std::uint64_t cache_row(const Params& p, std::uint64_t slot, std::uint32_t head) {
+    std::uint64_t page, offset;
+    if (p.wide) {
+        page = slot / p.block_size.divisor;
+        offset = slot - page * p.block_size.divisor;
+    } else {
+        const auto s = static_cast<std::uint32_t>(slot);
+        page = p.block_size.div(s);
+        offset = s - static_cast<std::uint32_t>(page) * p.block_size.divisor;
+    }
+    return ((page * p.kv_heads + head) * p.block_size.divisor + offset) * p.head_dim;
+}
+
+// One wavefront a row; any head size up to kMaxHead, any even rotation, any
+// alignment.
+template <typename In, typename Cache, typename Place>
+__global__ __launch_bounds__(64) void norm_rope_write_generic_kernel(Params p, Place place) {
+    constexpr int kPer = static_cast<int>(kMaxHead) / 64;
+    __shared__ float normed[kMaxHead];
+    const std::uint32_t token = p.token_rows.div(blockIdx.x);
+    const std::uint32_t row = blockIdx.x - token * p.token_rows.divisor;
+    const int lane = threadIdx.x;
+    if (!place.live(token)) return;  // uniform
+    const bool is_query = row < p.query_heads;
+    const bool is_value = row >= p.query_heads + p.kv_heads;
+    const std::uint32_t head = is_query ? row : is_value ? row - p.query_heads - p.kv_heads : row - p.query_heads;
+    const void* in = is_query ? p.query_in : is_value ? p.value_in : p.key_in;
+    const std::uint64_t stride = is_query ? p.query_stride : is_value ? p.value_stride : p.key_stride;
+    const auto* src = static_cast<const typename In::Storage*>(in) + token * stride +
+                      static_cast<std::uint64_t>(head) * p.head_dim;
+    std::uint64_t slot = 0;
+    if (!is_query) {
+        slot = place.slot(token);
+        if (slot >= p.slot_count) return;
+    }
+    if (is_value) {
+        auto* dst = static_cast<typename Cache::Storage*>(p.value_cache) + cache_row(p, slot, head);
+        for (std::uint32_t d = lane; d < p.head_dim; d += 64) {
+            if constexpr (std::is_same<In, Cache>::value) dst[d] = src[d];
+            else dst[d] = from_float<Cache>(to_float<In>(src[d]));
+        }
+        return;
+    }
+    const float* norm = is_query ? p.query_norm : p.key_norm;
+    float x[kPer], square = 0.0f;
+#pragma unroll
+    for (int k = 0; k < kPer; ++k) {
+        const std::uint32_t d = lane + 64 * k;
+        x[k] = d < p.head_dim ? to_float<In>(src[d]) : 0.0f;
+        square = fmaf(x[k], x[k], square);
+    }
+#pragma unroll
+    for (int m = 1; m < 64; m <<= 1) square += __shfl_xor(square, m);
+    const float scale = 1.0f / sqrtf(square / static_cast<float>(p.head_dim) + p.eps);
+#pragma unroll
+    for (int k = 0; k < kPer; ++k) {
+        const std::uint32_t d = lane + 64 * k;
+        if (d < p.head_dim) normed[d] = norm ? x[k] * scale * norm[d] : x[k];
+    }
+    __syncthreads();
+    const std::uint64_t position = place.position(token);
+    const std::uint32_t half = p.rotary / 2;
+    for (std::uint32_t d = lane; d < p.head_dim; d += 64) {
+        float y = normed[d];
+        if (d < p.rotary) {
+            const std::uint32_t j = p.interleaved ? d / 2 : d < half ? d : d - half;
+            const bool first = p.interleaved ? d % 2 == 0 : d < half;
+            const float other = normed[p.interleaved ? d ^ 1u : first ? d + half : d - half];
+            float c, s;
+            rotation(position, p.inv_freq[j], &c, &s);
+            y = first ? y * c - other * s : y * c + other * s;
+        }
+        if (is_query)
+            p.query_out[(static_cast<std::uint64_t>(token) * p.query_heads + head) * p.head_dim + d] = y;
+        else
+            static_cast<typename Cache::Storage*>(p.key_cache)[cache_row(p, slot, head) + d] = from_float<Cache>(y);
+    }
+}
+
+template <typename In, typename Cache, typename Place>
+int launch(const Params& p, const Place& place, hipStream_t s) {
+    hipLaunchKernelGGL((norm_rope_write_generic_kernel<In, Cache, Place>), dim3(p.rows), dim3(64), 0, s, p, place);
+    return launch_status("norm_rope_write_generic_kernel");
+}
+
+template <typename In, typename Place>
+int launch_cache(const Params& p, int dtype, const Place& place, hipStream_t s) {
+    switch (dtype) {
+    case KVFLUX_DTYPE_BF16: return launch<In, Bf16>(p, place, s);
+    case KVFLUX_DTYPE_F16: return launch<In, F16>(p, place, s);
+    default: return launch<In, F32>(p, place, s);
+    }
+}
+
+// Checks and launch shared by both entry points.
+template <typename Place>
+int norm_rope_write(void* key_cache, void* value_cache, uint64_t num_blocks, uint64_t num_kv_heads,
+                    uint64_t block_size, uint64_t head_size, int dtype, const void* query_in, const void* key_in,
+                    const void* value_in, int input_dtype, uint64_t query_stride, uint64_t key_stride,
+                    uint64_t value_stride, uint64_t query_heads, const float* query_norm, const float* key_norm,
+                    float eps, const double* inv_freq, uint64_t rotary_dim, int interleaved, const Place& place,
+                    uint64_t num_tokens, float* query_out, void* stream) {
+    const std::size_t in_bytes = dtype_bytes(input_dtype), cache_bytes = dtype_bytes(dtype);
+    if (cache_bytes == 0) return fail(KVFLUX_ERR_INVALID_ARGUMENT, "unknown dtype %d", dtype);
+    if (in_bytes == 0) return fail(KVFLUX_ERR_INVALID_ARGUMENT, "unknown input dtype %d", input_dtype);
+    if (!key_cache || !value_cache || !query_in || !key_in || !value_in || !query_out)
+        return fail(KVFLUX_ERR_INVALID_ARGUMENT, "norm, rotation and write: null pointer");
+    if (num_blocks == 0 || num_kv_heads == 0 || block_size == 0 || head_size == 0 || query_heads == 0)
+        return fail(KVFLUX_ERR_INVALID_ARGUMENT, "norm, rotation and write: zero dimension");
+    if (rotary_dim % 2 != 0 || rotary_dim > head_size)
+        return fail(KVFLUX_ERR_INVALID_ARGUMENT, "norm, rotation and write: rotary_dim %llu of head_size %llu",
+                    static_cast<unsigned long long>(rotary_dim), static_cast<unsigned long long>(head_size));
+    if (rotary_dim != 0 && !inv_freq)
+        return fail(KVFLUX_ERR_INVALID_ARGUMENT, "norm, rotation and write: null inv_freq");
+    if (!(eps >= 0.0f) || eps == INFINITY)
+        return fail(KVFLUX_ERR_INVALID_ARGUMENT, "norm, rotation and write: eps is negative or not finite");
+    if (head_size > kMaxHead)
+        return fail(KVFLUX_ERR_UNSUPPORTED, "norm, rotation and write: head_size %llu > %llu",
+                    static_cast<unsigned long long>(head_size), static_cast<unsigned long long>(kMaxHead));
+    if (num_blocks > (~0ULL) / block_size)
+        return fail(KVFLUX_ERR_OVERFLOW, "norm, rotation and write: size overflow");
+    // Rows of a launch: a wavefront each in the generic kernel, and fewer than 2^32 threads.
+    constexpr std::uint64_t limit = (1ULL << 26) - 1;
+    if (query_heads > limit || num_kv_heads > limit || block_size > 0x7fffffffULL ||
+        num_tokens > limit / (query_heads + 2 * num_kv_heads))
+        return fail(KVFLUX_ERR_UNSUPPORTED, "norm, rotation and write: dimension too large");
+    if (query_stride < query_heads * head_size || key_stride < num_kv_heads * head_size ||
+        value_stride < num_kv_heads * head_size)
+        return fail(KVFLUX_ERR_INVALID_ARGUMENT, "norm, rotation and write: a stride is shorter than a token's heads");
+    const auto misaligned = [](const void* ptr, std::size_t bytes) {
+        return reinterpret_cast<std::uintptr_t>(ptr) % bytes != 0;
+    };
+    if (misaligned(query_in, in_bytes) || misaligned(key_in, in_bytes) || misaligned(value_in, in_bytes) ||
+        misaligned(key_cache, cache_bytes) || misaligned(value_cache, cache_bytes) ||
+        misaligned(query_out, sizeof(float)) || misaligned(query_norm, sizeof(float)) ||
+        misaligned(key_norm, sizeof(float)) || misaligned(inv_freq, sizeof(double)))
+        return fail(KVFLUX_ERR_INVALID_ARGUMENT, "norm, rotation and write: misaligned buffers");
+
+    Params p{};
+    p.query_in = query_in;
+    p.key_in = key_in;
+    p.value_in = value_in;
+    p.query_stride = query_stride;
+    p.key_stride = key_stride;
+    p.value_stride = value_stride;
+    p.key_cache = key_cache;
+    p.value_cache = value_cache;
+    p.slot_count = num_blocks * block_size;
+    p.block_size = FastDiv(static_cast<std::uint32_t>(block_size));
+    p.wide = p.slot_count > 0xffffffffULL;
+    p.kv_heads = static_cast<std::uint32_t>(num_kv_heads);
+    p.query_heads = static_cast<std::uint32_t>(query_heads);
+    p.head_dim = static_cast<std::uint32_t>(head_size);
+    p.token_rows = FastDiv(static_cast<std::uint32_t>(query_heads + 2 * num_kv_heads));
+    p.tokens = static_cast<std::uint32_t>(num_tokens);
+    p.rows = p.tokens * p.token_rows.divisor;
+    p.query_norm = query_norm;
+    p.key_norm = key_norm;
+    p.eps = eps;
+    p.inv_freq = inv_freq;
+    p.rotary = static_cast<std::uint32_t>(rotary_dim);
+    p.interleaved = interleaved != 0;
+    p.query_out = query_out;
+    const hipStream_t s = as_stream(stream);
+    switch (input_dtype) {
+    case KVFLUX_DTYPE_BF16: return launch_cache<Bf16>(p, dtype, place, s);
+    case KVFLUX_DTYPE_F16: return launch_cache<F16>(p, dtype, place, s);
+    default: return launch_cache<F32>(p, dtype, place, s);
+    }
+}
+
+} // namespace
+} // namespace kvflux_hip
+
+using namespace kvflux_hip;
+
+extern "C" int kvflux_norm_rope_write(void* key_cache, void* value_cache, uint64_t num_blocks, uint64_t num_kv_heads,
+                                      uint64_t block_size, uint64_t head_size, int dtype, const void* query_in,
+                                      const void* key_in, const void* value_in, int input_dtype,
+                                      uint64_t query_stride, uint64_t key_stride, uint64_t value_stride,
+                                      uint64_t query_heads, const float* query_norm, const float* key_norm, float eps,
+                                      const double* inv_freq, uint64_t rotary_dim, int interleaved,
+                                      const uint64_t* positions, const uint64_t* slots, uint64_t num_tokens,
+                                      float* query_out, void* stream) {
+    if (num_tokens == 0) return KVFLUX_OK;
+    if (!positions || !slots) return fail(KVFLUX_ERR_INVALID_ARGUMENT, "norm, rotation and write: null pointer");
+    return norm_rope_write(key_cache, value_cache, num_blocks, num_kv_heads, block_size, head_size, dtype, query_in,
+                           key_in, value_in, input_dtype, query_stride, key_stride, value_stride, query_heads,
+                           query_norm, key_norm, eps, inv_freq, rotary_dim, interleaved, Listed{positions, slots},
+                           num_tokens, query_out, stream);
+}
+
+extern "C" int kvflux_norm_rope_write_tail(void* key_cache, void* value_cache, uint64_t num_blocks,
+                                           uint64_t num_kv_heads, uint64_t block_size, uint64_t head_size, int dtype,
+                                           const void* query_in, const void* key_in, const void* value_in,
+                                           int input_dtype, uint64_t query_stride, uint64_t key_stride,
+                                           uint64_t value_stride, uint64_t query_heads, const float* query_norm,
+                                           const float* key_norm, float eps, const double* inv_freq,
+                                           uint64_t rotary_dim, int interleaved, const uint64_t* block_table,
+                                           uint64_t table_width, const uint64_t* seq_lens, uint64_t num_rows,
+                                           float* query_out, void* stream) {
+    if (num_rows == 0) return KVFLUX_OK;
+    if (!block_table || !seq_lens || table_width == 0)
+        return fail(KVFLUX_ERR_INVALID_ARGUMENT, "norm, rotation and tail write: null table");
+    if (num_rows > (~0ULL) / table_width)
+        return fail(KVFLUX_ERR_OVERFLOW, "norm, rotation and tail write: size overflow");
+    return norm_rope_write(key_cache, value_cache, num_blocks, num_kv_heads, block_size, head_size, dtype, query_in,
+                           key_in, value_in, input_dtype, query_stride, key_stride, value_stride, query_heads,
+                           query_norm, key_norm, eps, inv_freq, rotary_dim, interleaved,
+                           Tail{block_table, table_width, seq_lens, block_size, num_blocks}, num_rows, query_out,
+                           stream);
+}
