@@ -21,6 +21,8 @@ namespace {
 
 constexpr std::uint64_t kMaxHead = 512;
 
+typedef __attribute__((ext_vector_type(4))) float f32x4_t;
+
 struct Bf16 { using Storage = std::uint16_t; };
 struct F16 { using Storage = std::uint16_t; };
 struct F32 { using Storage = std::uint32_t; };
@@ -49,15 +51,17 @@ struct Params {
     std::uint64_t slot_count;
     FastDiv block_size;       // slots below 2^32; wide: 64-bit divisions
     bool wide;
+    std::uint64_t head_step;  // block_size * head_dim
     std::uint32_t kv_heads, query_heads, head_dim;
     FastDiv token_rows;       // query_heads + 2 * kv_heads: rows of a token, queries, keys, values
     std::uint32_t rows;       // num_tokens * token_rows
     std::uint32_t tokens;
     const float* query_norm;  // null: no norm
     const float* key_norm;
-    float eps;
+    float eps, inv_dim;       // inv_dim = 1 / head_dim
     const double* inv_freq;   // [rotary / 2]
     std::uint32_t rotary;
+    FastDiv half;             // rotary / 2 (1 without a rotation)
     bool interleaved;
     float* query_out;
 };
@@ -103,8 +107,11 @@ __device__ inline void rotation(std::uint64_t position, double inv_freq, float* 
     *s = k == 0 ? sn : k == 1 ? cs : k == 2 ? -sn : -cs;
 }
 
-// Start of row `head` of `slot` in a cache, in elements.
-__device__ inline std::uint64_t cache_row(const Params& p, std::uint64_t slot, std::uint32_t head) {
+// Element of a cache where head 0 of `slot` starts (head h: h * head_step on),
+// or kNowhere.
+constexpr std::uint64_t kNowhere = ~0ULL;
+__device__ inline std::uint64_t cache_place(const Params& p, std::uint64_t slot) {
+    if (slot >= p.slot_count) return kNowhere;
     std::uint64_t page, offset;
     if (p.wide) {
         page = slot / p.block_size.divisor;
@@ -114,7 +121,199 @@ __device__ inline std::uint64_t cache_row(const Params& p, std::uint64_t slot, s
         page = p.block_size.div(s);
         offset = s - static_cast<std::uint32_t>(page) * p.block_size.divisor;
     }
-    return ((page * p.kv_heads + head) * p.block_size.divisor + offset) * p.head_dim;
+    return page * p.kv_heads * p.head_step + offset * p.head_dim;
+}
+
+// Sum over aligned groups of `lanes` lanes (a power of two, uniform), in every
+// lane of the group: lane moves within 16, a swizzle and a shuffle beyond.
+__device__ inline float row_sum(float x, std::uint32_t lanes) {
+    const auto moved = [](float v, auto ctrl) {
+        return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), decltype(ctrl)::value, 0xf, 0xf, true));
+    };
+    if (lanes >= 2) x += moved(x, std::integral_constant<int, 0xb1>{});    // lanes 1 apart
+    if (lanes >= 4) x += moved(x, std::integral_constant<int, 0x4e>{});    // lanes 2 apart
+    if (lanes >= 8) x += moved(x, std::integral_constant<int, 0x141>{});   // the other half of 8
+    if (lanes >= 16) x += moved(x, std::integral_constant<int, 0x128>{});  // the other half of 16
+    if (lanes >= 32) x += __int_as_float(__builtin_amdgcn_ds_swizzle(__float_as_int(x), 0x401f));
+    if (lanes >= 64) x += __shfl_xor(x, 32);
+    return x;
+}
+
+// Four values of a row: 8 bytes of a 16-bit type, 16 of FP32.
+template <typename E>
+using Four = typename std::conditional<std::is_same<E, F32>::value, V16, V8>::type;
+template <typename E>
+__device__ inline void widen(const Four<E>& v, float (&x)[4]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if constexpr (std::is_same<E, F32>::value) x[i] = __uint_as_float(v.w[i]);
+        else x[i] = to_float<E>(static_cast<std::uint16_t>(v.w[i / 2] >> (16 * (i % 2))));
+    }
+}
+template <typename E>
+__device__ inline Four<E> narrow(const float (&x)[4]) {
+    Four<E> v;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if constexpr (std::is_same<E, F32>::value) v.w[i] = __float_as_uint(x[i]);
+        else if (i % 2 == 0)
+            v.w[i / 2] = from_float<E>(x[i]) | static_cast<std::uint32_t>(from_float<E>(x[i + 1])) << 16;
+    }
+    return v;
+}
+
+// The fast kernel, for vectors of four values (head size and rotation
+// multiples of 8, aligned rows). 2^lane_shift lanes hold a row, each lane two vectors:
+// values 4l and 4l + R/2 on of the rotated part in the half form, so a pair's
+// two values are in one lane, and 8l and 8l + 4 on elsewhere. A workgroup
+// takes kUnroll * 256 / lanes consecutive rows (token by token: queries, keys,
+// values), so any number of heads fills it; cos and sin of its tokens, and the
+// place of each in the caches, are worked out once into LDS while the rows'
+// loads are in flight.
+//
+// Bound: HBM, and the launch below about 300 tokens. BF16, 32/8 heads of 128, MI355X:
+// 4096 tokens (134 MB) 22.2 us, 6.05 TB/s; 64/8 heads, 16384 tokens (940 MB)
+// 158 us, 5.95 TB/s; 64 tokens 4.2 us. What it took:
+//  * a wavefront a row, a sincos a value: 120 and 775 us;
+//  * this layout, with the slot's page found by each row: 46 and 270 us, about 500
+//    instructions a row, the divisions the larger part; found once a token: 30 and 168;
+//  * non-temporal stores (each row is written once, in whole lines): 22.1 and 159 us;
+//    non-temporal loads as well: 26 and 159;
+//  * rows of a thread (kUnroll): one 23-25 and 171 us, two 22.2 and 158, four 22.1 and
+//    158 but 5.2 us instead of 4.2 for 64 tokens. Two everywhere.
+constexpr int kThreads = 256;
+constexpr int kUnroll = 2;
+// Rows of a workgroup are at most kThreads * kUnroll (one lane a row, head size
+// 8), their values 8 * kThreads * kUnroll, and a token has three rows at least:
+// the tokens they touch, and those tokens' rotated values.
+constexpr int kSpanTokens = kThreads * kUnroll / 3 + 2;
+constexpr int kSpanRotated = 8 * kThreads * kUnroll / 3 + 2 * static_cast<int>(kMaxHead);
+
+template <typename In, typename Cache, typename Place>
+__global__ __launch_bounds__(kThreads) void norm_rope_write_kernel(Params p, Place place, std::uint32_t lane_shift) {
+    __shared__ __attribute__((aligned(16))) float turn[kSpanRotated];  // [token][cos R/2, sin R/2]
+    __shared__ std::uint64_t places[kSpanTokens];
+    __shared__ bool live[kSpanTokens];
+    using Vec = Four<In>;
+    const std::uint32_t tid = threadIdx.x, lanes = 1u << lane_shift, l = tid & (lanes - 1);
+    const std::uint32_t pass_rows = kThreads >> lane_shift;
+    const std::uint32_t first = blockIdx.x * pass_rows * kUnroll;
+    const std::uint32_t last = first + pass_rows * kUnroll < p.rows ? first + pass_rows * kUnroll - 1 : p.rows - 1;
+    const bool inside = 8 * l < p.head_dim;
+    const bool rotated = 8 * l < p.rotary;
+    const std::uint32_t a = rotated && !p.interleaved ? 4 * l : 8 * l;
+    const std::uint32_t b = rotated && !p.interleaved ? 4 * l + p.rotary / 2 : 8 * l + 4;
+
+    // Every row's loads, unconditional (a lane past a row's values rereads its
+    // first vectors, a row past the last one the last).
+    Vec va[kUnroll], vb[kUnroll];
+    std::uint32_t token[kUnroll], row[kUnroll];
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+        const std::uint32_t item = first + u * pass_rows + (tid >> lane_shift);
+        const std::uint32_t at = item < p.rows ? item : p.rows - 1;
+        token[u] = p.token_rows.div(at);
+        row[u] = at - token[u] * p.token_rows.divisor;
+        const bool is_query = row[u] < p.query_heads, is_key = row[u] < p.query_heads + p.kv_heads;
+        const void* in = is_query ? p.query_in : is_key ? p.key_in : p.value_in;
+        const std::uint64_t stride = is_query ? p.query_stride : is_key ? p.key_stride : p.value_stride;
+        const std::uint32_t head = is_query ? row[u] : row[u] - p.query_heads - (is_key ? 0u : p.kv_heads);
+        const auto* src = static_cast<const typename In::Storage*>(in) + token[u] * stride +
+                          static_cast<std::uint64_t>(head) * p.head_dim;
+        va[u] = *reinterpret_cast<const Vec*>(src + (inside ? a : 0u));
+        vb[u] = *reinterpret_cast<const Vec*>(src + (inside ? b : 4u));
+        if (item >= p.rows) row[u] = ~0u;
+    }
+    const auto weights = [&](const float* norm, std::uint32_t at) {
+        return norm ? *reinterpret_cast<const f32x4_t*>(norm + at) : f32x4_t{1.0f, 1.0f, 1.0f, 1.0f};  // uniform
+    };
+    const f32x4_t wqa = weights(p.query_norm, inside ? a : 0u), wqb = weights(p.query_norm, inside ? b : 4u);
+    const f32x4_t wka = weights(p.key_norm, inside ? a : 0u), wkb = weights(p.key_norm, inside ? b : 4u);
+
+    const std::uint32_t token0 = p.token_rows.div(first), tokens = p.token_rows.div(last) - token0 + 1;
+    const std::uint32_t half = p.rotary / 2;
+    for (std::uint32_t i = tid; i < tokens * half; i += kThreads) {
+        const std::uint32_t t = p.half.div(i), j = i - t * half;
+        rotation(place.position(token0 + t), p.inv_freq[j], &turn[t * p.rotary + j], &turn[t * p.rotary + half + j]);
+    }
+    for (std::uint32_t t = tid; t < tokens; t += kThreads) {
+        places[t] = cache_place(p, place.slot(token0 + t));
+        live[t] = place.live(token0 + t);
+    }
+    __syncthreads();
+
+    auto finish = [&](const Vec& row_a, const Vec& row_b, std::uint32_t token_u, std::uint32_t row_u) {
+        float xa[4], xb[4], square = 0.0f;
+        widen<In>(row_a, xa);
+        widen<In>(row_b, xb);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) square = fmaf(xa[i], xa[i], fmaf(xb[i], xb[i], square));
+        if (!inside) square = 0.0f;
+        square = row_sum(square, lanes);
+        if (row_u == ~0u || !inside) return;
+        const std::uint32_t t = token_u - token0;
+        const bool is_query = row_u < p.query_heads, is_key = row_u < p.query_heads + p.kv_heads;
+        const std::uint64_t at = places[t];
+        if (is_query ? !live[t] : at == kNowhere) return;
+        const std::uint32_t head = row_u - (is_query ? 0u : is_key ? p.query_heads : p.query_heads + p.kv_heads);
+        if (!is_query && !is_key) {
+            auto* dst = static_cast<typename Cache::Storage*>(p.value_cache) + at + head * p.head_step;
+            Four<Cache> ca, cb;
+            if constexpr (std::is_same<In, Cache>::value) {
+                ca = row_a;
+                cb = row_b;
+            } else {
+                ca = narrow<Cache>(xa);
+                cb = narrow<Cache>(xb);
+            }
+            stream_store(reinterpret_cast<Four<Cache>*>(dst + a), ca);
+            stream_store(reinterpret_cast<Four<Cache>*>(dst + b), cb);
+            return;
+        }
+        if (is_query ? p.query_norm != nullptr : p.key_norm != nullptr) {
+            const float scale = __builtin_amdgcn_rsqf(fmaf(square, p.inv_dim, p.eps));
+            const f32x4_t wa = is_query ? wqa : wka, wb = is_query ? wqb : wkb;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                xa[i] *= scale * wa[i];
+                xb[i] *= scale * wb[i];
+            }
+        }
+        if (rotated) {
+            const float4 c4 = *reinterpret_cast<const float4*>(turn + t * p.rotary + 4 * l);
+            const float4 s4 = *reinterpret_cast<const float4*>(turn + t * p.rotary + half + 4 * l);
+            const float c[4] = {c4.x, c4.y, c4.z, c4.w}, s[4] = {s4.x, s4.y, s4.z, s4.w};
+            if (p.interleaved) {
+#pragma unroll
+                for (int i = 0; i < 4; i += 2) {
+                    const float ya = xa[i] * c[i / 2] - xa[i + 1] * s[i / 2];
+                    xa[i + 1] = xa[i + 1] * c[i / 2] + xa[i] * s[i / 2];
+                    xa[i] = ya;
+                    const float yb = xb[i] * c[2 + i / 2] - xb[i + 1] * s[2 + i / 2];
+                    xb[i + 1] = xb[i + 1] * c[2 + i / 2] + xb[i] * s[2 + i / 2];
+                    xb[i] = yb;
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float y = xa[i] * c[i] - xb[i] * s[i];
+                    xb[i] = xb[i] * c[i] + xa[i] * s[i];
+                    xa[i] = y;
+                }
+            }
+        }
+        if (is_query) {
+            float* dst = p.query_out + (static_cast<std::uint64_t>(token_u) * p.query_heads + head) * p.head_dim;
+            stream_store(reinterpret_cast<V16*>(dst + a), narrow<F32>(xa));
+            stream_store(reinterpret_cast<V16*>(dst + b), narrow<F32>(xb));
+        } else {
+            auto* dst = static_cast<typename Cache::Storage*>(p.key_cache) + at + head * p.head_step;
+            stream_store(reinterpret_cast<Four<Cache>*>(dst + a), narrow<Cache>(xa));
+            stream_store(reinterpret_cast<Four<Cache>*>(dst + b), narrow<Cache>(xb));
+        }
+    };
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) finish(va[u], vb[u], token[u], row[u]);
 }
 
 // One wavefront a row; any head size up to kMaxHead, any even rotation, any
@@ -134,13 +333,14 @@ __global__ __launch_bounds__(64) void norm_rope_write_generic_kernel(Params p, P
     const std::uint64_t stride = is_query ? p.query_stride : is_value ? p.value_stride : p.key_stride;
     const auto* src = static_cast<const typename In::Storage*>(in) + token * stride +
                       static_cast<std::uint64_t>(head) * p.head_dim;
-    std::uint64_t slot = 0;
+    std::uint64_t at = 0;
     if (!is_query) {
-        slot = place.slot(token);
-        if (slot >= p.slot_count) return;
+        at = cache_place(p, place.slot(token));
+        if (at == kNowhere) return;
+        at += head * p.head_step;
     }
     if (is_value) {
-        auto* dst = static_cast<typename Cache::Storage*>(p.value_cache) + cache_row(p, slot, head);
+        auto* dst = static_cast<typename Cache::Storage*>(p.value_cache) + at;
         for (std::uint32_t d = lane; d < p.head_dim; d += 64) {
             if constexpr (std::is_same<In, Cache>::value) dst[d] = src[d];
             else dst[d] = from_float<Cache>(to_float<In>(src[d]));
@@ -157,7 +357,7 @@ __global__ __launch_bounds__(64) void norm_rope_write_generic_kernel(Params p, P
     }
 #pragma unroll
     for (int m = 1; m < 64; m <<= 1) square += __shfl_xor(square, m);
-    const float scale = 1.0f / sqrtf(square / static_cast<float>(p.head_dim) + p.eps);
+    const float scale = __builtin_amdgcn_rsqf(fmaf(square, p.inv_dim, p.eps));
 #pragma unroll
     for (int k = 0; k < kPer; ++k) {
         const std::uint32_t d = lane + 64 * k;
@@ -179,12 +379,32 @@ __global__ __launch_bounds__(64) void norm_rope_write_generic_kernel(Params p, P
         if (is_query)
             p.query_out[(static_cast<std::uint64_t>(token) * p.query_heads + head) * p.head_dim + d] = y;
         else
-            static_cast<typename Cache::Storage*>(p.key_cache)[cache_row(p, slot, head) + d] = from_float<Cache>(y);
+            static_cast<typename Cache::Storage*>(p.key_cache)[at + d] = from_float<Cache>(y);
     }
+}
+
+// Whether rows can be read and written in vectors of four values.
+template <typename In, typename Cache>
+bool in_vectors(const Params& p) {
+    if (p.head_dim % 8 != 0 || p.rotary % 8 != 0) return false;
+    if ((p.query_stride | p.key_stride | p.value_stride) % 4 != 0) return false;
+    const void* in[3] = {p.query_in, p.key_in, p.value_in};
+    const void* cache[2] = {p.key_cache, p.value_cache};
+    const void* floats[3] = {p.query_out, p.query_norm, p.key_norm};
+    return copy_width(sizeof(Four<In>), in, 3) == sizeof(Four<In>) &&
+           copy_width(sizeof(Four<Cache>), cache, 2) == sizeof(Four<Cache>) && copy_width(16, floats, 3) == 16;
 }
 
 template <typename In, typename Cache, typename Place>
 int launch(const Params& p, const Place& place, hipStream_t s) {
+    if (in_vectors<In, Cache>(p)) {
+        std::uint32_t lane_shift = 0;
+        while ((8u << lane_shift) < p.head_dim) ++lane_shift;
+        const std::uint32_t rows = (kThreads >> lane_shift) * kUnroll;
+        hipLaunchKernelGGL((norm_rope_write_kernel<In, Cache, Place>), dim3((p.rows + rows - 1) / rows), dim3(kThreads),
+                           0, s, p, place, lane_shift);
+        return launch_status("norm_rope_write_kernel");
+    }
     hipLaunchKernelGGL((norm_rope_write_generic_kernel<In, Cache, Place>), dim3(p.rows), dim3(64), 0, s, p, place);
     return launch_status("norm_rope_write_generic_kernel");
 }
@@ -253,6 +473,7 @@ int norm_rope_write(void* key_cache, void* value_cache, uint64_t num_blocks, uin
     p.value_cache = value_cache;
     p.slot_count = num_blocks * block_size;
     p.block_size = FastDiv(static_cast<std::uint32_t>(block_size));
+    p.head_step = block_size * head_size;
     p.wide = p.slot_count > 0xffffffffULL;
     p.kv_heads = static_cast<std::uint32_t>(num_kv_heads);
     p.query_heads = static_cast<std::uint32_t>(query_heads);
@@ -263,8 +484,10 @@ int norm_rope_write(void* key_cache, void* value_cache, uint64_t num_blocks, uin
     p.query_norm = query_norm;
     p.key_norm = key_norm;
     p.eps = eps;
+    p.inv_dim = 1.0f / static_cast<float>(head_size);
     p.inv_freq = inv_freq;
     p.rotary = static_cast<std::uint32_t>(rotary_dim);
+    p.half = FastDiv(p.rotary != 0 ? p.rotary / 2 : 1);
     p.interleaved = interleaved != 0;
     p.query_out = query_out;
     const hipStream_t s = as_stream(stream);
