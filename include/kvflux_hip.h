@@ -219,6 +219,46 @@ int kvflux_paged_attention_noalloc(const void* key_cache, const void* value_cach
                                    uint64_t kv_len, uint64_t num_rows, uint64_t query_heads,
                                    const float* query, float* output, void* stream);
 
+/* kvflux_paged_attention_shared: kvflux_paged_attention for a decode batch
+ * (seq_lens given) whose rows come in groups behind a shared prefix, each
+ * prefix computed once for all its rows instead of once a row. No counterpart
+ * in the reference, whose prefix cache shares pages but whose
+ * paged_attention_batch_kernel reads them for every row
+ * (src/v2/prefix_cache.cpp:7-57, src/v2/paged_attention.cu:130-153).
+ *   group_starts:   device uint64 [num_groups + 1], ascending: group g is rows
+ *                   group_starts[g] .. group_starts[g + 1]. Rows before the
+ *                   first group or behind the last have no shared prefix.
+ *   group_prefixes: device uint64 [num_groups]: the rows of group g have the
+ *                   same pages (table entries) for their first
+ *                   group_prefixes[g] tokens; they are read through the table
+ *                   row of the group's first row. A value above max_prefix
+ *                   or kv_len shares nothing: the group's rows are as rows
+ *                   without one.
+ * A row shorter than its group's prefix attends to its own seq_lens[r] tokens
+ * through its own table row, as a row without a group; a group of one row is
+ * the same. Other arguments, and the result, as for kvflux_paged_attention: FP32
+ * queries and outputs, the 1e-5 contract, rows of zero tokens give zeros,
+ * missing pages drop out. Results are the same bits from call to call; a
+ * row's bits may differ between batches and from kvflux_paged_attention's.
+ * 16-bit caches at head_size 64, 128 and 256 and FP32 caches at 64 and 128, pages
+ * of any size, up to 4096 rows and 512 groups; K, V and the workspace aligned to 16
+ * bytes there. Other calls, and num_groups = 0, run as kvflux_paged_attention
+ * does.
+ * workspace: kvflux_paged_attention_shared_workspace_size bytes, which for
+ * the shared kernel depend on neither kv_len nor the prefixes (no
+ * initialisation needed; calls that share one must be ordered). */
+int kvflux_paged_attention_shared_workspace_size(uint64_t num_rows, uint64_t kv_len, uint64_t num_kv_heads,
+                                                 uint64_t query_heads, uint64_t block_size, uint64_t head_size,
+                                                 int dtype, uint64_t num_groups, size_t* bytes);
+int kvflux_paged_attention_shared(const void* key_cache, const void* value_cache, uint64_t num_blocks,
+                                  uint64_t num_kv_heads, uint64_t block_size, uint64_t head_size, int dtype,
+                                  const uint64_t* block_table, uint64_t max_blocks_per_seq,
+                                  const uint64_t* seq_lens, uint64_t kv_len, uint64_t num_rows,
+                                  uint64_t query_heads, const uint64_t* group_starts,
+                                  const uint64_t* group_prefixes, uint64_t num_groups, uint64_t max_prefix,
+                                  const float* query, float* output, void* workspace, size_t workspace_bytes,
+                                  void* stream);
+
 /* ---------------------------------------------------------------------------
  * Hot path 3b: causal paged prefill on MFMA.
  * Replaces paged_attention_kernel for a whole-prompt call
