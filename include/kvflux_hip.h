@@ -241,7 +241,7 @@ int kvflux_paged_attention_noalloc(const void* key_cache, const void* value_cach
  * missing pages drop out. Results are the same bits from call to call; a
  * row's bits may differ between batches and from kvflux_paged_attention's.
  * 16-bit caches at head_size 64, 128 and 256 and FP32 caches at 64 and 128, pages
- * of any size, up to 4096 rows and 512 groups; K, V and the workspace aligned to 16
+ * of any size, up to 2048 rows and 512 groups; K, V and the workspace aligned to 16
  * bytes there. Other calls, and num_groups = 0, run as kvflux_paged_attention
  * does.
  * workspace: kvflux_paged_attention_shared_workspace_size bytes, which for

@@ -125,6 +125,10 @@ __device__ inline void wait_lgkm0() { __builtin_amdgcn_s_waitcnt(0xF | (3 << 14)
 __device__ inline void load_to_lds(const void* src, std::uint32_t lds_byte) {
     asm volatile("global_load_lds_dwordx4 %0, off" ::"v"(src), "{m0}"(lds_byte) : "memory");
 }
+// The same from `base` (wave-uniform) and a byte offset of each lane.
+__device__ inline void load_to_lds(std::uint64_t base, std::uint32_t offset, std::uint32_t lds_byte) {
+    asm volatile("global_load_lds_dwordx4 %0, %1" ::"v"(offset), "s"(base), "{m0}"(lds_byte) : "memory");
+}
 __device__ inline std::uint32_t lds_address(const void* p) {
     return static_cast<std::uint32_t>(reinterpret_cast<std::uintptr_t>((__attribute__((address_space(3))) const char*)p));
 }

@@ -37,7 +37,7 @@ constexpr int kThreads = 512;  // 8 wavefronts, two per SIMD
 constexpr int kWaves = kThreads / 64;
 constexpr std::uint32_t kCols = 128;        // columns of a stream: 16 a wavefront
 constexpr std::uint32_t kWorkgroups = 256;  // one per CU (two tiles fill its LDS)
-constexpr std::uint32_t kMaxRows = 4096;    // rows and groups whose costs are summed in LDS
+constexpr std::uint32_t kMaxRows = 2048;    // rows and groups whose plan is in LDS
 constexpr std::uint32_t kMaxGroups = 512;
 constexpr int kBufferBytes = 65536;         // K and V of a tile
 
@@ -49,18 +49,36 @@ struct Shape {
     static constexpr std::uint32_t kTile = kBufferBytes / 2 / kRowBytes;  // tokens
     static constexpr std::uint32_t kStep = kF32 ? 16 : 32;       // tokens of a wavefront's step
     static constexpr std::uint32_t kSteps = kTile / kStep;
-    // The fewest blocks of columns a tile's wavefronts are laid out for: with
-    // fewer, they would not have a step each.
-    static constexpr std::uint32_t kLeastBlocks = kSteps >= kWaves ? 1 : kWaves / kSteps;
+    // Blocks of 16 columns that a wavefront may hold: with two, every K and V
+    // operand read from LDS feeds twice the MFMAs. Head size 256 has no registers
+    // for two; FP32 MFMAs are slow enough for one.
+    static constexpr std::uint32_t kMostBlocks = kF32 || kD >= 128 ? 1 : 2;
+    // The fewest wavefronts side by side over columns: with fewer, the others
+    // would not have a step of the tile's tokens each.
+    static constexpr std::uint32_t kLeastAcross = kSteps >= kWaves ? 1 : kWaves / kSteps;
     static constexpr int kLoads = kBufferBytes / 2 / (kThreads * 16);  // loads of a thread, K and V each
 };
 
-// Blocks of 16 columns that the wavefronts are laid out for (a power of two);
-// kWaves / it groups of wavefronts share a tile's tokens.
-__host__ __device__ inline std::uint32_t layout_blocks(std::uint32_t blocks, std::uint32_t least) {
-    std::uint32_t n = least;
-    while (n < blocks) n *= 2;
-    return n < kWaves ? n : kWaves;
+// How the wavefronts take a stream of `cols` columns: `across` of them side by
+// side with `blocks` blocks of 16 columns each; kWaves / across groups of such
+// share a tile's tokens.
+struct Spread {
+    std::uint32_t across, blocks;
+};
+template <typename E, int kD>
+__device__ inline Spread spread_of(std::uint32_t cols) {
+    using S = Shape<E, kD>;
+    const std::uint32_t need = (cols + 15) / 16;
+    Spread s{S::kLeastAcross, 1};
+    while (s.across < need) {
+        // Two blocks where the merge of the shares' accumulators fits a buffer.
+        if (S::kMostBlocks == 2 && s.across * 2 >= need && (kWaves - s.across) * 2 * kD * 64 <= kBufferBytes) {
+            s.blocks = 2;
+            break;
+        }
+        s.across *= 2;
+    }
+    return s;
 }
 
 struct SharedParams {
@@ -83,8 +101,7 @@ struct SharedParams {
     const float* query;
     float* output;
     float scale_log2;            // log2(e) / sqrt(D)
-    // Workspace: total cost and the rows' plans for the merge, partials.
-    std::uint64_t* total;
+    // Workspace: the rows' plans for the merge, partials.
     struct RowPlan* plans;
     float* prefix_acc;  // [slot][kCols][D]
     float* prefix_ml;   // [slot][kCols][2]
@@ -96,32 +113,31 @@ struct SharedParams {
 
 // What the merge needs of a row.
 struct RowPlan {
-    std::uint64_t prefix_cost, own_cost;  // costs before the segments
-    std::uint32_t prefix_tiles, prefix_weight, prefix_col_tiles, prefix_stream;
-    std::uint32_t first_row, own_tiles, own_weight, len;
+    std::uint32_t prefix_cost, own_cost;  // costs before the segments
+    std::uint32_t prefix_tiles, prefix_shift, prefix_col_tiles, prefix_stream;
+    std::uint32_t first_row, own_tiles, own_shift, total;
 };
 
 // A segment: the columns (of row first_row on), the tokens [begin, end) of
-// table row first_row, its tiles and the cost of one.
+// table row first_row, its tiles and the cost of one (1 << shift).
 struct Segment {
-    std::uint32_t first_row, cols, col_tiles, begin, end, tiles, weight;
-    __device__ std::uint64_t stream_cost() const { return static_cast<std::uint64_t>(tiles) * weight; }
-    __device__ std::uint64_t cost(std::uint32_t heads) const { return stream_cost() * (heads * col_tiles); }
+    std::uint32_t first_row, cols, col_tiles, begin, end, tiles, shift;
+    __device__ std::uint32_t stream_cost() const { return tiles << shift; }
+    __device__ std::uint32_t cost(std::uint32_t heads) const { return stream_cost() * (heads * col_tiles); }
 };
 
-// Cost of a tile by its layout's blocks of columns.
+// Cost of a tile, as a power of two.
 template <typename E, int kD>
-__device__ inline std::uint32_t tile_weight(std::uint32_t cols) {
-    const std::uint32_t blocks = layout_blocks((cols + 15) / 16, Shape<E, kD>::kLeastBlocks);
-    return blocks < kWaves ? 1u : 2u;
+__device__ inline std::uint32_t tile_shift(std::uint32_t cols) {
+    return cols > kCols / 2 ? 1 : 0;
 }
 
 template <typename E, int kD>
 __device__ inline Segment make_segment(std::uint32_t first_row, std::uint32_t cols, std::uint32_t begin, std::uint32_t end) {
     constexpr std::uint32_t kTile = Shape<E, kD>::kTile;
-    Segment s{first_row, cols, (cols + kCols - 1) / kCols, begin, end, 0, 1};
+    Segment s{first_row, cols, (cols + kCols - 1) / kCols, begin, end, 0, 0};
     s.tiles = end > begin ? (end - begin - 1) / kTile + 1 : 0;
-    s.weight = tile_weight<E, kD>(cols < kCols ? cols : kCols);
+    s.shift = tile_shift<E, kD>(cols);
     return s;
 }
 
@@ -143,8 +159,14 @@ __device__ inline std::uint32_t group_stream(const SharedParams& p, std::uint32_
     return (g + first_row * p.group.divisor / kCols) * p.heads;
 }
 
-__device__ inline std::uint64_t share_begin(std::uint64_t total, std::uint32_t w) {
-    return (total * w + kWorkgroups - 1) / kWorkgroups;
+// Where the share of workgroup w begins, ceil(total * w / kWorkgroups), in 32 bits.
+__device__ inline std::uint32_t share_begin(std::uint32_t total, std::uint32_t w) {
+    return total / kWorkgroups * w + (total % kWorkgroups * w + kWorkgroups - 1) / kWorkgroups;
+}
+// The tiles before the first that starts at `at` or behind it, of a stream whose
+// first tile starts at `cost`.
+__device__ inline std::uint32_t tiles_before(std::uint32_t at, std::uint32_t cost, std::uint32_t shift) {
+    return at > cost ? (at - cost + (1u << shift) - 1) >> shift : 0;
 }
 
 // exp2(m - top) for merging partials: 0 for a part that saw no key.
@@ -154,7 +176,11 @@ __device__ inline float merge_weight(float m, float top) {
 
 __device__ __attribute__((aligned(16))) unsigned char sh_zero_row[512];
 
-template <typename E, int kD>
+// kWhole: pages of a multiple of 16 tokens. Then 16 neighbouring rows of a tile
+// that starts at a multiple of 16 lie in one page, and a wavefront's loads are
+// one scalar address and constant lane offsets; else every lane looks up the
+// page of each of its rows.
+template <typename E, int kD, bool kWhole>
 __global__ __launch_bounds__(kThreads) void shared_attention_kernel(SharedParams p) {
     using S = Shape<E, kD>;
     constexpr bool kF32 = S::kF32;
@@ -162,6 +188,7 @@ __global__ __launch_bounds__(kThreads) void shared_attention_kernel(SharedParams
     using Vec = typename M::Vec;
     constexpr std::uint32_t kTile = S::kTile, kStep = S::kStep;
     constexpr int kRowBytes = S::kRowBytes, kCpr = S::kCpr, kLoads = S::kLoads;
+    constexpr int kBlocks = static_cast<int>(S::kMostBlocks);
     constexpr int kKk = kD / 32;   // 16-bit: K steps of S^T
     constexpr int kDt = kD / 16;   // accumulator tiles of O^T
     constexpr float kWeightScale = kF32 ? 1.0f : M::kWeightScale;
@@ -169,25 +196,33 @@ __global__ __launch_bounds__(kThreads) void shared_attention_kernel(SharedParams
 
     __shared__ __attribute__((aligned(16))) unsigned char buffers[2][kBufferBytes];
     __shared__ std::uint32_t first_of[kMaxGroups + 1];  // first row of a group, and the end
-    __shared__ std::uint32_t prefix_of[kMaxGroups];     // its shared tokens (0: fewer than two rows, or past the bound)
-    __shared__ float2 part_ml[kWaves][16];
+    __shared__ std::uint32_t prefix_of[kMaxGroups];     // its prefix (0: past the bound)
+    __shared__ std::uint32_t begin_of[kMaxRows], end_of[kMaxRows];  // a row's own tokens
+    __shared__ float2 part_ml[kWaves][kBlocks][16];
     __shared__ std::uint32_t bad_tile[2];               // the serial number of a tile with a missing page
     __shared__ std::uint32_t found;
 
-    const int tid = threadIdx.x, wave = tid / 64, lane = tid % 64;
-    const int col = lane % 16, quad = lane / 16;
+    const int tid = threadIdx.x, lane = tid % 64;
     const auto uniform = [](std::uint32_t x) {
         return static_cast<std::uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(x)));
     };
-    const auto uniform64 = [&](std::uint64_t x) {
-        return static_cast<std::uint64_t>(uniform(static_cast<std::uint32_t>(x >> 32))) << 32 |
-               uniform(static_cast<std::uint32_t>(x));
-    };
+    const int wave = static_cast<int>(uniform(tid / 64));
+    const int col = lane % 16, quad = lane / 16;
 
     // ---- plan: the groups (starts made monotone, whatever the caller gave),
-    // then the sum of costs over all segments: groups first, then rows.
+    // every row's own tokens, and the sum of costs over all segments: groups
+    // first, then rows. All loads of it are in one round trip.
+    for (std::uint32_t r = tid; r < p.rows; r += kThreads) {
+        const std::uint64_t n = p.lens[r];
+        end_of[r] = n < p.kv_len ? static_cast<std::uint32_t>(n) : p.kv_len;
+    }
+    for (std::uint32_t g = tid; g < p.groups; g += kThreads) {
+        const std::uint64_t n = p.prefixes[g];
+        prefix_of[g] = n <= p.max_prefix ? static_cast<std::uint32_t>(n) & (kWhole ? ~15u : ~0u) : 0u;
+    }
     if (wave == 0) {
         std::uint32_t carry = 0;
+#pragma unroll 1
         for (std::uint32_t base = 0; base <= p.groups; base += 64) {
             const std::uint32_t g = base + lane;
             std::uint32_t v = 0;
@@ -195,7 +230,7 @@ __global__ __launch_bounds__(kThreads) void shared_attention_kernel(SharedParams
                 const std::uint64_t s = p.starts[g];
                 v = s < p.rows ? static_cast<std::uint32_t>(s) : p.rows;
             }
-#pragma unroll
+#pragma unroll 1
             for (int off = 1; off < 64; off <<= 1) {
                 const auto o = static_cast<std::uint32_t>(__shfl_up(static_cast<int>(v), off));
                 if (lane >= off && o > v) v = o;
@@ -206,79 +241,73 @@ __global__ __launch_bounds__(kThreads) void shared_attention_kernel(SharedParams
         }
     }
     if (tid < 2) bad_tile[tid] = 0;
+    if (tid == 0) found = ~0u;
     __syncthreads();
-    for (std::uint32_t g = tid; g < p.groups; g += kThreads) {
-        const std::uint64_t n = p.prefixes[g];
-        prefix_of[g] = first_of[g + 1] - first_of[g] >= 2 && n <= p.max_prefix ? static_cast<std::uint32_t>(n) : 0u;
-    }
-    __syncthreads();
-    const auto group_segment = [&](std::uint32_t g) {
-        return make_segment<E, kD>(first_of[g], (first_of[g + 1] - first_of[g]) * p.group.divisor, 0, prefix_of[g]);
-    };
-    // A row shorter than its group's prefix takes no part in it.
-    const auto row_segment = [&](std::uint32_t r, std::uint32_t* group) {
-        const std::uint64_t full = p.lens[r];
-        const std::uint32_t len = full < p.kv_len ? static_cast<std::uint32_t>(full) : p.kv_len;
-        const std::uint32_t g = group_of(first_of, p.groups, r);
-        const std::uint32_t shared = g < p.groups && prefix_of[g] <= len ? prefix_of[g] : 0u;
-        if (group) *group = shared ? g : p.groups;
-        return make_segment<E, kD>(r, p.group.divisor, shared, len);
-    };
+    // Tokens that the rows of a group share: none with fewer than two rows. A
+    // row shorter than that takes no part in it.
+    const auto shared_tokens = [&](std::uint32_t g) { return first_of[g + 1] - first_of[g] >= 2 ? prefix_of[g] : 0u; };
     const auto segment = [&](std::uint32_t s) {
-        return s < p.groups ? group_segment(s) : row_segment(s - p.groups, nullptr);
+        const bool group = s < p.groups;
+        const std::uint32_t r = s - p.groups;
+        return make_segment<E, kD>(group ? first_of[s] : r, (group ? first_of[s + 1] - first_of[s] : 1u) * p.group.divisor,
+                                   group ? 0u : begin_of[r], group ? shared_tokens(s) : end_of[r]);
     };
     const std::uint32_t segments = p.groups + p.rows;
-    // The buffers hold no tile yet: costs before every segment, and wave totals.
-    auto* const cost_before = reinterpret_cast<std::uint64_t*>(buffers[0]);
-    auto* const wave_cost = reinterpret_cast<std::uint64_t*>(buffers[1]);
-    static_assert((kMaxRows + kMaxGroups) * 8 <= kBufferBytes, "costs fit a buffer");
+    // The buffers hold no tile yet: every segment's cost, then the costs before
+    // it, and wave totals. A thread's segments are neighbours.
+    auto* const cost_of = reinterpret_cast<std::uint32_t*>(buffers[0]);
+    auto* const wave_cost = reinterpret_cast<std::uint32_t*>(buffers[1]);
+    static_assert((kMaxRows + kMaxGroups) * 4 <= kBufferBytes, "costs fit a buffer");
     const std::uint32_t per = (segments + kThreads - 1) / kThreads;
-    std::uint64_t mine = 0;
-    for (std::uint32_t i = 0; i < per; ++i) {
-        const std::uint32_t s = tid * per + i;
-        if (s < segments) mine += segment(s).cost(p.heads);
+    std::uint32_t mine = 0;
+#pragma unroll 1
+    for (std::uint32_t s = tid * per; s < (tid + 1) * per && s < segments; ++s) {
+        if (s >= p.groups) {
+            const std::uint32_t r = s - p.groups, g = group_of(first_of, p.groups, r);
+            const std::uint32_t shared = g < p.groups ? shared_tokens(g) : 0u;
+            begin_of[r] = shared <= end_of[r] ? shared : 0u;
+        }
+        const std::uint32_t cost = segment(s).cost(p.heads);
+        cost_of[s] = cost;
+        mine += cost;
     }
-    std::uint64_t upto = mine;
+    std::uint32_t upto = mine;
 #pragma unroll
     for (int off = 1; off < 64; off <<= 1) {
-        const std::uint64_t add = __shfl_up(static_cast<unsigned long long>(upto), off);
+        const auto add = static_cast<std::uint32_t>(__shfl_up(static_cast<int>(upto), off));
         if (lane >= off) upto += add;
     }
     if (lane == 63) wave_cost[wave] = upto;
-    if (tid == 0) found = ~0u;
     __syncthreads();
-    std::uint64_t before = upto - mine, total = 0;
+    std::uint32_t before = upto - mine, total = 0;
 #pragma unroll
     for (int w = 0; w < kWaves; ++w) {
         before += w < wave ? wave_cost[w] : 0;
         total += wave_cost[w];
     }
-    total = uniform64(total);
+    total = uniform(total);
     // Neighbouring shares on one XCD (workgroups go round the 8 XCDs), so the
     // streams of a kv head meet in its L2.
     const std::uint32_t w = (blockIdx.x % 8) * (kWorkgroups / 8) + blockIdx.x / 8;
-    const std::uint64_t share = share_begin(total, w), share_end = share_begin(total, w + 1);
-    for (std::uint32_t i = 0; i < per; ++i) {
-        const std::uint32_t s = tid * per + i;
-        if (s < segments) {
-            const std::uint64_t cost = segment(s).cost(p.heads);
-            cost_before[s] = before;
-            if (before <= share && share < before + cost) found = s;  // one segment at most
-            before += cost;
-        }
+    const std::uint32_t share = share_begin(total, w), share_end = share_begin(total, w + 1);
+#pragma unroll 1
+    for (std::uint32_t s = tid * per; s < (tid + 1) * per && s < segments; ++s) {
+        const std::uint32_t cost = cost_of[s];
+        cost_of[s] = before;
+        if (before <= share && share < before + cost) found = s;  // one segment at most
+        before += cost;
     }
     __syncthreads();
     if (w == 0) {  // uniform: the rows' plans for the merge
-        if (tid == 0) *p.total = total;
         for (std::uint32_t r = tid; r < p.rows; r += kThreads) {
-            std::uint32_t g;
-            const Segment own = row_segment(r, &g);
-            RowPlan plan{0, cost_before[p.groups + r], 0, 1, 1, 0, 0, own.tiles, own.weight, own.end};
-            if (g < p.groups) {
-                const Segment prefix = group_segment(g);
-                plan.prefix_cost = cost_before[g];
+            const Segment own = segment(p.groups + r);
+            RowPlan plan{0, cost_of[p.groups + r], 0, 0, 1, 0, 0, own.tiles, own.shift, total};
+            if (own.begin != 0) {
+                const std::uint32_t g = group_of(first_of, p.groups, r);
+                const Segment prefix = segment(g);
+                plan.prefix_cost = cost_of[g];
                 plan.prefix_tiles = prefix.tiles;
-                plan.prefix_weight = prefix.weight;
+                plan.prefix_shift = prefix.shift;
                 plan.prefix_col_tiles = prefix.col_tiles;
                 plan.prefix_stream = group_stream(p, g, prefix.first_row);
                 plan.first_row = prefix.first_row;
@@ -286,97 +315,136 @@ __global__ __launch_bounds__(kThreads) void shared_attention_kernel(SharedParams
             p.plans[r] = plan;
         }
     }
-    std::uint32_t seg = uniform(found);
-    if (share >= share_end || seg == ~0u) return;  // uniform: no tile starts in this share
+    // A tile: its segment, stream (kv head and tile of columns) and number, and
+    // the cost before the stream. `ok`: there is one, in this share.
+    struct Cursor {
+        Segment s;
+        std::uint32_t seg, kvh, col_tile, tile, cost;
+        bool ok;
+    };
     const auto uniform_segment = [&](std::uint32_t s) {
         const Segment x = segment(s);
         return Segment{uniform(x.first_row), uniform(x.cols), uniform(x.col_tiles), uniform(x.begin), uniform(x.end),
-                       uniform(x.tiles), uniform(x.weight)};
+                       uniform(x.tiles), uniform(x.shift)};
     };
-    Segment cur = uniform_segment(seg);
-    std::uint64_t cost = uniform64(cost_before[seg]);  // costs before the current stream
-    std::uint32_t stream = uniform(static_cast<std::uint32_t>((share - cost) / cur.stream_cost()));
-    cost += stream * cur.stream_cost();
-    std::uint32_t tile = uniform(static_cast<std::uint32_t>((share - cost + cur.weight - 1) / cur.weight));
-    __syncthreads();  // cost_before is read: the buffers are free
-
-    // The part at hand: tiles [tile, tile_end) of stream `stream` of segment
-    // `seg`. settle() moves to the next part that has tiles; false at the end
-    // of the share.
-    std::uint32_t tile_end = 0;
-    const auto settle = [&]() -> bool {
+    Cursor ahead;  // the tile whose page ids are fetched next
+    ahead.seg = uniform(found);
+    if (share >= share_end || ahead.seg == ~0u) return;  // uniform: an empty share
+    ahead.s = uniform_segment(ahead.seg);                 // has tiles: its cost is above 0
+    ahead.cost = uniform(cost_of[ahead.seg]);
+    {
+        const std::uint32_t stream = (share - ahead.cost) / ahead.s.stream_cost();
+        ahead.cost += stream * ahead.s.stream_cost();
+        ahead.kvh = stream / ahead.s.col_tiles;
+        ahead.col_tile = stream - ahead.kvh * ahead.s.col_tiles;
+    }
+    ahead.tile = tiles_before(share, ahead.cost, ahead.s.shift);
+    // A cursor past its stream's end moves on to the next tile there is.
+    const auto settle = [&](Cursor& c) {
+#pragma unroll 1
         while (true) {
-            if (tile < cur.tiles) {
-                const std::uint64_t at = cost + static_cast<std::uint64_t>(tile) * cur.weight;
-                if (at >= share_end) return false;
-                const std::uint64_t left = (share_end - cost + cur.weight - 1) / cur.weight;
-                tile_end = left < cur.tiles ? static_cast<std::uint32_t>(left) : cur.tiles;
-                return true;
+            if (c.tile < c.s.tiles) {
+                c.ok = c.cost + (c.tile << c.s.shift) < share_end;
+                return;
             }
-            cost += cur.stream_cost();
-            tile = 0;
-            if (cost >= share_end) return false;
-            if (cur.tiles != 0 && ++stream < p.heads * cur.col_tiles) continue;
-            stream = 0;
+            c.cost += c.s.stream_cost();
+            c.tile = 0;
+            c.ok = false;
+            if (c.cost >= share_end) return;
+            if (++c.col_tile < c.s.col_tiles) continue;
+            c.col_tile = 0;
+            if (++c.kvh < p.heads) continue;
+            c.kvh = 0;
             do {
-                if (++seg >= segments) return false;
-                cur = uniform_segment(seg);
-            } while (cur.tiles == 0);
+                if (++c.seg >= segments) return;
+                c.s = uniform_segment(c.seg);
+            } while (c.s.tiles == 0);
         }
     };
-    if (!settle()) return;  // uniform
+    __syncthreads();  // cost_of is read: the buffers are free
 
-    // ---- tile loads. Load i of a wavefront fills 1 KiB of the buffer in lane
-    // order: chunk e = (i * 8 + wave) * 64 + lane is slot e % kCpr of row
-    // e / kCpr. Which chunk of the row a lane fetches sets the swizzle that
-    // keeps the reads below free of bank conflicts.
+    // ---- tile loads. A wavefront fills 4 KiB of K and of V, kWaveRows rows, in
+    // loads of 1 KiB in lane order: chunk i * 64 + lane is slot % kCpr of row
+    // / kCpr. Which chunk of the row a lane fetches sets the swizzle that keeps
+    // the reads below free of bank conflicts.
+    constexpr std::uint32_t kWaveRows = 4096 / kRowBytes;
+    constexpr int kIds = kWhole ? (kWaveRows > 16 ? kWaveRows / 16 : 1) : kLoads;
     const auto kswz = [](int row) { return kCpr >= 16 ? (row & 15) : ((row >> 1) & 7); };
     const auto vswz = [](int row) { return kF32 ? 0 : kCpr / 8 * (row & 7); };
     const std::uint32_t bs = p.block_size.divisor;
-    const std::uint64_t head_bytes = static_cast<std::uint64_t>(bs) * kRowBytes;
-    const std::uint64_t page_bytes = head_bytes * p.heads;
-    std::uint32_t row_of[kLoads];
-#pragma unroll
-    for (int i = 0; i < kLoads; ++i) row_of[i] = ((i * kWaves + wave) * 64 + lane) / kCpr;
-    const int slot = lane % kCpr;
-    struct Where {  // a tile to load
-        const std::uint64_t* table;
-        std::uint32_t first, end, kvh;
+    const std::uint32_t wave_row = wave * kWaveRows;  // first row of the tile
+    const auto row_of = [&](int i) { return wave_row + (i * 64 + lane) / kCpr; };
+    // Byte of its row at which the lane's chunk of load i starts.
+    const auto chunk = [&](int i, bool of_key) {
+        const int row = row_of(i);
+        return static_cast<std::uint32_t>(((lane % kCpr) ^ (of_key ? kswz(row) : vswz(row))) * 16);
     };
-    const auto where = [&](std::uint32_t t) {
-        return Where{p.table + static_cast<std::uint64_t>(cur.first_row) * p.width, cur.begin + t * kTile, cur.end,
-                     stream / cur.col_tiles};
-    };
-    std::uint64_t ids[kLoads];
-    const auto fetch_ids = [&](const Where& at) {
+    const auto first_token = [](const Cursor& c) { return c.s.begin + c.tile * kTile; };
+    // The page ids of a tile's rows are fetched a tile before its loads go out.
+    std::uint64_t ids[kIds];
+    const auto fetch_ids = [&](const Cursor& c) {
+        const std::uint64_t* const table = p.table + static_cast<std::uint64_t>(c.s.first_row) * p.width;
 #pragma unroll
-        for (int i = 0; i < kLoads; ++i) {
-            const std::uint32_t token = at.first + row_of[i] < at.end ? at.first + row_of[i] : at.end - 1;
-            ids[i] = at.table[p.block_size.div(token)];
+        for (int i = 0; i < kIds; ++i) {
+            const std::uint32_t token = first_token(c) + (kWhole ? wave_row + 16 * i : row_of(i));
+            ids[i] = table[p.block_size.div(token < c.s.end ? token : c.s.end - 1)];
         }
     };
-    const auto issue = [&](const Where& at, std::uint32_t buffer, std::uint32_t serial) {
-        const char* kc = static_cast<const char*>(p.key_cache) + at.kvh * head_bytes;
-        const char* vc = static_cast<const char*>(p.value_cache) + at.kvh * head_bytes;
-        const std::uint32_t base = lds_address(buffers[0]) + buffer * kBufferBytes + wave * 1024;
+    const auto issue = [&](const Cursor& c, std::uint32_t buffer, std::uint32_t serial) {
+        // The ids are here (all loads before the barrier are); the compiler's own
+        // wait for them must not fall between the loads below, which it does not
+        // count.
 #pragma unroll
-        for (int i = 0; i < kLoads; ++i) {
-            const std::uint32_t token = at.first + row_of[i];
-            const bool inside = token < at.end, present = ids[i] < p.num_blocks;
-            if (inside && !present) bad_tile[buffer] = serial;
-            const int kchunk = (slot ^ kswz(row_of[i])) * 16, vchunk = (slot ^ vswz(row_of[i])) * 16;
-            const char *k, *v;
-            if (inside && present) {
-                const std::uint32_t off = token - p.block_size.div(token) * bs;
-                const std::uint64_t row = ids[i] * page_bytes + off * static_cast<std::uint64_t>(kRowBytes);
-                k = kc + row + kchunk;
-                v = vc + row + vchunk;
-            } else {  // a token past the end, or of a missing page: zeros, under a weight of zero
-                k = reinterpret_cast<const char*>(sh_zero_row) + kchunk;
-                v = reinterpret_cast<const char*>(sh_zero_row) + vchunk;
+        for (int i = 0; i < kIds; ++i) asm volatile("" : "+v"(ids[i]));
+        const std::uint32_t to = uniform(lds_address(buffers[0]) + buffer * kBufferBytes + wave * 4096);
+        const auto key = reinterpret_cast<std::uint64_t>(p.key_cache), value = reinterpret_cast<std::uint64_t>(p.value_cache);
+        const std::uint32_t first = first_token(c), end = c.s.end;
+        bool direct = false;
+        if constexpr (kWhole) {
+            direct = first + wave_row + kWaveRows <= end;
+#pragma unroll
+            for (int j = 0; j < kIds; ++j) {
+                ids[j] = static_cast<std::uint64_t>(uniform(static_cast<std::uint32_t>(ids[j] >> 32))) << 32 |
+                         uniform(static_cast<std::uint32_t>(ids[j]));
+                direct &= ids[j] < p.num_blocks;
             }
-            load_to_lds(k, uniform(base + i * (kWaves * 1024)));
-            load_to_lds(v, uniform(base + kBufferBytes / 2 + i * (kWaves * 1024)));
+            if (direct) {  // uniform in a wavefront
+#pragma unroll
+                for (int j = 0; j < kIds; ++j) {
+                    const std::uint32_t token = first + wave_row + 16 * j;
+                    const std::uint64_t from =
+                        ((ids[j] * p.heads + c.kvh) * bs + (token - p.block_size.div(token) * bs)) * kRowBytes;
+#pragma unroll
+                    for (int i = j * (kLoads / kIds); i < (j + 1) * (kLoads / kIds); ++i) {
+                        const std::uint32_t row = ((i - j * (kLoads / kIds)) * 64 + lane) / kCpr * kRowBytes;
+                        load_to_lds(key + from, row + chunk(i, true), to + i * 1024);
+                        load_to_lds(value + from, row + chunk(i, false), to + kBufferBytes / 2 + i * 1024);
+                    }
+                }
+            }
+        }
+        if (!direct) {
+            const auto zero = reinterpret_cast<std::uint64_t>(sh_zero_row);
+            std::uint64_t k[kLoads], v[kLoads];
+            bool missing = false;
+#pragma unroll
+            for (int i = 0; i < kLoads; ++i) {
+                const std::uint64_t id = ids[kWhole ? i * kIds / kLoads : i];
+                const std::uint32_t token = first + row_of(i), off = token - p.block_size.div(token) * bs;
+                const bool inside = token < end, present = id < p.num_blocks;
+                missing |= inside && !present;
+                // A token past the end, or of a missing page: zeros, under a weight of zero.
+                const bool live = inside && present;
+                const std::uint64_t row = ((id * p.heads + c.kvh) * bs + off) * kRowBytes;
+                k[i] = (live ? key + row : zero) + chunk(i, true);
+                v[i] = (live ? value + row : zero) + chunk(i, false);
+            }
+            if (missing) bad_tile[buffer] = serial;
+#pragma unroll
+            for (int i = 0; i < kLoads; ++i) {
+                load_to_lds(reinterpret_cast<const void*>(k[i]), to + i * 1024);
+                load_to_lds(reinterpret_cast<const void*>(v[i]), to + kBufferBytes / 2 + i * 1024);
+            }
         }
     };
 
@@ -389,256 +457,331 @@ __global__ __launch_bounds__(kThreads) void shared_attention_kernel(SharedParams
         v_read = r * kRowBytes + ((c ^ vswz(r)) * 16) + (s % 2) * 8;
     }
 
-    std::uint32_t buffer = 0, serial = 1;
-    {
-        const Where at = where(tile);
-        fetch_ids(at);
-        issue(at, buffer, serial);
-    }
-    bool more = true;
-    while (more) {
-        // ---- a part: its columns and this wavefront's place.
-        const std::uint32_t first_row = cur.first_row, kvh = stream / cur.col_tiles;
-        const std::uint32_t col0 = (stream - kvh * cur.col_tiles) * kCols;
-        const std::uint32_t cols = cur.cols - col0 < kCols ? cur.cols - col0 : kCols;
-        const std::uint32_t layout = uniform(layout_blocks((cols + 15) / 16, S::kLeastBlocks));
-        const std::uint32_t shares = kWaves / layout;  // groups of wavefronts over a tile's tokens
-        const std::uint32_t block = uniform(wave / shares), token_share = uniform(wave % shares);
-        const bool active = block * 16 < cols;  // uniform in a wavefront
-        const bool is_prefix = seg < p.groups;
-        const std::uint32_t slot_of_part =
-            is_prefix ? group_stream(p, seg, first_row) + stream + w
-                      : (seg - p.groups) * p.heads * p.row_tiles + stream + w;
-        const std::uint32_t my_col = block * 16 + col;
-        const std::uint32_t c = col0 + (my_col < cols ? my_col : 0);
-        const std::uint32_t row_in = p.group.div(c);
-        const float* q = p.query + (static_cast<std::uint64_t>(first_row + row_in) * p.query_heads +
-                                    kvh * p.group.divisor + (c - row_in * p.group.divisor)) * kD;
-        Vec qb[kF32 ? 1 : 3][kKk];
-        float qf[kF32 ? kD / 4 : 1];
-        if constexpr (kF32) {
+    // ---- the tile loop, three tiles deep: `cur` is computed while `next` is
+    // loaded and the page ids of `ahead` are fetched. Its code is in one place
+    // only, the first rounds doing less: a launch starts with a cold instruction
+    // cache, and straight code runs at the speed of its misses.
+    Cursor cur = ahead, next = ahead;
+    next.ok = ahead.ok = false;
+    --ahead.tile;  // the first round moves it on
+    bool more = true, new_part = true;
+    std::uint32_t buffer = 1, serial = 0;  // of the tile in flight
+    // The part (the share's tiles of one stream) at hand: its columns and this
+    // wavefront's place.
+    std::uint32_t cols = 0, blocks = 1, shares = 1, across = 0, token_share = 0, first_col = 0;
+    bool active = false;
+    const std::uint64_t* table_row = p.table;
+    Vec qb[kBlocks][kF32 ? 1 : 3][kKk];
+    float qf[kF32 ? kD / 4 : 1];
+    pf_f32x4_t acc[kBlocks][kDt];
+    // Minus the column's reference (in all accumulator lanes: the seed of the
+    // score chains), and what a score may pass it by; -inf until the column has
+    // seen a key.
+    float nref[kBlocks], lazy[kBlocks], sum_hi[kBlocks], sum_lo[kBlocks];
+#pragma unroll 1
+    do {
+        if (next.ok && new_part) {
+            const Segment& part = next.s;
+            const std::uint32_t col0 = next.col_tile * kCols;
+            cols = part.cols - col0 < kCols ? part.cols - col0 : kCols;
+            const Spread spread = spread_of<E, kD>(cols);
+            blocks = spread.blocks;
+            shares = kWaves / spread.across;
+            across = wave / shares;
+            token_share = wave % shares;
+            first_col = across * blocks * 16;
+            active = first_col < cols;  // uniform in a wavefront
+            table_row = p.table + static_cast<std::uint64_t>(part.first_row) * p.width;
 #pragma unroll
-            for (int m = 0; m < kD / 16; ++m) {
-                const float4 x = *reinterpret_cast<const float4*>(q + 16 * m + 4 * quad);
-                qf[4 * m] = x.x * p.scale_log2;
-                qf[4 * m + 1] = x.y * p.scale_log2;
-                qf[4 * m + 2] = x.z * p.scale_log2;
-                qf[4 * m + 3] = x.w * p.scale_log2;
-            }
-        } else {
+            for (int n = 0; n < kBlocks; ++n) {
+                const std::uint32_t mine = first_col + 16 * n + col, c = col0 + (mine < cols ? mine : 0);
+                const std::uint32_t row_in = p.group.div(c);
+                const float* q = p.query + (static_cast<std::uint64_t>(part.first_row + row_in) * p.query_heads +
+                                            next.kvh * p.group.divisor + (c - row_in * p.group.divisor)) * kD;
+                if constexpr (kF32) {
 #pragma unroll
-            for (int kk = 0; kk < kKk; ++kk) {
-                const float4 lo = *reinterpret_cast<const float4*>(q + 32 * kk + 8 * quad);
-                const float4 hi = *reinterpret_cast<const float4*>(q + 32 * kk + 8 * quad + 4);
-                const float v[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
-                std::uint32_t parts[3][4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    std::uint32_t x[3];
-                    M::split3(v[2 * e] * p.scale_log2, v[2 * e + 1] * p.scale_log2, x);
-#pragma unroll
-                    for (int k = 0; k < 3; ++k) parts[k][e] = x[k];
-                }
-#pragma unroll
-                for (int k = 0; k < 3; ++k)
-                    qb[k][kk] = __builtin_bit_cast(Vec, make_uint4(parts[k][0], parts[k][1], parts[k][2], parts[k][3]));
-            }
-        }
-        pf_f32x4_t acc[kDt];
-#pragma unroll
-        for (int dt = 0; dt < kDt; ++dt) acc[dt] = pf_f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
-        // Minus the column's reference (in all accumulator lanes: the seed of
-        // the score chains), and what a score may pass it by; -inf until the
-        // column has seen a key.
-        float nref = 0.0f, lazy = -INFINITY, sum_hi = 0.0f, sum_lo = 0.0f;
-
-        const std::uint32_t seg_begin = cur.begin, seg_end = cur.end;
-        const std::uint64_t* const table_row = p.table + static_cast<std::uint64_t>(first_row) * p.width;
-        for (std::uint32_t left = tile_end - tile; left != 0; --left) {
-            // The tile has landed, for every wavefront, and the other buffer is
-            // no longer read.
-            wait_vm<0>();
-            wait_lgkm0();
-            lds_barrier();
-            const std::uint32_t here = buffer, here_serial = serial, here_first = seg_begin + tile * kTile;
-            buffer ^= 1;
-            ++serial;
-            ++tile;
-            if (left > 1 || (more = settle())) {  // settle() moves on to the next part
-                const Where at = where(tile);
-                fetch_ids(at);
-                issue(at, buffer, serial);
-            }
-            if (active) {
-                const unsigned char* kt = buffers[here];
-                const unsigned char* vt = buffers[here] + kBufferBytes / 2;
-                const bool bad = bad_tile[here] == here_serial;
-                const std::uint32_t per_wave = S::kSteps / shares;
-                for (std::uint32_t st = 0; st < per_wave; ++st) {
-                    const std::uint32_t row0 = (token_share * per_wave + st) * kStep;
-                    const std::uint32_t token0 = here_first + row0;
-                    if (token0 >= seg_end) break;  // uniform in a wavefront
-                    constexpr int kSubs = kF32 ? 1 : 2;  // 16-token score tiles of a step
-                    pf_f32x4_t s[kSubs];
-#pragma unroll
-                    for (int b = 0; b < kSubs; ++b) s[b] = pf_f32x4_t{nref, nref, nref, nref};
-                    if constexpr (kF32) {
-#pragma unroll
-                        for (int m = 0; m < kD / 16; ++m) {
-                            const float4 x = *reinterpret_cast<const float4*>(kt + row0 * kRowBytes + (k_read ^ (m << 6)));
-                            s[0] = __builtin_amdgcn_mfma_f32_16x16x4f32(x.x, qf[4 * m], s[0], 0, 0, 0);
-                            s[0] = __builtin_amdgcn_mfma_f32_16x16x4f32(x.y, qf[4 * m + 1], s[0], 0, 0, 0);
-                            s[0] = __builtin_amdgcn_mfma_f32_16x16x4f32(x.z, qf[4 * m + 2], s[0], 0, 0, 0);
-                            s[0] = __builtin_amdgcn_mfma_f32_16x16x4f32(x.w, qf[4 * m + 3], s[0], 0, 0, 0);
-                        }
-                    } else {
-#pragma unroll
-                        for (int kk = 0; kk < kKk; ++kk)
-#pragma unroll
-                            for (int b = 0; b < 2; ++b) {
-                                const Vec a = __builtin_bit_cast(
-                                    Vec, *reinterpret_cast<const uint4*>(kt + (row0 + 16 * b) * kRowBytes + (k_read ^ (kk << 6))));
-#pragma unroll
-                                for (int k = 0; k < 3; ++k) s[b] = M::mma(a, qb[k][kk], s[b]);
-                            }
+                    for (int m = 0; m < kD / 16; ++m) {
+                        const float4 x = *reinterpret_cast<const float4*>(q + 16 * m + 4 * quad);
+                        qf[4 * m] = x.x * p.scale_log2;
+                        qf[4 * m + 1] = x.y * p.scale_log2;
+                        qf[4 * m + 2] = x.z * p.scale_log2;
+                        qf[4 * m + 3] = x.w * p.scale_log2;
                     }
-                    if (bad || seg_end - token0 < kStep) {
+                } else {
 #pragma unroll
-                        for (int b = 0; b < kSubs; ++b)
-#pragma unroll
-                            for (int r = 0; r < 4; ++r) {
-                                const std::uint32_t token = token0 + 16 * b + 4 * quad + r;
-                                bool live = token < seg_end;
-                                if (bad && live) live = table_row[p.block_size.div(token)] < p.num_blocks;
-                                s[b][r] = live ? s[b][r] : -INFINITY;
-                            }
-                    }
-                    float top = -INFINITY;
-#pragma unroll
-                    for (int b = 0; b < kSubs; ++b) top = max3(top, max3(s[b][0], s[b][1], s[b][2]), s[b][3]);
-                    if (__builtin_expect(__builtin_amdgcn_ballot_w64(top > lazy) != 0, 0)) {
-                        top = max_across_quads(top);
-                        const bool moves = top > lazy;
-                        const float shift = moves ? top : 0.0f;
-                        if (moves) lazy = kLazy;
-                        const float alpha = __builtin_amdgcn_exp2f(fminf(-shift, 0.0f));
-                        nref -= shift;
-                        sum_hi *= alpha;
-                        sum_lo *= alpha;
-#pragma unroll
-                        for (int b = 0; b < kSubs; ++b) s[b] -= shift;
-#pragma unroll
-                        for (int dt = 0; dt < kDt; ++dt) acc[dt] *= alpha;
-                    }
-                    float pr[4 * kSubs];
-#pragma unroll
-                    for (int e = 0; e < 4 * kSubs; ++e) pr[e] = __builtin_amdgcn_exp2f(s[e / 4][e % 4]);
-                    if constexpr (kF32) {
-                        two_sum_add(sum_hi, sum_lo, (pr[0] + pr[1]) + (pr[2] + pr[3]));
-                        // MFMA r takes token 4 * quad + r of lane (quad, col); block
-                        // 4 * mm + j of O^T is dims 64 * mm + 4 * i + j, i = 0..15.
-#pragma unroll
-                        for (int r = 0; r < 4; ++r)
-#pragma unroll
-                            for (int mm = 0; mm < kD / 64; ++mm) {
-                                const float4 x = *reinterpret_cast<const float4*>(
-                                    vt + (row0 + r) * kRowBytes + v_read + 256 * mm);
-                                acc[4 * mm] = __builtin_amdgcn_mfma_f32_16x16x4f32(x.x, pr[r], acc[4 * mm], 0, 0, 0);
-                                acc[4 * mm + 1] = __builtin_amdgcn_mfma_f32_16x16x4f32(x.y, pr[r], acc[4 * mm + 1], 0, 0, 0);
-                                acc[4 * mm + 2] = __builtin_amdgcn_mfma_f32_16x16x4f32(x.z, pr[r], acc[4 * mm + 2], 0, 0, 0);
-                                acc[4 * mm + 3] = __builtin_amdgcn_mfma_f32_16x16x4f32(x.w, pr[r], acc[4 * mm + 3], 0, 0, 0);
-                            }
-                    } else {
-                        two_sum_add(sum_hi, sum_lo,
-                                    ((pr[0] + pr[1]) + (pr[2] + pr[3])) + ((pr[4] + pr[5]) + (pr[6] + pr[7])));
+                    for (int kk = 0; kk < kKk; ++kk) {
+                        const float4 lo = *reinterpret_cast<const float4*>(q + 32 * kk + 8 * quad);
+                        const float4 hi = *reinterpret_cast<const float4*>(q + 32 * kk + 8 * quad + 4);
+                        const float v[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
                         std::uint32_t parts[3][4];
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
                             std::uint32_t x[3];
-                            M::split3(pr[2 * e] * kWeightScale, pr[2 * e + 1] * kWeightScale, x);
+                            M::split3(v[2 * e] * p.scale_log2, v[2 * e + 1] * p.scale_log2, x);
 #pragma unroll
                             for (int k = 0; k < 3; ++k) parts[k][e] = x[k];
                         }
-                        Vec pb[3];
 #pragma unroll
                         for (int k = 0; k < 3; ++k)
-                            pb[k] = __builtin_bit_cast(Vec, make_uint4(parts[k][0], parts[k][1], parts[k][2], parts[k][3]));
-                        const auto* vbase = (__attribute__((address_space(3))) char*)(
-                            (__attribute__((address_space(3))) unsigned char*)vt);
+                            qb[n][k][kk] =
+                                __builtin_bit_cast(Vec, make_uint4(parts[k][0], parts[k][1], parts[k][2], parts[k][3]));
+                    }
+                }
 #pragma unroll
-                        for (int dt = 0; dt < kDt; ++dt) {
-                            const std::uint32_t off = row0 * kRowBytes + (v_read ^ (dt << 5));
-                            const pf_i16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((pf_lds_i16x4_t*)(vbase + off));
-                            const pf_i16x4_t hi =
-                                __builtin_amdgcn_ds_read_tr16_b64_v4i16((pf_lds_i16x4_t*)(vbase + off + 16 * kRowBytes));
-                            const Vec a = __builtin_bit_cast(Vec, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+                for (int dt = 0; dt < kDt; ++dt) acc[n][dt] = pf_f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+                nref[n] = sum_hi[n] = sum_lo[n] = 0.0f;
+                lazy[n] = -INFINITY;
+            }
+            new_part = false;
+        }
+        // The tile has landed, for every wavefront, and the other buffer is no
+        // longer read.
+        wait_vm<0>();
+        wait_lgkm0();
+        lds_barrier();
+        const std::uint32_t here = buffer, here_serial = serial;
+        cur = next;
+        next = ahead;
+        if (next.ok) {
+            buffer ^= 1;
+            issue(next, buffer, ++serial);
+        }
+        if (more) {
+            ++ahead.tile;
+            settle(ahead);
+            more = ahead.ok;
+            if (more) fetch_ids(ahead);
+        }
+        if (!cur.ok) continue;
+
+        // This wavefront's share of the tile.
+        const unsigned char *const kt = buffers[here], *const vt = kt + kBufferBytes / 2;
+        const bool bad = bad_tile[here] == here_serial;
+        const std::uint32_t first = first_token(cur), end = cur.s.end;
+        const auto compute = [&](auto block_count) {
+            constexpr int kN = decltype(block_count)::value;
+            const std::uint32_t steps = S::kSteps / shares;
+#pragma unroll 1
+            for (std::uint32_t st = 0; st < steps; ++st) {
+                const std::uint32_t row0 = (token_share * steps + st) * kStep;
+                const std::uint32_t token0 = first + row0;
+                if (token0 >= end) break;  // uniform in a wavefront
+                constexpr int kSubs = kF32 ? 1 : 2;  // 16-token score tiles of a step
+                pf_f32x4_t s[kN][kSubs];
 #pragma unroll
-                            for (int k = 0; k < 3; ++k) acc[dt] = M::mma(a, pb[k], acc[dt]);
+                for (int n = 0; n < kN; ++n)
+#pragma unroll
+                    for (int b = 0; b < kSubs; ++b) s[n][b] = pf_f32x4_t{nref[n], nref[n], nref[n], nref[n]};
+                if constexpr (kF32) {
+#pragma unroll
+                    for (int m = 0; m < kD / 16; ++m) {
+                        const float4 x = *reinterpret_cast<const float4*>(kt + row0 * kRowBytes + (k_read ^ (m << 6)));
+                        s[0][0] = __builtin_amdgcn_mfma_f32_16x16x4f32(x.x, qf[4 * m], s[0][0], 0, 0, 0);
+                        s[0][0] = __builtin_amdgcn_mfma_f32_16x16x4f32(x.y, qf[4 * m + 1], s[0][0], 0, 0, 0);
+                        s[0][0] = __builtin_amdgcn_mfma_f32_16x16x4f32(x.z, qf[4 * m + 2], s[0][0], 0, 0, 0);
+                        s[0][0] = __builtin_amdgcn_mfma_f32_16x16x4f32(x.w, qf[4 * m + 3], s[0][0], 0, 0, 0);
+                    }
+                } else {
+#pragma unroll
+                    for (int kk = 0; kk < kKk; ++kk)
+#pragma unroll
+                        for (int b = 0; b < 2; ++b) {
+                            const Vec a = __builtin_bit_cast(
+                                Vec, *reinterpret_cast<const uint4*>(kt + (row0 + 16 * b) * kRowBytes + (k_read ^ (kk << 6))));
+#pragma unroll
+                            for (int k = 0; k < 3; ++k)
+#pragma unroll
+                                for (int n = 0; n < kN; ++n) s[n][b] = M::mma(a, qb[n][k][kk], s[n][b]);
                         }
+                }
+                if (bad || end - token0 < kStep) {
+#pragma unroll
+                    for (int b = 0; b < kSubs; ++b)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) {
+                            const std::uint32_t token = token0 + 16 * b + 4 * quad + r;
+                            bool live = token < end;
+                            if (bad && live) live = table_row[p.block_size.div(token)] < p.num_blocks;
+#pragma unroll
+                            for (int n = 0; n < kN; ++n) s[n][b][r] = live ? s[n][b][r] : -INFINITY;
+                        }
+                }
+                float top[kN];
+                bool moves = false;
+#pragma unroll
+                for (int n = 0; n < kN; ++n) {
+                    top[n] = -INFINITY;
+#pragma unroll
+                    for (int b = 0; b < kSubs; ++b)
+                        top[n] = max3(top[n], max3(s[n][b][0], s[n][b][1], s[n][b][2]), s[n][b][3]);
+                    moves |= top[n] > lazy[n];
+                }
+                if (__builtin_expect(__builtin_amdgcn_ballot_w64(moves) != 0, 0)) {
+#pragma unroll
+                    for (int n = 0; n < kN; ++n) {
+                        const float high = max_across_quads(top[n]);
+                        const float shift = high > lazy[n] ? high : 0.0f;
+                        if (high > lazy[n]) lazy[n] = kLazy;
+                        const float alpha = __builtin_amdgcn_exp2f(fminf(-shift, 0.0f));
+                        nref[n] -= shift;
+                        sum_hi[n] *= alpha;
+                        sum_lo[n] *= alpha;
+#pragma unroll
+                        for (int b = 0; b < kSubs; ++b) s[n][b] -= shift;
+#pragma unroll
+                        for (int dt = 0; dt < kDt; ++dt) acc[n][dt] *= alpha;
+                    }
+                }
+                Vec pb[kN][3];
+                float pr[kN][4 * kSubs];
+#pragma unroll
+                for (int n = 0; n < kN; ++n) {
+#pragma unroll
+                    for (int e = 0; e < 4 * kSubs; ++e) pr[n][e] = __builtin_amdgcn_exp2f(s[n][e / 4][e % 4]);
+                    float of_step = (pr[n][0] + pr[n][1]) + (pr[n][2] + pr[n][3]);
+                    if constexpr (!kF32) {
+                        of_step += (pr[n][4] + pr[n][5]) + (pr[n][6] + pr[n][7]);
+                        std::uint32_t parts[3][4];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            std::uint32_t x[3];
+                            M::split3(pr[n][2 * e] * kWeightScale, pr[n][2 * e + 1] * kWeightScale, x);
+#pragma unroll
+                            for (int k = 0; k < 3; ++k) parts[k][e] = x[k];
+                        }
+#pragma unroll
+                        for (int k = 0; k < 3; ++k)
+                            pb[n][k] =
+                                __builtin_bit_cast(Vec, make_uint4(parts[k][0], parts[k][1], parts[k][2], parts[k][3]));
+                    }
+                    two_sum_add(sum_hi[n], sum_lo[n], of_step);
+                }
+                if constexpr (kF32) {
+                    // MFMA r takes token 4 * quad + r of lane (quad, col); block
+                    // 4 * mm + j of O^T is dims 64 * mm + 4 * i + j, i = 0..15.
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+#pragma unroll
+                        for (int mm = 0; mm < kD / 64; ++mm) {
+                            const float4 x = *reinterpret_cast<const float4*>(vt + (row0 + r) * kRowBytes + v_read + 256 * mm);
+                            pf_f32x4_t* const o = &acc[0][4 * mm];
+                            o[0] = __builtin_amdgcn_mfma_f32_16x16x4f32(x.x, pr[0][r], o[0], 0, 0, 0);
+                            o[1] = __builtin_amdgcn_mfma_f32_16x16x4f32(x.y, pr[0][r], o[1], 0, 0, 0);
+                            o[2] = __builtin_amdgcn_mfma_f32_16x16x4f32(x.z, pr[0][r], o[2], 0, 0, 0);
+                            o[3] = __builtin_amdgcn_mfma_f32_16x16x4f32(x.w, pr[0][r], o[3], 0, 0, 0);
+                        }
+                } else {
+                    const auto* vbase = (__attribute__((address_space(3))) char*)(
+                        (__attribute__((address_space(3))) unsigned char*)vt);
+#pragma unroll
+                    for (int dt = 0; dt < kDt; ++dt) {
+                        const std::uint32_t off = row0 * kRowBytes + (v_read ^ (dt << 5));
+                        const pf_i16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((pf_lds_i16x4_t*)(vbase + off));
+                        const pf_i16x4_t hi =
+                            __builtin_amdgcn_ds_read_tr16_b64_v4i16((pf_lds_i16x4_t*)(vbase + off + 16 * kRowBytes));
+                        const Vec a = __builtin_bit_cast(Vec, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+#pragma unroll
+                        for (int k = 0; k < 3; ++k)
+#pragma unroll
+                            for (int n = 0; n < kN; ++n) acc[n][dt] = M::mma(a, pb[n][k], acc[n][dt]);
                     }
                 }
             }
+        };
+        if (active) {
+            if constexpr (kBlocks > 1) {
+                if (blocks > 1) compute(std::integral_constant<int, kBlocks>{});
+                else compute(std::integral_constant<int, 1>{});
+            } else {
+                compute(std::integral_constant<int, 1>{});
+            }
         }
+        if (next.ok && next.seg == cur.seg && next.kvh == cur.kvh && next.col_tile == cur.col_tile) continue;
 
         // ---- the part's partials: merged over the wavefronts that shared its
         // tokens (through the buffer just computed), then to the workspace.
-        float sum = sum_across_quads(sum_hi + sum_lo);
-        float top = lazy == -INFINITY ? -INFINITY : -nref;
+        new_part = true;
+        const bool is_prefix = cur.seg < p.groups;
+        const std::uint32_t slot_of_part = (is_prefix ? group_stream(p, cur.seg, cur.s.first_row)
+                                                      : (cur.seg - p.groups) * p.heads * p.row_tiles) +
+                                           cur.kvh * cur.s.col_tiles + cur.col_tile + w;
+        float sum[kBlocks], top[kBlocks];
+#pragma unroll
+        for (int n = 0; n < kBlocks; ++n) {
+            sum[n] = sum_across_quads(sum_hi[n] + sum_lo[n]);
+            top[n] = lazy[n] == -INFINITY ? -INFINITY : -nref[n];
+        }
         if (shares > 1) {  // uniform
-            auto* const scratch = reinterpret_cast<pf_f32x4_t*>(buffers[buffer ^ 1]);
+            // [across][token share but the first][block][dt][lane]
+            auto* const scratch = reinterpret_cast<pf_f32x4_t*>(buffers[here]) + lane;
+            const auto place = [&](std::uint32_t share, int n) {
+                return ((across * (shares - 1) + share - 1) * blocks + n) * kDt * 64;
+            };
             wait_lgkm0();
             lds_barrier();  // every wavefront is done with the buffer
-            if (active && quad == 0) part_ml[wave][col] = make_float2(top, sum);
             if (active && token_share != 0) {
 #pragma unroll
-                for (int dt = 0; dt < kDt; ++dt)
-                    scratch[((block * (shares - 1) + token_share - 1) * kDt + dt) * 64 + lane] = acc[dt];
+                for (int n = 0; n < kBlocks; ++n) {
+                    if (n >= static_cast<int>(blocks)) break;
+                    if (quad == 0) part_ml[wave][n][col] = make_float2(top[n], sum[n]);
+#pragma unroll
+                    for (int dt = 0; dt < kDt; ++dt) scratch[place(token_share, n) + dt * 64] = acc[n][dt];
+                }
             }
             wait_lgkm0();
             lds_barrier();
             if (active && token_share == 0) {
-                float all = top;
-                for (std::uint32_t o = 1; o < shares; ++o) all = fmaxf(all, part_ml[wave + o][col].x);
-                const float f0 = merge_weight(top, all);
-                sum *= f0;
 #pragma unroll
-                for (int dt = 0; dt < kDt; ++dt) acc[dt] *= f0;
-                for (std::uint32_t o = 1; o < shares; ++o) {
-                    const float2 ml = part_ml[wave + o][col];
-                    const float f = merge_weight(ml.x, all);
-                    sum = fmaf(ml.y, f, sum);
+                for (int n = 0; n < kBlocks; ++n) {
+                    if (n >= static_cast<int>(blocks)) break;
+                    float all = top[n];
+                    for (std::uint32_t o = 1; o < shares; ++o) all = fmaxf(all, part_ml[wave + o][n][col].x);
+                    const float f0 = merge_weight(top[n], all);
+                    sum[n] *= f0;
+#pragma unroll
+                    for (int dt = 0; dt < kDt; ++dt) acc[n][dt] *= f0;
+                    for (std::uint32_t o = 1; o < shares; ++o) {
+                        const float2 ml = part_ml[wave + o][n][col];
+                        const float f = merge_weight(ml.x, all);
+                        sum[n] = fmaf(ml.y, f, sum[n]);
+#pragma unroll
+                        for (int dt = 0; dt < kDt; ++dt) {
+                            const pf_f32x4_t x = scratch[place(o, n) + dt * 64];
+#pragma unroll
+                            for (int r = 0; r < 4; ++r) acc[n][dt][r] = fmaf(x[r], f, acc[n][dt][r]);
+                        }
+                    }
+                    top[n] = all;
+                }
+            }
+        }
+        if (active && token_share == 0) {
+#pragma unroll
+            for (int n = 0; n < kBlocks; ++n) {
+                const std::uint32_t mine = first_col + 16 * n + col;
+                if (n >= static_cast<int>(blocks) || mine >= cols) continue;
+                const std::uint64_t at = static_cast<std::uint64_t>(slot_of_part) * (is_prefix ? kCols : p.row_cols) + mine;
+                float* out = (is_prefix ? p.prefix_acc : p.row_acc) + at * kD;
+                if (quad == 0)
+                    *reinterpret_cast<float2*>((is_prefix ? p.prefix_ml : p.row_ml) + 2 * at) = make_float2(top[n], sum[n]);
+                if constexpr (kF32) {
+#pragma unroll
+                    for (int mm = 0; mm < kD / 64; ++mm)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r)
+                            *reinterpret_cast<float4*>(out + 64 * mm + 16 * quad + 4 * r) =
+                                make_float4(acc[n][4 * mm][r], acc[n][4 * mm + 1][r], acc[n][4 * mm + 2][r],
+                                            acc[n][4 * mm + 3][r]);
+                } else {
 #pragma unroll
                     for (int dt = 0; dt < kDt; ++dt) {
-                        const pf_f32x4_t x = scratch[((block * (shares - 1) + o - 1) * kDt + dt) * 64 + lane];
-#pragma unroll
-                        for (int r = 0; r < 4; ++r) acc[dt][r] = fmaf(x[r], f, acc[dt][r]);
+                        const pf_f32x4_t x = acc[n][dt] * (1.0f / kWeightScale);  // a power of two: exact
+                        *reinterpret_cast<float4*>(out + 16 * dt + 4 * quad) = make_float4(x[0], x[1], x[2], x[3]);
                     }
                 }
-                top = all;
             }
         }
-        if (active && token_share == 0 && my_col < cols) {
-            const std::uint64_t at = is_prefix ? static_cast<std::uint64_t>(slot_of_part) * kCols + my_col
-                                               : static_cast<std::uint64_t>(slot_of_part) * p.row_cols + my_col;
-            float* out = (is_prefix ? p.prefix_acc : p.row_acc) + at * kD;
-            if (quad == 0)
-                *reinterpret_cast<float2*>((is_prefix ? p.prefix_ml : p.row_ml) + 2 * at) = make_float2(top, sum);
-            if constexpr (kF32) {
-#pragma unroll
-                for (int mm = 0; mm < kD / 64; ++mm)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r)
-                        *reinterpret_cast<float4*>(out + 64 * mm + 16 * quad + 4 * r) =
-                            make_float4(acc[4 * mm][r], acc[4 * mm + 1][r], acc[4 * mm + 2][r], acc[4 * mm + 3][r]);
-            } else {
-#pragma unroll
-                for (int dt = 0; dt < kDt; ++dt) {
-                    const pf_f32x4_t x = acc[dt] * (1.0f / kWeightScale);  // a power of two: exact
-                    *reinterpret_cast<float4*>(out + 16 * dt + 4 * quad) = make_float4(x[0], x[1], x[2], x[3]);
-                }
-            }
-        }
-    }
+    } while (next.ok || more);
 }
 
 // Merges the partials of every (row, query head): those of its prefix's stream
@@ -656,31 +799,38 @@ __global__ __launch_bounds__(kMergeThreads) void shared_merge_kernel(SharedParam
     __shared__ float4 sums[kMergeThreads];
     const std::uint32_t row = blockIdx.x / p.query_heads, head = blockIdx.x % p.query_heads;
     const std::uint32_t tid = threadIdx.x, wave = tid / 64, lane = tid % 64;
-    const std::uint64_t total = *p.total;
     const RowPlan plan = p.plans[row];
+    const std::uint32_t total = plan.total;
     const std::uint32_t kvh = p.group.div(head), g = head - kvh * p.group.divisor;
 
     // A stream's partials: workgroups first .. first + count - 1.
     struct Stream {
-        std::uint64_t cost;
-        std::uint32_t tiles, weight, first, count;
+        std::uint32_t cost, tiles, shift, first, count;
         std::uint64_t slot;  // partial of workgroup w: row slot + w * step of the arrays
         std::uint32_t step;
+    };
+    // The workgroup in whose share `at` lies: a guess in FP32, put right.
+    const float per_cost = static_cast<float>(kWorkgroups) / static_cast<float>(total);
+    const auto owner = [&](std::uint32_t at) {
+        auto w = static_cast<std::uint32_t>(static_cast<float>(at) * per_cost);
+        if (w >= kWorkgroups) w = kWorkgroups - 1;
+        while (share_begin(total, w) > at) --w;
+        while (share_begin(total, w + 1) <= at) ++w;
+        return w;
     };
     const auto span = [&](Stream& s) {
         s.first = s.count = 0;
         if (s.tiles == 0) return;
-        s.first = static_cast<std::uint32_t>(s.cost * kWorkgroups / total);
-        const std::uint64_t last = s.cost + static_cast<std::uint64_t>(s.tiles - 1) * s.weight;
-        s.count = static_cast<std::uint32_t>(last * kWorkgroups / total) - s.first + 1;
+        s.first = owner(s.cost);
+        s.count = owner(s.cost + ((s.tiles - 1) << s.shift)) - s.first + 1;
     };
     Stream prefix, own;
     {
         const std::uint32_t c = (row - plan.first_row) * p.group.divisor + g;  // column of the prefix
         const std::uint32_t stream = kvh * plan.prefix_col_tiles + c / kCols;
         prefix.tiles = plan.prefix_tiles;
-        prefix.weight = plan.prefix_weight;
-        prefix.cost = plan.prefix_cost + static_cast<std::uint64_t>(stream) * prefix.tiles * prefix.weight;
+        prefix.shift = plan.prefix_shift;
+        prefix.cost = plan.prefix_cost + (stream * prefix.tiles << prefix.shift);
         prefix.slot = static_cast<std::uint64_t>(plan.prefix_stream + stream) * kCols + c % kCols;
         prefix.step = kCols;
         span(prefix);
@@ -688,8 +838,8 @@ __global__ __launch_bounds__(kMergeThreads) void shared_merge_kernel(SharedParam
     {
         const std::uint32_t stream = kvh * p.row_tiles + g / kCols;
         own.tiles = plan.own_tiles;
-        own.weight = plan.own_weight;
-        own.cost = plan.own_cost + static_cast<std::uint64_t>(stream) * own.tiles * own.weight;
+        own.shift = plan.own_shift;
+        own.cost = plan.own_cost + (stream * own.tiles << own.shift);
         own.slot = (static_cast<std::uint64_t>(row) * p.heads * p.row_tiles + stream) * p.row_cols + g % kCols;
         own.step = p.row_cols;
         span(own);
@@ -707,9 +857,8 @@ __global__ __launch_bounds__(kMergeThreads) void shared_merge_kernel(SharedParam
         const bool of_prefix = i < prefix.count;
         const Stream& s = of_prefix ? prefix : own;
         const std::uint32_t w = s.first + (of_prefix ? i : i - prefix.count);
-        const std::uint64_t begin = share_begin(total, w), end = share_begin(total, w + 1);
-        const std::uint64_t t = begin > s.cost ? (begin - s.cost + s.weight - 1) / s.weight : 0;
-        return t < s.tiles && s.cost + t * s.weight < end;
+        const std::uint32_t t = tiles_before(share_begin(total, w), s.cost, s.shift);
+        return t < s.tiles && s.cost + (t << s.shift) < share_begin(total, w + 1);
     };
 
     float top = -INFINITY;
@@ -775,7 +924,7 @@ __global__ __launch_bounds__(kMergeThreads) void shared_merge_kernel(SharedParam
 
 // Bytes of the workspace's parts, each a multiple of 256.
 struct Layout {
-    std::uint64_t total = 0, plans = 0, prefix_acc = 0, prefix_ml = 0, row_acc = 0, row_ml = 0, bytes = 0;
+    std::uint64_t prefix_acc = 0, prefix_ml = 0, row_acc = 0, row_ml = 0, bytes = 0;
 };
 
 // Whether the shared kernel takes the call; if not it runs as an ordinary
@@ -784,8 +933,12 @@ bool takes(std::uint64_t rows, std::uint64_t kv_len, std::uint64_t kv_heads, std
            std::uint64_t block_size, std::uint64_t head_size, int dtype, std::uint64_t groups) {
     if (groups == 0 || groups > kMaxGroups || rows > kMaxRows) return false;
     if (head_size != 64 && head_size != 128 && (head_size != 256 || dtype == KVFLUX_DTYPE_F32)) return false;
-    return kv_len < 0x80000000ULL && block_size < 0x80000000ULL && kv_heads <= 65535 && query_heads <= 65535 &&
-           rows * query_heads < (1ULL << 24);  // workgroups of the merge
+    if (kv_len >= 0x80000000ULL || block_size >= 0x80000000ULL || kv_heads > 65535 || query_heads > 65535) return false;
+    if (rows * query_heads >= (1ULL << 24)) return false;  // workgroups of the merge
+    // Costs are summed in 32 bits: two for a tile at most, of 64 tokens at least.
+    const std::uint64_t group = query_heads / kv_heads;
+    const std::uint64_t streams = kv_heads * (rows * ((group + kCols - 1) / kCols) + groups + rows * group / kCols);
+    return streams * (kv_len / 64 + 1) < (1ULL << 30);
 }
 
 Layout layout_of(std::uint64_t rows, std::uint64_t kv_heads, std::uint64_t query_heads, std::uint64_t head_size,
@@ -796,8 +949,7 @@ Layout layout_of(std::uint64_t rows, std::uint64_t kv_heads, std::uint64_t query
     const std::uint64_t row_slots = rows * kv_heads * ((group + kCols - 1) / kCols) + kWorkgroups;
     const std::uint64_t row_cols = group < kCols ? group : kCols;
     Layout l;
-    l.plans = 256;
-    l.prefix_acc = l.plans + whole(rows * sizeof(RowPlan));
+    l.prefix_acc = whole(rows * sizeof(RowPlan));  // the plans come first
     l.prefix_ml = l.prefix_acc + whole(prefix_slots * kCols * head_size * sizeof(float));
     l.row_acc = l.prefix_ml + whole(prefix_slots * kCols * 2 * sizeof(float));
     l.row_ml = l.row_acc + whole(row_slots * row_cols * head_size * sizeof(float));
@@ -807,7 +959,10 @@ Layout layout_of(std::uint64_t rows, std::uint64_t kv_heads, std::uint64_t query
 
 template <typename E, int kD>
 int launch(const SharedParams& p, hipStream_t s) {
-    hipLaunchKernelGGL((shared_attention_kernel<E, kD>), dim3(kWorkgroups), dim3(kThreads), 0, s, p);
+    if (p.block_size.divisor % 16 == 0)
+        hipLaunchKernelGGL((shared_attention_kernel<E, kD, true>), dim3(kWorkgroups), dim3(kThreads), 0, s, p);
+    else
+        hipLaunchKernelGGL((shared_attention_kernel<E, kD, false>), dim3(kWorkgroups), dim3(kThreads), 0, s, p);
     const int status = launch_status("shared_attention_kernel");
     if (status != KVFLUX_OK) return status;
     hipLaunchKernelGGL((shared_merge_kernel<kD>), dim3(p.rows * p.query_heads), dim3(kMergeThreads), 0, s, p);
@@ -901,8 +1056,7 @@ extern "C" int kvflux_paged_attention_shared(const void* key_cache, const void* 
     p.output = output;
     p.scale_log2 = static_cast<float>(1.4426950408889634 / std::sqrt(static_cast<double>(head_size)));
     char* base = static_cast<char*>(workspace);
-    p.total = reinterpret_cast<std::uint64_t*>(base);
-    p.plans = reinterpret_cast<RowPlan*>(base + l.plans);
+    p.plans = reinterpret_cast<RowPlan*>(base);
     p.prefix_acc = reinterpret_cast<float*>(base + l.prefix_acc);
     p.prefix_ml = reinterpret_cast<float*>(base + l.prefix_ml);
     p.row_acc = reinterpret_cast<float*>(base + l.row_acc);
