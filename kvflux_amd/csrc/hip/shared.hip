@@ -114,30 +114,36 @@ struct SharedParams {
 // What the merge needs of a row.
 struct RowPlan {
     std::uint32_t prefix_cost, own_cost;  // costs before the segments
-    std::uint32_t prefix_tiles, prefix_shift, prefix_col_tiles, prefix_stream;
-    std::uint32_t first_row, own_tiles, own_shift, total;
+    std::uint32_t prefix_tiles, prefix_weight, prefix_col_tiles, prefix_stream;
+    std::uint32_t first_row, own_tiles, own_weight, total;
 };
+
+// Cost of a tile in about 1000 cycles, by the blocks of 16 columns it is computed
+// for (rounded up to a power of two, as the wavefronts are laid out): what any
+// tile takes, to be loaded, and its products, which a tile of a fixed size in
+// bytes has as many of at every head size. A part starts with its queries and
+// ends with its partials: kPartCost, in the stream's first tile.
+constexpr std::uint32_t kPartCost = 4, kTileCost = 4, kMostTileCost = kTileCost + 3 * kCols / 16;
+template <typename E, int kD>
+__device__ inline std::uint32_t tile_cost(std::uint32_t cols) {
+    const std::uint32_t blocks = cols > 64 ? 8 : cols > 32 ? 4 : cols > 16 ? 2 : 1;
+    return kTileCost + (Shape<E, kD>::kF32 ? 3 : 1) * blocks;
+}
 
 // A segment: the columns (of row first_row on), the tokens [begin, end) of
-// table row first_row, its tiles and the cost of one (1 << shift).
+// table row first_row, its tiles and the cost of one.
 struct Segment {
-    std::uint32_t first_row, cols, col_tiles, begin, end, tiles, shift;
-    __device__ std::uint32_t stream_cost() const { return tiles << shift; }
+    std::uint32_t first_row, cols, col_tiles, begin, end, tiles, weight;
+    __device__ std::uint32_t stream_cost() const { return tiles != 0 ? tiles * weight + kPartCost : 0; }
     __device__ std::uint32_t cost(std::uint32_t heads) const { return stream_cost() * (heads * col_tiles); }
 };
-
-// Cost of a tile, as a power of two.
-template <typename E, int kD>
-__device__ inline std::uint32_t tile_shift(std::uint32_t cols) {
-    return cols > kCols / 2 ? 1 : 0;
-}
 
 template <typename E, int kD>
 __device__ inline Segment make_segment(std::uint32_t first_row, std::uint32_t cols, std::uint32_t begin, std::uint32_t end) {
     constexpr std::uint32_t kTile = Shape<E, kD>::kTile;
     Segment s{first_row, cols, (cols + kCols - 1) / kCols, begin, end, 0, 0};
     s.tiles = end > begin ? (end - begin - 1) / kTile + 1 : 0;
-    s.shift = tile_shift<E, kD>(cols);
+    s.weight = tile_cost<E, kD>(cols);
     return s;
 }
 
@@ -163,10 +169,13 @@ __device__ inline std::uint32_t group_stream(const SharedParams& p, std::uint32_
 __device__ inline std::uint32_t share_begin(std::uint32_t total, std::uint32_t w) {
     return total / kWorkgroups * w + (total % kWorkgroups * w + kWorkgroups - 1) / kWorkgroups;
 }
-// The tiles before the first that starts at `at` or behind it, of a stream whose
-// first tile starts at `cost`.
-__device__ inline std::uint32_t tiles_before(std::uint32_t at, std::uint32_t cost, std::uint32_t shift) {
-    return at > cost ? (at - cost + (1u << shift) - 1) >> shift : 0;
+// Where tile t of a stream starts, behind the stream's start; and the tiles
+// before the first that starts at `at` or behind it.
+__device__ inline std::uint32_t tile_start(std::uint32_t t, std::uint32_t weight) {
+    return t == 0 ? 0 : t * weight + kPartCost;
+}
+__device__ inline std::uint32_t tiles_before(std::uint32_t at, std::uint32_t weight) {
+    return at == 0 ? 0 : at <= weight + kPartCost ? 1 : (at - kPartCost + weight - 1) / weight;
 }
 
 // exp2(m - top) for merging partials: 0 for a part that saw no key.
@@ -301,13 +310,13 @@ __global__ __launch_bounds__(kThreads) void shared_attention_kernel(SharedParams
     if (w == 0) {  // uniform: the rows' plans for the merge
         for (std::uint32_t r = tid; r < p.rows; r += kThreads) {
             const Segment own = segment(p.groups + r);
-            RowPlan plan{0, cost_of[p.groups + r], 0, 0, 1, 0, 0, own.tiles, own.shift, total};
+            RowPlan plan{0, cost_of[p.groups + r], 0, 0, 1, 0, 0, own.tiles, own.weight, total};
             if (own.begin != 0) {
                 const std::uint32_t g = group_of(first_of, p.groups, r);
                 const Segment prefix = segment(g);
                 plan.prefix_cost = cost_of[g];
                 plan.prefix_tiles = prefix.tiles;
-                plan.prefix_shift = prefix.shift;
+                plan.prefix_weight = prefix.weight;
                 plan.prefix_col_tiles = prefix.col_tiles;
                 plan.prefix_stream = group_stream(p, g, prefix.first_row);
                 plan.first_row = prefix.first_row;
@@ -325,7 +334,7 @@ __global__ __launch_bounds__(kThreads) void shared_attention_kernel(SharedParams
     const auto uniform_segment = [&](std::uint32_t s) {
         const Segment x = segment(s);
         return Segment{uniform(x.first_row), uniform(x.cols), uniform(x.col_tiles), uniform(x.begin), uniform(x.end),
-                       uniform(x.tiles), uniform(x.shift)};
+                       uniform(x.tiles), uniform(x.weight)};
     };
     Cursor ahead;  // the tile whose page ids are fetched next
     ahead.seg = uniform(found);
@@ -338,13 +347,13 @@ __global__ __launch_bounds__(kThreads) void shared_attention_kernel(SharedParams
         ahead.kvh = stream / ahead.s.col_tiles;
         ahead.col_tile = stream - ahead.kvh * ahead.s.col_tiles;
     }
-    ahead.tile = tiles_before(share, ahead.cost, ahead.s.shift);
+    ahead.tile = tiles_before(share - ahead.cost, ahead.s.weight);
     // A cursor past its stream's end moves on to the next tile there is.
     const auto settle = [&](Cursor& c) {
 #pragma unroll 1
         while (true) {
             if (c.tile < c.s.tiles) {
-                c.ok = c.cost + (c.tile << c.s.shift) < share_end;
+                c.ok = c.cost + tile_start(c.tile, c.s.weight) < share_end;
                 return;
             }
             c.cost += c.s.stream_cost();
@@ -805,7 +814,7 @@ __global__ __launch_bounds__(kMergeThreads) void shared_merge_kernel(SharedParam
 
     // A stream's partials: workgroups first .. first + count - 1.
     struct Stream {
-        std::uint32_t cost, tiles, shift, first, count;
+        std::uint32_t cost, tiles, weight, first, count;
         std::uint64_t slot;  // partial of workgroup w: row slot + w * step of the arrays
         std::uint32_t step;
     };
@@ -822,15 +831,15 @@ __global__ __launch_bounds__(kMergeThreads) void shared_merge_kernel(SharedParam
         s.first = s.count = 0;
         if (s.tiles == 0) return;
         s.first = owner(s.cost);
-        s.count = owner(s.cost + ((s.tiles - 1) << s.shift)) - s.first + 1;
+        s.count = owner(s.cost + tile_start(s.tiles - 1, s.weight)) - s.first + 1;
     };
     Stream prefix, own;
     {
         const std::uint32_t c = (row - plan.first_row) * p.group.divisor + g;  // column of the prefix
         const std::uint32_t stream = kvh * plan.prefix_col_tiles + c / kCols;
         prefix.tiles = plan.prefix_tiles;
-        prefix.shift = plan.prefix_shift;
-        prefix.cost = plan.prefix_cost + (stream * prefix.tiles << prefix.shift);
+        prefix.weight = plan.prefix_weight;
+        prefix.cost = plan.prefix_cost + stream * (prefix.tiles * prefix.weight + kPartCost);
         prefix.slot = static_cast<std::uint64_t>(plan.prefix_stream + stream) * kCols + c % kCols;
         prefix.step = kCols;
         span(prefix);
@@ -838,8 +847,8 @@ __global__ __launch_bounds__(kMergeThreads) void shared_merge_kernel(SharedParam
     {
         const std::uint32_t stream = kvh * p.row_tiles + g / kCols;
         own.tiles = plan.own_tiles;
-        own.shift = plan.own_shift;
-        own.cost = plan.own_cost + (stream * own.tiles << own.shift);
+        own.weight = plan.own_weight;
+        own.cost = plan.own_cost + stream * (own.tiles * own.weight + kPartCost);
         own.slot = (static_cast<std::uint64_t>(row) * p.heads * p.row_tiles + stream) * p.row_cols + g % kCols;
         own.step = p.row_cols;
         span(own);
@@ -857,8 +866,8 @@ __global__ __launch_bounds__(kMergeThreads) void shared_merge_kernel(SharedParam
         const bool of_prefix = i < prefix.count;
         const Stream& s = of_prefix ? prefix : own;
         const std::uint32_t w = s.first + (of_prefix ? i : i - prefix.count);
-        const std::uint32_t t = tiles_before(share_begin(total, w), s.cost, s.shift);
-        return t < s.tiles && s.cost + (t << s.shift) < share_begin(total, w + 1);
+        const std::uint32_t begin = share_begin(total, w), t = tiles_before(begin > s.cost ? begin - s.cost : 0, s.weight);
+        return t < s.tiles && s.cost + tile_start(t, s.weight) < share_begin(total, w + 1);
     };
 
     float top = -INFINITY;
@@ -935,10 +944,10 @@ bool takes(std::uint64_t rows, std::uint64_t kv_len, std::uint64_t kv_heads, std
     if (head_size != 64 && head_size != 128 && (head_size != 256 || dtype == KVFLUX_DTYPE_F32)) return false;
     if (kv_len >= 0x80000000ULL || block_size >= 0x80000000ULL || kv_heads > 65535 || query_heads > 65535) return false;
     if (rows * query_heads >= (1ULL << 24)) return false;  // workgroups of the merge
-    // Costs are summed in 32 bits: two for a tile at most, of 64 tokens at least.
+    // Costs are summed in 32 bits; a tile has 64 tokens at least.
     const std::uint64_t group = query_heads / kv_heads;
     const std::uint64_t streams = kv_heads * (rows * ((group + kCols - 1) / kCols) + groups + rows * group / kCols);
-    return streams * (kv_len / 64 + 1) < (1ULL << 30);
+    return streams * (kv_len / 64 + 1) < (1ULL << 31) / (kMostTileCost + kPartCost);
 }
 
 Layout layout_of(std::uint64_t rows, std::uint64_t kv_heads, std::uint64_t query_heads, std::uint64_t head_size,
