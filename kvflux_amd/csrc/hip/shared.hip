@@ -576,6 +576,7 @@ __global__ __launch_bounds__(kThreads) void shared_attention_kernel(SharedParams
                 const std::uint32_t token0 = first + row0;
                 if (token0 >= end) break;  // uniform in a wavefront
                 constexpr int kSubs = kF32 ? 1 : 2;  // 16-token score tiles of a step
+                set_priority<1>();
                 pf_f32x4_t s[kN][kSubs];
 #pragma unroll
                 for (int n = 0; n < kN; ++n)
@@ -603,6 +604,30 @@ __global__ __launch_bounds__(kThreads) void shared_attention_kernel(SharedParams
                                 for (int n = 0; n < kN; ++n) s[n][b] = M::mma(a, qb[n][k][kk], s[n][b]);
                         }
                 }
+                // V^T operand of dims 16 dt on. At head size 128 all of them are read
+                // behind K, under the score MFMAs, and those run at a raised
+                // priority, the SIMD's other wavefront in its softmax meanwhile
+                // (48 rows behind 60000 tokens: 270 -> 254 us); at 256 they do not
+                // fit the registers.
+                constexpr bool kEarlyV = !kF32 && kD == 128;
+                Vec vop[kEarlyV ? kDt : 1];
+                const auto read_v = [&](int dt) {
+                    const auto* base = (__attribute__((address_space(3))) char*)(
+                        (__attribute__((address_space(3))) unsigned char*)vt);
+                    const std::uint32_t off = row0 * kRowBytes + (v_read ^ (dt << 5));
+                    const pf_i16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((pf_lds_i16x4_t*)(base + off));
+                    const pf_i16x4_t hi =
+                        __builtin_amdgcn_ds_read_tr16_b64_v4i16((pf_lds_i16x4_t*)(base + off + 16 * kRowBytes));
+                    return __builtin_bit_cast(Vec, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+                };
+                if constexpr (kEarlyV) {
+#pragma unroll
+                    for (int dt = 0; dt < kDt; ++dt) vop[dt] = read_v(dt);
+                    __builtin_amdgcn_sched_group_barrier(0x100, 2 * kKk, 0);       // the K reads
+                    __builtin_amdgcn_sched_group_barrier(0x008, 6 * kKk * kN, 0);  // the score MFMAs
+                    __builtin_amdgcn_sched_group_barrier(0x100, 2 * kDt, 0);       // the V reads
+                }
+                set_priority<0>();
                 if (bad || end - token0 < kStep) {
 #pragma unroll
                     for (int b = 0; b < kSubs; ++b)
@@ -680,15 +705,9 @@ __global__ __launch_bounds__(kThreads) void shared_attention_kernel(SharedParams
                             o[3] = __builtin_amdgcn_mfma_f32_16x16x4f32(x.w, pr[0][r], o[3], 0, 0, 0);
                         }
                 } else {
-                    const auto* vbase = (__attribute__((address_space(3))) char*)(
-                        (__attribute__((address_space(3))) unsigned char*)vt);
 #pragma unroll
                     for (int dt = 0; dt < kDt; ++dt) {
-                        const std::uint32_t off = row0 * kRowBytes + (v_read ^ (dt << 5));
-                        const pf_i16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((pf_lds_i16x4_t*)(vbase + off));
-                        const pf_i16x4_t hi =
-                            __builtin_amdgcn_ds_read_tr16_b64_v4i16((pf_lds_i16x4_t*)(vbase + off + 16 * kRowBytes));
-                        const Vec a = __builtin_bit_cast(Vec, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+                        const Vec a = kEarlyV ? vop[kEarlyV ? dt : 0] : read_v(dt);
 #pragma unroll
                         for (int k = 0; k < 3; ++k)
 #pragma unroll
@@ -794,121 +813,142 @@ __global__ __launch_bounds__(kThreads) void shared_attention_kernel(SharedParams
 }
 
 // Merges the partials of every (row, query head): those of its prefix's stream
-// and of its own, in the order of the workgroups that left them. Both streams'
-// workgroups are neighbours, from the one whose share their first tile starts
-// in to the one of their last; a workgroup in between has a partial where a
-// tile of the stream starts in its share.
-constexpr int kMergeThreads = 128;
-template <int kD>
+// and of its own, in the order of the workgroups that left them. A stream's
+// workgroups are neighbours, from the one whose share its first tile starts in
+// to the one of its last; one in between has a partial where a tile of the
+// stream starts in its share (a share may be shorter than a tile's cost).
+// Latency is all there is to it: the plan, then the partials' (m, sum) and the
+// first four accumulators of every group of lanes at once, then the others four
+// at a time (20 rows of 48 parts at head size 256, one load after the other:
+// 15.0 us).
+// Launches of more workgroups than the chip holds at once hide the latency behind
+// each other: there one wavefront does it, without barriers to wait at (4096
+// workgroups: 14.6 us with 256 threads).
+constexpr std::uint64_t kManyMerges = 2048;
+template <int kD, int kMergeThreads>
 __global__ __launch_bounds__(kMergeThreads) void shared_merge_kernel(SharedParams p) {
     constexpr std::uint32_t kMost = 2 * kWorkgroups;
-    constexpr std::uint32_t kLanes = kD / 4, kGroups = kMergeThreads / kLanes;
-    __shared__ float weight[kMost];  // the part's factor; below 0: no partial
-    __shared__ float wave_value[2][kMergeThreads / 64];
+    constexpr int kMergeWaves = kMergeThreads / 64, kPer = kMost / kMergeThreads;
+    constexpr std::uint32_t kLanes = kD / 4, kGroups = kMergeThreads / kLanes, kAhead = 4;
+    struct Stream {
+        std::uint32_t cost, tiles, weight, first, count;  // partials of workgroups first .. first + count - 1
+        std::uint32_t slot, step;  // of workgroup w: row slot + w * step of the arrays
+    };
+    __shared__ Stream streams[2];  // the prefix's, the row's own
+    __shared__ float weight[kMost];  // a part's factor; below 0: there is no partial
+    __shared__ float wave_value[2][kMergeWaves];
     __shared__ float4 sums[kMergeThreads];
     const std::uint32_t row = blockIdx.x / p.query_heads, head = blockIdx.x % p.query_heads;
     const std::uint32_t tid = threadIdx.x, wave = tid / 64, lane = tid % 64;
     const RowPlan plan = p.plans[row];
     const std::uint32_t total = plan.total;
-    const std::uint32_t kvh = p.group.div(head), g = head - kvh * p.group.divisor;
-
-    // A stream's partials: workgroups first .. first + count - 1.
-    struct Stream {
-        std::uint32_t cost, tiles, weight, first, count;
-        std::uint64_t slot;  // partial of workgroup w: row slot + w * step of the arrays
-        std::uint32_t step;
-    };
-    // The workgroup in whose share `at` lies: a guess in FP32, put right.
-    const float per_cost = static_cast<float>(kWorkgroups) / static_cast<float>(total);
-    const auto owner = [&](std::uint32_t at) {
-        auto w = static_cast<std::uint32_t>(static_cast<float>(at) * per_cost);
-        if (w >= kWorkgroups) w = kWorkgroups - 1;
-        while (share_begin(total, w) > at) --w;
-        while (share_begin(total, w + 1) <= at) ++w;
-        return w;
-    };
-    const auto span = [&](Stream& s) {
+    for (std::uint32_t which = wave; which < 2; which += kMergeWaves) {
+        const bool of_prefix = which == 0;
+        const std::uint32_t kvh = p.group.div(head), g = head - kvh * p.group.divisor;
+        const std::uint32_t c = of_prefix ? (row - plan.first_row) * p.group.divisor + g : g;  // column
+        const std::uint32_t stream = kvh * (of_prefix ? plan.prefix_col_tiles : p.row_tiles) + c / kCols;
+        Stream s;
+        s.tiles = of_prefix ? plan.prefix_tiles : plan.own_tiles;
+        s.weight = of_prefix ? plan.prefix_weight : plan.own_weight;
+        s.cost = (of_prefix ? plan.prefix_cost : plan.own_cost) + stream * (s.tiles * s.weight + kPartCost);
+        s.step = of_prefix ? kCols : p.row_cols;
+        s.slot = ((of_prefix ? plan.prefix_stream : row * p.heads * p.row_tiles) + stream) * s.step + c % kCols;
+        // The workgroup in whose share a cost lies: a guess in FP32, put right.
+        const float per_cost = static_cast<float>(kWorkgroups) / static_cast<float>(total);
+        const auto owner = [&](std::uint32_t at) {
+            auto w = static_cast<std::uint32_t>(static_cast<float>(at) * per_cost);
+            if (w >= kWorkgroups) w = kWorkgroups - 1;
+            while (share_begin(total, w) > at) --w;
+            while (share_begin(total, w + 1) <= at) ++w;
+            return w;
+        };
         s.first = s.count = 0;
-        if (s.tiles == 0) return;
-        s.first = owner(s.cost);
-        s.count = owner(s.cost + tile_start(s.tiles - 1, s.weight)) - s.first + 1;
-    };
-    Stream prefix, own;
-    {
-        const std::uint32_t c = (row - plan.first_row) * p.group.divisor + g;  // column of the prefix
-        const std::uint32_t stream = kvh * plan.prefix_col_tiles + c / kCols;
-        prefix.tiles = plan.prefix_tiles;
-        prefix.weight = plan.prefix_weight;
-        prefix.cost = plan.prefix_cost + stream * (prefix.tiles * prefix.weight + kPartCost);
-        prefix.slot = static_cast<std::uint64_t>(plan.prefix_stream + stream) * kCols + c % kCols;
-        prefix.step = kCols;
-        span(prefix);
-    }
-    {
-        const std::uint32_t stream = kvh * p.row_tiles + g / kCols;
-        own.tiles = plan.own_tiles;
-        own.weight = plan.own_weight;
-        own.cost = plan.own_cost + stream * (own.tiles * own.weight + kPartCost);
-        own.slot = (static_cast<std::uint64_t>(row) * p.heads * p.row_tiles + stream) * p.row_cols + g % kCols;
-        own.step = p.row_cols;
-        span(own);
-    }
-    const std::uint32_t parts = prefix.count + own.count;
-    const auto partial = [&](std::uint32_t i, const float** acc) {  // its (m, sum), and its place
-        const bool of_prefix = i < prefix.count;
-        const Stream& s = of_prefix ? prefix : own;
-        const std::uint32_t w = s.first + (of_prefix ? i : i - prefix.count);
-        const std::uint64_t at = s.slot + static_cast<std::uint64_t>(w) * s.step;
-        *acc = (of_prefix ? p.prefix_acc : p.row_acc) + at * kD;
-        return (of_prefix ? p.prefix_ml : p.row_ml) + 2 * at;
-    };
-    const auto exists = [&](std::uint32_t i) {
-        const bool of_prefix = i < prefix.count;
-        const Stream& s = of_prefix ? prefix : own;
-        const std::uint32_t w = s.first + (of_prefix ? i : i - prefix.count);
-        const std::uint32_t begin = share_begin(total, w), t = tiles_before(begin > s.cost ? begin - s.cost : 0, s.weight);
-        return t < s.tiles && s.cost + tile_start(t, s.weight) < share_begin(total, w + 1);
-    };
-
-    float top = -INFINITY;
-    for (std::uint32_t i = tid; i < parts; i += kMergeThreads) {
-        const float* acc;
-        const float* ml = partial(i, &acc);
-        if (exists(i)) top = fmaxf(top, ml[0]);
-    }
-#pragma unroll
-    for (int x = 1; x < 64; x <<= 1) top = fmaxf(top, __shfl_xor(top, x));
-    if (lane == 0) wave_value[0][wave] = top;
-    __syncthreads();
-    top = fmaxf(wave_value[0][0], wave_value[0][1]);
-    float sum = 0.0f;
-    for (std::uint32_t i = tid; i < parts; i += kMergeThreads) {
-        const float* acc;
-        const float* ml = partial(i, &acc);
-        float f = -1.0f;
-        if (exists(i)) {
-            f = merge_weight(ml[0], top);
-            sum = fmaf(ml[1], f, sum);
+        if (s.tiles != 0) {
+            s.first = owner(s.cost);
+            s.count = owner(s.cost + tile_start(s.tiles - 1, s.weight)) - s.first + 1;
         }
-        weight[i] = f;
+        if (lane == 0) streams[which] = s;
     }
-#pragma unroll
-    for (int x = 1; x < 64; x <<= 1) sum += __shfl_xor(sum, x);
-    if (lane == 0) wave_value[1][wave] = sum;
     __syncthreads();
-    sum = wave_value[1][0] + wave_value[1][1];
-    const std::uint32_t part0 = tid / kLanes, d4 = tid % kLanes;
+    const std::uint32_t prefix_parts = streams[0].count, parts = prefix_parts + streams[1].count;
+    // Row of part i in its arrays (past the parts: of the last one).
+    const auto place = [&](std::uint32_t i, bool* of_prefix, std::uint32_t* w) {
+        if (i >= parts) i = parts - 1;
+        *of_prefix = i < prefix_parts;
+        const Stream& s = streams[*of_prefix ? 0 : 1];
+        *w = s.first + i - (*of_prefix ? 0u : prefix_parts);
+        return s.slot + static_cast<std::uint64_t>(*w) * s.step;
+    };
+    const std::uint32_t group = tid / kLanes, d4 = tid % kLanes;
+    const auto accumulator = [&](std::uint32_t i) {
+        bool of_prefix;
+        std::uint32_t w;
+        const std::uint64_t at = place(i, &of_prefix, &w);
+        return *reinterpret_cast<const float4*>((of_prefix ? p.prefix_acc : p.row_acc) + at * kD + 4 * d4);
+    };
     float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    for (std::uint32_t i = part0; i < parts; i += kGroups) {
-        const float f = weight[i];
-        if (f < 0.0f) continue;
-        const float* acc;
-        partial(i, &acc);
-        const float4 x = *reinterpret_cast<const float4*>(acc + 4 * d4);
-        o.x = fmaf(x.x, f, o.x);
-        o.y = fmaf(x.y, f, o.y);
-        o.z = fmaf(x.z, f, o.z);
-        o.w = fmaf(x.w, f, o.w);
+    float sum = 0.0f;
+    if (parts != 0) {  // uniform
+        float4 ahead[kAhead];
+#pragma unroll
+        for (std::uint32_t u = 0; u < kAhead; ++u) ahead[u] = accumulator(group + u * kGroups);
+        float m[kPer], l[kPer];  // a thread's parts: tid + k * kMergeThreads
+        float top = -INFINITY;
+#pragma unroll
+        for (int k = 0; k < kPer; ++k) {
+            m[k] = -INFINITY;
+            l[k] = -1.0f;  // sums are never negative
+            if (k * kMergeThreads >= parts) break;  // uniform
+            bool of_prefix;
+            std::uint32_t w;
+            const std::uint64_t at = place(tid + k * kMergeThreads, &of_prefix, &w);
+            const float2 ml = *reinterpret_cast<const float2*>((of_prefix ? p.prefix_ml : p.row_ml) + 2 * at);
+            const Stream& s = streams[of_prefix ? 0 : 1];
+            const std::uint32_t begin = share_begin(total, w);
+            const std::uint32_t t = tiles_before(begin > s.cost ? begin - s.cost : 0, s.weight);
+            const bool there = tid + k * kMergeThreads < parts && t < s.tiles &&
+                               s.cost + tile_start(t, s.weight) < share_begin(total, w + 1);
+            m[k] = there ? ml.x : -INFINITY;
+            l[k] = there ? ml.y : -1.0f;
+            top = fmaxf(top, m[k]);
+        }
+#pragma unroll
+        for (int x = 1; x < 64; x <<= 1) top = fmaxf(top, __shfl_xor(top, x));
+        if (lane == 0) wave_value[0][wave] = top;
+        __syncthreads();
+#pragma unroll
+        for (int x = 0; x < kMergeWaves; ++x) top = fmaxf(top, wave_value[0][x]);
+#pragma unroll
+        for (int k = 0; k < kPer; ++k) {
+            if (k * kMergeThreads >= parts) break;  // uniform
+            const float f = merge_weight(m[k], top);
+            if (l[k] != -1.0f) sum = fmaf(l[k], f, sum);
+            weight[tid + k * kMergeThreads] = l[k] != -1.0f ? f : -1.0f;
+        }
+#pragma unroll
+        for (int x = 1; x < 64; x <<= 1) sum += __shfl_xor(sum, x);
+        if (lane == 0) wave_value[1][wave] = sum;
+        __syncthreads();
+        sum = 0.0f;
+#pragma unroll
+        for (int x = 0; x < kMergeWaves; ++x) sum += wave_value[1][x];
+#pragma unroll 1
+        for (std::uint32_t i = group;; i += kAhead * kGroups) {
+#pragma unroll
+            for (std::uint32_t u = 0; u < kAhead; ++u) {
+                const std::uint32_t part = i + u * kGroups;
+                const float f = part < parts ? weight[part] : -1.0f;
+                if (f >= 0.0f) {
+                    o.x = fmaf(ahead[u].x, f, o.x);
+                    o.y = fmaf(ahead[u].y, f, o.y);
+                    o.z = fmaf(ahead[u].z, f, o.z);
+                    o.w = fmaf(ahead[u].w, f, o.w);
+                }
+            }
+            if (i + kAhead * kGroups >= parts) break;
+#pragma unroll
+            for (std::uint32_t u = 0; u < kAhead; ++u) ahead[u] = accumulator(i + (kAhead + u) * kGroups);
+        }
     }
     sums[tid] = o;
     __syncthreads();
@@ -974,7 +1014,11 @@ int launch(const SharedParams& p, hipStream_t s) {
         hipLaunchKernelGGL((shared_attention_kernel<E, kD, false>), dim3(kWorkgroups), dim3(kThreads), 0, s, p);
     const int status = launch_status("shared_attention_kernel");
     if (status != KVFLUX_OK) return status;
-    hipLaunchKernelGGL((shared_merge_kernel<kD>), dim3(p.rows * p.query_heads), dim3(kMergeThreads), 0, s, p);
+    const unsigned merges = p.rows * p.query_heads;
+    if (merges > kManyMerges)
+        hipLaunchKernelGGL((shared_merge_kernel<kD, 64>), dim3(merges), dim3(64), 0, s, p);
+    else
+        hipLaunchKernelGGL((shared_merge_kernel<kD, 256>), dim3(merges), dim3(256), 0, s, p);
     return launch_status("shared_merge_kernel");
 }
 
