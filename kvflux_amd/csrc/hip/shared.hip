@@ -147,6 +147,23 @@ __device__ inline Segment make_segment(std::uint32_t first_row, std::uint32_t co
     return s;
 }
 
+// Inclusive scans over a wavefront by lane moves within rows of 16 and their
+// broadcasts to the rows behind (six shuffles through LDS: 700 cycles more).
+template <int kCtrl, int kRows>
+__device__ inline std::uint32_t moved(std::uint32_t x) {  // 0 where no lane is moved from
+    return static_cast<std::uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(x), kCtrl, kRows, 0xf, false));
+}
+template <typename Op>
+__device__ inline std::uint32_t wave_scan(std::uint32_t x, Op op) {
+    x = op(x, moved<0x111, 0xf>(x));  // 1, 2, 4 and 8 lanes below, in a row
+    x = op(x, moved<0x112, 0xf>(x));
+    x = op(x, moved<0x114, 0xf>(x));
+    x = op(x, moved<0x118, 0xf>(x));
+    x = op(x, moved<0x142, 0xa>(x));  // lane 15 of a row into rows 1 and 3
+    x = op(x, moved<0x143, 0xc>(x));  // lane 31 into rows 2 and 3
+    return x;
+}
+
 // Group of a row: the last whose first row is not behind it (rows past the
 // last group's end, or before the first group's start: none).
 __device__ inline std::uint32_t group_of(const std::uint32_t* first, std::uint32_t groups, std::uint32_t row) {
@@ -209,7 +226,7 @@ __global__ __launch_bounds__(kThreads) void shared_attention_kernel(SharedParams
     __shared__ std::uint32_t begin_of[kMaxRows], end_of[kMaxRows];  // a row's own tokens
     __shared__ float2 part_ml[kWaves][kBlocks][16];
     __shared__ std::uint32_t bad_tile[2];               // the serial number of a tile with a missing page
-    __shared__ std::uint32_t found;
+    __shared__ std::uint32_t found[2];                  // the segment this share starts in, the cost before it
 
     const int tid = threadIdx.x, lane = tid % 64;
     const auto uniform = [](std::uint32_t x) {
@@ -239,18 +256,14 @@ __global__ __launch_bounds__(kThreads) void shared_attention_kernel(SharedParams
                 const std::uint64_t s = p.starts[g];
                 v = s < p.rows ? static_cast<std::uint32_t>(s) : p.rows;
             }
-#pragma unroll 1
-            for (int off = 1; off < 64; off <<= 1) {
-                const auto o = static_cast<std::uint32_t>(__shfl_up(static_cast<int>(v), off));
-                if (lane >= off && o > v) v = o;
-            }
+            v = wave_scan(v, [](std::uint32_t a, std::uint32_t b) { return a > b ? a : b; });
             v = v > carry ? v : carry;
             if (g <= p.groups) first_of[g] = v;
             carry = static_cast<std::uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(v), 63));
         }
     }
     if (tid < 2) bad_tile[tid] = 0;
-    if (tid == 0) found = ~0u;
+    if (tid == 0) found[0] = ~0u;
     __syncthreads();
     // Tokens that the rows of a group share: none with fewer than two rows. A
     // row shorter than that takes no part in it.
@@ -280,12 +293,7 @@ __global__ __launch_bounds__(kThreads) void shared_attention_kernel(SharedParams
         cost_of[s] = cost;
         mine += cost;
     }
-    std::uint32_t upto = mine;
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
-        const auto add = static_cast<std::uint32_t>(__shfl_up(static_cast<int>(upto), off));
-        if (lane >= off) upto += add;
-    }
+    const std::uint32_t upto = wave_scan(mine, [](std::uint32_t a, std::uint32_t b) { return a + b; });
     if (lane == 63) wave_cost[wave] = upto;
     __syncthreads();
     std::uint32_t before = upto - mine, total = 0;
@@ -303,7 +311,10 @@ __global__ __launch_bounds__(kThreads) void shared_attention_kernel(SharedParams
     for (std::uint32_t s = tid * per; s < (tid + 1) * per && s < segments; ++s) {
         const std::uint32_t cost = cost_of[s];
         cost_of[s] = before;
-        if (before <= share && share < before + cost) found = s;  // one segment at most
+        if (before <= share && share < before + cost) {  // one segment at most
+            found[0] = s;
+            found[1] = before;
+        }
         before += cost;
     }
     __syncthreads();
@@ -337,10 +348,10 @@ __global__ __launch_bounds__(kThreads) void shared_attention_kernel(SharedParams
                        uniform(x.tiles), uniform(x.weight)};
     };
     Cursor ahead;  // the tile whose page ids are fetched next
-    ahead.seg = uniform(found);
+    ahead.seg = uniform(found[0]);
     if (share >= share_end || ahead.seg == ~0u) return;  // uniform: an empty share
     ahead.s = uniform_segment(ahead.seg);                 // has tiles: its cost is above 0
-    ahead.cost = uniform(cost_of[ahead.seg]);
+    ahead.cost = uniform(found[1]);
     {
         const std::uint32_t stream = (share - ahead.cost) / ahead.s.stream_cost();
         ahead.cost += stream * ahead.s.stream_cost();
@@ -507,20 +518,25 @@ __global__ __launch_bounds__(kThreads) void shared_attention_kernel(SharedParams
                 const std::uint32_t row_in = p.group.div(c);
                 const float* q = p.query + (static_cast<std::uint64_t>(part.first_row + row_in) * p.query_heads +
                                             next.kvh * p.group.divisor + (c - row_in * p.group.divisor)) * kD;
+                // All loads first: one round trip, and not one for each few.
+                float4 raw[kD / 16];
+#pragma unroll
+                for (int m = 0; m < kD / 16; ++m)
+                    raw[m] = *reinterpret_cast<const float4*>(
+                        q + (kF32 ? 16 * m + 4 * quad : 32 * (m / 2) + 8 * quad + 4 * (m % 2)));
+                __builtin_amdgcn_sched_barrier(0);
                 if constexpr (kF32) {
 #pragma unroll
                     for (int m = 0; m < kD / 16; ++m) {
-                        const float4 x = *reinterpret_cast<const float4*>(q + 16 * m + 4 * quad);
-                        qf[4 * m] = x.x * p.scale_log2;
-                        qf[4 * m + 1] = x.y * p.scale_log2;
-                        qf[4 * m + 2] = x.z * p.scale_log2;
-                        qf[4 * m + 3] = x.w * p.scale_log2;
+                        qf[4 * m] = raw[m].x * p.scale_log2;
+                        qf[4 * m + 1] = raw[m].y * p.scale_log2;
+                        qf[4 * m + 2] = raw[m].z * p.scale_log2;
+                        qf[4 * m + 3] = raw[m].w * p.scale_log2;
                     }
                 } else {
 #pragma unroll
                     for (int kk = 0; kk < kKk; ++kk) {
-                        const float4 lo = *reinterpret_cast<const float4*>(q + 32 * kk + 8 * quad);
-                        const float4 hi = *reinterpret_cast<const float4*>(q + 32 * kk + 8 * quad + 4);
+                        const float4 lo = raw[2 * kk], hi = raw[2 * kk + 1];
                         const float v[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
                         std::uint32_t parts[3][4];
 #pragma unroll
