@@ -514,6 +514,7 @@ __global__ __launch_bounds__(kThreads) void shared_attention_kernel(SharedParams
             table_row = p.table + static_cast<std::uint64_t>(part.first_row) * p.width;
 #pragma unroll
             for (int n = 0; n < kBlocks; ++n) {
+                if (!active || n >= static_cast<int>(blocks)) break;
                 const std::uint32_t mine = first_col + 16 * n + col, c = col0 + (mine < cols ? mine : 0);
                 const std::uint32_t row_in = p.group.div(c);
                 const float* q = p.query + (static_cast<std::uint64_t>(part.first_row + row_in) * p.query_heads +
@@ -644,17 +645,28 @@ __global__ __launch_bounds__(kThreads) void shared_attention_kernel(SharedParams
                     __builtin_amdgcn_sched_group_barrier(0x100, 2 * kDt, 0);       // the V reads
                 }
                 set_priority<0>();
-                if (bad || end - token0 < kStep) {
+                if (bad) {  // uniform: some page of the tile is missing
+#pragma unroll
+                    for (int b = 0; b < kSubs; ++b)
+#pragma unroll 1
+                        for (int r = 0; r < 4; ++r) {
+                            const std::uint32_t token = token0 + 16 * b + 4 * quad + r;
+                            const bool live = token >= end || table_row[p.block_size.div(token)] < p.num_blocks;
+#pragma unroll
+                            for (int n = 0; n < kN; ++n) {
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) s[n][b][e] = live || e != r ? s[n][b][e] : -INFINITY;
+                            }
+                        }
+                }
+                if (end - token0 < kStep) {  // uniform: the last tokens
+                    const std::int32_t left = static_cast<std::int32_t>(end - token0) - 4 * quad;
 #pragma unroll
                     for (int b = 0; b < kSubs; ++b)
 #pragma unroll
-                        for (int r = 0; r < 4; ++r) {
-                            const std::uint32_t token = token0 + 16 * b + 4 * quad + r;
-                            bool live = token < end;
-                            if (bad && live) live = table_row[p.block_size.div(token)] < p.num_blocks;
+                        for (int r = 0; r < 4; ++r)
 #pragma unroll
-                            for (int n = 0; n < kN; ++n) s[n][b][r] = live ? s[n][b][r] : -INFINITY;
-                        }
+                            for (int n = 0; n < kN; ++n) s[n][b][r] = 16 * b + r < left ? s[n][b][r] : -INFINITY;
                 }
                 float top[kN];
                 bool moves = false;
