@@ -242,10 +242,11 @@ int kvflux_paged_attention_noalloc(const void* key_cache, const void* value_cach
  * row's bits may differ between batches and from kvflux_paged_attention's.
  * 16-bit caches at head_size 64, 128 and 256 and FP32 caches at 64 and 128, pages
  * of any size, up to 2048 rows and 512 groups; K, V and the workspace aligned to 16
- * bytes there. Other calls, and num_groups = 0, run as kvflux_paged_attention
- * does.
- * workspace: kvflux_paged_attention_shared_workspace_size bytes, which for
- * the shared kernel depend on neither kv_len nor the prefixes (no
+ * bytes. Other shapes, and calls whose bounds say that sharing cannot pay (few
+ * rows more than groups, short prefixes), run as kvflux_paged_attention does,
+ * bit for bit: max_prefix and kv_len decide that, so bounds that are far too
+ * large choose the shared kernel where it does not pay.
+ * workspace: kvflux_paged_attention_shared_workspace_size bytes (no
  * initialisation needed; calls that share one must be ordered). */
 int kvflux_paged_attention_shared_workspace_size(uint64_t num_rows, uint64_t kv_len, uint64_t num_kv_heads,
                                                  uint64_t query_heads, uint64_t block_size, uint64_t head_size,

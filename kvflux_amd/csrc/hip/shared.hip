@@ -1004,9 +1004,9 @@ struct Layout {
     std::uint64_t prefix_acc = 0, prefix_ml = 0, row_acc = 0, row_ml = 0, bytes = 0;
 };
 
-// Whether the shared kernel takes the call; if not it runs as an ordinary
+// Whether the shared kernel can take a call's shape; others run as an ordinary
 // decode batch (the same results: a shared page is only read more often).
-bool takes(std::uint64_t rows, std::uint64_t kv_len, std::uint64_t kv_heads, std::uint64_t query_heads,
+bool can_take(std::uint64_t rows, std::uint64_t kv_len, std::uint64_t kv_heads, std::uint64_t query_heads,
            std::uint64_t block_size, std::uint64_t head_size, int dtype, std::uint64_t groups) {
     if (groups == 0 || groups > kMaxGroups || rows > kMaxRows) return false;
     if (head_size != 64 && head_size != 128 && (head_size != 256 || dtype == KVFLUX_DTYPE_F32)) return false;
@@ -1016,6 +1016,23 @@ bool takes(std::uint64_t rows, std::uint64_t kv_len, std::uint64_t kv_heads, std
     const std::uint64_t group = query_heads / kv_heads;
     const std::uint64_t streams = kv_heads * (rows * ((group + kCols - 1) / kCols) + groups + rows * group / kCols);
     return streams * (kv_len / 64 + 1) < (1ULL << 31) / (kMostTileCost + kPartCost);
+}
+
+// Whether sharing pays, as far as the host can know. An ordinary decode reads a
+// prefix again for every further row of its group, from L2, at about 9 MB a
+// microsecond; the shared kernel pays its plan and merge, about 5 us, and for every row
+// and kv head a part of its own, of which a round of the workgroups takes about
+// 4.5 us more than the ordinary decode's items. Measured, shared and ordinary:
+// 17 rows in 2 groups behind 1500-2500 tokens, 28/4 heads of 128 (77 MB read again) 23.8
+// and 25.3 us; 27 in 2 behind up to 7061, 32/8 (723 MB) 25.1 and 35.9; 34 in 4 behind
+// 347, 24/8 (43 MB) 21.7 and 15.0; 116 in 11 behind 423, 24/8 (182 MB) 34.8 and 30.7; 60
+// in 3 behind 221, 40/8 heads of 64 (26 MB) 28.9 and 9.8.
+bool pays(std::uint64_t rows, std::uint64_t groups, std::uint64_t prefix, std::uint64_t kv_heads,
+          std::uint64_t head_size, int dtype) {
+    if (rows <= groups) return false;
+    const double again = static_cast<double>(rows - groups) * static_cast<double>(prefix) *
+                         static_cast<double>(2 * kv_heads * head_size * dtype_bytes(dtype));
+    return again > 9e6 * (5.0 + 4.5 * static_cast<double>(rows * kv_heads) / kWorkgroups);
 }
 
 Layout layout_of(std::uint64_t rows, std::uint64_t kv_heads, std::uint64_t query_heads, std::uint64_t head_size,
@@ -1078,12 +1095,14 @@ extern "C" int kvflux_paged_attention_shared_workspace_size(uint64_t num_rows, u
                                                             size_t* bytes) {
     if (!bytes) return fail(KVFLUX_ERR_INVALID_ARGUMENT, "bytes is null");
     *bytes = 0;
-    const int status = check_shape(num_kv_heads, block_size, head_size, dtype, query_heads);
+    int status = check_shape(num_kv_heads, block_size, head_size, dtype, query_heads);
     if (status != KVFLUX_OK) return status;
-    if (!takes(num_rows, kv_len, num_kv_heads, query_heads, block_size, head_size, dtype, num_groups))
-        return kvflux_paged_attention_workspace_size(num_rows, kv_len, num_kv_heads, query_heads, block_size, head_size,
-                                                     bytes);
-    *bytes = layout_of(num_rows, num_kv_heads, query_heads, head_size, num_groups).bytes;
+    status = kvflux_paged_attention_workspace_size(num_rows, kv_len, num_kv_heads, query_heads, block_size, head_size, bytes);
+    if (status != KVFLUX_OK) return status;
+    if (can_take(num_rows, kv_len, num_kv_heads, query_heads, block_size, head_size, dtype, num_groups)) {
+        const std::uint64_t need = layout_of(num_rows, num_kv_heads, query_heads, head_size, num_groups).bytes;
+        if (need > *bytes) *bytes = need;
+    }
     return KVFLUX_OK;
 }
 
@@ -1103,7 +1122,8 @@ extern "C" int kvflux_paged_attention_shared(const void* key_cache, const void* 
         return fail(KVFLUX_ERR_INVALID_ARGUMENT, "shared attention: null pointer");
     if (num_blocks == 0 || max_blocks_per_seq == 0)
         return fail(KVFLUX_ERR_INVALID_ARGUMENT, "shared attention: invalid shape");
-    if (!takes(num_rows, kv_len, num_kv_heads, query_heads, block_size, head_size, dtype, num_groups))
+    if (!can_take(num_rows, kv_len, num_kv_heads, query_heads, block_size, head_size, dtype, num_groups) ||
+        !pays(num_rows, num_groups, max_prefix < kv_len ? max_prefix : kv_len, num_kv_heads, head_size, dtype))
         return kvflux_paged_attention(key_cache, value_cache, num_blocks, num_kv_heads, block_size, head_size, dtype,
                                       block_table, max_blocks_per_seq, seq_lens, kv_len, num_rows, query_heads, query,
                                       output, workspace, workspace_bytes, stream);

@@ -19,6 +19,9 @@ from kvflux_amd import capi, device
 CODE = {"f16": capi.DTYPE_F16, "bf16": capi.DTYPE_BF16, "f32": capi.DTYPE_F32}
 TOL = 1e-5
 NONE = 2 ** 64 - 1
+# Small batches run as an ordinary decode by their bounds; these bounds, as large
+# as a caller may give, choose the shared kernel.
+BOUND = 1 << 18
 
 
 def to_bits(x, name):
@@ -105,11 +108,12 @@ class Batch:
                 out[r, h * G:(h + 1) * G] = (w @ vv) / w.sum(-1, keepdims=True)
         return out
 
-    def upload(self):
+    def upload(self, bound=BOUND):
         self.dev = {n: device.to_device(getattr(self, n)) for n in ("k", "v", "table", "lens", "starts", "prefixes", "q")}
         self.out = device.to_device(np.full(self.q.shape, 999.0, np.float32))
         size = C.c_size_t()
-        self.max_len = int(self.lens.max()) if len(self.lens) else 0
+        self.max_len = bound or int(self.lens.max())
+        self.max_prefix = bound or int(self.prefixes.max())
         capi.call("kvflux_paged_attention_shared_workspace_size", len(self.lens), self.max_len, self.H, self.Hq, self.bs,
                   self.D, CODE[self.dtype], self.groups, C.byref(size))
         self.ws = device.DeviceBuffer(size.value)
@@ -120,7 +124,7 @@ class Batch:
         d = self.dev
         return (d["k"].ptr, d["v"].ptr, self.pages, self.H, self.bs, self.D, CODE[self.dtype], d["table"].ptr,
                 self.table.shape[1], d["lens"].ptr, self.max_len, len(self.lens), self.Hq, d["starts"].ptr,
-                d["prefixes"].ptr, self.groups, int(self.prefixes.max()), d["q"].ptr, self.out.ptr, self.ws.ptr,
+                d["prefixes"].ptr, self.groups, self.max_prefix, d["q"].ptr, self.out.ptr, self.ws.ptr,
                 self.ws.nbytes, stream)
 
     def run(self, stream=0):
@@ -128,8 +132,8 @@ class Batch:
         device.synchronize(stream)
         return self.out.download(np.float32).reshape(self.q.shape)
 
-    def check(self, tol=TOL):
-        got, want = self.upload().run(), self.expected()
+    def check(self, tol=TOL, bound=BOUND):
+        got, want = self.upload(bound).run(), self.expected()
         assert np.isfinite(got).all()
         assert np.abs(got - want).max() <= tol, np.abs(got - want).max()
         return got
@@ -337,15 +341,34 @@ def test_near_the_ordinary_decode(gpu):
     """The result is that of kvflux_paged_attention on the same batch."""
     rng = np.random.default_rng(20)
     b = Batch(rng, [(1000, [100, 3, 5, 800]), (64, [10, 70])], before=[300], heads=(32, 8)).upload()
-    shared = b.run()
+    shared, plain = b.run(), ordinary(b)
+    assert np.abs(plain - shared).max() <= TOL
+
+
+def ordinary(b):
+    """kvflux_paged_attention's output for the batch."""
     size = C.c_size_t()
     capi.call("kvflux_paged_attention_workspace_size", len(b.lens), b.max_len, b.H, b.Hq, b.bs, b.D, C.byref(size))
     ws = device.DeviceBuffer(size.value)
     a = b.args()
+    b.out.fill(0xff)
     capi.call("kvflux_paged_attention", *a[:13], a[17], a[18], ws.ptr, size.value, None)
     device.synchronize()
-    plain = b.out.download(np.float32).reshape(b.q.shape)
-    assert np.abs(plain - shared).max() <= TOL
+    return b.out.download(np.float32).reshape(b.q.shape)
+
+
+@pytest.mark.gpu
+def test_calls_that_sharing_cannot_pay_for(gpu):
+    """Short prefixes and batches without sharers run as the ordinary decode, bit for bit; long prefixes do not."""
+    rng = np.random.default_rng(25)
+    for groups in ([(96, [3, 40, 7])], [(700, [5]), (40, [9]), (900, [1])]):
+        b = Batch(rng, groups)
+        got = b.check(bound=None)
+        assert np.array_equal(got, ordinary(b))
+    b = Batch(rng, [(6000, [5, 9, 40, 2, 3, 8, 1, 1, 7, 200])], heads=(8, 4))
+    got = b.check(bound=None)
+    plain = ordinary(b)
+    assert not np.array_equal(got, plain) and np.abs(got - plain).max() <= TOL
 
 
 @pytest.mark.gpu
@@ -372,12 +395,7 @@ def test_odd_group_arrays_stay_in_bounds(gpu):
     for starts, prefixes in (([5, 2, 9, 1], [64, 64, 64]), ([1, 1, 1, 1], [64, 64, 64]),
                              ([7, 100, 2 ** 63, NONE], [64, 64, 64]), ([1, 3, 5, 7], [NONE, 2 ** 40, 100000])):
         b.starts, b.prefixes = np.array(starts, np.uint64), np.array(prefixes, np.uint64)
-        b.upload()
-        d = list(b.args())
-        d[16] = b.max_len
-        capi.call("kvflux_paged_attention_shared", *d)
-        device.synchronize()
-        got = b.out.download(np.float32).reshape(b.q.shape)
+        got = b.upload().run()
         assert np.isfinite(got).all()
         assert np.abs(got[0] - want[0]).max() <= TOL
         if prefixes[0] == NONE:  # every row is shorter: all on their own
@@ -394,8 +412,8 @@ def test_on_another_stream(gpu):
 
 def test_refusals():
     """Checked on the host before anything is launched (no GPU needed)."""
-    ok = dict(k=4096, v=4096, blocks=8, H=2, bs=16, D=128, dtype=1, table=4096, width=4, lens=4096, kv=64, rows=3, Hq=4,
-              starts=4096, prefixes=4096, groups=1, most=32, q=4096, out=4096, ws=4096, size=1 << 40)
+    ok = dict(k=4096, v=4096, blocks=8, H=2, bs=16, D=128, dtype=1, table=4096, width=4, lens=4096, kv=BOUND, rows=3, Hq=4,
+              starts=4096, prefixes=4096, groups=1, most=BOUND, q=4096, out=4096, ws=4096, size=1 << 40)
 
     def status(**change):
         return capi.lib().kvflux_paged_attention_shared(*({**ok, **change}[x] for x in ok), None)
@@ -413,13 +431,15 @@ def test_refusals():
     assert fn(3, 64, 2, 5, 16, 128, 1, 1, C.byref(size)) == capi.ERR_INVALID and size.value == 0
     assert fn(3, 64, 2, 4, 16, 128, 9, 1, C.byref(size)) == capi.ERR_INVALID
     assert fn(3, 64, 2, 4, 16, 128, 1, 1, C.byref(size)) == capi.OK and size.value > 0
-    need = size.value
-    assert status(size=need - 1) == capi.ERR_INVALID
-    for kv in (1, 1 << 30):  # lengths do not matter
-        assert fn(3, kv, 2, 4, 16, 128, 1, 1, C.byref(size)) == capi.OK and size.value == need
+    assert fn(3, BOUND, 2, 4, 16, 128, 1, 1, C.byref(size)) == capi.OK
+    assert status(size=100000) == capi.ERR_INVALID  # less than the shared kernel takes
     ordinary = C.c_size_t()
     capi.call("kvflux_paged_attention_workspace_size", 3, 9000, 2, 4, 16, 128, C.byref(ordinary))
     assert fn(3, 9000, 2, 4, 16, 128, 1, 0, C.byref(size)) == capi.OK and size.value == ordinary.value
     assert fn(5000, 9000, 2, 4, 16, 128, 1, 4, C.byref(size)) == capi.OK
     capi.call("kvflux_paged_attention_workspace_size", 5000, 9000, 2, 4, 16, 128, C.byref(ordinary))
     assert size.value == ordinary.value
+    # Where either kernel may take the call the workspace serves both.
+    for kv in (64, 100000):
+        capi.call("kvflux_paged_attention_workspace_size", 64, kv, 8, 32, 16, 128, C.byref(ordinary))
+        assert fn(64, kv, 8, 32, 16, 128, 1, 3, C.byref(size)) == capi.OK and size.value >= max(1, ordinary.value)
