@@ -51,6 +51,16 @@ public:
     // Library-internal: enqueues the refresh on the default stream without
     // waiting (the caller synchronises before the next refresh).
     void enqueue_refresh();
+    // Library-internal: the rows' shared prefixes (shared_prefix.h) as device
+    // arrays uint64 [groups + 1] and [groups], found and uploaded at the first
+    // call after the whole table was; most: the longest prefix.
+    struct Groups {
+        const std::uint64_t* starts = nullptr;
+        const std::uint64_t* prefixes = nullptr;
+        std::size_t count = 0;
+        std::uint64_t most = 0;
+    };
+    const Groups& enqueue_groups();
 
 private:
     struct Device;
@@ -63,6 +73,8 @@ private:
     std::vector<std::uint64_t> lengths_;  // host copy of the device lengths
     std::vector<std::uint64_t> blocks_;   // pages per row at the last refresh
     bool stale_ = true;                   // device copy must be uploaded whole
+    bool grouped_ = false;                // groups_ holds for the rows
+    Groups groups_;
     std::unique_ptr<Device> device_;
 };
 

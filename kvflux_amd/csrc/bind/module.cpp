@@ -11,12 +11,14 @@
 #include "kvflux/v2/batch_block_table.h"
 #include "kvflux/v2/copy_on_write.h"
 #include "kvflux/v2/device_batch_table.h"
+#include "kvflux/v2/norm_rope_write.h"
 #include "kvflux/v2/prefix_cache.h"
 #include "kvflux/v2/sequence_lifecycle.h"
 #include "kvflux/v2/paged_attention.h"
 #include "kvflux/v2/paged_kv_read.h"
 #include "kvflux/v2/paged_kv_write.h"
 #include "kvflux/v2/reference_attention.h"
+#include "kvflux/v2/shared_prefix.h"
 #include "kvflux/v3/cache_directory.h"
 #include "kvflux/v3/gpu_chunk_store.h"
 #include "kvflux/v3/gpu_cpu_transfer.h"
@@ -393,6 +395,51 @@ PYBIND11_MODULE(_kvflux, m) {
         py::gil_scoped_release release;
         return decode_step(s, t, ptr(k), ptr(v), static_cast<const float*>(ptr(q)),
                            static_cast<float*>(ptr(o)), query_heads);
+    });
+
+    py::class_<ProjectedRows>(m, "ProjectedRows")
+        .def(py::init([](std::uintptr_t q, std::uintptr_t k, std::uintptr_t v, DType dtype, std::size_t qs,
+                         std::size_t ks, std::size_t vs) {
+                 return ProjectedRows{ptr(q), ptr(k), ptr(v), dtype, qs, ks, vs};
+             }),
+             py::arg("query"), py::arg("key"), py::arg("value"), py::arg("dtype"), py::arg("query_stride") = 0,
+             py::arg("key_stride") = 0, py::arg("value_stride") = 0);
+    py::class_<NormRope>(m, "NormRope")
+        .def(py::init([](std::uintptr_t qn, std::uintptr_t kn, float eps, std::uintptr_t inv_freq,
+                         std::size_t rotary_dim, bool interleaved) {
+                 return NormRope{static_cast<const float*>(ptr(qn)), static_cast<const float*>(ptr(kn)), eps,
+                                 static_cast<const double*>(ptr(inv_freq)), rotary_dim, interleaved};
+             }),
+             py::arg("query_norm") = 0, py::arg("key_norm") = 0, py::arg("eps") = 1e-6f, py::arg("inv_freq") = 0,
+             py::arg("rotary_dim") = 0, py::arg("interleaved") = false);
+    m.def("norm_rope_write", [](PagedKVStorage& s, const ProjectedRows& rows, const NormRope& form,
+                                std::size_t query_heads, const std::vector<std::uint64_t>& positions,
+                                const SlotMapping& slots, std::uintptr_t query_out) {
+        py::gil_scoped_release release;
+        norm_rope_write(s, rows, form, query_heads, positions, slots, static_cast<float*>(ptr(query_out)));
+    });
+    m.def("find_shared_prefixes", [](const std::vector<const SequenceState*>& seqs) {
+        const auto found = find_shared_prefixes(seqs);
+        return std::make_pair(found.starts, found.prefixes);
+    });
+    m.def("paged_attention_batch_shared", [](const PagedKVStorage& s, const std::vector<const SequenceState*>& seqs,
+                                             std::uintptr_t q, std::uintptr_t o, std::size_t query_heads) {
+        py::gil_scoped_release release;
+        paged_attention_batch_shared(s, seqs, static_cast<const float*>(ptr(q)), static_cast<float*>(ptr(o)),
+                                     query_heads);
+    });
+    m.def("paged_attention_batch_shared", [](const PagedKVStorage& s, DeviceBatchTable& t, std::uintptr_t q,
+                                             std::uintptr_t o, std::size_t query_heads) {
+        py::gil_scoped_release release;
+        paged_attention_batch_shared(s, t, static_cast<const float*>(ptr(q)), static_cast<float*>(ptr(o)),
+                                     query_heads);
+    });
+    m.def("decode_step_projected", [](PagedKVStorage& s, DeviceBatchTable& t, const ProjectedRows& rows,
+                                      const NormRope& form, std::uintptr_t q, std::uintptr_t o,
+                                      std::size_t query_heads) {
+        py::gil_scoped_release release;
+        return decode_step_projected(s, t, rows, form, static_cast<float*>(ptr(q)), static_cast<float*>(ptr(o)),
+                                     query_heads);
     });
 
     py::class_<SequenceLifecycle>(m, "SequenceLifecycle")

@@ -6,8 +6,10 @@
 // (src/v2/sequence_lifecycle.cpp:53-69), for a whole batch at once.
 #include "kvflux/v2/copy_on_write.h"
 #include "kvflux/v2/device_batch_table.h"
+#include "kvflux/v2/shared_prefix.h"
 
 #include "device_runtime.h"
+#include "row_checks.h"
 
 #include <algorithm>
 #include <limits>
@@ -157,8 +159,8 @@ std::vector<TokenLocation> append_tokens_cow(const PagedKVStorage& storage,
 // ---------------------------------------------------------------- DeviceBatchTable
 
 struct DeviceBatchTable::Device {
-    detail::DeviceBuffer table, lengths, updates;
-    detail::PinnedBuffer staging;
+    detail::DeviceBuffer table, lengths, updates, groups;
+    detail::PinnedBuffer staging, groups_staging;
 };
 
 namespace {
@@ -205,6 +207,7 @@ const std::uint64_t* DeviceBatchTable::device_lengths() const noexcept {
 }
 
 void DeviceBatchTable::upload_all() {
+    grouped_ = false;
     for (std::size_t r = 0; r < sequences_.size(); ++r) {
         const SequenceState& s = *sequences_[r];
         const std::size_t n = s.num_allocated_blocks();
@@ -284,6 +287,29 @@ void DeviceBatchTable::enqueue_refresh() {
     }
 }
 
+const DeviceBatchTable::Groups& DeviceBatchTable::enqueue_groups() {
+    if (grouped_) return groups_;
+    std::vector<detail::RowPages> rows;
+    for (std::size_t r = 0; r < sequences_.size(); ++r)
+        rows.push_back({shadow_.data() + r * capacity_, lengths_[r] / storage_.layout().block_size()});
+    const auto found = detail::group_rows(rows, storage_.layout().block_size());
+    groups_ = Groups{};
+    if (found.groups() != 0) {
+        const std::size_t starts_bytes = found.starts.size() * 8, bytes = starts_bytes + found.prefixes.size() * 8;
+        auto* host = static_cast<unsigned char*>(device_->groups_staging.reserve(bytes));
+        std::memcpy(host, found.starts.data(), starts_bytes);
+        std::memcpy(host + starts_bytes, found.prefixes.data(), bytes - starts_bytes);
+        auto* dev = static_cast<unsigned char*>(device_->groups.reserve(bytes));
+        check(kvflux_memcpy_async(dev, host, bytes, nullptr), "upload batch groups");
+        groups_.starts = reinterpret_cast<const std::uint64_t*>(dev);
+        groups_.prefixes = reinterpret_cast<const std::uint64_t*>(dev + starts_bytes);
+        groups_.count = found.groups();
+        groups_.most = *std::max_element(found.prefixes.begin(), found.prefixes.end());
+    }
+    grouped_ = true;
+    return groups_;
+}
+
 void DeviceBatchTable::refresh() {
     detail::DeviceGuard guard(storage_.device());
     try {
@@ -348,20 +374,15 @@ void paged_attention_batch(const PagedKVStorage& storage, const DeviceBatchTable
     check(kvflux_stream_synchronize(nullptr), "paged attention batch synchronize");
 }
 
-std::vector<TokenLocation> decode_step(PagedKVStorage& storage, DeviceBatchTable& batch,
-                                       const void* key_new_device, const void* value_new_device,
-                                       const float* query_device, float* output_device,
-                                       std::size_t query_heads) {
+namespace {
+
+// What decode_step and decode_step_projected have in common: the appends with
+// their copies, the refresh, and `enqueue`, which launches the write and the
+// attention.
+template <typename Enqueue>
+std::vector<TokenLocation> append_and_run(PagedKVStorage& storage, DeviceBatchTable& batch, const Enqueue& enqueue) {
     const auto& layout = storage.layout();
     const auto& sequences = batch.sequences();
-    detail::DeviceGuard guard(storage.device());
-    validate_batch_attention(storage, batch, query_device, output_device, query_heads);
-    if (sequences.empty()) return {};
-    if (!key_new_device || !value_new_device) {
-        throw std::invalid_argument("K_new and V_new device pointers are required");
-    }
-    detail::require_device_pointer(key_new_device, storage.device(), "K_new");
-    detail::require_device_pointer(value_new_device, storage.device(), "V_new");
     for (const auto* s : sequences) {
         if (s->num_tokens() % layout.block_size() == 0 &&
             s->num_allocated_blocks() + 1 > batch.capacity_blocks()) {
@@ -379,6 +400,52 @@ std::vector<TokenLocation> decode_step(PagedKVStorage& storage, DeviceBatchTable
     commit(sequences, plan);
     try {
         batch.enqueue_refresh();
+        enqueue();
+        check(kvflux_stream_synchronize(nullptr), "decode step synchronize");
+    } catch (...) {
+        (void)kvflux_stream_synchronize(nullptr);
+        throw;
+    }
+    return plan.locations;
+}
+
+// The attention's launch with the rows' shared prefixes computed once.
+void enqueue_shared_attention(const PagedKVStorage& storage, DeviceBatchTable& batch, const float* query,
+                              float* output, std::size_t query_heads) {
+    const auto& layout = storage.layout();
+    const auto& lengths = batch.lengths();
+    if (std::find(lengths.begin(), lengths.end(), 0) != lengths.end()) {
+        throw std::invalid_argument("invalid batch attention sequence");
+    }
+    const std::size_t max_len = *std::max_element(lengths.begin(), lengths.end());
+    const auto& groups = batch.enqueue_groups();
+    std::size_t ws_bytes = 0;
+    void* ws = detail::shared_attention_workspace(storage, batch.rows(), max_len, query_heads, groups.count, &ws_bytes);
+    check(kvflux_paged_attention_shared(storage.key_base(), storage.value_base(), layout.num_blocks(),
+                                        layout.num_kv_heads(), layout.block_size(), layout.head_size(),
+                                        detail::abi_dtype(layout.dtype()), batch.device_table(),
+                                        batch.capacity_blocks(), batch.device_lengths(), max_len, batch.rows(),
+                                        query_heads, groups.starts, groups.prefixes, groups.count, groups.most, query,
+                                        output, ws, ws_bytes, nullptr),
+          "shared attention batch kernel launch");
+}
+
+}  // namespace
+
+std::vector<TokenLocation> decode_step(PagedKVStorage& storage, DeviceBatchTable& batch,
+                                       const void* key_new_device, const void* value_new_device,
+                                       const float* query_device, float* output_device,
+                                       std::size_t query_heads) {
+    const auto& layout = storage.layout();
+    detail::DeviceGuard guard(storage.device());
+    validate_batch_attention(storage, batch, query_device, output_device, query_heads);
+    if (batch.rows() == 0) return {};
+    if (!key_new_device || !value_new_device) {
+        throw std::invalid_argument("K_new and V_new device pointers are required");
+    }
+    detail::require_device_pointer(key_new_device, storage.device(), "K_new");
+    detail::require_device_pointer(value_new_device, storage.device(), "V_new");
+    return append_and_run(storage, batch, [&] {
         check(kvflux_write_paged_kv_tail(storage.key_base(), storage.value_base(), layout.num_blocks(),
                                          layout.num_kv_heads(), layout.block_size(),
                                          layout.head_size(), detail::abi_dtype(layout.dtype()),
@@ -387,12 +454,39 @@ std::vector<TokenLocation> decode_step(PagedKVStorage& storage, DeviceBatchTable
                                          batch.rows(), nullptr),
               "decode step KV write");
         enqueue_batch_attention(storage, batch, query_device, output_device, query_heads);
-        check(kvflux_stream_synchronize(nullptr), "decode step synchronize");
-    } catch (...) {
-        (void)kvflux_stream_synchronize(nullptr);
-        throw;
-    }
-    return plan.locations;
+    });
+}
+
+void paged_attention_batch_shared(const PagedKVStorage& storage, DeviceBatchTable& batch,
+                                  const float* query_device, float* output_device, std::size_t query_heads) {
+    detail::DeviceGuard guard(storage.device());
+    validate_batch_attention(storage, batch, query_device, output_device, query_heads);
+    if (batch.rows() == 0) return;
+    enqueue_shared_attention(storage, batch, query_device, output_device, query_heads);
+    check(kvflux_stream_synchronize(nullptr), "paged attention batch synchronize");
+}
+
+std::vector<TokenLocation> decode_step_projected(PagedKVStorage& storage, DeviceBatchTable& batch,
+                                                 const ProjectedRows& rows, const NormRope& form,
+                                                 float* query_device, float* output_device,
+                                                 std::size_t query_heads) {
+    const auto& layout = storage.layout();
+    detail::DeviceGuard guard(storage.device());
+    validate_batch_attention(storage, batch, query_device, output_device, query_heads);
+    if (batch.rows() == 0) return {};
+    const auto strides = detail::check_projection(storage, rows, form, query_heads, batch.rows(), query_device);
+    return append_and_run(storage, batch, [&] {
+        check(kvflux_norm_rope_write_tail(storage.key_base(), storage.value_base(), layout.num_blocks(),
+                                          layout.num_kv_heads(), layout.block_size(), layout.head_size(),
+                                          detail::abi_dtype(layout.dtype()), rows.query, rows.key, rows.value,
+                                          detail::abi_dtype(rows.dtype), strides.query, strides.key, strides.value,
+                                          query_heads, form.query_norm, form.key_norm, form.eps, form.inv_freq,
+                                          form.rotary_dim, form.interleaved, batch.device_table(),
+                                          batch.capacity_blocks(), batch.device_lengths(), batch.rows(), query_device,
+                                          nullptr),
+              "decode step norm, rotation and KV write");
+        enqueue_shared_attention(storage, batch, query_device, output_device, query_heads);
+    });
 }
 
 } // namespace kvflux::v2

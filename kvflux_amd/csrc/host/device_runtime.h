@@ -188,6 +188,17 @@ inline void* attention_workspace(const PagedKVStorage& storage, std::size_t rows
     return *bytes ? storage.scratch().workspace.reserve(*bytes) : nullptr;
 }
 
+// Workspace of a decode batch whose rows share prefixes.
+inline void* shared_attention_workspace(const PagedKVStorage& storage, std::size_t rows, std::size_t kv_len,
+                                        std::size_t query_heads, std::size_t groups, std::size_t* bytes) {
+    const auto& layout = storage.layout();
+    check(kvflux_paged_attention_shared_workspace_size(rows, kv_len, layout.num_kv_heads(), query_heads,
+                                                       layout.block_size(), layout.head_size(),
+                                                       abi_dtype(layout.dtype()), groups, bytes),
+          "attention workspace size");
+    return *bytes ? storage.scratch().workspace.reserve(*bytes) : nullptr;
+}
+
 // Workspace of the split-key MFMA prefill (nullptr when the call does not split).
 inline void* prefill_workspace(const PagedKVStorage& storage, std::size_t query_tokens, std::size_t kv_len,
                                std::size_t query_heads, std::size_t* bytes) {

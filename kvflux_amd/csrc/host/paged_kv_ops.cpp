@@ -5,14 +5,18 @@
 //   read_paged_kv          reference src/v2/paged_kv_read.cu:106-155
 //   paged_attention        reference src/v2/paged_attention.cu:193-246
 //   paged_attention_batch  reference src/v2/paged_attention.cu:248-313
+//   norm_rope_write        no counterpart; checks as write_paged_kv
 #include "kvflux/v2/batch_block_table.h"
+#include "kvflux/v2/norm_rope_write.h"
 #include "kvflux/v2/paged_attention.h"
 #include "kvflux/v2/paged_kv_read.h"
 #include "kvflux/v2/paged_kv_write.h"
 
 #include "device_runtime.h"
+#include "row_checks.h"
 
 #include <algorithm>
+#include <cmath>
 #include <stdexcept>
 
 namespace kvflux::v2 {
@@ -83,6 +87,102 @@ void write_paged_kv(PagedKVStorage& storage, const void* key_new_device,
                                 dev[0], slot_mapping.size(), nullptr),
           "paged KV write kernel launch");
     finish("paged KV write synchronize");
+}
+
+namespace detail {
+
+ProjectionStrides check_projection(const PagedKVStorage& storage, const ProjectedRows& rows, const NormRope& form,
+                                   std::size_t query_heads, std::size_t tokens, const float* query_out) {
+    constexpr const char* too_large = "projected rows size overflow";
+    const auto& layout = storage.layout();
+    if (query_heads == 0 || query_heads % layout.num_kv_heads() != 0) {
+        throw std::invalid_argument("invalid query head count");
+    }
+    if (!rows.query || !rows.key || !rows.value || !query_out) {
+        throw std::invalid_argument("projected rows and query output device pointers are required");
+    }
+    if (form.rotary_dim % 2 != 0 || form.rotary_dim > layout.head_size() || (form.rotary_dim != 0 && !form.inv_freq)) {
+        throw std::invalid_argument("invalid rotation");
+    }
+    if (!(form.eps >= 0.0f) || std::isinf(form.eps)) throw std::invalid_argument("eps is negative or not finite");
+    // The kernel's limits, here so that a decode step refuses before it appends.
+    constexpr std::size_t most_rows = (std::size_t{1} << 26) - 1, most_dims = 512;
+    if (layout.head_size() > most_dims || layout.block_size() > 0x7fffffff || query_heads > most_rows ||
+        tokens > most_rows / (query_heads + 2 * layout.num_kv_heads())) {
+        throw std::runtime_error("projected rows are too large");
+    }
+    const std::size_t element = abi_dtype(rows.dtype) == KVFLUX_DTYPE_F32 ? 4 : 2;
+    const auto query_row = mul_checked(query_heads, layout.head_size(), too_large);
+    const auto kv_row = mul_checked(layout.num_kv_heads(), layout.head_size(), too_large);
+    const ProjectionStrides strides{rows.query_stride ? rows.query_stride : query_row,
+                                    rows.key_stride ? rows.key_stride : kv_row,
+                                    rows.value_stride ? rows.value_stride : kv_row};
+    if (strides.query < query_row || strides.key < kv_row || strides.value < kv_row) {
+        throw std::invalid_argument("a stride is shorter than a token's heads");
+    }
+    // Bytes from the first token's rows to the last one's end.
+    const auto extent = [&](std::size_t stride, std::size_t row) {
+        const auto before = mul_checked(tokens - 1, stride, too_large);
+        if (before > std::numeric_limits<std::size_t>::max() - row) throw std::overflow_error(too_large);
+        return mul_checked(before + row, element, too_large);
+    };
+    const auto out_bytes = mul_checked(mul_checked(tokens, query_row, too_large), sizeof(float), too_large);
+    const struct {
+        const void* data;
+        std::size_t bytes;
+        std::size_t alignment;
+        const char* name;
+    } inputs[] = {
+        {rows.query, extent(strides.query, query_row), element, "projected queries"},
+        {rows.key, extent(strides.key, kv_row), element, "projected keys"},
+        {rows.value, extent(strides.value, kv_row), element, "projected values"},
+        {form.query_norm, layout.head_size() * sizeof(float), sizeof(float), "query norm weights"},
+        {form.key_norm, layout.head_size() * sizeof(float), sizeof(float), "key norm weights"},
+        {form.inv_freq, form.rotary_dim / 2 * sizeof(double), sizeof(double), "rotation frequencies"}};
+    require_device_pointer(query_out, storage.device(), "query output");
+    if (reinterpret_cast<std::uintptr_t>(query_out) % sizeof(float) != 0) {
+        throw std::invalid_argument("misaligned query output");
+    }
+    if (overlaps(query_out, out_bytes, storage.key_base(), layout.total_bytes())) {
+        throw std::invalid_argument("query output must not overlap the KV cache");
+    }
+    for (const auto& in : inputs) {
+        if (!in.data) continue;
+        require_device_pointer(in.data, storage.device(), in.name);
+        if (reinterpret_cast<std::uintptr_t>(in.data) % in.alignment != 0) {
+            throw std::invalid_argument(std::string("misaligned ") + in.name);
+        }
+        if (overlaps(in.data, in.bytes, query_out, out_bytes) ||
+            overlaps(in.data, in.bytes, storage.key_base(), layout.total_bytes())) {
+            throw std::invalid_argument(std::string(in.name) + " must not overlap the query output or the KV cache");
+        }
+    }
+    return strides;
+}
+
+} // namespace detail
+
+void norm_rope_write(PagedKVStorage& storage, const ProjectedRows& rows, const NormRope& form,
+                     std::size_t query_heads, const std::vector<std::uint64_t>& positions,
+                     const SlotMapping& slot_mapping, float* query_out) {
+    if (positions.size() != slot_mapping.size()) {
+        throw std::invalid_argument("as many positions as slots are required");
+    }
+    if (slot_mapping.empty()) return;
+    const auto& layout = storage.layout();
+    validate_slots(layout, slot_mapping, storage.scratch().seen_slots);
+    const auto bytes = mul_checked(slot_mapping.size(), sizeof(PhysicalSlot), "projected rows size overflow");
+    detail::DeviceGuard guard(storage.device());
+    const auto strides = detail::check_projection(storage, rows, form, query_heads, slot_mapping.size(), query_out);
+    const auto dev = storage.scratch().upload({{positions.data(), bytes}, {slot_mapping.data(), bytes}});
+    check(kvflux_norm_rope_write(storage.key_base(), storage.value_base(), layout.num_blocks(),
+                                 layout.num_kv_heads(), layout.block_size(), layout.head_size(),
+                                 abi_dtype(layout.dtype()), rows.query, rows.key, rows.value, abi_dtype(rows.dtype),
+                                 strides.query, strides.key, strides.value, query_heads, form.query_norm,
+                                 form.key_norm, form.eps, form.inv_freq, form.rotary_dim, form.interleaved, dev[0],
+                                 dev[1], slot_mapping.size(), query_out, nullptr),
+          "norm, rotation and paged KV write kernel launch");
+    finish("norm, rotation and paged KV write synchronize");
 }
 
 namespace {
