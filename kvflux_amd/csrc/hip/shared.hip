@@ -1027,6 +1027,11 @@ bool can_take(std::uint64_t rows, std::uint64_t kv_len, std::uint64_t kv_heads, 
 // and 25.3 us; 27 in 2 behind up to 7061, 32/8 (723 MB) 25.1 and 35.9; 34 in 4 behind
 // 347, 24/8 (43 MB) 21.7 and 15.0; 116 in 11 behind 423, 24/8 (182 MB) 34.8 and 30.7; 60
 // in 3 behind 221, 40/8 heads of 64 (26 MB) 28.9 and 9.8.
+// The host knows no prefix but the longest, so groups of unequal sizes count for more
+// than they share. That costs little, an own part being read as fast either way: 2
+// rows behind 32768 tokens and 126 of U[1000, 32768], 32/8 heads of 128, 1470 and 1402
+// us; 2 behind 8192 and 126 of U[200, 6000] 302 and 309; 2 behind 8192 and 30 of U[50,
+// 300] 23.9 and 26.3.
 bool pays(std::uint64_t rows, std::uint64_t groups, std::uint64_t prefix, std::uint64_t kv_heads,
           std::uint64_t head_size, int dtype) {
     if (rows <= groups) return false;

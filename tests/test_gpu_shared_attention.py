@@ -403,6 +403,41 @@ def test_odd_group_arrays_stay_in_bounds(gpu):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_pages_past_32_bits(gpu, dtype):
+    """The batch's pages are the last of a cache of over 2^32 elements a tensor; whole pages and small ones."""
+    rng = np.random.default_rng(26)
+    for bs in (16, 8):
+        b = Batch(rng, [(200 // bs * bs, [30, 5, 70])], dtype, heads=(16, 8), bs=bs)
+        want, used, page = b.expected(), b.pages, b.k[0].nbytes
+        b.pages = (1 << 32) // b.k[0].size + used + 1
+        first = b.pages - used
+        b.table[b.table != NONE] += np.uint64(first)
+        k, v, b.k, b.v = b.k, b.v, b.k[:1], b.v[:1]
+        b.upload()
+        for name, part in (("k", k), ("v", v)):
+            b.dev[name] = device.DeviceBuffer(b.pages * page)
+            b.dev[name].upload(part, first * page)
+        assert np.abs(b.run() - want).max() <= TOL
+
+
+@pytest.mark.gpu
+def test_queries_and_outputs_at_any_float(gpu):
+    """Query and output arrays aligned to 4 bytes, and nothing written past the output."""
+    rng = np.random.default_rng(27)
+    for dtype, D in (("bf16", 128), ("f16", 64), ("f32", 64), ("bf16", 256)):
+        b = Batch(rng, [(300, [10, 20, 30])], dtype, D=D).upload()
+        q, out = device.DeviceBuffer(b.q.nbytes + 16), device.to_device(np.full(b.q.size + 2, 999.0, np.float32))
+        q.upload(b.q, 4)
+        a = list(b.args())
+        a[17], a[18] = q.ptr + 4, out.ptr + 4
+        capi.call("kvflux_paged_attention_shared", *a)
+        got = out.download(np.float32)
+        assert got[0] == 999.0 and got[-1] == 999.0
+        assert np.abs(got[1:-1].reshape(b.q.shape) - b.expected()).max() <= TOL
+
+
+@pytest.mark.gpu
 def test_on_another_stream(gpu):
     rng = np.random.default_rng(24)
     b = Batch(rng, [(300, [10, 20, 30])]).upload()
