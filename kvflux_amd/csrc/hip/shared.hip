@@ -21,8 +21,8 @@
 // 8 blocks of columns, fewer where there are fewer blocks, merged through LDS
 // at a part's end.
 //   S^T = K Q^T, O^T += V^T P^T  on v_mfma_f32_16x16x32 with Q (scale folded
-// in) and the weights as three 16-bit parts each: products exact in FP32, sums
-// FP32. FP32 caches: v_mfma_f32_16x16x4_f32 on the values as they are.
+// in) and the weights as three BF16 or two FP16 parts each: products as exact as
+// FP32's, sums FP32. FP32 caches: v_mfma_f32_16x16x4_f32 on the values as they are.
 #include "mfma_parts.h"
 
 #include <cmath>
@@ -217,6 +217,11 @@ __global__ __launch_bounds__(kThreads) void shared_attention_kernel(SharedParams
     constexpr int kBlocks = static_cast<int>(S::kMostBlocks);
     constexpr int kKk = kD / 32;   // 16-bit: K steps of S^T
     constexpr int kDt = kD / 16;   // accumulator tiles of O^T
+    // 16-bit parts of a query value and of a weight. Three BF16 parts hold an FP32
+    // value; two FP16 parts are off by at most 2^-23 of it, twice an FP32 rounding
+    // (and a third adds nothing below 2^-2, where the parts end at 2^-25): 48 rows
+    // behind 60000 tokens in FP16 263 -> 225 us, error against 64 bits unchanged.
+    constexpr int kParts = std::is_same<E, PfF16Exact>::value ? 2 : 3;
     constexpr float kWeightScale = kF32 ? 1.0f : M::kWeightScale;
     constexpr float kLazy = kF32 ? 8.0f : M::kLazyLog2;
 
@@ -491,7 +496,7 @@ __global__ __launch_bounds__(kThreads) void shared_attention_kernel(SharedParams
     std::uint32_t cols = 0, blocks = 1, shares = 1, across = 0, token_share = 0, first_col = 0;
     bool active = false;
     const std::uint64_t* table_row = p.table;
-    Vec qb[kBlocks][kF32 ? 1 : 3][kKk];
+    Vec qb[kBlocks][kF32 ? 1 : kParts][kKk];
     float qf[kF32 ? kD / 4 : 1];
     pf_f32x4_t acc[kBlocks][kDt];
     // Minus the column's reference (in all accumulator lanes: the seed of the
@@ -539,16 +544,16 @@ __global__ __launch_bounds__(kThreads) void shared_attention_kernel(SharedParams
                     for (int kk = 0; kk < kKk; ++kk) {
                         const float4 lo = raw[2 * kk], hi = raw[2 * kk + 1];
                         const float v[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
-                        std::uint32_t parts[3][4];
+                        std::uint32_t parts[kParts][4];
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
                             std::uint32_t x[3];
                             M::split3(v[2 * e] * p.scale_log2, v[2 * e + 1] * p.scale_log2, x);
 #pragma unroll
-                            for (int k = 0; k < 3; ++k) parts[k][e] = x[k];
+                            for (int k = 0; k < kParts; ++k) parts[k][e] = x[k];
                         }
 #pragma unroll
-                        for (int k = 0; k < 3; ++k)
+                        for (int k = 0; k < kParts; ++k)
                             qb[n][k][kk] =
                                 __builtin_bit_cast(Vec, make_uint4(parts[k][0], parts[k][1], parts[k][2], parts[k][3]));
                     }
@@ -616,7 +621,7 @@ __global__ __launch_bounds__(kThreads) void shared_attention_kernel(SharedParams
                             const Vec a = __builtin_bit_cast(
                                 Vec, *reinterpret_cast<const uint4*>(kt + (row0 + 16 * b) * kRowBytes + (k_read ^ (kk << 6))));
 #pragma unroll
-                            for (int k = 0; k < 3; ++k)
+                            for (int k = 0; k < kParts; ++k)
 #pragma unroll
                                 for (int n = 0; n < kN; ++n) s[n][b] = M::mma(a, qb[n][k][kk], s[n][b]);
                         }
@@ -641,7 +646,7 @@ __global__ __launch_bounds__(kThreads) void shared_attention_kernel(SharedParams
 #pragma unroll
                     for (int dt = 0; dt < kDt; ++dt) vop[dt] = read_v(dt);
                     __builtin_amdgcn_sched_group_barrier(0x100, 2 * kKk, 0);       // the K reads
-                    __builtin_amdgcn_sched_group_barrier(0x008, 6 * kKk * kN, 0);  // the score MFMAs
+                    __builtin_amdgcn_sched_group_barrier(0x008, 2 * kParts * kKk * kN, 0);  // the score MFMAs
                     __builtin_amdgcn_sched_group_barrier(0x100, 2 * kDt, 0);       // the V reads
                 }
                 set_priority<0>();
@@ -694,7 +699,7 @@ __global__ __launch_bounds__(kThreads) void shared_attention_kernel(SharedParams
                         for (int dt = 0; dt < kDt; ++dt) acc[n][dt] *= alpha;
                     }
                 }
-                Vec pb[kN][3];
+                Vec pb[kN][kParts];
                 float pr[kN][4 * kSubs];
 #pragma unroll
                 for (int n = 0; n < kN; ++n) {
@@ -703,16 +708,16 @@ __global__ __launch_bounds__(kThreads) void shared_attention_kernel(SharedParams
                     float of_step = (pr[n][0] + pr[n][1]) + (pr[n][2] + pr[n][3]);
                     if constexpr (!kF32) {
                         of_step += (pr[n][4] + pr[n][5]) + (pr[n][6] + pr[n][7]);
-                        std::uint32_t parts[3][4];
+                        std::uint32_t parts[kParts][4];
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
                             std::uint32_t x[3];
                             M::split3(pr[n][2 * e] * kWeightScale, pr[n][2 * e + 1] * kWeightScale, x);
 #pragma unroll
-                            for (int k = 0; k < 3; ++k) parts[k][e] = x[k];
+                            for (int k = 0; k < kParts; ++k) parts[k][e] = x[k];
                         }
 #pragma unroll
-                        for (int k = 0; k < 3; ++k)
+                        for (int k = 0; k < kParts; ++k)
                             pb[n][k] =
                                 __builtin_bit_cast(Vec, make_uint4(parts[k][0], parts[k][1], parts[k][2], parts[k][3]));
                     }
@@ -737,7 +742,7 @@ __global__ __launch_bounds__(kThreads) void shared_attention_kernel(SharedParams
                     for (int dt = 0; dt < kDt; ++dt) {
                         const Vec a = kEarlyV ? vop[kEarlyV ? dt : 0] : read_v(dt);
 #pragma unroll
-                        for (int k = 0; k < 3; ++k)
+                        for (int k = 0; k < kParts; ++k)
 #pragma unroll
                             for (int n = 0; n < kN; ++n) acc[n][dt] = M::mma(a, pb[n][k], acc[n][dt]);
                     }

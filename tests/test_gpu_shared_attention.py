@@ -2,8 +2,9 @@
 
 Tolerance: the decode attention's contract, 1e-5 for unit-scale data (scores of
 standard deviation 1, values of 1). With u = 2^-24: a score is a sum of D
-products of FP32-exact parts in FP32 chains, off by at most D u |q||k| in the
-worst case and about sqrt(D) u of its size in practice, under 3e-7 here; a
+products of FP32-exact parts (FP16: a query value and a weight are off by 2u) in
+FP32 chains, off by at most 3 D u |q||k| in the worst case and about 2 sqrt(D) u
+of its size in practice, under 3e-7 here; a
 weight is off by its score's error and exp2's 2u; an output is a weighted mean
 of values below 5, so off by under 5 * (3e-7 + 4u + merge 4u) = 4e-6.
 """
