@@ -50,8 +50,8 @@ struct Shape {
     static constexpr std::uint32_t kStep = kF32 ? 16 : 32;       // tokens of a wavefront's step
     static constexpr std::uint32_t kSteps = kTile / kStep;
     // Blocks of 16 columns that a wavefront may hold: with two, every K and V
-    // operand read from LDS feeds twice the MFMAs. Head size 256 has no registers
-    // for two; FP32 MFMAs are slow enough for one.
+    // operand read from LDS feeds twice the MFMAs. Head sizes 128 and 256 have no
+    // registers for two; FP32 MFMAs are slow enough for one.
     static constexpr std::uint32_t kMostBlocks = kF32 || kD >= 128 ? 1 : 2;
     // The fewest wavefronts side by side over columns: with fewer, the others
     // would not have a step of the tile's tokens each.

@@ -320,6 +320,17 @@ def test_many_rows_and_groups(gpu):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("more", [0, 1], ids=["most rows", "a row more"])
+def test_most_rows_and_groups(gpu, more):
+    """2048 rows in 512 groups, the most that one plan holds; a row more runs as the ordinary decode."""
+    rng = np.random.default_rng(28)
+    b = Batch(rng, [(16 * int(rng.integers(0, 4)), list(rng.integers(0, 30, 4))) for _ in range(512)], "bf16",
+              heads=(2, 1), D=64, after=[9] * more)
+    got = b.check()
+    assert np.array_equal(got, ordinary(b)) == bool(more)
+
+
+@pytest.mark.gpu
 def test_long_prefix(gpu):
     """A prefix over many tiles, so its streams are split over workgroups, beside short and long own parts."""
     rng = np.random.default_rng(18)
