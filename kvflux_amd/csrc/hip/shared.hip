@@ -21,7 +21,7 @@
 // 8 blocks of columns, fewer where there are fewer blocks, merged through LDS
 // at a part's end.
 //   S^T = K Q^T, O^T += V^T P^T  on v_mfma_f32_16x16x32 with Q (scale folded
-// in) and the weights as three BF16 or two FP16 parts each: products as exact as
+// in) and the weights as three 16-bit parts each: products as exact as
 // FP32's, sums FP32. FP32 caches: v_mfma_f32_16x16x4_f32 on the values as they are.
 #include "mfma_parts.h"
 
@@ -217,11 +217,10 @@ __global__ __launch_bounds__(kThreads) void shared_attention_kernel(SharedParams
     constexpr int kBlocks = static_cast<int>(S::kMostBlocks);
     constexpr int kKk = kD / 32;   // 16-bit: K steps of S^T
     constexpr int kDt = kD / 16;   // accumulator tiles of O^T
-    // 16-bit parts of a query value and of a weight. Three BF16 parts hold an FP32
-    // value; two FP16 parts are off by at most 2^-23 of it, twice an FP32 rounding
-    // (and a third adds nothing below 2^-2, where the parts end at 2^-25): 48 rows
-    // behind 60000 tokens in FP16 263 -> 225 us, error against 64 bits unchanged.
-    constexpr int kParts = std::is_same<E, PfF16Exact>::value ? 2 : 3;
+    // 16-bit parts of a query value and of a weight: three hold all 24 bits of an
+    // FP32 value, as in the ordinary decode (two FP16 parts miss its last: 48 rows
+    // behind 60000 tokens in FP16 216 us, and 254 with three).
+    constexpr int kParts = 3;
     constexpr float kWeightScale = kF32 ? 1.0f : M::kWeightScale;
     constexpr float kLazy = kF32 ? 8.0f : M::kLazyLog2;
 
