@@ -195,6 +195,14 @@ __device__ inline std::uint32_t tiles_before(std::uint32_t at, std::uint32_t wei
     return at == 0 ? 0 : at <= weight + kPartCost ? 1 : (at - kPartCost + weight - 1) / weight;
 }
 
+// Exponent of the power of two that takes `largest` into [2^14, 2^15): 0 for zero,
+// NaN, infinity and what passes 2^100 (whose scores could pass FP32), and 126 at
+// most, as 2^-126 is the last normal number.
+__device__ inline int column_exponent(float largest) {
+    const int e = largest > 0.0f && largest < 0x1p100f ? 15 - __builtin_amdgcn_frexp_expf(largest) : 0;
+    return e < 126 ? e : 126;
+}
+
 // exp2(m - top) for merging partials: 0 for a part that saw no key.
 __device__ inline float merge_weight(float m, float top) {
     return m == -INFINITY ? 0.0f : m == top ? 1.0f : __builtin_amdgcn_exp2f(m - top);
@@ -221,8 +229,14 @@ __global__ __launch_bounds__(kThreads) void shared_attention_kernel(SharedParams
     // FP32 value, as in the ordinary decode (two FP16 parts miss its last: 48 rows
     // behind 60000 tokens in FP16 216 us, and 254 with three).
     constexpr int kParts = 3;
+    // FP16 parts end at 2^-24 and at 65504, whatever the query's size: a column's
+    // queries are split times the power of two that brings the largest into
+    // [2^14, 2^15), so only values below 2^-16 of it lose bits. Its scores, the
+    // reference among them, carry that factor up to the exponentials (exact).
+    constexpr bool kScaled = std::is_same<E, PfF16Exact>::value;
     constexpr float kWeightScale = kF32 ? 1.0f : M::kWeightScale;
     constexpr float kLazy = kF32 ? 8.0f : M::kLazyLog2;
+    static_assert(!kScaled || kLazy == 0.0f, "a scaled score is compared with kLazy");
 
     __shared__ __attribute__((aligned(16))) unsigned char buffers[2][kBufferBytes];
     __shared__ std::uint32_t first_of[kMaxGroups + 1];  // first row of a group, and the end
@@ -502,6 +516,7 @@ __global__ __launch_bounds__(kThreads) void shared_attention_kernel(SharedParams
     // score chains), and what a score may pass it by; -inf until the column has
     // seen a key.
     float nref[kBlocks], lazy[kBlocks], sum_hi[kBlocks], sum_lo[kBlocks];
+    float down[kBlocks];  // one over the column's factor
 #pragma unroll 1
     do {
         if (next.ok && new_part) {
@@ -539,6 +554,18 @@ __global__ __launch_bounds__(kThreads) void shared_attention_kernel(SharedParams
                         qf[4 * m + 3] = raw[m].w * p.scale_log2;
                     }
                 } else {
+                    float up = 1.0f;
+                    if constexpr (kScaled) {
+                        float largest = 0.0f;
+#pragma unroll
+                        for (int m = 0; m < kD / 16; ++m)
+                            largest = max3(max3(largest, __builtin_fabsf(raw[m].x), __builtin_fabsf(raw[m].y)),
+                                           __builtin_fabsf(raw[m].z), __builtin_fabsf(raw[m].w));
+                        largest = max_across_quads(largest) * p.scale_log2;
+                        const int e = column_exponent(largest);
+                        up = __builtin_amdgcn_ldexpf(1.0f, e);
+                        down[n] = __builtin_amdgcn_ldexpf(1.0f, -e);
+                    }
 #pragma unroll
                     for (int kk = 0; kk < kKk; ++kk) {
                         const float4 lo = raw[2 * kk], hi = raw[2 * kk + 1];
@@ -547,7 +574,7 @@ __global__ __launch_bounds__(kThreads) void shared_attention_kernel(SharedParams
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
                             std::uint32_t x[3];
-                            M::split3(v[2 * e] * p.scale_log2, v[2 * e + 1] * p.scale_log2, x);
+                            M::split3(v[2 * e] * p.scale_log2 * up, v[2 * e + 1] * p.scale_log2 * up, x);
 #pragma unroll
                             for (int k = 0; k < kParts; ++k) parts[k][e] = x[k];
                         }
@@ -688,7 +715,7 @@ __global__ __launch_bounds__(kThreads) void shared_attention_kernel(SharedParams
                         const float high = max_across_quads(top[n]);
                         const float shift = high > lazy[n] ? high : 0.0f;
                         if (high > lazy[n]) lazy[n] = kLazy;
-                        const float alpha = __builtin_amdgcn_exp2f(fminf(-shift, 0.0f));
+                        const float alpha = __builtin_amdgcn_exp2f(fminf(kScaled ? -shift * down[n] : -shift, 0.0f));
                         nref[n] -= shift;
                         sum_hi[n] *= alpha;
                         sum_lo[n] *= alpha;
@@ -703,7 +730,8 @@ __global__ __launch_bounds__(kThreads) void shared_attention_kernel(SharedParams
 #pragma unroll
                 for (int n = 0; n < kN; ++n) {
 #pragma unroll
-                    for (int e = 0; e < 4 * kSubs; ++e) pr[n][e] = __builtin_amdgcn_exp2f(s[n][e / 4][e % 4]);
+                    for (int e = 0; e < 4 * kSubs; ++e)
+                        pr[n][e] = __builtin_amdgcn_exp2f(kScaled ? s[n][e / 4][e % 4] * down[n] : s[n][e / 4][e % 4]);
                     float of_step = (pr[n][0] + pr[n][1]) + (pr[n][2] + pr[n][3]);
                     if constexpr (!kF32) {
                         of_step += (pr[n][4] + pr[n][5]) + (pr[n][6] + pr[n][7]);
@@ -769,7 +797,7 @@ __global__ __launch_bounds__(kThreads) void shared_attention_kernel(SharedParams
 #pragma unroll
         for (int n = 0; n < kBlocks; ++n) {
             sum[n] = sum_across_quads(sum_hi[n] + sum_lo[n]);
-            top[n] = lazy[n] == -INFINITY ? -INFINITY : -nref[n];
+            top[n] = lazy[n] == -INFINITY ? -INFINITY : kScaled ? -nref[n] * down[n] : -nref[n];
         }
         if (shares > 1) {  // uniform
             // [across][token share but the first][block][dt][lane]

@@ -1,4 +1,5 @@
-"""Numbers that kvflux_paged_attention_shared has to hold: every bit of a query.
+"""Numbers that kvflux_paged_attention_shared has to hold: every bit of a query,
+queries and keys of any size.
 
 Tolerance: the 1e-5 of the decode attention's contract; what a case can lose is
 worked out at the case.
@@ -53,3 +54,38 @@ def test_f16_every_bit_of_a_query(gpu, D, e):
             for s, first in ((1, 0), (-1, 1)):
                 b.q[r, h, first::2] = rng.permutation(queries_past_22_bits(rng, D, e, s))[:D // 2]
     b.check()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,D", [("f16", 64), ("f16", 128), ("f16", 256), ("bf16", 128), ("f32", 64)])
+@pytest.mark.parametrize("size", [1e-3, 1e-4, 1e-8, 1024.0, 2.0 ** 20])
+def test_queries_of_any_size(gpu, dtype, D, size):
+    """Queries of standard deviation `size` and keys of 1 / size (FP16 keys: at most 10000, and of 16 of their least
+    steps at 2^-20): scores of the size of every other test's, or smaller ones, so the same error."""
+    rng = np.random.default_rng(32)
+    keys = min(1 / size, 1e4) if dtype == "f16" else 1 / size
+    b = Batch(rng, [(300, [10, 200, 31]), (64, [3, 3])], dtype, D=D, scale=keys)
+    b.q *= np.float32(size)
+    b.check()
+
+
+@pytest.mark.parametrize("size", [1e-30, 1e-8, 1e-3, 1.0, 1e3, 1e20])
+def test_split_of_a_scaled_column(size):
+    """The arithmetic of the split (no GPU needed): the column's largest value taken into [2^14, 2^15), then three FP16
+    parts. Their least step is 2^-24, so a value is off by 2^-25 * 2^-14 of the largest at most, or, above 2^-15 of it,
+    by nothing: 33 bits hold FP32's 24. Without the factor, values of 0.2 and less keep an error of 2^-25 whatever
+    their size, and those past 65504 have no parts."""
+    rng = np.random.default_rng(34)
+    x = (rng.standard_normal((200, 128)) * size).astype(np.float32) * scale_of(128)
+    largest = np.abs(x).max(-1, keepdims=True)
+    up = np.ldexp(np.float32(1), np.minimum(15 - np.frexp(largest)[1], 126))
+    y = x * up
+    assert (np.abs(y).max(-1) >= 2.0 ** 14).all() and (np.abs(y) < 2.0 ** 15).all()
+    rest, parts = y.copy(), np.zeros(y.shape)
+    for _ in range(3):
+        part = rest.astype(np.float16)
+        rest = rest - part.astype(np.float32)
+        parts += part.astype(np.float64)
+    off = np.abs(parts - y.astype(np.float64))
+    assert off.max() <= 2.0 ** -25
+    assert (off[np.abs(y) >= 0.5] == 0).all()
