@@ -236,6 +236,14 @@ __global__ __launch_bounds__(kThreads) void shared_attention_kernel(SharedParams
     constexpr bool kScaled = std::is_same<E, PfF16Exact>::value;
     constexpr float kWeightScale = kF32 ? 1.0f : M::kWeightScale;
     constexpr float kLazy = kF32 ? 8.0f : M::kLazyLog2;
+    // Where the weighted sums gather before they are added to the part's: an MFMA
+    // rounds a sum with a large accumulator to fewer bits and toward zero, and
+    // thousands of weights of 2^-25 behind one large one lost 2e-5 that way (FP32
+    // caches 9e-5). Over a tile, in registers of their own, where those are there
+    // (48 rows behind 60000 tokens 262 -> 249 us, head size 64 51.4 -> 50.3); over a
+    // step at head size 256, and on FP16 caches, whose reference moves too often
+    // to scale two sets of sums (64 rows behind 8192, head size 64: 56.5, else 59).
+    constexpr bool kTileSums = !kScaled && kD <= 128;
     static_assert(!kScaled || kLazy == 0.0f, "a scaled score is compared with kLazy");
 
     __shared__ __attribute__((aligned(16))) unsigned char buffers[2][kBufferBytes];
@@ -618,6 +626,7 @@ __global__ __launch_bounds__(kThreads) void shared_attention_kernel(SharedParams
         const auto compute = [&](auto block_count) {
             constexpr int kN = decltype(block_count)::value;
             const std::uint32_t steps = S::kSteps / shares;
+            pf_f32x4_t of_tile[kTileSums ? kN : 1][kTileSums ? kDt : 1] = {};
 #pragma unroll 1
             for (std::uint32_t st = 0; st < steps; ++st) {
                 const std::uint32_t row0 = (token_share * steps + st) * kStep;
@@ -722,7 +731,10 @@ __global__ __launch_bounds__(kThreads) void shared_attention_kernel(SharedParams
 #pragma unroll
                         for (int b = 0; b < kSubs; ++b) s[n][b] -= shift;
 #pragma unroll
-                        for (int dt = 0; dt < kDt; ++dt) acc[n][dt] *= alpha;
+                        for (int dt = 0; dt < kDt; ++dt) {
+                            acc[n][dt] *= alpha;
+                            if constexpr (kTileSums) of_tile[n][dt] *= alpha;
+                        }
                     }
                 }
                 Vec pb[kN][kParts];
@@ -750,30 +762,55 @@ __global__ __launch_bounds__(kThreads) void shared_attention_kernel(SharedParams
                     }
                     two_sum_add(sum_hi[n], sum_lo[n], of_step);
                 }
+                // Weighted sums of the step, from zero or on the tile's.
+                const auto gathered = [&](int n, int dt) {
+                    if constexpr (kTileSums) return of_tile[n][dt];
+                    else return pf_f32x4_t{};
+                };
+                const auto gather = [&](int n, int dt, const pf_f32x4_t& x) {
+                    if constexpr (kTileSums) of_tile[n][dt] = x;
+                    else acc[n][dt] += x;
+                };
                 if constexpr (kF32) {
                     // MFMA r takes token 4 * quad + r of lane (quad, col); block
                     // 4 * mm + j of O^T is dims 64 * mm + 4 * i + j, i = 0..15.
 #pragma unroll
-                    for (int r = 0; r < 4; ++r)
+                    for (int mm = 0; mm < kD / 64; ++mm) {
+                        pf_f32x4_t o[4];
 #pragma unroll
-                        for (int mm = 0; mm < kD / 64; ++mm) {
+                        for (int j = 0; j < 4; ++j) o[j] = gathered(0, 4 * mm + j);
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) {
                             const float4 x = *reinterpret_cast<const float4*>(vt + (row0 + r) * kRowBytes + v_read + 256 * mm);
-                            pf_f32x4_t* const o = &acc[0][4 * mm];
                             o[0] = __builtin_amdgcn_mfma_f32_16x16x4f32(x.x, pr[0][r], o[0], 0, 0, 0);
                             o[1] = __builtin_amdgcn_mfma_f32_16x16x4f32(x.y, pr[0][r], o[1], 0, 0, 0);
                             o[2] = __builtin_amdgcn_mfma_f32_16x16x4f32(x.z, pr[0][r], o[2], 0, 0, 0);
                             o[3] = __builtin_amdgcn_mfma_f32_16x16x4f32(x.w, pr[0][r], o[3], 0, 0, 0);
                         }
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) gather(0, 4 * mm + j, o[j]);
+                    }
                 } else {
 #pragma unroll
                     for (int dt = 0; dt < kDt; ++dt) {
                         const Vec a = kEarlyV ? vop[kEarlyV ? dt : 0] : read_v(dt);
+                        pf_f32x4_t o[kN];
+#pragma unroll
+                        for (int n = 0; n < kN; ++n) o[n] = gathered(n, dt);
 #pragma unroll
                         for (int k = 0; k < kParts; ++k)
 #pragma unroll
-                            for (int n = 0; n < kN; ++n) acc[n][dt] = M::mma(a, pb[n][k], acc[n][dt]);
+                            for (int n = 0; n < kN; ++n) o[n] = M::mma(a, pb[n][k], o[n]);
+#pragma unroll
+                        for (int n = 0; n < kN; ++n) gather(n, dt, o[n]);
                     }
                 }
+            }
+            if constexpr (kTileSums) {
+#pragma unroll
+                for (int n = 0; n < kN; ++n)
+#pragma unroll
+                    for (int dt = 0; dt < kDt; ++dt) acc[n][dt] += of_tile[n][dt];
             }
         };
         if (active) {

@@ -1,5 +1,5 @@
 """Numbers that kvflux_paged_attention_shared has to hold: every bit of a query,
-queries and keys of any size.
+queries and keys of any size, rows dominated by one key.
 
 Tolerance: the 1e-5 of the decode attention's contract; what a case can lose is
 worked out at the case.
@@ -9,7 +9,7 @@ from __future__ import annotations
 import numpy as np
 import pytest
 
-from test_gpu_shared_attention import Batch, to_bits
+from test_gpu_shared_attention import TOL, Batch, from_bits, to_bits
 
 
 def scale_of(D):
@@ -89,3 +89,36 @@ def test_split_of_a_scaled_column(size):
     off = np.abs(parts - y.astype(np.float64))
     assert off.max() <= 2.0 ** -25
     assert (off[np.abs(y) >= 0.5] == 0).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["f16", "bf16", "f32"])
+def test_rows_dominated_by_one_key(gpu, dtype):
+    """The first key 25 to 26 above all others in log2, whose weights, 2^-25.5 of it each, come to 3e-4 of the row and
+    whose values lie about 1: they have to reach the numerator as they reach the sum. 128 columns in 64 streams, so a
+    wavefront walks 4096 tokens."""
+    rng = np.random.default_rng(33)
+    D, prefix, rows, H, G = 64, 16384, 16, 8, 8
+    b = Batch(rng, [(prefix, [16] * rows)] * 8, dtype, heads=(H * G, H), D=D)
+    a, top = 8.0, 30.0
+    k = rng.uniform(-1, 1, b.k.shape).astype(np.float32)
+    k[..., 0] = top - rng.uniform(25.0, 26.0, b.k.shape[:-1]) / (a * scale_of(D))
+    v = (1 + 0.5 * rng.standard_normal(b.v.shape)).astype(np.float32)
+    for g in range(8):
+        first = int(b.table[g * rows, 0])
+        k[first, :, 0, 0] = top
+        v[first, :, 0] = rng.standard_normal((H, D))
+    b.k, b.v = to_bits(k, dtype), to_bits(v, dtype)
+    b.q = (0.01 * rng.standard_normal(b.q.shape)).astype(np.float32)
+    b.q[..., 0] = a
+    got = b.upload().run()
+    k, v = from_bits(b.k, dtype), from_bits(b.v, dtype)
+    for r in range(0, len(b.lens), 7):
+        h = r % H
+        tokens = np.arange(int(b.lens[r]))
+        page = b.table[r, tokens // b.bs].astype(np.int64)
+        s = b.q[r, h * G:(h + 1) * G].astype(np.float64) @ k[page, h, tokens % b.bs].T / np.sqrt(D)
+        w = np.exp(s - s.max(-1, keepdims=True))
+        want = w @ v[page, h, tokens % b.bs] / w.sum(-1, keepdims=True)
+        error = np.abs(got[r, h * G:(h + 1) * G] - want).max()
+        assert error <= TOL, (r, error)
