@@ -471,6 +471,10 @@ struct Mfma<Bf16> {
     __device__ static f32x4_t mma16(const i16x4_t& a, const i16x4_t& b, const f32x4_t& c) {
         return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(a, b, c, 0, 0, 0);
     }
+    // A query's parts are held times kUp[k] (exact) and their scores taken
+    // back: 1 here, as BF16 has FP32's exponents.
+    static constexpr bool kQueryScaled = false;
+    static constexpr float kUp[3] = {1.0f, 1.0f, 1.0f};
     __device__ static std::uint16_t split(float x, float* rest) {  // RNE to BF16
         std::uint32_t u = __float_as_uint(x);
         u += 0x7fffu + ((u >> 16) & 1u);
@@ -505,6 +509,15 @@ struct Mfma<F16> {
         return __builtin_amdgcn_mfma_f32_16x16x16f16(__builtin_bit_cast(f16x4_t, a),
                                                      __builtin_bit_cast(f16x4_t, b), c, 0, 0, 0);
     }
+    // FP16 parts end at 2^-24 and at 65504: unscaled ones leave 2^-25 of a query
+    // whatever its size (1e-3 beside keys of 1e3: outputs off by 1e-4) and hold none
+    // past 65504. The parts' scores come in columns of their own, so each part has
+    // its own factor: together they hold scaled queries of up to 2^20 to the last of
+    // FP32's bits or to 2^-42. (A first factor of 2^-8, for queries of up to 2^24,
+    // makes small ones subnormal, whose products the MFMA sums to fewer bits: 1.7e-5
+    // at queries of 1e-4, where this is under 2e-6.)
+    static constexpr bool kQueryScaled = true;
+    static constexpr float kUp[3] = {0x1p-4f, 0x1p6f, 0x1p17f};
     __device__ static std::uint16_t split(float x, float* rest) {
         const _Float16 h = static_cast<_Float16>(x);
         *rest = x - static_cast<float>(h);
@@ -926,9 +939,9 @@ __global__ __launch_bounds__(kThreads, (bs16_occupancy_g<E, kD, kG, kSmall>())) 
                     reinterpret_cast<float*>(qsplit[s])[g * kD + d] = x;
                 } else {
                     float rest;
-                    qsplit[s][(0 * kG + g) * kD + d] = M::split(x, &rest);
-                    qsplit[s][(1 * kG + g) * kD + d] = M::split(rest, &rest);
-                    qsplit[s][(2 * kG + g) * kD + d] = M::split(rest, &rest);
+                    qsplit[s][(0 * kG + g) * kD + d] = M::split(x * M::kUp[0], &rest);
+                    qsplit[s][(1 * kG + g) * kD + d] = M::split(rest * (M::kUp[1] / M::kUp[0]), &rest);
+                    qsplit[s][(2 * kG + g) * kD + d] = M::split(rest * (M::kUp[2] / M::kUp[1]), &rest);
                 }
             }
         }
@@ -1139,13 +1152,19 @@ __global__ __launch_bounds__(kThreads, (bs16_occupancy_g<E, kD, kG, kSmall>())) 
             float sc[4];
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                if constexpr (kSets == 1) {
-                    sc[r] = in.s0[r] + row_shl<kG>(in.s0[r]) + row_shl<2 * kG>(in.s0[r]);
-                } else if constexpr (kSets == 2) {
-                    sc[r] = in.s0[r] + row_shl<kG>(in.s0[r]) + in.s1[r];
+                float mid, lo;  // the parts' scores
+                if constexpr (kSets == 3) {
+                    mid = in.s1[r];
+                    lo = in.s2[r];
                 } else {
-                    sc[r] = (in.s0[r] + in.s1[r]) + in.s2[r];
+                    mid = row_shl<kG>(in.s0[r]);
+                    if constexpr (kSets == 2) lo = in.s1[r];
+                    else lo = row_shl<2 * kG>(in.s0[r]);
                 }
+                if constexpr (M::kQueryScaled)
+                    sc[r] = fmaf(lo, 1.0f / M::kUp[2], fmaf(mid, 1.0f / M::kUp[1], in.s0[r] * (1.0f / M::kUp[0])));
+                else
+                    sc[r] = in.s0[r] + mid + lo;
                 if (valid < kBs && static_cast<std::uint32_t>(quad * 4 + r) >= valid) sc[r] = -INFINITY;
             }
             float tmax = fmaxf(fmaxf(sc[0], sc[1]), fmaxf(sc[2], sc[3]));
