@@ -89,6 +89,15 @@ struct PfF16Exact : PfF16 {
     static constexpr float kWeightScale = 32768.0f;
     static constexpr float kLazyLog2 = 0.0f;
 };
+// Exponent of the power of two by which a row of scaled queries is split into FP16
+// parts, whose range is fixed: it takes the `largest` into [2^14, 2^15), so only
+// values below 2^-16 of that lose bits of FP32's 24. 0 for zero,
+// NaN, infinity and what passes 2^100 (whose scores could pass FP32), and 126 at
+// most, as 2^-126 is the last normal number.
+__device__ inline int split_exponent(float largest) {
+    const int e = largest > 0.0f && largest < 0x1p100f ? 15 - __builtin_amdgcn_frexp_expf(largest) : 0;
+    return e < 126 ? e : 126;
+}
 // NaN-propagating maximum of three (one v_maximum3_f32).
 __device__ inline float max3(float a, float b, float c) {
     return __builtin_elementwise_maximum(__builtin_elementwise_maximum(a, b), c);

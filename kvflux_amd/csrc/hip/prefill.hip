@@ -180,6 +180,11 @@ __global__ __launch_bounds__(kPfThreads) void paged_prefill_kernel(PrefillParams
     constexpr int kVSwz = kCpr / 8;  // V slot swizzle multiplier
     constexpr float kLazy = E::kLazyLog2;
     constexpr float kWeightScale = E::kWeightScale;
+    // FP16 parts end at 2^-24 and at 65504 whatever the query's size (queries of
+    // 1e-4 beside keys of 1e4: outputs off by 1e-3): a row's queries are split times
+    // a power of two, which its scores and reference carry up to the exponentials.
+    constexpr bool kScaled = std::is_same<E, PfF16Exact>::value;
+    static_assert(!kScaled || kLazy == 0.0f, "a scaled score is compared with kLazy");
     static_assert(kDma >= 1 && kTileBytes % (kPfThreads * 16) == 0, "tile split");
 
     __shared__ __attribute__((aligned(16))) std::uint16_t lds_tiles[4][kTileBytes / 2];
@@ -266,8 +271,20 @@ __global__ __launch_bounds__(kPfThreads) void paged_prefill_kernel(PrefillParams
     }
     stage(first_page(tile_begin & ~win_mask));
     Vec qb_op[kParts][kPfNt][kSteps];
+    float down[kPfNt];  // one over the row's factor
 #pragma unroll
     for (int n = 0; n < kPfNt; ++n) {
+        float up = 1.0f;
+        if constexpr (kScaled) {
+            float largest = 0.0f;
+#pragma unroll
+            for (int c = 0; c < kQuads; ++c)
+                largest = max3(max3(largest, __builtin_fabsf(qraw[n][c].x), __builtin_fabsf(qraw[n][c].y)),
+                               __builtin_fabsf(qraw[n][c].z), __builtin_fabsf(qraw[n][c].w));
+            const int e = split_exponent(max_across_quads(largest) * p.scale_log2);
+            up = __builtin_amdgcn_ldexpf(1.0f, e);
+            down[n] = __builtin_amdgcn_ldexpf(1.0f, -e);
+        }
 #pragma unroll
         for (int kk = 0; kk < kSteps; ++kk) {
             const float4 lo = qraw[n][2 * kk], hi = qraw[n][2 * kk + 1];
@@ -277,7 +294,10 @@ __global__ __launch_bounds__(kPfThreads) void paged_prefill_kernel(PrefillParams
             for (int e = 0; e < 4; ++e) {
                 if constexpr (kExact) {
                     std::uint32_t parts[3];
-                    M::split3(v[2 * e] * p.scale_log2, v[2 * e + 1] * p.scale_log2, parts);
+                    if constexpr (kScaled)
+                        M::split3(v[2 * e] * p.scale_log2 * up, v[2 * e + 1] * p.scale_log2 * up, parts);
+                    else
+                        M::split3(v[2 * e] * p.scale_log2, v[2 * e + 1] * p.scale_log2, parts);
 #pragma unroll
                     for (int k = 0; k < kParts; ++k) w[k][e] = parts[k];
                 } else {
@@ -466,7 +486,7 @@ __global__ __launch_bounds__(kPfThreads) void paged_prefill_kernel(PrefillParams
                     const bool moves = (kKs == 1 && !have_ref) || tmax > lazy_of[n];
                     const float shift = moves ? tmax : 0.0f;
                     if (kKs == 2 && moves) lazy_of[n] = kLazy;
-                    const float alpha = __builtin_amdgcn_exp2f(fminf(-shift, 0.0f));
+                    const float alpha = __builtin_amdgcn_exp2f(fminf(kScaled ? -shift * down[n] : -shift, 0.0f));
                     nref[n] -= shift;
                     lsum[n] *= alpha;
 #pragma unroll
@@ -483,7 +503,8 @@ __global__ __launch_bounds__(kPfThreads) void paged_prefill_kernel(PrefillParams
 #pragma unroll
                 for (int kt2 = 0; kt2 < 2; ++kt2)
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) pr[4 * kt2 + r] = __builtin_amdgcn_exp2f(s[kt2][n][r]);
+                    for (int r = 0; r < 4; ++r)
+                        pr[4 * kt2 + r] = __builtin_amdgcn_exp2f(kScaled ? s[kt2][n][r] * down[n] : s[kt2][n][r]);
                 std::uint32_t w[kParts][4];
                 if constexpr (kExact) {
                     float hi = lsum[n][0], lo = lsum[n][1];  // [1]: the sum's low word
@@ -588,6 +609,10 @@ __global__ __launch_bounds__(kPfThreads) void paged_prefill_kernel(PrefillParams
         lds_barrier();
     }
 
+    if constexpr (kScaled) {
+#pragma unroll
+        for (int n = 0; n < kPfNt; ++n) nref[n] *= down[n];
+    }
     // kKs = 2: the second halves' wavefronts hand their sums over, one row
     // block at a time through the tile buffers (free after the loop's last
     // barrier); the first halves' wavefronts rescale both to the higher

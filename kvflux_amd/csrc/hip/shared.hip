@@ -195,14 +195,6 @@ __device__ inline std::uint32_t tiles_before(std::uint32_t at, std::uint32_t wei
     return at == 0 ? 0 : at <= weight + kPartCost ? 1 : (at - kPartCost + weight - 1) / weight;
 }
 
-// Exponent of the power of two that takes `largest` into [2^14, 2^15): 0 for zero,
-// NaN, infinity and what passes 2^100 (whose scores could pass FP32), and 126 at
-// most, as 2^-126 is the last normal number.
-__device__ inline int column_exponent(float largest) {
-    const int e = largest > 0.0f && largest < 0x1p100f ? 15 - __builtin_amdgcn_frexp_expf(largest) : 0;
-    return e < 126 ? e : 126;
-}
-
 // exp2(m - top) for merging partials: 0 for a part that saw no key.
 __device__ inline float merge_weight(float m, float top) {
     return m == -INFINITY ? 0.0f : m == top ? 1.0f : __builtin_amdgcn_exp2f(m - top);
@@ -570,7 +562,7 @@ __global__ __launch_bounds__(kThreads) void shared_attention_kernel(SharedParams
                             largest = max3(max3(largest, __builtin_fabsf(raw[m].x), __builtin_fabsf(raw[m].y)),
                                            __builtin_fabsf(raw[m].z), __builtin_fabsf(raw[m].w));
                         largest = max_across_quads(largest) * p.scale_log2;
-                        const int e = column_exponent(largest);
+                        const int e = split_exponent(largest);
                         up = __builtin_amdgcn_ldexpf(1.0f, e);
                         down[n] = __builtin_amdgcn_ldexpf(1.0f, -e);
                     }
