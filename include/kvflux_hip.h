@@ -414,7 +414,8 @@ int kvflux_write_paged_kv_tail(void* key_cache, void* value_cache, uint64_t num_
  *   They are only read; query_out must not overlap them.
  * For a query or key row x and position t:
  *   n = x / sqrt(mean(x^2) + eps) * w     (w = query_norm or key_norm, device
- *       float [head_size]; NULL: n = x), eps >= 0
+ *       float [head_size]; NULL: n = x), eps >= 0, rows of any size (of zeros with
+ *       eps 0: 0 / 0, NaN)
  *   over the first rotary_dim dims (even, at most head_size; 0: no rotation),
  *   angle_j = t * inv_freq[j], inv_freq device double [rotary_dim / 2]:
  *     y_a = n_a cos - n_b sin, y_b = n_b cos + n_a sin for the pairs (a, b) =

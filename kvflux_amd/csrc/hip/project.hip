@@ -139,6 +139,18 @@ __device__ inline float row_sum(float x, std::uint32_t lanes) {
     return x;
 }
 
+// Rows whose squares or their mean leave FP32's normal range (a mean under 2^-100,
+// which a tiny eps leaves there; a sum of 2^120 and more, up to infinity): the
+// reciprocal root takes no denormals, and a sum that overflowed has none. Such a
+// row is normed times f^2 = 2^100 or 2^-100, with eps times f^4, and scaled in two
+// steps of f, so no step leaves the range.
+__device__ inline bool out_of_range(float mean, float square) { return mean < 0x1p-100f || square >= 0x1p120f; }
+__device__ inline float range_factor(float mean) { return mean < 0x1p-100f ? 0x1p50f : 0x1p-50f; }
+// What (x * f) is multiplied by, `square` being the sum of the squares of x f^2.
+__device__ inline float ranged_scale(float square, float inv_dim, float eps, float f) {
+    return __builtin_amdgcn_rsqf(fmaf(square, inv_dim, eps * (f * f) * (f * f))) * f;
+}
+
 // Four values of a row: 8 bytes of a 16-bit type, 16 of FP32.
 template <typename E>
 using Four = typename std::conditional<std::is_same<E, F32>::value, V16, V8>::type;
@@ -250,9 +262,32 @@ __global__ __launch_bounds__(kThreads) void norm_rope_write_kernel(Params p, Pla
         for (int i = 0; i < 4; ++i) square = fmaf(xa[i], xa[i], fmaf(xb[i], xb[i], square));
         if (!inside) square = 0.0f;
         square = row_sum(square, lanes);
+        const bool is_query = row_u < p.query_heads, is_key = row_u < p.query_heads + p.kv_heads;
+        const bool normed = is_query ? p.query_norm != nullptr : is_key && p.key_norm != nullptr;
+        const float mean = fmaf(square, p.inv_dim, p.eps);
+        float scale = __builtin_amdgcn_rsqf(mean);
+        const bool odd = normed && out_of_range(mean, square);
+        if (__builtin_expect(__builtin_amdgcn_ballot_w64(odd) != 0, 0)) {  // uniform
+            const float f = range_factor(mean);
+            float again = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float ya = xa[i] * f * f, yb = xb[i] * f * f;
+                again = fmaf(ya, ya, fmaf(yb, yb, again));
+            }
+            again = row_sum(inside ? again : 0.0f, lanes);
+            if (odd) {
+                const float by = ranged_scale(again, p.inv_dim, p.eps, f);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    xa[i] = xa[i] * f * by;
+                    xb[i] = xb[i] * f * by;
+                }
+                scale = 1.0f;
+            }
+        }
         if (row_u == ~0u || !inside) return;
         const std::uint32_t t = token_u - token0;
-        const bool is_query = row_u < p.query_heads, is_key = row_u < p.query_heads + p.kv_heads;
         const std::uint64_t at = places[t];
         if (is_query ? !live[t] : at == kNowhere) return;
         const std::uint32_t head = row_u - (is_query ? 0u : is_key ? p.query_heads : p.query_heads + p.kv_heads);
@@ -270,8 +305,7 @@ __global__ __launch_bounds__(kThreads) void norm_rope_write_kernel(Params p, Pla
             stream_store(reinterpret_cast<Four<Cache>*>(dst + b), cb);
             return;
         }
-        if (is_query ? p.query_norm != nullptr : p.key_norm != nullptr) {
-            const float scale = __builtin_amdgcn_rsqf(fmaf(square, p.inv_dim, p.eps));
+        if (normed) {
             const f32x4_t wa = is_query ? wqa : wka, wb = is_query ? wqb : wkb;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
@@ -357,7 +391,21 @@ __global__ __launch_bounds__(64) void norm_rope_write_generic_kernel(Params p, P
     }
 #pragma unroll
     for (int m = 1; m < 64; m <<= 1) square += __shfl_xor(square, m);
-    const float scale = __builtin_amdgcn_rsqf(fmaf(square, p.inv_dim, p.eps));
+    const float mean = fmaf(square, p.inv_dim, p.eps);
+    float scale = __builtin_amdgcn_rsqf(mean);
+    if (norm && out_of_range(mean, square)) {  // uniform
+        const float f = range_factor(mean);
+        square = 0.0f;
+#pragma unroll
+        for (int k = 0; k < kPer; ++k) {
+            const float y = x[k] * f * f;
+            square = fmaf(y, y, square);
+            x[k] *= f;
+        }
+#pragma unroll
+        for (int m = 1; m < 64; m <<= 1) square += __shfl_xor(square, m);
+        scale = ranged_scale(square, p.inv_dim, p.eps, f);
+    }
 #pragma unroll
     for (int k = 0; k < kPer; ++k) {
         const std::uint32_t d = lane + 64 * k;
