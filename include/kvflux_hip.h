@@ -231,7 +231,8 @@ int kvflux_paged_attention_noalloc(const void* key_cache, const void* value_cach
  *   group_prefixes: device uint64 [num_groups]: the rows of group g have the
  *                   same pages (table entries) for their first
  *                   group_prefixes[g] tokens; they are read through the table
- *                   row of the group's first row. A value above max_prefix
+ *                   row of the group's first row that has so many (shorter rows
+ *                   need not have those pages). A value above max_prefix
  *                   or kv_len shares nothing: the group's rows are as rows
  *                   without one.
  * A row shorter than its group's prefix attends to its own seq_lens[r] tokens

@@ -131,9 +131,9 @@ __device__ inline std::uint32_t tile_cost(std::uint32_t cols) {
 }
 
 // A segment: the columns (of row first_row on), the tokens [begin, end) of
-// table row first_row, its tiles and the cost of one.
+// table row `table_row`, its tiles and the cost of one.
 struct Segment {
-    std::uint32_t first_row, cols, col_tiles, begin, end, tiles, weight;
+    std::uint32_t first_row, table_row, cols, col_tiles, begin, end, tiles, weight;
     __device__ std::uint32_t stream_cost() const { return tiles != 0 ? tiles * weight + kPartCost : 0; }
     __device__ std::uint32_t cost(std::uint32_t heads) const { return stream_cost() * (heads * col_tiles); }
 };
@@ -141,7 +141,7 @@ struct Segment {
 template <typename E, int kD>
 __device__ inline Segment make_segment(std::uint32_t first_row, std::uint32_t cols, std::uint32_t begin, std::uint32_t end) {
     constexpr std::uint32_t kTile = Shape<E, kD>::kTile;
-    Segment s{first_row, cols, (cols + kCols - 1) / kCols, begin, end, 0, 0};
+    Segment s{first_row, first_row, cols, (cols + kCols - 1) / kCols, begin, end, 0, 0};
     s.tiles = end > begin ? (end - begin - 1) / kTile + 1 : 0;
     s.weight = tile_cost<E, kD>(cols);
     return s;
@@ -362,7 +362,21 @@ __global__ __launch_bounds__(kThreads) void shared_attention_kernel(SharedParams
     };
     const auto uniform_segment = [&](std::uint32_t s) {
         const Segment x = segment(s);
-        return Segment{uniform(x.first_row), uniform(x.cols), uniform(x.col_tiles), uniform(x.begin), uniform(x.end),
+        // A prefix is read through the first of its rows that reach it: a shorter
+        // row's table need not have those pages.
+        std::uint32_t table_row = uniform(x.first_row);
+        if (s < p.groups) {
+            const std::uint32_t end = uniform(first_of[s + 1]);
+#pragma unroll 1
+            for (std::uint32_t base = table_row; base < end; base += 64) {
+                const std::uint32_t r = base + lane;
+                const std::uint64_t reach = __builtin_amdgcn_ballot_w64(r < end && begin_of[r] != 0);
+                if (reach == 0) continue;
+                table_row = base + static_cast<std::uint32_t>(__builtin_ctzll(reach));
+                break;
+            }
+        }
+        return Segment{uniform(x.first_row), table_row, uniform(x.cols), uniform(x.col_tiles), uniform(x.begin), uniform(x.end),
                        uniform(x.tiles), uniform(x.weight)};
     };
     Cursor ahead;  // the tile whose page ids are fetched next
@@ -421,7 +435,7 @@ __global__ __launch_bounds__(kThreads) void shared_attention_kernel(SharedParams
     // The page ids of a tile's rows are fetched a tile before its loads go out.
     std::uint64_t ids[kIds];
     const auto fetch_ids = [&](const Cursor& c) {
-        const std::uint64_t* const table = p.table + static_cast<std::uint64_t>(c.s.first_row) * p.width;
+        const std::uint64_t* const table = p.table + static_cast<std::uint64_t>(c.s.table_row) * p.width;
 #pragma unroll
         for (int i = 0; i < kIds; ++i) {
             const std::uint32_t token = first_token(c) + (kWhole ? wave_row + 16 * i : row_of(i));
@@ -530,7 +544,7 @@ __global__ __launch_bounds__(kThreads) void shared_attention_kernel(SharedParams
             token_share = wave % shares;
             first_col = across * blocks * 16;
             active = first_col < cols;  // uniform in a wavefront
-            table_row = p.table + static_cast<std::uint64_t>(part.first_row) * p.width;
+            table_row = p.table + static_cast<std::uint64_t>(part.table_row) * p.width;
 #pragma unroll
             for (int n = 0; n < kBlocks; ++n) {
                 if (!active || n >= static_cast<int>(blocks)) break;
