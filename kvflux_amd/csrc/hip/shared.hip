@@ -262,7 +262,7 @@ __global__ __launch_bounds__(kThreads) void shared_attention_kernel(SharedParams
     }
     for (std::uint32_t g = tid; g < p.groups; g += kThreads) {
         const std::uint64_t n = p.prefixes[g];
-        prefix_of[g] = n <= p.max_prefix ? static_cast<std::uint32_t>(n) & (kWhole ? ~15u : ~0u) : 0u;
+        prefix_of[g] = n <= p.max_prefix ? static_cast<std::uint32_t>(n) : 0u;
     }
     if (wave == 0) {
         std::uint32_t carry = 0;
@@ -283,9 +283,12 @@ __global__ __launch_bounds__(kThreads) void shared_attention_kernel(SharedParams
     if (tid < 2) bad_tile[tid] = 0;
     if (tid == 0) found[0] = ~0u;
     __syncthreads();
-    // Tokens that the rows of a group share: none with fewer than two rows. A
-    // row shorter than that takes no part in it.
-    const auto shared_tokens = [&](std::uint32_t g) { return first_of[g + 1] - first_of[g] >= 2 ? prefix_of[g] : 0u; };
+    // Tokens that the rows of a group share, in steps of 16 where pages are whole
+    // ones: none with fewer than two rows. A row shorter than the prefix takes no
+    // part in it.
+    const auto shared_tokens = [&](std::uint32_t g) {
+        return first_of[g + 1] - first_of[g] >= 2 ? prefix_of[g] & (kWhole ? ~15u : ~0u) : 0u;
+    };
     const auto segment = [&](std::uint32_t s) {
         const bool group = s < p.groups;
         const std::uint32_t r = s - p.groups;
@@ -304,8 +307,7 @@ __global__ __launch_bounds__(kThreads) void shared_attention_kernel(SharedParams
     for (std::uint32_t s = tid * per; s < (tid + 1) * per && s < segments; ++s) {
         if (s >= p.groups) {
             const std::uint32_t r = s - p.groups, g = group_of(first_of, p.groups, r);
-            const std::uint32_t shared = g < p.groups ? shared_tokens(g) : 0u;
-            begin_of[r] = shared <= end_of[r] ? shared : 0u;
+            begin_of[r] = g < p.groups && prefix_of[g] <= end_of[r] ? shared_tokens(g) : 0u;
         }
         const std::uint32_t cost = segment(s).cost(p.heads);
         cost_of[s] = cost;

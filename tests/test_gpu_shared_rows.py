@@ -35,3 +35,17 @@ def test_pages_behind_a_short_first_row(gpu):
     b.lens[0] = 100
     b.table[0] = rng.permutation(b.pages)[:b.table.shape[1]]
     b.check()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("prefix,length", [(330, 325), (330, 320), (330, 329), (17, 16), (343, 336)])
+@pytest.mark.parametrize("bs", [16, 48])
+def test_rows_shorter_than_a_prefix_inside_a_page(gpu, bs, prefix, length):
+    """A prefix that ends inside a page, and a row that ends between the last whole step before it and its end: its pages
+    are its own from the first on."""
+    rng = np.random.default_rng(63)
+    for row in (0, 2):
+        b = Batch(rng, [(prefix, [20, 40, 60, 80])], bs=bs)
+        b.lens[row] = length
+        b.table[row, :-(-length // bs)] = rng.choice(b.table[3][b.table[3] < b.pages], -(-length // bs))
+        b.check()
