@@ -53,14 +53,16 @@ public:
     void enqueue_refresh();
     // Library-internal: the rows' shared prefixes (shared_prefix.h) as device
     // arrays uint64 [groups + 1] and [groups], found and uploaded at the first
-    // call after the whole table was; most: the longest prefix.
+    // call after the whole table was; most: the longest prefix. grouped(): they are.
     struct Groups {
         const std::uint64_t* starts = nullptr;
         const std::uint64_t* prefixes = nullptr;
         std::size_t count = 0;
         std::uint64_t most = 0;
+        std::uint64_t shared_tokens = 0;  // sum of (rows - 1) * prefix
     };
     const Groups& enqueue_groups();
+    bool grouped() const noexcept { return grouped_; }
 
 private:
     struct Device;

@@ -32,14 +32,16 @@ SharedPrefixGroups find_shared_prefixes(const std::vector<const SequenceState*>&
 // paged_attention_batch with every group's prefix computed once (see
 // kvflux_paged_attention_shared); groups from find_shared_prefixes. Same contract:
 // FP32 Q and O, Exact, the same exceptions. Results agree with
-// paged_attention_batch to 1e-5; where sharing cannot pay they are its bits.
+// paged_attention_batch to 1e-5; where sharing, as the groups really share, does not
+// pay they are its bits.
 void paged_attention_batch_shared(const PagedKVStorage& storage,
                                   const std::vector<const SequenceState*>& sequences,
                                   const float* query_device, float* output_device,
                                   std::size_t query_heads);
 
 // The same over a refreshed device table, whose groups are found at the first
-// such call and stay: rows only ever append pages behind the whole ones.
+// such call that they could pay for and stay: rows only ever append pages behind
+// the whole ones.
 void paged_attention_batch_shared(const PagedKVStorage& storage, DeviceBatchTable& batch,
                                   const float* query_device, float* output_device,
                                   std::size_t query_heads);

@@ -245,13 +245,22 @@ int kvflux_paged_attention_noalloc(const void* key_cache, const void* value_cach
  * of any size, up to 2048 rows and 512 groups; K, V and the workspace aligned to 16
  * bytes. Other shapes, and calls whose bounds say that sharing cannot pay (few
  * rows more than groups, short prefixes), run as kvflux_paged_attention does,
- * bit for bit: max_prefix and kv_len decide that, so bounds that are far too
- * large choose the shared kernel where it does not pay.
+ * bit for bit. This entry knows no lengths: num_rows - num_groups times max_prefix
+ * stands for what is shared, so bounds that are far too large, or a long prefix of
+ * a few rows among many, choose the shared kernel where it does not pay. A caller
+ * who knows the groups asks kvflux_paged_attention_shared_pays first.
  * workspace: kvflux_paged_attention_shared_workspace_size bytes (no
  * initialisation needed; calls that share one must be ordered). */
 int kvflux_paged_attention_shared_workspace_size(uint64_t num_rows, uint64_t kv_len, uint64_t num_kv_heads,
                                                  uint64_t query_heads, uint64_t block_size, uint64_t head_size,
                                                  int dtype, uint64_t num_groups, size_t* bytes);
+/* kvflux_paged_attention_shared_pays: whether the shared kernel takes such a call
+ * and is the faster one for it. shared_tokens: the sum over the groups of (rows - 1)
+ * * prefix, the tokens that need not be read again. *pays 0: kvflux_paged_attention
+ * (and its workspace) serves the call better. Host arithmetic only. */
+int kvflux_paged_attention_shared_pays(uint64_t num_rows, uint64_t kv_len, uint64_t num_kv_heads,
+                                       uint64_t query_heads, uint64_t block_size, uint64_t head_size, int dtype,
+                                       uint64_t num_groups, uint64_t shared_tokens, int* pays);
 int kvflux_paged_attention_shared(const void* key_cache, const void* value_cache, uint64_t num_blocks,
                                   uint64_t num_kv_heads, uint64_t block_size, uint64_t head_size, int dtype,
                                   const uint64_t* block_table, uint64_t max_blocks_per_seq,

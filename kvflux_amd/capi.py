@@ -65,6 +65,8 @@ SIGNATURES = {
                                               _u64, _u64, _u64, _vp, _vp, _vp]),
     "kvflux_paged_attention_shared_workspace_size": (_i32, [_u64, _u64, _u64, _u64, _u64, _u64, _i32, _u64,
                                                             C.POINTER(C.c_size_t)]),
+    "kvflux_paged_attention_shared_pays": (_i32, [_u64, _u64, _u64, _u64, _u64, _u64, _i32, _u64, _u64,
+                                                  C.POINTER(C.c_int)]),
     "kvflux_paged_attention_shared": (_i32, [_vp, _vp, _u64, _u64, _u64, _u64, _i32, _vp, _u64, _vp, _u64, _u64, _u64,
                                              _vp, _vp, _u64, _u64, _vp, _vp, _vp, _sz, _vp]),
     "kvflux_paged_prefill": (_i32, [_vp, _vp, _u64, _u64, _u64, _u64, _i32, _vp, _u64, _u64,

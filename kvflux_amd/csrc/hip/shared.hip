@@ -1095,26 +1095,24 @@ bool can_take(std::uint64_t rows, std::uint64_t kv_len, std::uint64_t kv_heads, 
     return streams * (kv_len / 64 + 1) < (1ULL << 31) / (kMostTileCost + kPartCost);
 }
 
-// Whether sharing pays, as far as the host can know. An ordinary decode reads a
-// prefix again for every further row of its group, from L2, at about 9 MB a
-// microsecond; the shared kernel pays its plan and merge, about 5 us, and for every row
+// Whether sharing pays: `again` is the tokens that an ordinary decode reads again,
+// once for every further row of a group, from L2, at about 9 MB a microsecond; the
+// shared kernel pays its plan and merge, about 5 us, and for every row
 // and kv head a part of its own, of which a round of the workgroups takes about
 // 4.5 us more than the ordinary decode's items. Measured, shared and ordinary:
 // 17 rows in 2 groups behind 1500-2500 tokens, 28/4 heads of 128 (77 MB read again) 23.8
 // and 25.3 us; 27 in 2 behind up to 7061, 32/8 (723 MB) 25.1 and 35.9; 34 in 4 behind
 // 347, 24/8 (43 MB) 21.7 and 15.0; 116 in 11 behind 423, 24/8 (182 MB) 34.8 and 30.7; 60
 // in 3 behind 221, 40/8 heads of 64 (26 MB) 28.9 and 9.8.
-// The host knows no prefix but the longest, so groups of unequal sizes count for more
-// than they share. That costs little, an own part being read as fast either way: 2
-// rows behind 32768 tokens and 126 of U[1000, 32768], 32/8 heads of 128, 1470 and 1402
-// us; 2 behind 8192 and 126 of U[200, 6000] 302 and 309; 2 behind 8192 and 30 of U[50,
-// 300] 23.9 and 26.3.
-bool pays(std::uint64_t rows, std::uint64_t groups, std::uint64_t prefix, std::uint64_t kv_heads,
-          std::uint64_t head_size, int dtype) {
-    if (rows <= groups) return false;
-    const double again = static_cast<double>(rows - groups) * static_cast<double>(prefix) *
-                         static_cast<double>(2 * kv_heads * head_size * dtype_bytes(dtype));
-    return again > 9e6 * (5.0 + 4.5 * static_cast<double>(rows * kv_heads) / kWorkgroups);
+bool pays(std::uint64_t rows, double again, std::uint64_t kv_heads, std::uint64_t head_size, int dtype) {
+    return again * static_cast<double>(2 * kv_heads * head_size * dtype_bytes(dtype)) >
+           9e6 * (5.0 + 4.5 * static_cast<double>(rows * kv_heads) / kWorkgroups);
+}
+// What a caller of the attention's entry has read again at the most: every row but
+// one of a group behind the longest prefix.
+double most_again(std::uint64_t rows, std::uint64_t groups, std::uint64_t max_prefix, std::uint64_t kv_len) {
+    if (rows <= groups) return 0.0;
+    return static_cast<double>(rows - groups) * static_cast<double>(max_prefix < kv_len ? max_prefix : kv_len);
 }
 
 Layout layout_of(std::uint64_t rows, std::uint64_t kv_heads, std::uint64_t query_heads, std::uint64_t head_size,
@@ -1188,6 +1186,18 @@ extern "C" int kvflux_paged_attention_shared_workspace_size(uint64_t num_rows, u
     return KVFLUX_OK;
 }
 
+extern "C" int kvflux_paged_attention_shared_pays(uint64_t num_rows, uint64_t kv_len, uint64_t num_kv_heads,
+                                                  uint64_t query_heads, uint64_t block_size, uint64_t head_size,
+                                                  int dtype, uint64_t num_groups, uint64_t shared_tokens, int* result) {
+    if (!result) return fail(KVFLUX_ERR_INVALID_ARGUMENT, "pays is null");
+    *result = 0;
+    const int status = check_shape(num_kv_heads, block_size, head_size, dtype, query_heads);
+    if (status != KVFLUX_OK) return status;
+    *result = can_take(num_rows, kv_len, num_kv_heads, query_heads, block_size, head_size, dtype, num_groups) &&
+              pays(num_rows, static_cast<double>(shared_tokens), num_kv_heads, head_size, dtype);
+    return KVFLUX_OK;
+}
+
 extern "C" int kvflux_paged_attention_shared(const void* key_cache, const void* value_cache, uint64_t num_blocks,
                                              uint64_t num_kv_heads, uint64_t block_size, uint64_t head_size, int dtype,
                                              const uint64_t* block_table, uint64_t max_blocks_per_seq,
@@ -1205,7 +1215,7 @@ extern "C" int kvflux_paged_attention_shared(const void* key_cache, const void* 
     if (num_blocks == 0 || max_blocks_per_seq == 0)
         return fail(KVFLUX_ERR_INVALID_ARGUMENT, "shared attention: invalid shape");
     if (!can_take(num_rows, kv_len, num_kv_heads, query_heads, block_size, head_size, dtype, num_groups) ||
-        !pays(num_rows, num_groups, max_prefix < kv_len ? max_prefix : kv_len, num_kv_heads, head_size, dtype))
+        !pays(num_rows, most_again(num_rows, num_groups, max_prefix, kv_len), num_kv_heads, head_size, dtype))
         return kvflux_paged_attention(key_cache, value_cache, num_blocks, num_kv_heads, block_size, head_size, dtype,
                                       block_table, max_blocks_per_seq, seq_lens, kv_len, num_rows, query_heads, query,
                                       output, workspace, workspace_bytes, stream);

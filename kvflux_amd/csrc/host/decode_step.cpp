@@ -305,6 +305,7 @@ const DeviceBatchTable::Groups& DeviceBatchTable::enqueue_groups() {
         groups_.prefixes = reinterpret_cast<const std::uint64_t*>(dev + starts_bytes);
         groups_.count = found.groups();
         groups_.most = *std::max_element(found.prefixes.begin(), found.prefixes.end());
+        groups_.shared_tokens = detail::shared_tokens(found);
     }
     grouped_ = true;
     return groups_;
@@ -409,7 +410,8 @@ std::vector<TokenLocation> append_and_run(PagedKVStorage& storage, DeviceBatchTa
     return plan.locations;
 }
 
-// The attention's launch with the rows' shared prefixes computed once.
+// The attention's launch with the rows' shared prefixes computed once, where that
+// pays; the rows are not even grouped while nothing they could share would.
 void enqueue_shared_attention(const PagedKVStorage& storage, DeviceBatchTable& batch, const float* query,
                               float* output, std::size_t query_heads) {
     const auto& layout = storage.layout();
@@ -418,7 +420,13 @@ void enqueue_shared_attention(const PagedKVStorage& storage, DeviceBatchTable& b
         throw std::invalid_argument("invalid batch attention sequence");
     }
     const std::size_t max_len = *std::max_element(lengths.begin(), lengths.end());
+    if (!batch.grouped() && !detail::sharing_could_pay(storage, batch.rows(), max_len, query_heads)) {
+        return enqueue_batch_attention(storage, batch, query, output, query_heads);
+    }
     const auto& groups = batch.enqueue_groups();
+    if (!detail::sharing_pays(storage, batch.rows(), max_len, query_heads, groups.count, groups.shared_tokens)) {
+        return enqueue_batch_attention(storage, batch, query, output, query_heads);
+    }
     std::size_t ws_bytes = 0;
     void* ws = detail::shared_attention_workspace(storage, batch.rows(), max_len, query_heads, groups.count, &ws_bytes);
     check(kvflux_paged_attention_shared(storage.key_base(), storage.value_base(), layout.num_blocks(),

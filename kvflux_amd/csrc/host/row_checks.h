@@ -20,6 +20,16 @@ struct RowPages {
 // The grouping of neighbouring rows that shares the most tokens.
 SharedPrefixGroups group_rows(const std::vector<RowPages>& rows, std::size_t block_size);
 
+// Tokens that the groups' further rows need not have read again: the sum of
+// (rows - 1) * prefix.
+std::uint64_t shared_tokens(const SharedPrefixGroups& groups);
+
+// Whether the shared attention serves a batch better than the ordinary one; and
+// whether it could, whatever the rows (one at least) share.
+bool sharing_pays(const PagedKVStorage& storage, std::size_t rows, std::size_t kv_len, std::size_t query_heads,
+                  std::size_t groups, std::uint64_t shared_tokens);
+bool sharing_could_pay(const PagedKVStorage& storage, std::size_t rows, std::size_t kv_len, std::size_t query_heads);
+
 // Elements from one token of a projection to the next.
 struct ProjectionStrides {
     std::size_t query, key, value;

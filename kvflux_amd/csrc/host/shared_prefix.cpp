@@ -60,6 +60,30 @@ SharedPrefixGroups group_rows(const std::vector<RowPages>& rows, std::size_t blo
     return out;
 }
 
+std::uint64_t shared_tokens(const SharedPrefixGroups& groups) {
+    std::uint64_t sum = 0;
+    for (std::size_t g = 0; g < groups.groups(); ++g)
+        sum += (groups.starts[g + 1] - groups.starts[g] - 1) * groups.prefixes[g];
+    return sum;
+}
+
+bool sharing_pays(const PagedKVStorage& storage, std::size_t rows, std::size_t kv_len, std::size_t query_heads,
+                  std::size_t groups, std::uint64_t shared_tokens) {
+    const auto& layout = storage.layout();
+    int pays = 0;
+    check(kvflux_paged_attention_shared_pays(rows, kv_len, layout.num_kv_heads(), query_heads, layout.block_size(),
+                                             layout.head_size(), abi_dtype(layout.dtype()), groups, shared_tokens,
+                                             &pays),
+          "shared attention");
+    return pays != 0;
+}
+
+bool sharing_could_pay(const PagedKVStorage& storage, std::size_t rows, std::size_t kv_len, std::size_t query_heads) {
+    std::uint64_t most = 0;  // one group of all rows that is all prefix; an overflow is past what the kernel takes
+    return !__builtin_mul_overflow(static_cast<std::uint64_t>(rows - 1), static_cast<std::uint64_t>(kv_len), &most) &&
+           sharing_pays(storage, rows, kv_len, query_heads, 1, most);
+}
+
 } // namespace detail
 
 SharedPrefixGroups find_shared_prefixes(const std::vector<const SequenceState*>& sequences) {
@@ -108,26 +132,38 @@ void paged_attention_batch_shared(const PagedKVStorage& storage, const std::vect
     }
     const auto table_bytes = detail::mul_checked(batch.block_table().size(), sizeof(PhysicalBlockID),
                                                  "paged attention size overflow");
-    const auto groups = find_shared_prefixes(sequences);
+    const std::vector<std::uint64_t> lengths(batch.sequence_lengths().begin(), batch.sequence_lengths().end());
+    const auto max_len = *std::max_element(lengths.begin(), lengths.end());
+    SharedPrefixGroups groups;
+    if (detail::sharing_could_pay(storage, sequences.size(), max_len, query_heads)) groups = find_shared_prefixes(sequences);
+    const bool pays = detail::sharing_pays(storage, sequences.size(), max_len, query_heads, groups.groups(),
+                                           detail::shared_tokens(groups));
     detail::DeviceGuard guard(storage.device());
     detail::validate_q_o(storage, query_device, output_device, tensor_bytes);
-    const std::vector<std::uint64_t> lengths(batch.sequence_lengths().begin(), batch.sequence_lengths().end());
     const auto dev = storage.scratch().upload({{batch.block_table().data(), table_bytes},
                                                {lengths.data(), lengths.size() * 8},
                                                {groups.starts.data(), groups.starts.size() * 8},
                                                {groups.prefixes.data(), groups.prefixes.size() * 8}});
-    const auto max_len = *std::max_element(lengths.begin(), lengths.end());
-    const auto most = groups.groups() ? *std::max_element(groups.prefixes.begin(), groups.prefixes.end()) : 0;
     std::size_t ws_bytes = 0;
-    void* ws = detail::shared_attention_workspace(storage, sequences.size(), max_len, query_heads, groups.groups(),
-                                                  &ws_bytes);
-    detail::check(kvflux_paged_attention_shared(storage.key_base(), storage.value_base(), layout.num_blocks(),
-                                                layout.num_kv_heads(), layout.block_size(), layout.head_size(),
-                                                detail::abi_dtype(layout.dtype()), dev[0],
-                                                batch.max_blocks_per_sequence(), dev[1], max_len, sequences.size(),
-                                                query_heads, dev[2], dev[3], groups.groups(), most, query_device,
-                                                output_device, ws, ws_bytes, nullptr),
-                  "shared attention batch kernel launch");
+    if (pays) {
+        const auto most = *std::max_element(groups.prefixes.begin(), groups.prefixes.end());
+        void* ws = detail::shared_attention_workspace(storage, sequences.size(), max_len, query_heads, groups.groups(),
+                                                      &ws_bytes);
+        detail::check(kvflux_paged_attention_shared(
+                          storage.key_base(), storage.value_base(), layout.num_blocks(), layout.num_kv_heads(),
+                          layout.block_size(), layout.head_size(), detail::abi_dtype(layout.dtype()), dev[0],
+                          batch.max_blocks_per_sequence(), dev[1], max_len, sequences.size(), query_heads, dev[2],
+                          dev[3], groups.groups(), most, query_device, output_device, ws, ws_bytes, nullptr),
+                      "shared attention batch kernel launch");
+    } else {
+        void* ws = detail::attention_workspace(storage, sequences.size(), max_len, query_heads, &ws_bytes);
+        detail::check(kvflux_paged_attention(storage.key_base(), storage.value_base(), layout.num_blocks(),
+                                             layout.num_kv_heads(), layout.block_size(), layout.head_size(),
+                                             detail::abi_dtype(layout.dtype()), dev[0],
+                                             batch.max_blocks_per_sequence(), dev[1], max_len, sequences.size(),
+                                             query_heads, query_device, output_device, ws, ws_bytes, nullptr),
+                      "paged attention batch kernel launch");
+    }
     detail::check(kvflux_stream_synchronize(nullptr), "paged attention batch synchronize");
 }
 
