@@ -103,8 +103,8 @@ struct SharedParams {
     float scale_log2;            // log2(e) / sqrt(D)
     // Workspace: the rows' plans for the merge, partials.
     struct RowPlan* plans;
-    float* prefix_acc;  // [slot][kCols][D]
-    float* prefix_ml;   // [slot][kCols][2]
+    float* prefix_acc;  // [prefix_place][D]
+    float* prefix_ml;   // [prefix_place][2]
     float* row_acc;     // [slot][row_cols][D]
     float* row_ml;      // [slot][row_cols][2]
     std::uint32_t row_cols;   // min(group, kCols)
@@ -114,7 +114,7 @@ struct SharedParams {
 // What the merge needs of a row.
 struct RowPlan {
     std::uint32_t prefix_cost, own_cost;  // costs before the segments
-    std::uint32_t prefix_tiles, prefix_weight, prefix_col_tiles, prefix_stream;
+    std::uint32_t prefix_tiles, prefix_weight, prefix_cols;
     std::uint32_t first_row, own_tiles, own_weight, total;
 };
 
@@ -176,10 +176,13 @@ __device__ inline std::uint32_t group_of(const std::uint32_t* first, std::uint32
     return first[lo] <= row && row < first[lo + 1] ? lo : groups;
 }
 
-// Stream numbers before a group's: every group may end in a started tile of
-// columns, so group + floor(columns of the rows before it / kCols).
-__device__ inline std::uint32_t group_stream(const SharedParams& p, std::uint32_t g, std::uint32_t first_row) {
-    return (g + first_row * p.group.divisor / kCols) * p.heads;
+// Where workgroup w's partials of a prefix's stream go, in columns: its columns lie
+// behind those of all streams before it (the groups' in order, a group's kv heads
+// in order), and another kCols on for every workgroup. Streams are taken up in that
+// order, so no two parts meet.
+__device__ inline std::uint32_t prefix_place(const SharedParams& p, std::uint32_t first_row, std::uint32_t cols,
+                                             std::uint32_t kvh, std::uint32_t col, std::uint32_t w) {
+    return first_row * p.query_heads + kvh * cols + col + w * kCols;
 }
 
 // Where the share of workgroup w begins, ceil(total * w / kWorkgroups), in 32 bits.
@@ -341,15 +344,14 @@ __global__ __launch_bounds__(kThreads) void shared_attention_kernel(SharedParams
     if (w == 0) {  // uniform: the rows' plans for the merge
         for (std::uint32_t r = tid; r < p.rows; r += kThreads) {
             const Segment own = segment(p.groups + r);
-            RowPlan plan{0, cost_of[p.groups + r], 0, 0, 1, 0, 0, own.tiles, own.weight, total};
+            RowPlan plan{0, cost_of[p.groups + r], 0, 0, 0, 0, own.tiles, own.weight, total};
             if (own.begin != 0) {
                 const std::uint32_t g = group_of(first_of, p.groups, r);
                 const Segment prefix = segment(g);
                 plan.prefix_cost = cost_of[g];
                 plan.prefix_tiles = prefix.tiles;
                 plan.prefix_weight = prefix.weight;
-                plan.prefix_col_tiles = prefix.col_tiles;
-                plan.prefix_stream = group_stream(p, g, prefix.first_row);
+                plan.prefix_cols = prefix.cols;
                 plan.first_row = prefix.first_row;
             }
             p.plans[r] = plan;
@@ -835,9 +837,10 @@ __global__ __launch_bounds__(kThreads) void shared_attention_kernel(SharedParams
         // tokens (through the buffer just computed), then to the workspace.
         new_part = true;
         const bool is_prefix = cur.seg < p.groups;
-        const std::uint32_t slot_of_part = (is_prefix ? group_stream(p, cur.seg, cur.s.first_row)
-                                                      : (cur.seg - p.groups) * p.heads * p.row_tiles) +
-                                           cur.kvh * cur.s.col_tiles + cur.col_tile + w;
+        // Its first column's place: a row's streams are numbered, row_cols columns each.
+        const std::uint32_t place_of_part =
+            is_prefix ? prefix_place(p, cur.s.first_row, cur.s.cols, cur.kvh, cur.col_tile * kCols, w)
+                      : (((cur.seg - p.groups) * p.heads + cur.kvh) * p.row_tiles + cur.col_tile + w) * p.row_cols;
         float sum[kBlocks], top[kBlocks];
 #pragma unroll
         for (int n = 0; n < kBlocks; ++n) {
@@ -893,7 +896,7 @@ __global__ __launch_bounds__(kThreads) void shared_attention_kernel(SharedParams
             for (int n = 0; n < kBlocks; ++n) {
                 const std::uint32_t mine = first_col + 16 * n + col;
                 if (n >= static_cast<int>(blocks) || mine >= cols) continue;
-                const std::uint64_t at = static_cast<std::uint64_t>(slot_of_part) * (is_prefix ? kCols : p.row_cols) + mine;
+                const std::uint64_t at = place_of_part + mine;
                 float* out = (is_prefix ? p.prefix_acc : p.row_acc) + at * kD;
                 if (quad == 0)
                     *reinterpret_cast<float2*>((is_prefix ? p.prefix_ml : p.row_ml) + 2 * at) = make_float2(top[n], sum[n]);
@@ -951,13 +954,15 @@ __global__ __launch_bounds__(kMergeThreads) void shared_merge_kernel(SharedParam
         const bool of_prefix = which == 0;
         const std::uint32_t kvh = p.group.div(head), g = head - kvh * p.group.divisor;
         const std::uint32_t c = of_prefix ? (row - plan.first_row) * p.group.divisor + g : g;  // column
-        const std::uint32_t stream = kvh * (of_prefix ? plan.prefix_col_tiles : p.row_tiles) + c / kCols;
+        const std::uint32_t stream =
+            kvh * (of_prefix ? (plan.prefix_cols + kCols - 1) / kCols : p.row_tiles) + c / kCols;
         Stream s;
         s.tiles = of_prefix ? plan.prefix_tiles : plan.own_tiles;
         s.weight = of_prefix ? plan.prefix_weight : plan.own_weight;
         s.cost = (of_prefix ? plan.prefix_cost : plan.own_cost) + stream * (s.tiles * s.weight + kPartCost);
         s.step = of_prefix ? kCols : p.row_cols;
-        s.slot = ((of_prefix ? plan.prefix_stream : row * p.heads * p.row_tiles) + stream) * s.step + c % kCols;
+        s.slot = of_prefix ? prefix_place(p, plan.first_row, plan.prefix_cols, kvh, c, 0)
+                           : (row * p.heads * p.row_tiles + stream) * p.row_cols + c % kCols;
         // The workgroup in whose share a cost lies: a guess in FP32, put right.
         const float per_cost = static_cast<float>(kWorkgroups) / static_cast<float>(total);
         const auto owner = [&](std::uint32_t at) {
@@ -1115,17 +1120,16 @@ double most_again(std::uint64_t rows, std::uint64_t groups, std::uint64_t max_pr
     return static_cast<double>(rows - groups) * static_cast<double>(max_prefix < kv_len ? max_prefix : kv_len);
 }
 
-Layout layout_of(std::uint64_t rows, std::uint64_t kv_heads, std::uint64_t query_heads, std::uint64_t head_size,
-                 std::uint64_t groups) {
+Layout layout_of(std::uint64_t rows, std::uint64_t kv_heads, std::uint64_t query_heads, std::uint64_t head_size) {
     const auto whole = [](std::uint64_t bytes) { return (bytes + 255) & ~std::uint64_t{255}; };
     const std::uint64_t group = query_heads / kv_heads;
-    const std::uint64_t prefix_slots = (groups + rows * group / kCols) * kv_heads + kWorkgroups;
+    const std::uint64_t prefix_columns = rows * query_heads + kWorkgroups * kCols;
     const std::uint64_t row_slots = rows * kv_heads * ((group + kCols - 1) / kCols) + kWorkgroups;
     const std::uint64_t row_cols = group < kCols ? group : kCols;
     Layout l;
     l.prefix_acc = whole(rows * sizeof(RowPlan));  // the plans come first
-    l.prefix_ml = l.prefix_acc + whole(prefix_slots * kCols * head_size * sizeof(float));
-    l.row_acc = l.prefix_ml + whole(prefix_slots * kCols * 2 * sizeof(float));
+    l.prefix_ml = l.prefix_acc + whole(prefix_columns * head_size * sizeof(float));
+    l.row_acc = l.prefix_ml + whole(prefix_columns * 2 * sizeof(float));
     l.row_ml = l.row_acc + whole(row_slots * row_cols * head_size * sizeof(float));
     l.bytes = l.row_ml + whole(row_slots * row_cols * 2 * sizeof(float));
     return l;
@@ -1180,7 +1184,7 @@ extern "C" int kvflux_paged_attention_shared_workspace_size(uint64_t num_rows, u
     status = kvflux_paged_attention_workspace_size(num_rows, kv_len, num_kv_heads, query_heads, block_size, head_size, bytes);
     if (status != KVFLUX_OK) return status;
     if (can_take(num_rows, kv_len, num_kv_heads, query_heads, block_size, head_size, dtype, num_groups)) {
-        const std::uint64_t need = layout_of(num_rows, num_kv_heads, query_heads, head_size, num_groups).bytes;
+        const std::uint64_t need = layout_of(num_rows, num_kv_heads, query_heads, head_size).bytes;
         if (need > *bytes) *bytes = need;
     }
     return KVFLUX_OK;
@@ -1219,7 +1223,7 @@ extern "C" int kvflux_paged_attention_shared(const void* key_cache, const void* 
         return kvflux_paged_attention(key_cache, value_cache, num_blocks, num_kv_heads, block_size, head_size, dtype,
                                       block_table, max_blocks_per_seq, seq_lens, kv_len, num_rows, query_heads, query,
                                       output, workspace, workspace_bytes, stream);
-    const Layout l = layout_of(num_rows, num_kv_heads, query_heads, head_size, num_groups);
+    const Layout l = layout_of(num_rows, num_kv_heads, query_heads, head_size);
     if (!workspace || workspace_bytes < l.bytes)
         return fail(KVFLUX_ERR_INVALID_ARGUMENT, "shared attention: workspace needs %llu bytes",
                     static_cast<unsigned long long>(l.bytes));

@@ -48,6 +48,18 @@ def test_refusals():
         assert fn(*bad, 1, 10 ** 9, C.byref(out)) == capi.ERR_INVALID and out.value == 0
 
 
+def test_workspace_holds_the_columns_there_are():
+    """Partials of every row and query head once for the prefix and once for the row's own tokens, and of 256 workgroups'
+    128 columns more for each, whatever the number of groups (2000 rows in 512 groups, 32/32 heads of 128: 84 MB)."""
+    for rows, groups, H, Hq, D in ((2000, 512, 32, 32, 128), (2048, 1, 8, 64, 256), (64, 1, 8, 32, 128), (3, 2, 1, 300, 64)):
+        size = C.c_size_t()
+        capi.call("kvflux_paged_attention_shared_workspace_size", rows, 200, H, Hq, 16, D, capi.DTYPE_BF16, groups,
+                  C.byref(size))
+        tiles = -(-Hq // H // 128) * min(Hq // H, 128) * H  # a row's own columns, in whole streams
+        most = (rows * Hq + rows * tiles + 2 * 256 * 128) * (D + 2) * 4 + rows * 64 + 5 * 256
+        assert 0 < size.value <= most
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("sharers", [2, 63])
 def test_batches_with_few_and_many_sharers(gpu, v2, sharers):
