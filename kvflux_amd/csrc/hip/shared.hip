@@ -57,6 +57,9 @@ struct Shape {
     // would not have a step of the tile's tokens each.
     static constexpr std::uint32_t kLeastAcross = kSteps >= kWaves ? 1 : kWaves / kSteps;
     static constexpr int kLoads = kBufferBytes / 2 / (kThreads * 16);  // loads of a thread, K and V each
+    // spread_of doubles the wavefronts side by side until they hold a stream's
+    // columns: more of them than there are would leave no shares of a tile.
+    static_assert(kCols <= 16 * kWaves && kLeastAcross <= kWaves && (kWaves & (kWaves - 1)) == 0, "columns of a stream");
 };
 
 // How the wavefronts take a stream of `cols` columns: `across` of them side by
