@@ -1129,19 +1129,24 @@ __global__ __launch_bounds__(kThreads, (bs16_occupancy_g<E, kD, kG, kSmall>())) 
         // O^T += V^T P^T over tokens: MFMA kk takes token 4 * quad + kk in
         // lane (quad, col), the weight the lane holds in pr[kk]; block dt of
         // O^T is dims 64 * (dt / 4) + 4 * i + dt % 4, i = 0..15. V rows of
-        // tokens past the end read as zero (0 * NaN would poison P*V).
+        // tokens past the end read as zero (0 * NaN would poison P*V). The tile's
+        // products are summed from zero and added with one rounding: one MFMA at
+        // a time on an accumulator that holds a dominant key's, thousands of weights
+        // of 2^-25 lost 2e-5 (3e-6 so, at the same time).
 #pragma unroll
-        for (int kk = 0; kk < 4; ++kk) {
-            const bool live = static_cast<std::uint32_t>(4 * quad + kk) < valid;
+        for (int mm = 0; mm < kD / 64; ++mm) {
+            f32x4_t o[4] = {};
 #pragma unroll
-            for (int mm = 0; mm < kD / 64; ++mm) {
+            for (int kk = 0; kk < 4; ++kk) {
+                const bool live = static_cast<std::uint32_t>(4 * quad + kk) < valid;
                 const uint4 w = b.v[kk * (kD / 64) + mm];
                 const float vx[4] = {live ? __uint_as_float(w.x) : 0.0f, live ? __uint_as_float(w.y) : 0.0f,
                                      live ? __uint_as_float(w.z) : 0.0f, live ? __uint_as_float(w.w) : 0.0f};
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    acc[0][4 * mm + j] = __builtin_amdgcn_mfma_f32_16x16x4f32(vx[j], pr[kk], acc[0][4 * mm + j], 0, 0, 0);
+                for (int j = 0; j < 4; ++j) o[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(vx[j], pr[kk], o[j], 0, 0, 0);
             }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) acc[0][4 * mm + j] += o[j];
         }
     };
 
