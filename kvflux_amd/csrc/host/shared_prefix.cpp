@@ -24,18 +24,33 @@ SharedPrefixGroups group_rows(const std::vector<RowPages>& rows, std::size_t blo
         while (k < most && rows[r].ids[k] == rows[r + 1].ids[k]) ++k;
         common[r] = k;
     }
-    // best[r]: pages not computed again in rows [0, r) under their best grouping,
-    // whose last segment starts at from[r]. A row that shares nothing with the one
+    // A cut between two rows of a run of equal `common` gains nothing over one at the
+    // run's end: moved by a row, one segment wins what it shares and the other loses
+    // what it does, until one of them is past the run. So segments start only next to
+    // where `common` changes: the work grows with those places, not with the rows
+    // (2048 rows behind one prefix: 1.1 ms otherwise).
+    std::vector<std::size_t> at{0};
+    for (std::size_t r = 1; r < n; ++r) {
+        const bool inside = r >= 2 && r + 1 < n && common[r - 2] == common[r - 1] && common[r - 1] == common[r];
+        if (!inside) at.push_back(r);
+    }
+    if (n != 0) at.push_back(n);
+    // best[i]: pages not computed again in rows [0, at[i]) under their best grouping,
+    // whose last segment starts at at[from[i]]. A row that shares nothing with the one
     // before it starts a segment, so a segment never reaches across such a place.
-    std::vector<std::size_t> best(n + 1, 0), from(n + 1, 0);
-    for (std::size_t end = 1; end <= n; ++end) {
+    std::vector<std::size_t> best(at.size(), 0), from(at.size(), 0);
+    for (std::size_t end = 1; end < at.size(); ++end) {
         best[end] = best[end - 1];
         from[end] = end - 1;
         std::size_t least = static_cast<std::size_t>(-1);
-        for (std::size_t begin = end - 1; begin-- > 0;) {
-            least = std::min(least, common[begin]);
+        for (std::size_t begin = end; begin-- > 0;) {
+            // The rows at[begin] .. at[begin + 1] join: what they have in common, and
+            // with the rows behind them.
+            if (at[begin] + 1 < at[begin + 1]) least = std::min(least, common[at[begin]]);
+            if (begin + 1 != end) least = std::min(least, common[at[begin + 1] - 1]);
             if (least == 0) break;
-            const std::size_t saved = best[begin] + (end - begin - 1) * least;
+            const std::size_t rows_saved = at[end] - at[begin] - 1;
+            const std::size_t saved = best[begin] + (rows_saved != 0 ? rows_saved * least : 0);
             if (saved > best[end]) {
                 best[end] = saved;
                 from[end] = begin;
@@ -43,9 +58,9 @@ SharedPrefixGroups group_rows(const std::vector<RowPages>& rows, std::size_t blo
         }
     }
     SharedPrefixGroups out;
-    if (n == 0 || best[n] == 0) return out;
+    if (best.back() == 0) return out;
     std::vector<std::size_t> cuts;
-    for (std::size_t at = n; at != 0; at = from[at]) cuts.push_back(from[at]);
+    for (std::size_t i = at.size() - 1; i != 0; i = from[i]) cuts.push_back(at[from[i]]);
     std::reverse(cuts.begin(), cuts.end());
     for (std::size_t g = 0; g < cuts.size(); ++g) {
         const std::size_t begin = cuts[g], end = g + 1 < cuts.size() ? cuts[g + 1] : n;
