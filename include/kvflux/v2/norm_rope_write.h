@@ -44,7 +44,7 @@ struct NormRope {
 // Token n, at positions[n], goes to slot_mapping[n]; its query to query_out
 // (device float [tokens][query_heads][head_size], as the attention takes it).
 // Checks and exceptions as write_paged_kv; positions and slots differing in
-// number, a query head count that is no multiple of the kv heads, a stride below
+// number, a position of 2^53 or more, a query head count that is no multiple of the kv heads, a stride below
 // a token's heads, an odd rotary_dim or one above head_size, a negative eps,
 // misaligned arrays, or query_out overlapping the inputs or the cache:
 // std::invalid_argument. A head_size above 512, or 2^26 heads of all tokens:

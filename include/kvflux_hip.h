@@ -249,8 +249,10 @@ int kvflux_paged_attention_noalloc(const void* key_cache, const void* value_cach
  * stands for what is shared, so bounds that are far too large, or a long prefix of
  * a few rows among many, choose the shared kernel where it does not pay. A caller
  * who knows the groups asks kvflux_paged_attention_shared_pays first.
- * workspace: kvflux_paged_attention_shared_workspace_size bytes (no
- * initialisation needed; calls that share one must be ordered). */
+ * workspace: kvflux_paged_attention_shared_workspace_size bytes for the call's own
+ * arguments (no initialisation needed; calls that share one must be ordered). More
+ * than 2048 rows or 512 groups need none of the shared kernel's, so one sized for
+ * them may be too small for a smaller call, which then fails. */
 int kvflux_paged_attention_shared_workspace_size(uint64_t num_rows, uint64_t kv_len, uint64_t num_kv_heads,
                                                  uint64_t query_heads, uint64_t block_size, uint64_t head_size,
                                                  int dtype, uint64_t num_groups, size_t* bytes);

@@ -168,6 +168,9 @@ void norm_rope_write(PagedKVStorage& storage, const ProjectedRows& rows, const N
     if (positions.size() != slot_mapping.size()) {
         throw std::invalid_argument("as many positions as slots are required");
     }
+    for (const auto position : positions) {  // past that an angle is another position's
+        if (position >> 53 != 0) throw std::invalid_argument("a position is 2^53 or more");
+    }
     if (slot_mapping.empty()) return;
     const auto& layout = storage.layout();
     validate_slots(layout, slot_mapping, storage.scratch().seen_slots);

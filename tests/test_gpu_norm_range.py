@@ -70,3 +70,21 @@ def test_one_large_value(gpu, monkeypatch, D, rotary, shift):
         slots = nrw.slots_for(rng, c)
         c.listed([3, 4], slots)
         c.check([3, 4], slots)
+
+
+@pytest.mark.gpu
+def test_positions_past_the_angles(gpu, v2):
+    """2^53 and more have no exact FP64 value: refused, nothing written; the last that has one is taken."""
+    from gpu_util import read_cache
+    from test_gpu_projected_step import Model, filled
+    rng = np.random.default_rng(53)
+    pool, storage = filled(v2, "BFloat16", 2, 64, 16, 3, 9)
+    model = Model(rng, "BFloat16", 4, 2, 64, 64, False)
+    rows, form, q = model.project(v2, rng, 2), model.form(v2), nrw.device.DeviceBuffer(2 * 4 * 64 * 4)
+    before = [x.copy() for x in read_cache(storage, "BFloat16")]
+    for bad in (2 ** 53, 2 ** 64 - 1):
+        with pytest.raises(ValueError):
+            v2.norm_rope_write(storage, rows, form, 4, [0, bad], [0, 1], q.ptr)
+    assert all(np.array_equal(a, b) for a, b in zip(before, read_cache(storage, "BFloat16")))
+    v2.norm_rope_write(storage, rows, form, 4, [0, 2 ** 53 - 1], [0, 1], q.ptr)
+    assert np.isfinite(q.download(np.float32)).all()
