@@ -150,7 +150,14 @@ void paged_attention_batch_shared(const PagedKVStorage& storage, const std::vect
     const std::vector<std::uint64_t> lengths(batch.sequence_lengths().begin(), batch.sequence_lengths().end());
     const auto max_len = *std::max_element(lengths.begin(), lengths.end());
     SharedPrefixGroups groups;
-    if (detail::sharing_could_pay(storage, sequences.size(), max_len, query_heads)) groups = find_shared_prefixes(sequences);
+    if (detail::sharing_could_pay(storage, sequences.size(), max_len, query_heads)) {
+        std::vector<detail::RowPages> rows(sequences.size());
+        for (std::size_t r = 0; r < rows.size(); ++r) {
+            rows[r] = {reinterpret_cast<const std::uint64_t*>(batch.block_table().data()) + r * batch.max_blocks_per_sequence(),
+                       lengths[r] / layout.block_size()};
+        }
+        groups = detail::group_rows(rows, layout.block_size());
+    }
     const bool pays = detail::sharing_pays(storage, sequences.size(), max_len, query_heads, groups.groups(),
                                            detail::shared_tokens(groups));
     detail::DeviceGuard guard(storage.device());
