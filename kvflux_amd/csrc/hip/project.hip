@@ -184,8 +184,8 @@ __device__ inline Four<E> narrow(const float (&x)[4]) {
 // loads are in flight.
 //
 // Bound: HBM, and the launch below about 300 tokens. BF16, 32/8 heads of 128, MI355X:
-// 4096 tokens (134 MB) 22.2 us, 6.05 TB/s; 64/8 heads, 16384 tokens (940 MB)
-// 158 us, 5.95 TB/s; 64 tokens 4.2 us. What it took:
+// 4096 tokens (134 MB) 22 to 25 us, 5.4 to 6.05 TB/s; 64/8 heads, 16384 tokens (940 MB)
+// 159 us, 5.9 TB/s; 64 tokens 4.2 us. What it took:
 //  * a wavefront a row, a sincos a value: 120 and 775 us;
 //  * this layout, with the slot's page found by each row: 46 and 270 us, about 500
 //    instructions a row, the divisions the larger part; found once a token: 30 and 168;
@@ -351,7 +351,9 @@ __global__ __launch_bounds__(kThreads) void norm_rope_write_kernel(Params p, Pla
 }
 
 // One wavefront a row; any head size up to kMaxHead, any even rotation, any
-// alignment.
+// alignment. Bound by its instructions, a sincos a value among them: 4096 tokens of
+// 32/8 heads of 80, 20 dims rotated, 81 us, 1.0 TB/s; heads of 128 an element off
+// their alignment 94 us.
 template <typename In, typename Cache, typename Place>
 __global__ __launch_bounds__(64) void norm_rope_write_generic_kernel(Params p, Place place) {
     constexpr int kPer = static_cast<int>(kMaxHead) / 64;
