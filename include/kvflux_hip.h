@@ -152,7 +152,8 @@ int kvflux_gather_paged_kv_live(const void* key_cache, const void* value_cache,
  *   seq_lens == NULL: every row uses table row 0 and row r attends to tokens
  *                     [0, kv_len - num_rows + r] (causal trailing queries of one
  *                     sequence, reference paged_attention.cu:123).
- * scale = 1/sqrt(head_size). query_heads % num_kv_heads == 0.
+ * scale = 1/sqrt(head_size). query_heads % num_kv_heads == 0. FP16 caches:
+ *   queries of up to 2^20 * sqrt(head_size) / log2(e).
  * workspace: device scratch of at least kvflux_paged_attention_workspace_size()
  *   bytes (no initialisation needed). Calls that share a workspace must be
  *   ordered (same stream).
