@@ -1020,12 +1020,25 @@ __global__ __launch_bounds__(kThreads, (bs16_occupancy_g<E, kD, kG, kSmall>())) 
             b.v[i] = stream_load(reinterpret_cast<const uint4*>(vb));
         }
     };
-    // Leading valid pages of tile jt (small pages): those before the tile's
-    // first missing page slot, from a wave-wide ballot of missing slots.
-    auto leading_pages = [&](std::uint64_t missing, std::uint32_t jt) -> std::uint32_t {
-        const std::uint32_t n = 1u << tps;
-        const std::uint64_t bits = (missing >> (jt << tps)) & ((n == 64 ? ~0ULL : (1ULL << n) - 1));
-        return bits ? static_cast<std::uint32_t>(__builtin_ctzll(bits)) : n;
+    // The tokens of a tile that count: how many lead it, or a bit for each where
+    // pages are smaller than a tile and a missing one can lie between others.
+    const auto is_whole = [](std::uint32_t valid) { return kSmall ? valid == 0xffffu : valid >= kBs; };
+    const auto counts = [](std::uint32_t token, std::uint32_t valid) {
+        return kSmall ? (valid >> token & 1u) != 0 : token < valid;
+    };
+    // The first n tokens of tile jt but for its missing pages, from a wave-wide
+    // ballot of missing page slots.
+    auto present = [&](std::uint64_t missing, std::uint32_t jt, std::uint32_t n) -> std::uint32_t {
+        std::uint32_t tokens = (1u << n) - 1;
+        // Missing pages among those that hold the n tokens (those behind matter to none).
+        std::uint32_t pages = static_cast<std::uint32_t>(missing >> (jt << tps)) &
+                              ((1u << ((n + (1u << bs_shift) - 1) >> bs_shift)) - 1);
+        while (pages != 0) {  // uniform
+            const std::uint32_t k = static_cast<std::uint32_t>(__builtin_ctz(pages));
+            tokens &= ~(((1u << (1u << bs_shift)) - 1) << (k << bs_shift));
+            pages &= pages - 1;
+        }
+        return tokens;
     };
 
     // run_max is a reference point, not always the exact maximum: it only
@@ -1073,10 +1086,10 @@ __global__ __launch_bounds__(kThreads, (bs16_occupancy_g<E, kD, kG, kSmall>())) 
         } else {
 #pragma unroll
             for (int i = 0; i < kVLoads; ++i) *reinterpret_cast<uint4*>(my_tile + v_store[i]) = b.v[i];
-            if (valid < kBs) {  // rows past the end read as zero (0 * NaN would poison P*V)
+            if (!is_whole(valid)) {  // tokens past the end read as zero (0 * NaN would poison P*V)
 #pragma unroll
                 for (int i = 0; i < kVLoads; ++i) {
-                    if (static_cast<std::uint32_t>(lane / kCpr + i * kRowStep) >= valid)
+                    if (!counts(static_cast<std::uint32_t>(lane / kCpr + i * kRowStep), valid))
                         *reinterpret_cast<uint4*>(my_tile + v_store[i]) = make_uint4(0, 0, 0, 0);
                 }
             }
@@ -1102,7 +1115,7 @@ __global__ __launch_bounds__(kThreads, (bs16_occupancy_g<E, kD, kG, kSmall>())) 
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
             sc[r] = in.s0[r];
-            if (valid < kBs && static_cast<std::uint32_t>(quad * 4 + r) >= valid) sc[r] = -INFINITY;
+            if (!is_whole(valid) && !counts(static_cast<std::uint32_t>(quad * 4 + r), valid)) sc[r] = -INFINITY;
         }
         float tmax = fmaxf(fmaxf(sc[0], sc[1]), fmaxf(sc[2], sc[3]));
         tmax = fmaxf(tmax, swizzle_xor16(tmax));
@@ -1138,7 +1151,7 @@ __global__ __launch_bounds__(kThreads, (bs16_occupancy_g<E, kD, kG, kSmall>())) 
             f32x4_t o[4] = {};
 #pragma unroll
             for (int kk = 0; kk < 4; ++kk) {
-                const bool live = static_cast<std::uint32_t>(4 * quad + kk) < valid;
+                const bool live = counts(static_cast<std::uint32_t>(4 * quad + kk), valid);
                 const uint4 w = b.v[kk * (kD / 64) + mm];
                 const float vx[4] = {live ? __uint_as_float(w.x) : 0.0f, live ? __uint_as_float(w.y) : 0.0f,
                                      live ? __uint_as_float(w.z) : 0.0f, live ? __uint_as_float(w.w) : 0.0f};
@@ -1170,7 +1183,7 @@ __global__ __launch_bounds__(kThreads, (bs16_occupancy_g<E, kD, kG, kSmall>())) 
                     sc[r] = fmaf(lo, 1.0f / M::kUp[2], fmaf(mid, 1.0f / M::kUp[1], in.s0[r] * (1.0f / M::kUp[0])));
                 else
                     sc[r] = in.s0[r] + mid + lo;
-                if (valid < kBs && static_cast<std::uint32_t>(quad * 4 + r) >= valid) sc[r] = -INFINITY;
+                if (!is_whole(valid) && !counts(static_cast<std::uint32_t>(quad * 4 + r), valid)) sc[r] = -INFINITY;
             }
             float tmax = fmaxf(fmaxf(sc[0], sc[1]), fmaxf(sc[2], sc[3]));
             tmax = fmaxf(tmax, swizzle_xor16(tmax));
@@ -1316,8 +1329,7 @@ __global__ __launch_bounds__(kThreads, (bs16_occupancy_g<E, kD, kG, kSmall>())) 
             const std::uint32_t begin = t * kBs;
             const std::uint32_t n = cur.ntok > begin ? (cur.ntok - begin < kBs ? cur.ntok - begin : kBs) : 0u;
             if constexpr (kSmall) {
-                const std::uint32_t ok = leading_pages(cur_missing, static_cast<std::uint32_t>(j)) << bs_shift;
-                return n < ok ? n : ok;
+                return present(cur_missing, static_cast<std::uint32_t>(j), n);
             } else {
                 return page_of(cur_pages, j) == kNoPage ? 0u : n;
             }
