@@ -242,7 +242,14 @@ __global__ __launch_bounds__(kThreads, 2) void paged_attention_split_kernel(Para
     const std::uint32_t kvh = blockIdx.y % p.heads;
     const std::uint64_t len = row_length(p, row);
     const std::uint64_t tok_begin = static_cast<std::uint64_t>(chunk) * kChunk;
-    if (tok_begin >= len) return;
+    if (tok_begin >= len) {
+        // A row without tokens gives zeros, as in the other kernels.
+        if (len == 0 && chunk == 0) {
+            float* out = p.output + (static_cast<std::uint64_t>(row) * p.query_heads + kvh * p.q_group + p.q_first) * kD;
+            for (int i = threadIdx.x; i < kG * kD; i += kThreads) out[i] = 0.0f;
+        }
+        return;
+    }
     const std::uint64_t tok_end = len - tok_begin > kChunk ? tok_begin + kChunk : len;
     const std::uint32_t ntok = static_cast<std::uint32_t>(tok_end - tok_begin);
     const std::uint32_t bs = p.block_size.divisor;
