@@ -42,6 +42,9 @@ enum kvflux_status {
 /* Same values as kvflux::DType (reference include/kvflux/kv_layout.h:7). */
 enum kvflux_dtype { KVFLUX_DTYPE_F16 = 0, KVFLUX_DTYPE_BF16 = 1, KVFLUX_DTYPE_F32 = 2 };
 
+/* What a value of an 8-bit cache is held as (kvflux_quant_* below). */
+enum kvflux_quant_format { KVFLUX_QUANT_E4M3 = 0, KVFLUX_QUANT_INT8 = 1 };
+
 /* Message of the last failing call on this thread ("" if none). */
 const char* kvflux_last_error(void);
 int kvflux_abi_version(void);
@@ -465,6 +468,69 @@ int kvflux_norm_rope_write_tail(void* key_cache, void* value_cache, uint64_t num
                                 uint64_t rotary_dim, int interleaved, const uint64_t* block_table,
                                 uint64_t table_width, const uint64_t* seq_lens, uint64_t num_rows,
                                 float* query_out, void* stream);
+
+/* ---------------------------------------------------------------------------
+ * The paged cache in 8 bits, a scale for each page and kv head. No counterpart
+ * in the reference, whose caches hold 16 or 32 bits a value
+ * (include/kvflux/v2/paged_kv_layout.h:12-40); the calls are those of hot paths
+ * 1, 2, 3a and 3b on such a cache.
+ *
+ * Layout: key_cache and value_cache [num_blocks][num_kv_heads][block_size]
+ *   [head_size] bytes, key_scales and value_scales float [num_blocks]
+ *   [num_kv_heads]. A value is its byte's value times its page's scale:
+ *   KVFLUX_QUANT_E4M3  8-bit floats (sign, 4 exponent bits, 3 mantissa bits, up
+ *                      to 448; 0x7f and 0xff are NaN)
+ *   KVFLUX_QUANT_INT8  integers; the writes give -127 to 127
+ *   Half the bytes of a 16-bit cache and 8 for each page and kv head. Pages are
+ *   copied (kvflux_copy_pages) with their scales: the same call on the scale
+ *   arrays, with page_bytes = num_kv_heads * 4.
+ *
+ * kvflux_quant_write: the last new_lens[i] of kv_lens[i] tokens of every sequence
+ *   i (device uint64 [num_seqs]), from rows new_offsets[i] .. of key_new and
+ *   value_new, into their places by table row i (device uint64 [num_seqs]
+ *   [table_width]): the metadata that kvflux_quant_prefill takes for the same
+ *   step. max_new_tokens bounds every new_lens[i] (tokens past it, counted from
+ *   the first, are not written). Rows are [num_kv_heads][head_size] of
+ *   `input_dtype`, key_stride and value_stride elements from one token to the
+ *   next. Two sequences of a call must not write to the same page.
+ * kvflux_quant_write_tail: one token a row, input row r at position seq_lens[r] -
+ *   1 of table row r (as kvflux_write_paged_kv_tail).
+ *   The scale of a page and head is the smallest power of two, 2^-110 at least,
+ *   that brings the largest magnitude among the new values to 448 or 127, or, if
+ *   the page has earlier tokens (of positions before the first new one), the
+ *   page's scale if that is larger. Values are divided by it (exactly) and rounded
+ *   to nearest, ties to even. Where it grows, the earlier tokens are rounded again
+ *   to it: exactly for E4M3 except for what falls below 2^-6 of the scale. Scales of
+ *   another origin stay as they are until they grow. An infinity or NaN makes the
+ *   scale of its page and head NaN, and with it all that is read there, until a
+ *   write that starts the page anew. Places behind the new tokens keep their
+ *   bytes. Nothing is written for lengths of zero, pages past table_width and page
+ *   ids >= num_blocks.
+ * kvflux_quant_gather: K and V of every sequence as [sum of lengths]
+ *   [num_kv_heads][head_size] of `output_dtype`, each value rounded once; its
+ *   other arguments as for kvflux_gather_paged_kv_live.
+ * Any head_size; block_size and head_size such that a page has fewer than 2^31
+ * values, heads below 2^16. Caches need no alignment; with 8 bytes (and inputs and
+ * outputs with 16, head_size and strides multiples of 8) the fast kernels run. All
+ * calls are safe under graph capture.
+ * ------------------------------------------------------------------------- */
+int kvflux_quant_write(void* key_cache, void* value_cache, float* key_scales, float* value_scales,
+                       uint64_t num_blocks, uint64_t num_kv_heads, uint64_t block_size, uint64_t head_size,
+                       int format, const void* key_new, const void* value_new, int input_dtype,
+                       uint64_t key_stride, uint64_t value_stride, const uint64_t* block_table,
+                       uint64_t table_width, const uint64_t* kv_lens, const uint64_t* new_lens,
+                       const uint64_t* new_offsets, uint64_t num_seqs, uint64_t max_new_tokens, void* stream);
+int kvflux_quant_write_tail(void* key_cache, void* value_cache, float* key_scales, float* value_scales,
+                            uint64_t num_blocks, uint64_t num_kv_heads, uint64_t block_size, uint64_t head_size,
+                            int format, const void* key_new, const void* value_new, int input_dtype,
+                            uint64_t key_stride, uint64_t value_stride, const uint64_t* block_table,
+                            uint64_t table_width, const uint64_t* seq_lens, uint64_t num_rows, void* stream);
+int kvflux_quant_gather(const void* key_cache, const void* value_cache, const float* key_scales,
+                        const float* value_scales, uint64_t num_blocks, uint64_t num_kv_heads,
+                        uint64_t block_size, uint64_t head_size, int format, const uint64_t* block_table,
+                        uint64_t max_blocks_per_seq, const uint64_t* seq_lens, const uint64_t* out_offsets,
+                        const uint64_t* page_starts, uint64_t num_seqs, uint64_t total_pages, void* key_out,
+                        void* value_out, int output_dtype, void* stream);
 
 /* ---------------------------------------------------------------------------
  * GPU <-> CPU chunk transfer (KV offload).

@@ -15,6 +15,7 @@ LIB_PATH = LIB_DIR / "libkvflux_hip.so"
 
 OK, ERR_INVALID, ERR_RANGE, ERR_OVERFLOW, ERR_RUNTIME, ERR_UNSUPPORTED = range(6)
 DTYPE_F16, DTYPE_BF16, DTYPE_F32 = 0, 1, 2
+QUANT_E4M3, QUANT_INT8 = 0, 1
 DIST_UNIFORM, DIST_NORMAL = 0, 1
 
 _vp, _u64, _sz, _i32 = C.c_void_p, C.c_uint64, C.c_size_t, C.c_int
@@ -88,6 +89,12 @@ SIGNATURES = {
     "kvflux_norm_rope_write_tail": (_i32, [_vp, _vp, _u64, _u64, _u64, _u64, _i32, _vp, _vp, _vp, _i32, _u64, _u64,
                                            _u64, _u64, _vp, _vp, C.c_float, _vp, _u64, _i32, _vp, _u64, _vp, _u64,
                                            _vp, _vp]),
+    "kvflux_quant_write": (_i32, [_vp, _vp, _vp, _vp, _u64, _u64, _u64, _u64, _i32, _vp, _vp, _i32, _u64, _u64, _vp,
+                                  _u64, _vp, _vp, _vp, _u64, _u64, _vp]),
+    "kvflux_quant_write_tail": (_i32, [_vp, _vp, _vp, _vp, _u64, _u64, _u64, _u64, _i32, _vp, _vp, _i32, _u64, _u64,
+                                       _vp, _u64, _vp, _u64, _vp]),
+    "kvflux_quant_gather": (_i32, [_vp, _vp, _vp, _vp, _u64, _u64, _u64, _u64, _i32, _vp, _u64, _vp, _vp, _vp, _u64,
+                                   _u64, _vp, _vp, _i32, _vp]),
     "kvflux_copy_chunks": (_i32, [_vp, _u64, _u64, _vp]),
     "kvflux_copy_page_list": (_i32, [_vp, _vp, _u64, _u64, _vp, _u64, _vp]),
     "kvflux_bandwidth_probe": (_i32, [_i32, _vp, _vp, _u64, C.c_uint32, C.c_uint32, C.c_uint32, _i32, _vp]),

@@ -127,6 +127,28 @@ __device__ inline void two_sum_add(float& hi, float& lo, float b) {
     lo += e;
 }
 
+// Last index i in [0, n) with starts[i] <= w, for a non-decreasing `starts`
+// with starts[0] <= w (the sequence holding flat page w; empty sequences,
+// whose start equals the next one's, are stepped over). Every lane of the
+// wavefront takes part and gets the same answer: each level probes 64 evenly
+// spaced entries and keeps the span between the last probe <= w and the next.
+__device__ inline std::uint32_t find_sequence(const std::uint64_t* __restrict__ starts, std::uint32_t n,
+                                              std::uint64_t w) {
+    const std::uint32_t lane = threadIdx.x & 63u;
+    std::uint32_t lo = 0;
+    while (n > 1) {  // uniform
+        const std::uint32_t step = (n + 63u) / 64u;
+        const std::uint32_t k = lane * step;
+        const bool below = k < n && starts[lo + k] <= w;
+        std::uint32_t c = static_cast<std::uint32_t>(__popcll(__ballot(below)));
+        if (c == 0) c = 1;  // starts[lo] > w only for a malformed scan: stay at lo
+        lo += (c - 1u) * step;
+        const std::uint32_t left = n - (c - 1u) * step;
+        n = left < step ? left : step;
+    }
+    return lo;
+}
+
 // Widest power-of-two byte width (<= 16) that divides `row_bytes` and every
 // address in `ptrs`.
 inline unsigned copy_width(std::uint64_t row_bytes, const void* const* ptrs, int n) {

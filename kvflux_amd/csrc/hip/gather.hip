@@ -89,28 +89,6 @@ __device__ inline void gather_part(const Vec* __restrict__ src, Vec* __restrict_
     }
 }
 
-// Last index i in [0, n) with starts[i] <= w, for a non-decreasing `starts`
-// with starts[0] <= w (the sequence holding flat page w; empty sequences,
-// whose start equals the next one's, are stepped over). Every lane of the
-// wavefront takes part and gets the same answer: each level probes 64 evenly
-// spaced entries and keeps the span between the last probe <= w and the next.
-__device__ inline std::uint32_t find_sequence(const std::uint64_t* __restrict__ starts, std::uint32_t n,
-                                              std::uint64_t w) {
-    const std::uint32_t lane = threadIdx.x & 63u;
-    std::uint32_t lo = 0;
-    while (n > 1) {  // uniform
-        const std::uint32_t step = (n + 63u) / 64u;
-        const std::uint32_t k = lane * step;
-        const bool below = k < n && starts[lo + k] <= w;
-        std::uint32_t c = static_cast<std::uint32_t>(__popcll(__ballot(below)));
-        if (c == 0) c = 1;  // starts[lo] > w only for a malformed scan: stay at lo
-        lo += (c - 1u) * step;
-        const std::uint32_t left = n - (c - 1u) * step;
-        n = left < step ? left : step;
-    }
-    return lo;
-}
-
 // kGroup threads (a workgroup, or a wavefront of it) move one part.
 template <typename Vec, int kVpt, int kGroup>
 __global__ __launch_bounds__(kThreads) void paged_kv_gather_live_kernel(

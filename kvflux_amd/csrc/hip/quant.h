@@ -1,0 +1,76 @@
+// The formats of an 8-bit cache: what a byte stands for, and the scale of the
+// values that share one.
+//
+// A value is q * s with s = 2^k, the smallest power of two that brings the largest
+// magnitude to the format's top (448 or 127). Powers of two, not top / largest:
+// dividing by s is exact, so rounding happens once and is the same whoever
+// computes it; raising the scale of a page that has tokens moves E4M3 values by
+// whole exponents (exact above their subnormals), where another factor would round
+// all of them anew at each step. E4M3 loses nothing by it (its relative precision
+// is the same at every size), integers at most one bit of seven.
+#pragma once
+
+#include "common.h"
+
+namespace kvflux_hip {
+namespace {
+
+typedef __attribute__((ext_vector_type(2))) float qt_f32x2_t;
+typedef __attribute__((ext_vector_type(2))) _Float16 qt_f16x2_t;
+
+// hold4: four values, divided by their scale, to bytes (nearest, ties to even).
+// values4: what four bytes stand for. pair16: bytes 2 * half and 2 * half + 1 of a word as two
+// FP16 values, exactly (448 and 2^-9 are normal there; bytes up to -128 are whole).
+struct QuantE4m3 {
+    static constexpr int kTopLog2 = 9;                     // 448 = 0.875 * 2^9
+    static constexpr std::uint32_t kTopMantissa = 0x600000u;  // of 1.75
+    __device__ static std::uint32_t hold4(float a, float b, float c, float d) {
+        const int lo = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
+        return static_cast<std::uint32_t>(__builtin_amdgcn_cvt_pk_fp8_f32(c, d, lo, true));
+    }
+    __device__ static void values4(std::uint32_t w, float (&out)[4]) {
+        const qt_f32x2_t lo = __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<int>(w), false);
+        const qt_f32x2_t hi = __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<int>(w), true);
+        out[0] = lo[0];
+        out[1] = lo[1];
+        out[2] = hi[0];
+        out[3] = hi[1];
+    }
+    template <int kHalf>
+    __device__ static std::uint32_t pair16(std::uint32_t w) {
+        return __builtin_bit_cast(std::uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, kHalf != 0));
+    }
+};
+struct QuantInt8 {
+    static constexpr int kTopLog2 = 7;                     // 127 = (127 / 128) * 2^7
+    static constexpr std::uint32_t kTopMantissa = 0x7e0000u;  // of 127 / 64
+    __device__ static std::uint32_t hold4(float a, float b, float c, float d) {
+        const auto byte = [](float x) { return static_cast<std::uint32_t>(static_cast<int>(__builtin_rintf(x))) & 0xffu; };
+        return byte(a) | byte(b) << 8 | byte(c) << 16 | byte(d) << 24;
+    }
+    __device__ static void values4(std::uint32_t w, float (&out)[4]) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) out[i] = static_cast<float>(static_cast<int>(w << (24 - 8 * i)) >> 24);
+    }
+    // The byte plus 128 is the mantissa of an FP16 of 1024 to 1279.
+    template <int kHalf>
+    __device__ static std::uint32_t pair16(std::uint32_t w) {
+        const std::uint32_t m = __builtin_amdgcn_perm(0x64646464u, w ^ 0x80808080u, kHalf == 0 ? 0x04010400u : 0x04030402u);
+        const qt_f16x2_t base{static_cast<_Float16>(-1152.0f), static_cast<_Float16>(-1152.0f)};
+        return __builtin_bit_cast(std::uint32_t, __builtin_bit_cast(qt_f16x2_t, m) + base);
+    }
+};
+
+// The scale for values whose largest magnitude has the FP32 bits `largest`; NaN for
+// an infinity or NaN. 2^-110 at least: every value of either format times it is a
+// normal FP32 number (2^-9 * 2^-110 > 2^-126), zeros apart.
+constexpr int kLeastScaleLog2 = -110;
+template <typename F>
+__device__ inline float quant_scale(std::uint32_t largest) {
+    int k = static_cast<int>(largest >> 23) - 126 - F::kTopLog2 + ((largest & 0x7fffffu) > F::kTopMantissa ? 1 : 0);
+    if (k < kLeastScaleLog2) k = kLeastScaleLog2;
+    return __uint_as_float(largest >= 0x7f800000u ? 0x7fc00000u : static_cast<std::uint32_t>(k + 127) << 23);
+}
+
+} // namespace
+} // namespace kvflux_hip
