@@ -532,6 +532,29 @@ int kvflux_quant_gather(const void* key_cache, const void* value_cache, const fl
                         const uint64_t* page_starts, uint64_t num_seqs, uint64_t total_pages, void* key_out,
                         void* value_out, int output_dtype, void* stream);
 
+/* kvflux_quant_attention: kvflux_paged_attention's batch decode (seq_lens given) on
+ * such a cache, with its arguments, FP32 queries and outputs, and the 1e-5 contract
+ * against the values that the cache holds. Rows of zero tokens give zeros, missing
+ * pages (ids >= num_blocks, entries past the table's rows) drop out, a scale or live
+ * E4M3 byte that is NaN makes the rows that see it NaN. Scales of any size and
+ * origin. Results are the same bits from call to call; a row's may differ between
+ * batches.
+ * head_size 64, 128 and 256, pages of any size, any group of query heads (16 to a
+ * launch's item); other head sizes up to 512, and caches that are not aligned to 16
+ * bytes, take a generic kernel (a lane a token, tens of times slower).
+ * workspace: kvflux_quant_attention_workspace_size bytes, aligned to 8 (no
+ * initialisation needed; calls that share one must be ordered); NULL where that is 0
+ * (kv_len of at most 512). */
+int kvflux_quant_attention_workspace_size(uint64_t num_rows, uint64_t kv_len, uint64_t num_kv_heads,
+                                          uint64_t query_heads, uint64_t block_size, uint64_t head_size,
+                                          size_t* bytes);
+int kvflux_quant_attention(const void* key_cache, const void* value_cache, const float* key_scales,
+                           const float* value_scales, uint64_t num_blocks, uint64_t num_kv_heads,
+                           uint64_t block_size, uint64_t head_size, int format, const uint64_t* block_table,
+                           uint64_t max_blocks_per_seq, const uint64_t* seq_lens, uint64_t kv_len,
+                           uint64_t num_rows, uint64_t query_heads, const float* query, float* output,
+                           void* workspace, size_t workspace_bytes, void* stream);
+
 /* ---------------------------------------------------------------------------
  * GPU <-> CPU chunk transfer (KV offload).
  *

@@ -12,6 +12,8 @@
 
 #include "common.h"
 
+#include <initializer_list>
+
 namespace kvflux_hip {
 namespace {
 
@@ -70,6 +72,31 @@ __device__ inline float quant_scale(std::uint32_t largest) {
     int k = static_cast<int>(largest >> 23) - 126 - F::kTopLog2 + ((largest & 0x7fffffu) > F::kTopMantissa ? 1 : 0);
     if (k < kLeastScaleLog2) k = kLeastScaleLog2;
     return __uint_as_float(largest >= 0x7f800000u ? 0x7fc00000u : static_cast<std::uint32_t>(k + 127) << 23);
+}
+
+inline bool aligned(std::uint64_t bytes, std::initializer_list<const void*> pointers) {
+    for (const void* x : pointers)
+        if (reinterpret_cast<std::uintptr_t>(x) % bytes != 0) return false;
+    return true;
+}
+
+// What every call on an 8-bit cache checks.
+inline int check_quant_cache(const char* op, const void* key_cache, const void* value_cache, const void* key_scales,
+                             const void* value_scales, std::uint64_t num_blocks, std::uint64_t heads,
+                             std::uint64_t block_size, std::uint64_t head_size, int format) {
+    if (format != KVFLUX_QUANT_E4M3 && format != KVFLUX_QUANT_INT8)
+        return fail(KVFLUX_ERR_INVALID_ARGUMENT, "%s: unknown format %d", op, format);
+    if (!key_cache || !value_cache || !key_scales || !value_scales)
+        return fail(KVFLUX_ERR_INVALID_ARGUMENT, "%s: null cache pointer", op);
+    if (num_blocks == 0 || heads == 0 || block_size == 0 || head_size == 0)
+        return fail(KVFLUX_ERR_INVALID_ARGUMENT, "%s: empty cache shape", op);
+    if (!aligned(4, {key_scales, value_scales}))
+        return fail(KVFLUX_ERR_INVALID_ARGUMENT, "%s: misaligned scales", op);
+    if (heads > 65535 || head_size > 0x7fffffffULL || block_size > 0x7fffffffULL / head_size)
+        return fail(KVFLUX_ERR_UNSUPPORTED, "%s: a page is too large", op);
+    if (num_blocks > (std::uint64_t{1} << 56) / (heads * block_size * head_size))
+        return fail(KVFLUX_ERR_OVERFLOW, "%s: cache size", op);
+    return KVFLUX_OK;
 }
 
 } // namespace

@@ -206,38 +206,13 @@ int launch_write_format(WriteParams& p, int format, bool wide, hipStream_t strea
     return wide ? launch_write<In, QuantInt8, 8>(p, stream) : launch_write<In, QuantInt8, 1>(p, stream);
 }
 
-bool aligned(std::uint64_t bytes, std::initializer_list<const void*> pointers) {
-    for (const void* x : pointers)
-        if (reinterpret_cast<std::uintptr_t>(x) % bytes != 0) return false;
-    return true;
-}
-
-// What every call on an 8-bit cache checks.
-int check_cache(const char* op, const void* key_cache, const void* value_cache, const void* key_scales,
-                const void* value_scales, std::uint64_t num_blocks, std::uint64_t heads, std::uint64_t block_size,
-                std::uint64_t head_size, int format) {
-    if (format != KVFLUX_QUANT_E4M3 && format != KVFLUX_QUANT_INT8)
-        return fail(KVFLUX_ERR_INVALID_ARGUMENT, "%s: unknown format %d", op, format);
-    if (!key_cache || !value_cache || !key_scales || !value_scales)
-        return fail(KVFLUX_ERR_INVALID_ARGUMENT, "%s: null cache pointer", op);
-    if (num_blocks == 0 || heads == 0 || block_size == 0 || head_size == 0)
-        return fail(KVFLUX_ERR_INVALID_ARGUMENT, "%s: empty cache shape", op);
-    if (!aligned(4, {key_scales, value_scales}))
-        return fail(KVFLUX_ERR_INVALID_ARGUMENT, "%s: misaligned scales", op);
-    if (heads > 65535 || head_size > 0x7fffffffULL || block_size > 0x7fffffffULL / head_size)
-        return fail(KVFLUX_ERR_UNSUPPORTED, "%s: a page is too large", op);
-    if (num_blocks > (std::uint64_t{1} << 60) / (heads * block_size * head_size))
-        return fail(KVFLUX_ERR_OVERFLOW, "%s: cache size", op);
-    return KVFLUX_OK;
-}
-
 int write(const char* op, void* key_cache, void* value_cache, float* key_scales, float* value_scales,
           std::uint64_t num_blocks, std::uint64_t heads, std::uint64_t block_size, std::uint64_t head_size, int format,
           const void* key_new, const void* value_new, int input_dtype, std::uint64_t key_stride,
           std::uint64_t value_stride, const std::uint64_t* table, std::uint64_t width, const std::uint64_t* kv_lens,
           const std::uint64_t* new_lens, const std::uint64_t* offsets, std::uint64_t num_seqs,
           std::uint64_t max_new, void* stream) {
-    if (const int s = check_cache(op, key_cache, value_cache, key_scales, value_scales, num_blocks, heads, block_size,
+    if (const int s = check_quant_cache(op, key_cache, value_cache, key_scales, value_scales, num_blocks, heads, block_size,
                                   head_size, format))
         return s;
     const std::uint64_t element = dtype_bytes(input_dtype);
@@ -445,7 +420,7 @@ extern "C" int kvflux_quant_gather(const void* key_cache, const void* value_cach
                                    const uint64_t* page_starts, uint64_t num_seqs, uint64_t total_pages, void* key_out,
                                    void* value_out, int output_dtype, void* stream) {
     if (num_seqs == 0 || total_pages == 0) return KVFLUX_OK;
-    if (const int s = check_cache("quant gather", key_cache, value_cache, key_scales, value_scales, num_blocks,
+    if (const int s = check_quant_cache("quant gather", key_cache, value_cache, key_scales, value_scales, num_blocks,
                                   num_kv_heads, block_size, head_size, format))
         return s;
     const std::uint64_t element = dtype_bytes(output_dtype);

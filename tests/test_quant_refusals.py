@@ -36,14 +36,19 @@ def gather(cache=None, **change):
     return status("kvflux_quant_gather", *(cache or cache_args()), *a.values())
 
 
-CALLS = [write, tail, gather]
+def attend(cache=None, **change):
+    a = dict(table=P, width=4, lens=P, kv_len=400, rows=3, Hq=8, q=P, o=P, ws=P, bytes=1 << 40, stream=None) | change
+    return status("kvflux_quant_attention", *(cache or cache_args()), *a.values())
+
+
+CALLS = [write, tail, gather, attend]
 BAD_CACHES = [
     (dict(fmt=2), capi.ERR_INVALID), (dict(fmt=-1), capi.ERR_INVALID), (dict(k=None), capi.ERR_INVALID),
     (dict(v=None), capi.ERR_INVALID), (dict(ks=None), capi.ERR_INVALID), (dict(vs=None), capi.ERR_INVALID),
     (dict(blocks=0), capi.ERR_INVALID), (dict(heads=0), capi.ERR_INVALID), (dict(bs=0), capi.ERR_INVALID),
     (dict(D=0), capi.ERR_INVALID), (dict(ks=P + 2), capi.ERR_INVALID), (dict(vs=P + 1), capi.ERR_INVALID),
     (dict(heads=1 << 16), capi.ERR_UNSUPPORTED), (dict(bs=1 << 30), capi.ERR_UNSUPPORTED),
-    (dict(blocks=1 << 60), capi.ERR_OVERFLOW)]
+    (dict(blocks=1 << 60), capi.ERR_OVERFLOW), (dict(blocks=2 ** 64 - 1), capi.ERR_OVERFLOW)]
 
 
 @pytest.mark.parametrize("call", CALLS)
@@ -81,3 +86,34 @@ def test_reads(change, want):
 
 def test_nothing_to_read():
     assert gather(seqs=0, table=None) == capi.OK and gather(pages=0, table=None) == capi.OK
+
+
+@pytest.mark.parametrize("change,want", [
+    (dict(table=None), capi.ERR_INVALID), (dict(lens=None), capi.ERR_INVALID), (dict(q=None), capi.ERR_INVALID),
+    (dict(o=None), capi.ERR_INVALID), (dict(width=0), capi.ERR_INVALID), (dict(Hq=0), capi.ERR_INVALID),
+    (dict(Hq=7), capi.ERR_INVALID), (dict(q=P + 2), capi.ERR_INVALID), (dict(o=P + 1), capi.ERR_INVALID),
+    (dict(table=P + 4), capi.ERR_INVALID), (dict(Hq=1 << 20), capi.ERR_UNSUPPORTED),
+    (dict(kv_len=1 << 32), capi.ERR_UNSUPPORTED), (dict(rows=1 << 32), capi.ERR_UNSUPPORTED),
+    (dict(kv_len=5000, ws=None), capi.ERR_INVALID), (dict(kv_len=5000, bytes=100), capi.ERR_INVALID),
+    (dict(kv_len=5000, ws=P + 4), capi.ERR_INVALID)])
+def test_attention(change, want):
+    assert attend(**change) == want
+
+
+def test_head_sizes_of_attention():
+    assert attend(cache_args(D=513)) == capi.ERR_UNSUPPORTED
+    assert attend(rows=0, table=None) == capi.OK
+
+
+def test_workspace_sizes_of_attention():
+    size = C.c_size_t(7)
+
+    def ask(rows=4, kv_len=2000, H=2, Hq=8, bs=16, D=128):
+        return status("kvflux_quant_attention_workspace_size", rows, kv_len, H, Hq, bs, D, C.byref(size))
+
+    assert ask() == capi.OK and size.value > 0
+    assert ask(kv_len=512) == capi.OK and size.value == 0
+    assert ask(rows=0) == capi.OK and size.value == 0
+    assert ask(D=96) == capi.OK and size.value == 0
+    assert ask(Hq=7) == capi.ERR_INVALID and ask(H=0) == capi.ERR_INVALID and ask(kv_len=1 << 32) == capi.ERR_UNSUPPORTED
+    assert status("kvflux_quant_attention_workspace_size", 1, 1, 1, 1, 1, 64, None) == capi.ERR_INVALID
