@@ -555,6 +555,29 @@ int kvflux_quant_attention(const void* key_cache, const void* value_cache, const
                            uint64_t num_rows, uint64_t query_heads, const float* query, float* output,
                            void* workspace, size_t workspace_bytes, void* stream);
 
+/* kvflux_quant_prefill: kvflux_paged_prefill_batch on such a cache: sequence i of
+ * kv_lens[i] tokens (device uint64 [num_seqs]), the last query_lens[i] of which are its
+ * queries, at rows query_offsets[i] .. of query and output ([.][query_heads][head_size]
+ * FP32); query j sees tokens [0, kv_lens[i] - query_lens[i] + j]. max_query_tokens and
+ * max_kv_len bound them and size the grid. Accuracy, missing pages, NaN and head sizes
+ * as kvflux_quant_attention; pages of any size, any group of query heads.
+ * A live E4M3 byte of V that is NaN (the writes make none) may reach queries before
+ * its token. workspace: kvflux_quant_prefill_workspace_size bytes for the same bounds,
+ * for calls of few queries behind many tokens, whose keys are split over workgroups
+ * (0: NULL will do; no initialisation; calls that share one must be ordered).
+ * KVFLUX_ERR_UNSUPPORTED: more than 65535 sequences, 2^31 pages or max_kv_len, or
+ * num_seqs * max_query_tokens * query_heads of 2^31 and more. */
+int kvflux_quant_prefill_workspace_size(uint64_t num_seqs, uint64_t max_query_tokens, uint64_t max_kv_len,
+                                        uint64_t num_kv_heads, uint64_t query_heads, uint64_t block_size,
+                                        uint64_t head_size, size_t* bytes);
+int kvflux_quant_prefill(const void* key_cache, const void* value_cache, const float* key_scales,
+                         const float* value_scales, uint64_t num_blocks, uint64_t num_kv_heads,
+                         uint64_t block_size, uint64_t head_size, int format, const uint64_t* block_table,
+                         uint64_t max_blocks_per_seq, const uint64_t* kv_lens, const uint64_t* query_lens,
+                         const uint64_t* query_offsets, uint64_t num_seqs, uint64_t max_query_tokens,
+                         uint64_t max_kv_len, uint64_t query_heads, const float* query, float* output,
+                         void* workspace, size_t workspace_bytes, void* stream);
+
 /* ---------------------------------------------------------------------------
  * GPU <-> CPU chunk transfer (KV offload).
  *

@@ -98,6 +98,9 @@ SIGNATURES = {
     "kvflux_quant_attention_workspace_size": (_i32, [_u64, _u64, _u64, _u64, _u64, _u64, C.POINTER(_sz)]),
     "kvflux_quant_attention": (_i32, [_vp, _vp, _vp, _vp, _u64, _u64, _u64, _u64, _i32, _vp, _u64, _vp, _u64, _u64, _u64,
                                       _vp, _vp, _vp, _sz, _vp]),
+    "kvflux_quant_prefill_workspace_size": (_i32, [_u64, _u64, _u64, _u64, _u64, _u64, _u64, C.POINTER(_sz)]),
+    "kvflux_quant_prefill": (_i32, [_vp, _vp, _vp, _vp, _u64, _u64, _u64, _u64, _i32, _vp, _u64, _vp, _vp, _vp, _u64,
+                                    _u64, _u64, _u64, _vp, _vp, _vp, _sz, _vp]),
     "kvflux_copy_chunks": (_i32, [_vp, _u64, _u64, _vp]),
     "kvflux_copy_page_list": (_i32, [_vp, _vp, _u64, _u64, _vp, _u64, _vp]),
     "kvflux_bandwidth_probe": (_i32, [_i32, _vp, _vp, _u64, C.c_uint32, C.c_uint32, C.c_uint32, _i32, _vp]),

@@ -15,6 +15,32 @@
 #include <initializer_list>
 
 namespace kvflux_hip {
+
+// Attention of any shape, a workgroup for each (query row, query head): quant_rows_kernel.
+struct QuantRows {
+    const std::uint8_t* key_cache;
+    const std::uint8_t* value_cache;
+    const float* key_scales;
+    const float* value_scales;
+    std::uint64_t num_blocks;
+    std::uint32_t heads, head_size;
+    FastDiv block_size;
+    const std::uint64_t* table;
+    std::uint64_t width;
+    const std::uint64_t* lens;
+    std::uint32_t kv_len;  // bound of every length
+    // Null: row r is the one query of sequence r. Else row r is query r % max_query of
+    // sequence r / max_query's last query_lens[.], at row query_offsets[.] on.
+    const std::uint64_t* query_lens;
+    const std::uint64_t* query_offsets;
+    std::uint32_t max_query;
+    std::uint32_t query_heads, group;
+    const float* query;
+    float* output;
+    float scale_log2;
+};
+int launch_quant_rows(const QuantRows& p, std::uint64_t rows, int format, hipStream_t stream);
+
 namespace {
 
 typedef __attribute__((ext_vector_type(2))) float qt_f32x2_t;

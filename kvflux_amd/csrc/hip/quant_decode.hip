@@ -600,22 +600,34 @@ __global__ __launch_bounds__(kMergeThreads) void quant_decode_merge_kernel(Quant
         Float4{o.x * inv, o.y * inv, o.z * inv, o.w * inv};
 }
 
-// Any head_size up to 512, and caches at any byte: a workgroup for each (row, query
+// Any head_size up to 512, and caches at any byte: a workgroup for each (query row, query
 // head), a lane for each of 64 tokens of a wavefront's step, FP32 products and sums.
 constexpr std::uint32_t kGenericD = 512;
 template <typename F>
-__global__ __launch_bounds__(kThreads) void quant_decode_generic_kernel(QuantDecodeParams p, std::uint32_t head_size) {
+__global__ __launch_bounds__(kThreads) void quant_rows_kernel(QuantRows p, std::uint32_t first_row) {
     __shared__ float q[kGenericD];
     __shared__ float weight[kWaves][64];
     __shared__ std::uint64_t at_of[kWaves][64];
     __shared__ float reduce[kWaves][kGenericD];
     __shared__ float2 stats[kWaves];
-    const std::uint32_t tid = threadIdx.x, wave = tid / 64, lane = tid % 64;
-    const std::uint32_t row = blockIdx.x / p.query_heads, head = blockIdx.x % p.query_heads, kvh = head / p.group;
-    const std::uint64_t out_row = (static_cast<std::uint64_t>(p.row_base) + row) * p.query_heads + head;
-    const std::uint64_t full = p.lens[p.row_base + row];
-    const std::uint32_t len = full < p.kv_len ? static_cast<std::uint32_t>(full) : p.kv_len;
-    for (std::uint32_t d = tid; d < head_size; d += kThreads) q[d] = p.query[out_row * head_size + d] * p.scale_log2;
+    const std::uint32_t tid = threadIdx.x, wave = tid / 64, lane = tid % 64, D = p.head_size;
+    const std::uint64_t row = static_cast<std::uint64_t>(first_row) + blockIdx.x / p.query_heads;
+    const std::uint32_t head = blockIdx.x % p.query_heads, kvh = head / p.group;
+    const std::uint64_t seq = p.query_lens ? row / p.max_query : row;
+    const std::uint64_t full = p.lens[seq];
+    std::uint32_t len = full < p.kv_len ? static_cast<std::uint32_t>(full) : p.kv_len;
+    std::uint64_t out_row = row;
+    if (p.query_lens) {
+        const std::uint32_t i = static_cast<std::uint32_t>(row % p.max_query);
+        const std::uint64_t queries = p.query_lens[seq];
+        std::uint32_t n = queries < len ? static_cast<std::uint32_t>(queries) : len;
+        if (n > p.max_query) n = p.max_query;
+        if (i >= n) return;  // uniform
+        len = len - n + i + 1;
+        out_row = p.query_offsets[seq] + i;
+    }
+    out_row = out_row * p.query_heads + head;
+    for (std::uint32_t d = tid; d < D; d += kThreads) q[d] = p.query[out_row * D + d] * p.scale_log2;
     __syncthreads();
     float top = -INFINITY, sum = 0.0f;
     float acc[kGenericD / 64] = {};
@@ -623,13 +635,13 @@ __global__ __launch_bounds__(kThreads) void quant_decode_generic_kernel(QuantDec
         const std::uint32_t token = static_cast<std::uint32_t>(base) + lane;
         const std::uint64_t page = p.block_size.div(token);
         bool live = base + lane < len && page < p.width;
-        std::uint64_t id = p.table[(static_cast<std::uint64_t>(p.row_base) + row) * p.width + (live ? page : 0)];
+        std::uint64_t id = p.table[seq * p.width + (live ? page : 0)];
         live = live && id < p.num_blocks;
         id = live ? id : 0;
         const std::uint64_t scale_at = id * p.heads + kvh;
-        const std::uint64_t at = (scale_at * p.block_size.divisor + (live ? p.block_size.mod(token) : 0)) * head_size;
+        const std::uint64_t at = (scale_at * p.block_size.divisor + (live ? p.block_size.mod(token) : 0)) * D;
         float dot = 0.0f, v4[4];
-        for (std::uint32_t d = 0; d < head_size; ++d) {
+        for (std::uint32_t d = 0; d < D; ++d) {
             F::values4(p.key_cache[at + d], v4);
             dot = fmaf(q[d], v4[0], dot);
         }
@@ -655,7 +667,7 @@ __global__ __launch_bounds__(kThreads) void quant_decode_generic_kernel(QuantDec
             const float wt = weight[wave][t];
 #pragma unroll
             for (std::uint32_t i = 0; i < kGenericD / 64; ++i) {
-                if (lane + 64 * i >= head_size) break;
+                if (lane + 64 * i >= D) break;
                 F::values4(p.value_cache[from + lane + 64 * i], v4);
                 acc[i] = fmaf(wt, v4[0], acc[i]);
             }
@@ -667,7 +679,7 @@ __global__ __launch_bounds__(kThreads) void quant_decode_generic_kernel(QuantDec
     if (lane == 0) stats[wave] = make_float2(top, sum);
 #pragma unroll
     for (std::uint32_t i = 0; i < kGenericD / 64; ++i)
-        if (lane + 64 * i < head_size) reduce[wave][lane + 64 * i] = acc[i];
+        if (lane + 64 * i < D) reduce[wave][lane + 64 * i] = acc[i];
     __syncthreads();
     float all = -INFINITY, total = 0.0f;
 #pragma unroll
@@ -678,11 +690,11 @@ __global__ __launch_bounds__(kThreads) void quant_decode_generic_kernel(QuantDec
         factor[w] = stats[w].y != stats[w].y ? stats[w].y : merge_weight(stats[w].x, all);
         total += stats[w].y * factor[w];
     }
-    for (std::uint32_t d = tid; d < head_size; d += kThreads) {
+    for (std::uint32_t d = tid; d < D; d += kThreads) {
         float o = 0.0f;
 #pragma unroll
         for (int w = 0; w < kWaves; ++w) o += reduce[w][d] * factor[w];
-        p.output[out_row * head_size + d] = total == 0.0f ? 0.0f : o / total;
+        p.output[out_row * D + d] = total == 0.0f ? 0.0f : o / total;
     }
 }
 
@@ -728,11 +740,7 @@ int launch_decode_pages(QuantDecodeParams& p, std::uint32_t grid, hipStream_t s)
     return p.block_size.divisor % 8 == 0 ? launch_decode<F, kD, 8>(p, grid, s) : launch_decode<F, kD, 1>(p, grid, s);
 }
 template <typename F>
-int launch_decode_format(QuantDecodeParams& p, std::uint64_t head_size, bool fast, std::uint32_t grid, hipStream_t s) {
-    if (!fast) {
-        quant_decode_generic_kernel<F><<<dim3(p.rows * p.query_heads), dim3(kThreads), 0, s>>>(p, static_cast<std::uint32_t>(head_size));
-        return launch_status("quant_decode_generic_kernel");
-    }
+int launch_decode_format(QuantDecodeParams& p, std::uint64_t head_size, std::uint32_t grid, hipStream_t s) {
     switch (head_size) {
     case 64: return launch_decode_pages<F, 64>(p, grid, s);
     case 128: return launch_decode_pages<F, 128>(p, grid, s);
@@ -751,6 +759,20 @@ int check_shape(const char* op, std::uint64_t num_rows, std::uint64_t kv_len, st
 }
 
 } // namespace
+
+int launch_quant_rows(const QuantRows& p, std::uint64_t rows, int format, hipStream_t stream) {
+    const std::uint64_t at_once = 0x7fffffffULL / p.query_heads;
+    for (std::uint64_t first = 0; first < rows; first += at_once) {
+        const dim3 grid(static_cast<unsigned>((rows - first < at_once ? rows - first : at_once) * p.query_heads));
+        if (format == KVFLUX_QUANT_E4M3)
+            quant_rows_kernel<QuantE4m3><<<grid, dim3(kThreads), 0, stream>>>(p, static_cast<std::uint32_t>(first));
+        else
+            quant_rows_kernel<QuantInt8><<<grid, dim3(kThreads), 0, stream>>>(p, static_cast<std::uint32_t>(first));
+        if (const int s = launch_status("quant_rows_kernel")) return s;
+    }
+    return KVFLUX_OK;
+}
+
 } // namespace kvflux_hip
 
 using namespace kvflux_hip;
@@ -787,7 +809,28 @@ extern "C" int kvflux_quant_attention(const void* key_cache, const void* value_c
         return s;
     if (!aligned(4, {query, output}) || !aligned(8, {block_table, seq_lens}))
         return fail(KVFLUX_ERR_INVALID_ARGUMENT, "quant attention: misaligned array");
-    const bool fast = fast_head_size(head_size) && aligned(16, {key_cache, value_cache});
+    const float scale_log2 = static_cast<float>(1.4426950408889634 / std::sqrt(static_cast<double>(head_size)));
+    if (!fast_head_size(head_size) || !aligned(16, {key_cache, value_cache})) {
+        QuantRows rows{};
+        rows.key_cache = static_cast<const std::uint8_t*>(key_cache);
+        rows.value_cache = static_cast<const std::uint8_t*>(value_cache);
+        rows.key_scales = key_scales;
+        rows.value_scales = value_scales;
+        rows.num_blocks = num_blocks;
+        rows.heads = static_cast<std::uint32_t>(num_kv_heads);
+        rows.head_size = static_cast<std::uint32_t>(head_size);
+        rows.block_size = FastDiv(static_cast<std::uint32_t>(block_size));
+        rows.table = block_table;
+        rows.width = max_blocks_per_seq;
+        rows.lens = seq_lens;
+        rows.kv_len = static_cast<std::uint32_t>(kv_len);
+        rows.query_heads = static_cast<std::uint32_t>(query_heads);
+        rows.group = static_cast<std::uint32_t>(query_heads / num_kv_heads);
+        rows.query = query;
+        rows.output = output;
+        rows.scale_log2 = scale_log2;
+        return launch_quant_rows(rows, num_rows, format, as_stream(stream));
+    }
     QuantDecodeParams p{};
     p.key_cache = static_cast<const std::uint8_t*>(key_cache);
     p.value_cache = static_cast<const std::uint8_t*>(value_cache);
@@ -805,10 +848,10 @@ extern "C" int kvflux_quant_attention(const void* key_cache, const void* value_c
     head_sets(p.group, &p.sets, &p.set_heads);
     p.query = query;
     p.output = output;
-    p.scale_log2 = static_cast<float>(1.4426950408889634 / std::sqrt(static_cast<double>(head_size)));
+    p.scale_log2 = scale_log2;
     const std::uint64_t streams = num_kv_heads * p.sets;
     const std::uint64_t slice = num_rows < kPlanRows ? num_rows : kPlanRows;
-    const std::uint32_t grid = fast ? decode_grid(slice, kv_len, streams, head_size) : 0;
+    const std::uint32_t grid = decode_grid(slice, kv_len, streams, head_size);
     if (grid != 0) {
         if (!workspace || workspace_bytes < decode_workspace(grid, p.set_heads, head_size))
             return fail(KVFLUX_ERR_INVALID_ARGUMENT, "quant attention: workspace too small");
@@ -821,8 +864,8 @@ extern "C" int kvflux_quant_attention(const void* key_cache, const void* value_c
         p.row_base = static_cast<std::uint32_t>(base);
         p.rows = static_cast<std::uint32_t>(num_rows - base < slice ? num_rows - base : slice);
         const int s = format == KVFLUX_QUANT_E4M3
-                          ? launch_decode_format<QuantE4m3>(p, head_size, fast, grid, as_stream(stream))
-                          : launch_decode_format<QuantInt8>(p, head_size, fast, grid, as_stream(stream));
+                          ? launch_decode_format<QuantE4m3>(p, head_size, grid, as_stream(stream))
+                          : launch_decode_format<QuantInt8>(p, head_size, grid, as_stream(stream));
         if (s != KVFLUX_OK) return s;
     }
     return KVFLUX_OK;

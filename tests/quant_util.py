@@ -148,18 +148,18 @@ def u64(x):
 
 def attention(cache, table, n, q, visible=None):
     """Outputs [rows][Hq][D] in 64 bits of queries [rows][Hq][D] over the first n tokens of a
-    table row (row i sees visible[i] of them, all by default; missing pages drop out), and the
-    largest value of V that a row sees, for tolerances."""
+    table row (row i sees visible[i] of them, all by default; missing pages drop out)."""
     Hq, D = q.shape[1:]
     G = Hq // cache.H
     pages = np.asarray(table[:-(-n // cache.bs)], np.uint64)
+    n = min(n, len(pages) * cache.bs)  # a table row may end before its tokens
     ok = np.repeat(pages < cache.blocks, cache.bs)[:n]
     ids = np.where(pages < cache.blocks, pages, 0).astype(np.int64)
     values = VALUES[cache.fmt][cache.bytes[:, ids]] * cache.scales[:, ids][..., None, None].astype(np.float64)
     k, v = values.transpose(0, 2, 1, 3, 4).reshape(2, cache.H, -1, D)[:, :, :n]
     out = np.zeros(q.shape)
     for i in range(q.shape[0]):
-        see = ok & (np.arange(n) < (n if visible is None else visible[i]))
+        see = ok & (np.arange(n) < (n if visible is None else int(visible[i])))
         if not see.any():
             continue
         for h in range(cache.H):

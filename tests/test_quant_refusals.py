@@ -41,7 +41,13 @@ def attend(cache=None, **change):
     return status("kvflux_quant_attention", *(cache or cache_args()), *a.values())
 
 
-CALLS = [write, tail, gather, attend]
+def prefill(cache=None, **change):
+    a = dict(table=P, width=40, lens=P, ql=P, qo=P, seqs=3, most=7, kv_len=400, Hq=8, q=P, o=P, ws=P, bytes=1 << 60,
+             stream=None) | change
+    return status("kvflux_quant_prefill", *(cache or cache_args()), *a.values())
+
+
+CALLS = [write, tail, gather, attend, prefill]
 BAD_CACHES = [
     (dict(fmt=2), capi.ERR_INVALID), (dict(fmt=-1), capi.ERR_INVALID), (dict(k=None), capi.ERR_INVALID),
     (dict(v=None), capi.ERR_INVALID), (dict(ks=None), capi.ERR_INVALID), (dict(vs=None), capi.ERR_INVALID),
@@ -117,3 +123,32 @@ def test_workspace_sizes_of_attention():
     assert ask(D=96) == capi.OK and size.value == 0
     assert ask(Hq=7) == capi.ERR_INVALID and ask(H=0) == capi.ERR_INVALID and ask(kv_len=1 << 32) == capi.ERR_UNSUPPORTED
     assert status("kvflux_quant_attention_workspace_size", 1, 1, 1, 1, 1, 64, None) == capi.ERR_INVALID
+
+
+@pytest.mark.parametrize("change,want", [
+    (dict(table=None), capi.ERR_INVALID), (dict(lens=None), capi.ERR_INVALID), (dict(ql=None), capi.ERR_INVALID),
+    (dict(qo=None), capi.ERR_INVALID), (dict(q=None), capi.ERR_INVALID), (dict(o=None), capi.ERR_INVALID),
+    (dict(width=0), capi.ERR_INVALID), (dict(Hq=0), capi.ERR_INVALID), (dict(Hq=7), capi.ERR_INVALID),
+    (dict(q=P + 2), capi.ERR_INVALID), (dict(qo=P + 4), capi.ERR_INVALID), (dict(most=401), capi.ERR_INVALID),
+    (dict(Hq=1 << 20), capi.ERR_UNSUPPORTED), (dict(kv_len=1 << 31), capi.ERR_UNSUPPORTED),
+    (dict(seqs=1 << 16), capi.ERR_UNSUPPORTED), (dict(seqs=60000, most=30000, kv_len=30000), capi.ERR_UNSUPPORTED),
+    (dict(kv_len=50000, ws=None), capi.ERR_INVALID), (dict(kv_len=50000, bytes=100), capi.ERR_INVALID),
+    (dict(kv_len=50000, ws=P + 2), capi.ERR_INVALID)])
+def test_prefill(change, want):
+    assert prefill(**change) == want
+
+
+def test_shapes_of_prefill():
+    assert prefill(cache_args(D=513)) == capi.ERR_UNSUPPORTED and prefill(cache_args(blocks=1 << 31)) == capi.ERR_UNSUPPORTED
+    assert prefill(seqs=0, table=None) == capi.OK and prefill(most=0, table=None) == capi.OK
+    size = C.c_size_t(7)
+
+    def ask(seqs=1, most=8, kv_len=50000, H=2, Hq=8, bs=16, D=128):
+        return status("kvflux_quant_prefill_workspace_size", seqs, most, kv_len, H, Hq, bs, D, C.byref(size))
+
+    assert ask() == capi.OK and size.value > 0
+    assert ask(seqs=64, most=4096, kv_len=4096, H=8, Hq=32) == capi.OK and size.value == 0
+    assert ask(D=80) == capi.OK and size.value == 0
+    assert ask(seqs=0) == capi.OK and size.value == 0
+    assert ask(most=50001) == capi.ERR_INVALID and ask(Hq=3) == capi.ERR_INVALID and ask(kv_len=1 << 31) == capi.ERR_UNSUPPORTED
+    assert status("kvflux_quant_prefill_workspace_size", 1, 1, 1, 1, 1, 1, 64, None) == capi.ERR_INVALID
