@@ -23,12 +23,17 @@
 
 namespace kvflux::v2 {
 
+class QuantizedKVStorage;  // quantized_kv.h
+
 class DeviceBatchTable {
 public:
     // Row r is sequences[r] (distinct, using storage's pool, each with at
     // most capacity_blocks pages). The sequences must outlive the table and
     // stay at their addresses. Uploads the full table once and waits.
     DeviceBatchTable(const PagedKVStorage& storage, std::vector<SequenceState*> sequences,
+                     std::size_t capacity_blocks);
+    // The same on a cache held in 8 bits.
+    DeviceBatchTable(const QuantizedKVStorage& storage, std::vector<SequenceState*> sequences,
                      std::size_t capacity_blocks);
     ~DeviceBatchTable();
     DeviceBatchTable(const DeviceBatchTable&) = delete;
@@ -66,9 +71,12 @@ public:
 
 private:
     struct Device;
+    template <typename Storage>
+    void check_sequences(const Storage& storage);
     void upload_all();
 
-    const PagedKVStorage& storage_;
+    int gpu_;                             // the storage's
+    std::size_t block_size_;
     std::vector<SequenceState*> sequences_;
     std::size_t capacity_;
     std::vector<std::uint64_t> shadow_;   // host copy of the device table

@@ -13,6 +13,7 @@
 #include "kvflux/v2/device_batch_table.h"
 #include "kvflux/v2/norm_rope_write.h"
 #include "kvflux/v2/prefix_cache.h"
+#include "kvflux/v2/quantized_kv.h"
 #include "kvflux/v2/sequence_lifecycle.h"
 #include "kvflux/v2/paged_attention.h"
 #include "kvflux/v2/paged_kv_read.h"
@@ -85,6 +86,79 @@ static void bind_timing(py::module_ t) {
             }
         });
     }, "all sequences' tokens as queries (whole-prompt prefill), one call per sequence");
+}
+
+static void bind_quantized(py::module_& m) {
+    py::enum_<QuantFormat>(m, "QuantFormat").value("E4M3", QuantFormat::E4M3).value("Int8", QuantFormat::Int8);
+    py::class_<QuantizedKVLayout>(m, "QuantizedKVLayout")
+        .def(py::init<std::size_t, std::size_t, std::size_t, std::size_t, QuantFormat>())
+        .def("num_blocks", &QuantizedKVLayout::num_blocks)
+        .def("num_kv_heads", &QuantizedKVLayout::num_kv_heads)
+        .def("block_size", &QuantizedKVLayout::block_size)
+        .def("head_size", &QuantizedKVLayout::head_size)
+        .def("format", &QuantizedKVLayout::format)
+        .def("page_bytes", &QuantizedKVLayout::page_bytes)
+        .def("cache_bytes", &QuantizedKVLayout::cache_bytes)
+        .def("cache_stride", &QuantizedKVLayout::cache_stride)
+        .def("scale_bytes", &QuantizedKVLayout::scale_bytes)
+        .def("total_bytes", &QuantizedKVLayout::total_bytes);
+    py::class_<QuantizedKVStorage>(m, "QuantizedKVStorage")
+        .def(py::init<PhysicalBlockPool&, std::size_t, std::size_t, QuantFormat, int>(), py::arg("pool"),
+             py::arg("num_kv_heads"), py::arg("head_size"), py::arg("format"), py::arg("device") = 0,
+             py::keep_alive<1, 2>())
+        .def("layout", &QuantizedKVStorage::layout, py::return_value_policy::reference_internal)
+        .def("device", &QuantizedKVStorage::device)
+        .def("uses_pool", &QuantizedKVStorage::uses_pool)
+        .def("key_base", [](const QuantizedKVStorage& s) { return addr(s.key_base()); })
+        .def("value_base", [](const QuantizedKVStorage& s) { return addr(s.value_base()); })
+        .def("key_scales", [](const QuantizedKVStorage& s) { return addr(s.key_scales()); })
+        .def("value_scales", [](const QuantizedKVStorage& s) { return addr(s.value_scales()); })
+        .def("copy_blocks", [](const QuantizedKVStorage& s,
+                               const std::vector<std::pair<PhysicalBlockHandle, PhysicalBlockHandle>>& pairs) {
+            py::gil_scoped_release release;
+            s.copy_blocks(pairs);
+        });
+    py::class_<NewRows>(m, "NewRows")
+        .def(py::init([](std::uintptr_t k, std::uintptr_t v, DType dtype, std::size_t ks, std::size_t vs) {
+                 return NewRows{ptr(k), ptr(v), dtype, ks, vs};
+             }),
+             py::arg("key"), py::arg("value"), py::arg("dtype"), py::arg("key_stride") = 0, py::arg("value_stride") = 0);
+    m.def("write_quantized_kv", [](QuantizedKVStorage& s, const std::vector<const SequenceState*>& seqs,
+                                   const std::vector<std::size_t>& new_tokens, const NewRows& rows) {
+        py::gil_scoped_release release;
+        write_quantized_kv(s, seqs, new_tokens, rows);
+    });
+    m.def("read_quantized_kv", [](const QuantizedKVStorage& s, const std::vector<const SequenceState*>& seqs, DType dtype,
+                                  std::uintptr_t k, std::uintptr_t v) {
+        py::gil_scoped_release release;
+        read_quantized_kv(s, seqs, dtype, ptr(k), ptr(v));
+    });
+    m.def("paged_attention_batch", [](const QuantizedKVStorage& s, const std::vector<const SequenceState*>& seqs,
+                                      std::uintptr_t q, std::uintptr_t o, std::size_t query_heads) {
+        py::gil_scoped_release release;
+        paged_attention_batch(s, seqs, static_cast<const float*>(ptr(q)), static_cast<float*>(ptr(o)), query_heads);
+    });
+    m.def("paged_attention_batch", [](const QuantizedKVStorage& s, const DeviceBatchTable& t, std::uintptr_t q,
+                                      std::uintptr_t o, std::size_t query_heads) {
+        py::gil_scoped_release release;
+        paged_attention_batch(s, t, static_cast<const float*>(ptr(q)), static_cast<float*>(ptr(o)), query_heads);
+    });
+    m.def("paged_attention_prompts", [](const QuantizedKVStorage& s, const std::vector<const SequenceState*>& seqs,
+                                        const std::vector<std::size_t>& query_tokens, std::uintptr_t q, std::uintptr_t o,
+                                        std::size_t query_heads) {
+        py::gil_scoped_release release;
+        paged_attention_prompts(s, seqs, query_tokens, static_cast<const float*>(ptr(q)), static_cast<float*>(ptr(o)),
+                                query_heads);
+    });
+    m.def("append_tokens_cow", [](const QuantizedKVStorage& s, const std::vector<SequenceState*>& seqs) {
+        py::gil_scoped_release release;
+        return append_tokens_cow(s, seqs);
+    });
+    m.def("decode_step", [](QuantizedKVStorage& s, DeviceBatchTable& t, const NewRows& rows, std::uintptr_t q,
+                            std::uintptr_t o, std::size_t query_heads) {
+        py::gil_scoped_release release;
+        return decode_step(s, t, rows, static_cast<const float*>(ptr(q)), static_cast<float*>(ptr(o)), query_heads);
+    });
 }
 
 static void bind_v3(py::module_ v3m) {
@@ -381,6 +455,9 @@ PYBIND11_MODULE(_kvflux, m) {
         .def(py::init<const PagedKVStorage&, std::vector<SequenceState*>, std::size_t>(),
              py::arg("storage"), py::arg("sequences"), py::arg("capacity_blocks"),
              py::keep_alive<1, 2>(), py::keep_alive<1, 3>())
+        .def(py::init<const QuantizedKVStorage&, std::vector<SequenceState*>, std::size_t>(),
+             py::arg("storage"), py::arg("sequences"), py::arg("capacity_blocks"),
+             py::keep_alive<1, 2>(), py::keep_alive<1, 3>())
         .def("refresh", [](DeviceBatchTable& t) {
             py::gil_scoped_release release;
             t.refresh();
@@ -505,6 +582,7 @@ PYBIND11_MODULE(_kvflux, m) {
         paged_attention_batch(s, seqs, static_cast<const float*>(ptr(q)),
                               static_cast<float*>(ptr(o)), query_heads);
     });
+    bind_quantized(m);
     bind_v3(m.def_submodule("v3", "kvflux::v3 tiered cache: tiers, directory, GPU <-> CPU transfer"));
     bind_timing(m.def_submodule("timing", "seconds per call of the synchronous C++ API, timed in C++"));
     m.def("paged_attention_batch", [](const PagedKVStorage& s, const DeviceBatchTable& t,

@@ -6,6 +6,7 @@
 // (src/v2/sequence_lifecycle.cpp:53-69), for a whole batch at once.
 #include "kvflux/v2/copy_on_write.h"
 #include "kvflux/v2/device_batch_table.h"
+#include "kvflux/v2/quantized_kv.h"
 #include "kvflux/v2/shared_prefix.h"
 
 #include "device_runtime.h"
@@ -56,8 +57,8 @@ struct AppendPlan {
     }
 };
 
-void plan_appends(const PagedKVStorage& storage, const std::vector<SequenceState*>& sequences,
-                  AppendPlan& plan) {
+template <typename Storage>
+void plan_appends(const Storage& storage, const std::vector<SequenceState*>& sequences, AppendPlan& plan) {
     const std::size_t bs = storage.layout().block_size();
     std::unordered_set<const SequenceState*> seen;
     for (const auto* s : sequences) {
@@ -115,6 +116,11 @@ void enqueue_copies(const PagedKVStorage& storage, const AppendPlan& plan) {
                             layout.page_bytes(), dev[0], plan.pairs.size() / 2, nullptr),
           "copy-on-write page copy");
 }
+void enqueue_copies(const QuantizedKVStorage& storage, const AppendPlan& plan) {
+    if (plan.pairs.empty()) return;
+    const auto dev = storage.scratch().upload({{plan.pairs.data(), plan.pairs.size() * 8}});
+    detail::copy_quantized_pages(storage, dev[0], plan.pairs.size() / 2);
+}
 
 void commit(const std::vector<SequenceState*>& sequences, AppendPlan& plan) noexcept {
     for (std::size_t i = 0; i < sequences.size(); ++i) {
@@ -135,10 +141,8 @@ void commit(const std::vector<SequenceState*>& sequences, AppendPlan& plan) noex
     plan.committed = true;
 }
 
-}  // namespace
-
-std::vector<TokenLocation> append_tokens_cow(const PagedKVStorage& storage,
-                                             const std::vector<SequenceState*>& sequences) {
+template <typename Storage>
+std::vector<TokenLocation> append_with_copies(const Storage& storage, const std::vector<SequenceState*>& sequences) {
     AppendPlan plan;
     plan_appends(storage, sequences, plan);
     if (sequences.empty()) return {};
@@ -156,6 +160,17 @@ std::vector<TokenLocation> append_tokens_cow(const PagedKVStorage& storage,
     return plan.locations;
 }
 
+}  // namespace
+
+std::vector<TokenLocation> append_tokens_cow(const PagedKVStorage& storage,
+                                             const std::vector<SequenceState*>& sequences) {
+    return append_with_copies(storage, sequences);
+}
+std::vector<TokenLocation> append_tokens_cow(const QuantizedKVStorage& storage,
+                                             const std::vector<SequenceState*>& sequences) {
+    return append_with_copies(storage, sequences);
+}
+
 // ---------------------------------------------------------------- DeviceBatchTable
 
 struct DeviceBatchTable::Device {
@@ -167,16 +182,12 @@ namespace {
 constexpr std::uint64_t kNoPage = std::numeric_limits<std::uint64_t>::max();
 }
 
-DeviceBatchTable::DeviceBatchTable(const PagedKVStorage& storage,
-                                   std::vector<SequenceState*> sequences,
-                                   std::size_t capacity_blocks)
-    : storage_(storage), sequences_(std::move(sequences)), capacity_(capacity_blocks),
-      device_(std::make_unique<Device>()) {
+template <typename Storage>
+void DeviceBatchTable::check_sequences(const Storage& storage) {
     if (capacity_ == 0) throw std::invalid_argument("device batch table needs a row capacity");
     std::unordered_set<const SequenceState*> seen;
     for (const auto* s : sequences_) {
-        if (!s || !storage_.uses_pool(s->block_table()) ||
-            s->block_size() != storage_.layout().block_size()) {
+        if (!s || !storage.uses_pool(s->block_table()) || s->block_size() != block_size_) {
             throw std::invalid_argument("sequence and KV storage must use one physical pool");
         }
         if (!seen.insert(s).second) throw std::invalid_argument("a sequence appears twice in the batch");
@@ -189,10 +200,23 @@ DeviceBatchTable::DeviceBatchTable(const PagedKVStorage& storage,
     refresh();
 }
 
+DeviceBatchTable::DeviceBatchTable(const PagedKVStorage& storage, std::vector<SequenceState*> sequences,
+                                   std::size_t capacity_blocks)
+    : gpu_(storage.device()), block_size_(storage.layout().block_size()), sequences_(std::move(sequences)),
+      capacity_(capacity_blocks), device_(std::make_unique<Device>()) {
+    check_sequences(storage);
+}
+DeviceBatchTable::DeviceBatchTable(const QuantizedKVStorage& storage, std::vector<SequenceState*> sequences,
+                                   std::size_t capacity_blocks)
+    : gpu_(storage.device()), block_size_(storage.layout().block_size()), sequences_(std::move(sequences)),
+      capacity_(capacity_blocks), device_(std::make_unique<Device>()) {
+    check_sequences(storage);
+}
+
 DeviceBatchTable::~DeviceBatchTable() {
     // The buffers belong to the storage's device; free them there.
     int previous = 0;
-    const int device = storage_.device();
+    const int device = gpu_;
     const bool switched = kvflux_get_device(&previous) == KVFLUX_OK &&
                           (previous == device || kvflux_set_device(device) == KVFLUX_OK);
     device_.reset();
@@ -232,7 +256,7 @@ void DeviceBatchTable::upload_all() {
 }
 
 void DeviceBatchTable::enqueue_refresh() {
-    detail::DeviceGuard guard(storage_.device());
+    detail::DeviceGuard guard(gpu_);
     if (stale_) {
         upload_all();
         stale_ = false;
@@ -291,8 +315,8 @@ const DeviceBatchTable::Groups& DeviceBatchTable::enqueue_groups() {
     if (grouped_) return groups_;
     std::vector<detail::RowPages> rows;
     for (std::size_t r = 0; r < sequences_.size(); ++r)
-        rows.push_back({shadow_.data() + r * capacity_, lengths_[r] / storage_.layout().block_size()});
-    const auto found = detail::group_rows(rows, storage_.layout().block_size());
+        rows.push_back({shadow_.data() + r * capacity_, lengths_[r] / block_size_});
+    const auto found = detail::group_rows(rows, block_size_);
     groups_ = Groups{};
     if (found.groups() != 0) {
         const std::size_t starts_bytes = found.starts.size() * 8, bytes = starts_bytes + found.prefixes.size() * 8;
@@ -312,7 +336,7 @@ const DeviceBatchTable::Groups& DeviceBatchTable::enqueue_groups() {
 }
 
 void DeviceBatchTable::refresh() {
-    detail::DeviceGuard guard(storage_.device());
+    detail::DeviceGuard guard(gpu_);
     try {
         enqueue_refresh();
         check(kvflux_stream_synchronize(nullptr), "synchronize batch table refresh");
@@ -327,7 +351,8 @@ void DeviceBatchTable::refresh() {
 
 namespace {
 
-std::size_t validate_batch_attention(const PagedKVStorage& storage, const DeviceBatchTable& batch,
+template <typename Storage>
+std::size_t validate_batch_attention(const Storage& storage, const DeviceBatchTable& batch,
                                      const float* query, float* output, std::size_t query_heads) {
     const auto& layout = storage.layout();
     if (query_heads == 0 || query_heads % layout.num_kv_heads() != 0) {
@@ -363,6 +388,17 @@ void enqueue_batch_attention(const PagedKVStorage& storage, const DeviceBatchTab
           "paged attention batch kernel launch");
 }
 
+void enqueue_batch_attention(const QuantizedKVStorage& storage, const DeviceBatchTable& batch, const float* query,
+                             float* output, std::size_t query_heads) {
+    const auto& lengths = batch.lengths();
+    if (std::find(lengths.begin(), lengths.end(), 0) != lengths.end()) {
+        throw std::invalid_argument("invalid batch attention sequence");
+    }
+    detail::enqueue_quantized_decode(storage, batch.device_table(), batch.capacity_blocks(), batch.device_lengths(),
+                                     *std::max_element(lengths.begin(), lengths.end()), batch.rows(), query, output,
+                                     query_heads);
+}
+
 }  // namespace
 
 void paged_attention_batch(const PagedKVStorage& storage, const DeviceBatchTable& batch,
@@ -377,11 +413,11 @@ void paged_attention_batch(const PagedKVStorage& storage, const DeviceBatchTable
 
 namespace {
 
-// What decode_step and decode_step_projected have in common: the appends with
+// What the decode steps have in common: the appends with
 // their copies, the refresh, and `enqueue`, which launches the write and the
 // attention.
-template <typename Enqueue>
-std::vector<TokenLocation> append_and_run(PagedKVStorage& storage, DeviceBatchTable& batch, const Enqueue& enqueue) {
+template <typename Storage, typename Enqueue>
+std::vector<TokenLocation> append_and_run(Storage& storage, DeviceBatchTable& batch, const Enqueue& enqueue) {
     const auto& layout = storage.layout();
     const auto& sequences = batch.sequences();
     for (const auto* s : sequences) {
@@ -494,6 +530,34 @@ std::vector<TokenLocation> decode_step_projected(PagedKVStorage& storage, Device
                                           nullptr),
               "decode step norm, rotation and KV write");
         enqueue_shared_attention(storage, batch, query_device, output_device, query_heads);
+    });
+}
+
+void paged_attention_batch(const QuantizedKVStorage& storage, const DeviceBatchTable& batch, const float* query_device,
+                           float* output_device, std::size_t query_heads) {
+    detail::DeviceGuard guard(storage.device());
+    validate_batch_attention(storage, batch, query_device, output_device, query_heads);
+    if (batch.rows() == 0) return;
+    enqueue_batch_attention(storage, batch, query_device, output_device, query_heads);
+    check(kvflux_stream_synchronize(nullptr), "paged attention batch synchronize");
+}
+
+std::vector<TokenLocation> decode_step(QuantizedKVStorage& storage, DeviceBatchTable& batch, const NewRows& rows,
+                                       const float* query_device, float* output_device, std::size_t query_heads) {
+    const auto& layout = storage.layout();
+    detail::DeviceGuard guard(storage.device());
+    validate_batch_attention(storage, batch, query_device, output_device, query_heads);
+    if (batch.rows() == 0) return {};
+    const auto strides = detail::check_new_rows(storage, rows, batch.rows());
+    return append_and_run(storage, batch, [&] {
+        check(kvflux_quant_write_tail(storage.key_base(), storage.value_base(), storage.key_scales(),
+                                      storage.value_scales(), layout.num_blocks(), layout.num_kv_heads(),
+                                      layout.block_size(), layout.head_size(), detail::abi_format(layout.format()),
+                                      rows.key, rows.value, detail::abi_dtype(rows.dtype), strides.first,
+                                      strides.second, batch.device_table(), batch.capacity_blocks(),
+                                      batch.device_lengths(), batch.rows(), nullptr),
+              "decode step quantised KV write");
+        enqueue_batch_attention(storage, batch, query_device, output_device, query_heads);
     });
 }
 

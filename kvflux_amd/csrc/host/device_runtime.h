@@ -166,8 +166,8 @@ inline int abi_dtype(DType dtype) {
 
 // Q and O must be device buffers on the storage GPU, disjoint from each
 // other and from the cache.
-inline void validate_q_o(const PagedKVStorage& storage, const float* query, float* output,
-                         std::size_t tensor_bytes) {
+template <typename Storage>
+void validate_q_o(const Storage& storage, const float* query, float* output, std::size_t tensor_bytes) {
     const auto& layout = storage.layout();
     require_device_pointer(query, storage.device(), "Q");
     require_device_pointer(output, storage.device(), "attention output");

@@ -1,12 +1,15 @@
-// Library-internal: grouping of a batch's rows by their shared pages, and the
-// checks of projected rows, for the calls of shared_prefix.h and norm_rope_write.h.
+// Library-internal: grouping of a batch's rows by their shared pages, the checks of
+// projected and of new rows, and what the calls on an 8-bit cache share, for
+// shared_prefix.h, norm_rope_write.h and quantized_kv.h.
 #pragma once
 
 #include "kvflux/v2/norm_rope_write.h"
+#include "kvflux/v2/quantized_kv.h"
 #include "kvflux/v2/shared_prefix.h"
 
 #include <cstddef>
 #include <cstdint>
+#include <utility>
 #include <vector>
 
 namespace kvflux::v2::detail {
@@ -39,5 +42,21 @@ struct ProjectionStrides {
 // be normed, rotated and written; the current device is the storage's.
 ProjectionStrides check_projection(const PagedKVStorage& storage, const ProjectedRows& rows, const NormRope& form,
                                    std::size_t query_heads, std::size_t tokens, const float* query_out);
+
+// kvflux_quant_format of a format.
+int abi_format(QuantFormat format);
+
+// Strides of K and V rows (never 0); throws std::invalid_argument (std::overflow_error for
+// sizes) unless `tokens` such rows can be written. The current device is the storage's.
+std::pair<std::size_t, std::size_t> check_new_rows(const QuantizedKVStorage& storage, const NewRows& rows,
+                                                   std::size_t tokens);
+
+// Enqueues the copies of {source, destination} pages (a device array) and of their scales.
+void copy_quantized_pages(const QuantizedKVStorage& storage, const std::uint64_t* pairs, std::size_t count);
+
+// Enqueues the decode attention of `rows` rows of a device table.
+void enqueue_quantized_decode(const QuantizedKVStorage& storage, const std::uint64_t* table, std::size_t width,
+                              const std::uint64_t* lengths, std::size_t max_len, std::size_t rows, const float* query,
+                              float* output, std::size_t query_heads);
 
 } // namespace kvflux::v2::detail
