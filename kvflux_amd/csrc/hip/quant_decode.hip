@@ -5,8 +5,13 @@
 //
 // What bounds it is the reading of K and V, one byte a value: half the time of a
 // 16-bit cache is left for the same arithmetic. So
-//  * bytes are widened in registers, where the matrix instructions take them (one
-//    conversion for two values; both formats are exact in FP16), never through LDS;
+//  * K and V are read past the caches, whole 128-byte lines by one instruction, two
+//    tiles ahead, and reach the matrix instructions through a wavefront's own LDS
+//    (no barrier). 128 rows of <= 32768 tokens, 8 kv heads of 128: 747 us, 6.3 TB/s;
+//    with loads in the operands' own layout, which split lines, 805 us. Loads alone
+//    take 705 us. The same loads without the streaming hint took 1611 us;
+//  * bytes are widened in registers, one conversion for two values; both formats are
+//    exact in FP16;
 //  * the products are FP16 MFMAs with FP32 sums, on Q and the weights in two FP16
 //    parts: x = hi + lo, off by at most 2^-23 of x (half a step of hi is 2^-12, and
 //    lo has 11 bits of what is left), the size of FP32's own rounding;
@@ -16,8 +21,7 @@
 //    are columns (up to 16), S^T = K Q^T and O^T += V^T P^T on 16x16x32. Row i of
 //    K's block b is token 8 (i / 4) + 4 b + i % 4, so that lane (quad, col) holds the
 //    scores of tokens 8 quad .. 8 quad + 7: the second product's operand as it is.
-//    V's operand wants eight tokens of one dim in a lane: the lane loads a few dims
-//    of each (D / 16 bytes) and takes bytes of two tokens together (v_perm_b32).
+//    V's operand wants eight tokens of one dim in a lane: the transposing LDS read.
 //
 // The work of a call is a list of streams, a row's tokens for one kv head (and up to
 // 16 of its query heads), cut into equal shares: workgroup w of N takes the tiles
@@ -48,6 +52,9 @@ constexpr std::uint64_t kOneLaunch = 512;
 // so two parts miss a weight by at most 2^-40 of the largest, or 2^-23 of itself.
 constexpr float kWeightScale = 32768.0f;
 
+typedef __attribute__((ext_vector_type(2))) int qd_i32x2_t;
+typedef __attribute__((address_space(3))) qd_i32x2_t qd_lds_i32x2_t;
+
 struct QuantDecodeParams {
     const std::uint8_t* key_cache;
     const std::uint8_t* value_cache;
@@ -68,7 +75,7 @@ struct QuantDecodeParams {
     float* output;
     float scale_log2;             // log2(e) / sqrt(D)
     // Workspace: for every workgroup the stream that it begins and does not end, with
-    // the last workgroup of it, and two partials (see part_slot).
+    // the last workgroup of it, and two partials.
     uint2* cuts;                  // [grid] {stream, last workgroup}, {~0, .}: none
     float* part_acc;              // [2 * grid][set_heads][D]
     float* part_ml;               // [2 * grid][set_heads][2]
@@ -82,23 +89,23 @@ __device__ inline float merge_weight(float m, float top) {
 // A caller's FP32 arrays are only known to be float-aligned.
 struct Float4 { float x, y, z, w; };
 
-// What the lanes of a wavefront know of kSub tokens of a tile: where the first one's
-// K and V rows lie in the caches, how many of them count (above bit 56), ks, and vs
-// over the wavefront's reference times kWeightScale.
-struct alignas(16) Record {
-    std::uint64_t at;
-    float ks, vs;
-};
+// A record is what the lanes of a wavefront know of kSub tokens of a tile: where the
+// first one's K and V rows lie in the caches and how many of them count (above bit 56);
+// ks, and vs over the wavefront's reference times kWeightScale.
 constexpr int kCountShift = 56;
 constexpr std::uint64_t kOffsetMask = (std::uint64_t{1} << kCountShift) - 1;
 
 template <int kD>
 struct Shape {
     static constexpr int kSteps = kD / 32;   // MFMAs of a 16-token block of S^T for one part of Q
-    static constexpr int kChunks = kD / 64;  // 16-byte loads of a K row by a lane
-    static constexpr int kDt = kD / 16;      // MFMAs of O^T for one part of the weights, and bytes of a V row a lane loads
-    static constexpr int kWords = kDt / 4;
+    static constexpr int kDt = kD / 16;      // MFMAs of O^T for one part of the weights
+    static constexpr int kCpr = kD / 16;     // 16-byte chunks of a row
+    static constexpr int kLoads = kCpr / 2;  // loads of a tile's K (and V) by a wavefront
+    static constexpr int kRowsOf = 64 / kCpr;  // rows of a load
     static constexpr int kPad = kD + 4;      // floats of a row of the merge buffer
+    // LDS of a wavefront: its tile, K then V, and at a part's end its sums.
+    static constexpr int kTileBytes = 2 * static_cast<int>(kTile) * kD;
+    static constexpr int kWaveBytes = kTileBytes > static_cast<int>(kCols) * kPad * 4 ? kTileBytes : static_cast<int>(kCols) * kPad * 4;
     static constexpr int kResident = kD == 256 ? 1 : 2;  // workgroups of a CU
     static constexpr std::uint32_t kGrid = 256 * kResident;
 };
@@ -110,14 +117,15 @@ template <typename F, int kD, int kSub, bool kWhole>
 __global__ __launch_bounds__(kThreads, Shape<kD>::kResident) void quant_decode_kernel(QuantDecodeParams p) {
     using S = Shape<kD>;
     using Vec = pf_f16x8_t;
-    constexpr int kSteps = S::kSteps, kChunks = S::kChunks, kDt = S::kDt, kWords = S::kWords;
+    constexpr int kSteps = S::kSteps, kDt = S::kDt, kCpr = S::kCpr, kLoads = S::kLoads, kRowsOf = S::kRowsOf;
     constexpr std::uint32_t kPerTile = kTile / kSub;      // records of a tile
     constexpr std::uint32_t kBatch = 64 / kPerTile;       // tiles whose records the lanes make at once
     __shared__ std::uint64_t before[kWhole ? 1 : kPlanRows + 1];  // costs of a stream of each row before
     __shared__ std::uint32_t lens_of[kWhole ? 1 : kPlanRows];
     __shared__ std::uint64_t wave_cost[kWaves];
-    __shared__ Record records[kWaves][2][64];
-    __shared__ __attribute__((aligned(16))) float reduce[kWaves * kCols * S::kPad];
+    __shared__ std::uint64_t places[kWaves][2][64];
+    __shared__ float2 scales_of[kWaves][2][64];
+    __shared__ __attribute__((aligned(16))) unsigned char wave_lds[kWaves][S::kWaveBytes];
     __shared__ float2 stats[kWaves][kCols];
 
     const int tid = threadIdx.x, lane = tid % 64;
@@ -168,26 +176,56 @@ __global__ __launch_bounds__(kThreads, Shape<kD>::kResident) void quant_decode_k
                 const std::uint64_t at = (id == ~0ull ? 0 : id) * p.heads + kvh;
                 return Scales{p.key_scales[at], p.value_scales[at]};
             };
-            float next_ref = 0.0f;
-            const auto put_records = [&](std::uint32_t batch, std::uint64_t id, const Scales& s) {
+            const auto put_places = [&](std::uint32_t batch, std::uint64_t id) {
                 const std::uint32_t token = token_of(batch);
+                std::uint64_t at = 0;
+                if (id != ~0ull) {
+                    const std::uint32_t count = len - token < kSub ? len - token : kSub;
+                    at = ((id * p.heads + kvh) * bs + p.block_size.mod(token)) * kD | static_cast<std::uint64_t>(count) << kCountShift;
+                }
+                places[wave][batch & 1][lane] = at;
+                __builtin_amdgcn_wave_barrier();  // a wavefront's LDS accesses are in order
+            };
+            float next_ref = 0.0f;
+            const auto put_scales = [&](std::uint32_t batch, std::uint64_t id, const Scales& s) {
                 const bool live = id != ~0ull;
                 const float mine = live ? s.v : 0.0f;
                 float top = __builtin_fabsf(mine);
 #pragma unroll
                 for (int d = 1; d < 64; d <<= 1) top = fmaxf(top, __shfl_xor(top, d));
                 next_ref = fmaxf(next_ref, top);
-                Record r{0, live ? s.k : 0.0f, next_ref > 0.0f ? mine / next_ref * kWeightScale : mine};
-                if (live) {
-                    const std::uint32_t in_page = p.block_size.mod(token);
-                    const std::uint32_t count = len - token < kSub ? len - token : kSub;
-                    r.at = ((id * p.heads + kvh) * bs + in_page) * kD | static_cast<std::uint64_t>(count) << kCountShift;
+                scales_of[wave][batch & 1][lane] = make_float2(live ? s.k : 0.0f, next_ref > 0.0f ? mine / next_ref * kWeightScale : mine);
+                __builtin_amdgcn_wave_barrier();
+            };
+
+            struct Tile {
+                uint4 k[kLoads], v[kLoads];
+            };
+            // Load i of a tile: kRowsOf whole rows, 16 bytes a lane; every 128-byte line is
+            // read by one instruction, so both caches are streamed past the others. Every
+            // load is unconditional: places past the last tile lead to the pool's first rows.
+            const std::uint32_t my_row = static_cast<std::uint32_t>(lane) / kCpr, my_chunk = static_cast<std::uint32_t>(lane) % kCpr;
+            const auto load = [&](std::uint32_t j, Tile& b) {
+                const std::uint64_t* const r = places[wave][j / kBatch & 1] + j % kBatch * kPerTile;
+#pragma unroll
+                for (int i = 0; i < kLoads; ++i) {
+                    std::uint64_t at;
+                    if constexpr (kSub == 8 && kRowsOf <= 8) {  // one place for all lanes
+                        const std::uint64_t x = r[i * kRowsOf / 8];
+                        const std::uint32_t lo = uniform(static_cast<std::uint32_t>(x)), hi = uniform(static_cast<std::uint32_t>(x >> 32));
+                        at = ((static_cast<std::uint64_t>(hi) << 32 | lo) & kOffsetMask) + i * kRowsOf % 8 * kD + (my_row * kD + my_chunk * 16);
+                    } else {
+                        const std::uint32_t token = i * kRowsOf + my_row;
+                        at = (r[token / kSub] & kOffsetMask) + token % kSub * kD + my_chunk * 16;
+                    }
+                    b.k[i] = __builtin_bit_cast(uint4, stream_load(reinterpret_cast<const V16*>(p.key_cache + at)));
+                    b.v[i] = __builtin_bit_cast(uint4, stream_load(reinterpret_cast<const V16*>(p.value_cache + at)));
                 }
-                records[wave][batch & 1][lane] = r;
-                __builtin_amdgcn_wave_barrier();  // a wavefront's LDS accesses are in order
             };
             std::uint64_t page_now = fetch_page(0);
             std::uint64_t page_next = fetch_page(1);
+            put_places(0, page_now);
+            Scales scales_now = fetch_scales(page_now);
 
             // Queries: column `col` is head col of the set (the others repeat the
             // last), lane (quad, col) holds dims 64 m + 16 quad + 8 h of step 2 m + h,
@@ -195,6 +233,7 @@ __global__ __launch_bounds__(kThreads, Shape<kD>::kResident) void quant_decode_k
             // is split times a power of two, undone with its scores' scale.
             Vec q_hi[kSteps], q_lo[kSteps];
             float down;
+            Tile b0, b1;
             {
                 const std::uint32_t head = kvh * p.group + first_head + (static_cast<std::uint32_t>(col) < heads ? col : heads - 1);
                 const float* const src = p.query + ((static_cast<std::uint64_t>(p.row_base) + row) * p.query_heads + head) * kD + 16 * quad;
@@ -204,7 +243,8 @@ __global__ __launch_bounds__(kThreads, Shape<kD>::kResident) void quant_decode_k
 #pragma unroll
                     for (int i = 0; i < 2; ++i)
                         raw[kk][i] = *reinterpret_cast<const Float4*>(src + 64 * (kk / 2) + 8 * (kk % 2) + 4 * i);
-                Scales s = fetch_scales(page_now);
+                load(0, b0);
+                load(1, b1);
                 float largest = 0.0f;
 #pragma unroll
                 for (int kk = 0; kk < kSteps; ++kk)
@@ -237,46 +277,33 @@ __global__ __launch_bounds__(kThreads, Shape<kD>::kResident) void quant_decode_k
                     q_hi[kk] = __builtin_bit_cast(Vec, make_uint4(hi[0], hi[1], hi[2], hi[3]));
                     q_lo[kk] = __builtin_bit_cast(Vec, make_uint4(lo[0], lo[1], lo[2], lo[3]));
                 }
-                put_records(0, page_now, s);
+                put_scales(0, page_now, scales_now);
                 if (next_ref > 0.0f) value_ref = next_ref;  // else all are 0 or NaN, in any unit
             }
             page_now = page_next;
-            Scales scales_now = fetch_scales(page_now);
+            scales_now = fetch_scales(page_now);
             page_next = fetch_page(2);
-            // Records of batch `b`, and the fetches for the ones behind it.
+            // Places and scales of batch `b`, and the fetches for the ones behind it.
             const auto stage = [&](std::uint32_t b) {
-                put_records(b, page_now, scales_now);
+                put_places(b, page_now);
+                put_scales(b, page_now, scales_now);
                 page_now = page_next;
                 scales_now = fetch_scales(page_now);
                 page_next = fetch_page(b + 2);
             };
 
-            struct Tile {
-                uint4 k[2][kChunks];
-                std::uint32_t v[8][kWords];
+            // Rows of a tile in LDS: chunk c of row t at slot c ^ f(t), so that the rows of a
+            // read fall on different banks: K 16 rows of one chunk (8 at a time, see the
+            // order of tokens), V 8 rows of one chunk.
+            unsigned char* const k_lds = wave_lds[wave];
+            unsigned char* const v_lds = k_lds + kTile * kD;
+            const auto k_slot = [](std::uint32_t t, std::uint32_t c) {
+                return c ^ (kCpr == 4 ? (t >> 1 & 1) | (t >> 3 & 1) << 1 : (t & 3) | (t >> 3 & 1) << 2);
             };
-            // Every load is unconditional: records past the last tile lead to the
-            // pool's first rows.
-            const auto load = [&](std::uint32_t j, Tile& b) {
-                const Record* const r = records[wave][j / kBatch & 1] + j % kBatch * kPerTile;
-                const auto row_of = [&](std::uint32_t token) -> std::uint64_t {
-                    if constexpr (kSub == 8) return (r[token / 8].at & kOffsetMask) + token % 8 * kD;
-                    return r[token].at & kOffsetMask;
-                };
-#pragma unroll
-                for (int blk = 0; blk < 2; ++blk) {
-                    const std::uint8_t* const src = p.key_cache + row_of(8 * (col / 4) + 4 * blk + col % 4) + 16 * quad;
-#pragma unroll
-                    for (int m = 0; m < kChunks; ++m) b.k[blk][m] = *reinterpret_cast<const uint4*>(src + 64 * m);
-                }
-#pragma unroll
-                for (int t = 0; t < 8; ++t) {
-                    const std::uint8_t* const src = p.value_cache + row_of(8 * quad + t) + kDt * col;
-                    __builtin_memcpy(b.v[t], __builtin_assume_aligned(src, kDt < 16 ? kDt : 16), kDt);
-                }
-            };
+            const auto v_slot = [](std::uint32_t t, std::uint32_t c) { return c ^ (kCpr == 4 ? t >> 1 & 3 : t & 7); };
             const auto compute = [&](std::uint32_t j, Tile& b) {
-                const Record* const r = records[wave][j / kBatch & 1] + j % kBatch * kPerTile;
+                const std::uint64_t* const r = places[wave][j / kBatch & 1] + j % kBatch * kPerTile;
+                const float2* const rs = scales_of[wave][j / kBatch & 1] + j % kBatch * kPerTile;
                 if (j % kBatch == 0 && value_ref != next_ref && next_ref > 0.0f) {  // uniform
                     const float f = value_ref / next_ref;
 #pragma unroll
@@ -289,21 +316,35 @@ __global__ __launch_bounds__(kThreads, Shape<kD>::kResident) void quant_decode_k
                 std::uint32_t live = 0;  // a bit for each of the eight that count
 #pragma unroll
                 for (int i = 0; i < kOwn; ++i) {
-                    const Record x = r[kSub == 8 ? quad : 8 * quad + i];
-                    const float k = x.ks * down;
+                    const int at = kSub == 8 ? quad : 8 * quad + i;
+                    const float2 x = rs[at];
+                    const float k = x.x * down;
                     ks[i] = k > 3.0e38f ? 3.0e38f : k;  // finite: a product of 0 stays 0
-                    vs[i] = x.vs;
-                    const std::uint32_t count = static_cast<std::uint32_t>(x.at >> kCountShift);
+                    vs[i] = x.y;
+                    const std::uint32_t count = static_cast<std::uint32_t>(r[at] >> kCountShift);
                     live |= ((1u << count) - 1) << i;
                 }
+                const bool part = __builtin_amdgcn_ballot_w64(live != 0xffu) != 0;  // a row's end, or a missing page
+#pragma unroll
+                for (int i = 0; i < kLoads; ++i) {
+                    const std::uint32_t t = i * kRowsOf + my_row;
+                    *reinterpret_cast<uint4*>(k_lds + t * kD + 16 * k_slot(t, my_chunk)) = b.k[i];
+                    *reinterpret_cast<uint4*>(v_lds + t * kD + 16 * v_slot(t, my_chunk)) = b.v[i];
+                    if (part) {  // uniform; 0 * NaN would stay
+                        const std::uint32_t count = static_cast<std::uint32_t>(r[kSub == 8 ? t / 8 : t] >> kCountShift);
+                        if (t % kSub >= count) *reinterpret_cast<uint4*>(v_lds + t * kD + 16 * v_slot(t, my_chunk)) = make_uint4(0, 0, 0, 0);
+                    }
+                }
+                __builtin_amdgcn_wave_barrier();
                 pf_f32x4_t s[2];
 #pragma unroll
                 for (int blk = 0; blk < 2; ++blk) {
                     s[blk] = pf_f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
                     Vec a[kSteps];
+                    const std::uint32_t t = 8 * (col / 4) + 4 * blk + col % 4;
 #pragma unroll
-                    for (int m = 0; m < kChunks; ++m) {
-                        const uint4 w = b.k[blk][m];
+                    for (int m = 0; m < kSteps / 2; ++m) {
+                        const uint4 w = *reinterpret_cast<const uint4*>(k_lds + t * kD + 16 * k_slot(t, 4 * m + quad));
                         a[2 * m] = __builtin_bit_cast(Vec, make_uint4(F::template pair16<0>(w.x), F::template pair16<1>(w.x),
                                                                       F::template pair16<0>(w.y), F::template pair16<1>(w.y)));
                         a[2 * m + 1] = __builtin_bit_cast(Vec, make_uint4(F::template pair16<0>(w.z), F::template pair16<1>(w.z),
@@ -317,15 +358,10 @@ __global__ __launch_bounds__(kThreads, Shape<kD>::kResident) void quant_decode_k
                 float x[8];
 #pragma unroll
                 for (int t = 0; t < 8; ++t) x[t] = s[t / 4][t % 4] * ks[kSub == 8 ? 0 : t];
-                const bool part = __builtin_amdgcn_ballot_w64(live != 0xffu) != 0;
-                if (part) {  // uniform: a row's end, or a missing page
+                if (part) {  // uniform
 #pragma unroll
-                    for (int t = 0; t < 8; ++t) {
-                        if (live >> t & 1) continue;
-                        x[t] = -INFINITY;
-#pragma unroll
-                        for (int i = 0; i < kWords; ++i) b.v[t][i] = 0;  // 0 * NaN would stay
-                    }
+                    for (int t = 0; t < 8; ++t)
+                        if (!(live >> t & 1)) x[t] = -INFINITY;
                 }
                 const float top = max3(max3(x[0], x[1], x[2]), max3(x[3], x[4], x[5]), __builtin_elementwise_maximum(x[6], x[7]));
                 if (__builtin_expect(__builtin_amdgcn_ballot_w64(top > run_max) != 0, 0)) {  // uniform
@@ -357,32 +393,22 @@ __global__ __launch_bounds__(kThreads, Shape<kD>::kResident) void quant_decode_k
                 }
                 const Vec p_hi = __builtin_bit_cast(Vec, make_uint4(hi[0], hi[1], hi[2], hi[3]));
                 const Vec p_lo = __builtin_bit_cast(Vec, make_uint4(lo[0], lo[1], lo[2], lo[3]));
-                // Bytes i and i + 1 of two tokens' words together, then two dims' operands.
-                // A tile's products are summed from zero and added with one rounding: an
-                // MFMA on an accumulator that holds a dominant key's sum drops bits of
-                // the small weights, always in the same direction.
+                // V^T: a group of 16 lanes reads 8 tokens of 16 dims and leaves lane i with the
+                // tokens of dim i. A tile's products are summed from zero and added with one
+                // rounding: an MFMA on an accumulator that holds a dominant key's sum drops
+                // bits of the small weights, always in the same direction.
+                const std::uint32_t row = 8 * quad + col / 2;
 #pragma unroll
-                for (int i = 0; i < kWords; ++i)
-#pragma unroll
-                    for (int half = 0; half < 2; ++half) {
-                        std::uint32_t two[4];
-#pragma unroll
-                        for (int t = 0; t < 4; ++t)
-                            two[t] = __builtin_amdgcn_perm(b.v[2 * t + 1][i], b.v[2 * t][i], half == 0 ? 0x05010400u : 0x07030602u);
-                        const Vec a0 = __builtin_bit_cast(Vec, make_uint4(F::template pair16<0>(two[0]), F::template pair16<0>(two[1]),
-                                                                          F::template pair16<0>(two[2]), F::template pair16<0>(two[3])));
-                        const Vec a1 = __builtin_bit_cast(Vec, make_uint4(F::template pair16<1>(two[0]), F::template pair16<1>(two[1]),
-                                                                          F::template pair16<1>(two[2]), F::template pair16<1>(two[3])));
-                        const int dt = 4 * i + 2 * half;
-                        const pf_f32x4_t zero{0.0f, 0.0f, 0.0f, 0.0f};
-                        acc[dt] += PfF16::mma(a0, p_hi, PfF16::mma(a0, p_lo, zero));
-                        acc[dt + 1] += PfF16::mma(a1, p_hi, PfF16::mma(a1, p_lo, zero));
-                    }
+                for (int dt = 0; dt < kDt; ++dt) {
+                    const auto w = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
+                        (qd_lds_i32x2_t*)((__attribute__((address_space(3))) unsigned char*)v_lds + row * kD + 16 * v_slot(row, dt) + col % 2 * 8));
+                    const auto lo = static_cast<std::uint32_t>(w[0]), hi = static_cast<std::uint32_t>(w[1]);
+                    const Vec a = __builtin_bit_cast(Vec, make_uint4(F::template pair16<0>(lo), F::template pair16<1>(lo),
+                                                                     F::template pair16<0>(hi), F::template pair16<1>(hi)));
+                    acc[dt] += PfF16::mma(a, p_hi, PfF16::mma(a, p_lo, pf_f32x4_t{0.0f, 0.0f, 0.0f, 0.0f}));
+                }
             };
 
-            Tile b0, b1;
-            load(0, b0);
-            load(1, b1);
 #pragma unroll 1
             for (std::uint32_t j = 0; j < tiles; j += 2) {
                 compute(j, b0);
@@ -393,19 +419,16 @@ __global__ __launch_bounds__(kThreads, Shape<kD>::kResident) void quant_decode_k
             }
         }
 
-        // The wavefronts' sums: in units of 1, then merged. acc[dt][r] is dim
-        // (4 quad + r) kDt + dt of head col.
+        // The wavefronts' sums: in units of 1, then merged. acc[dt][r] is dim 16 dt + 4 quad + r
+        // of head col.
         const float total = sum_across_quads(run_sum + run_low);
         if (quad == 0) stats[wave][col] = make_float2(run_max, total);
         const float unit = value_ref * (1.0f / kWeightScale);
         if (static_cast<std::uint32_t>(col) < heads) {
-            float* const row_to = reduce + (wave * kCols + col) * S::kPad + 4 * quad * kDt;
+            float* const row_to = reinterpret_cast<float*>(wave_lds[wave]) + col * S::kPad + 4 * quad;
 #pragma unroll
-            for (int r = 0; r < 4; ++r)
-#pragma unroll
-                for (int dt = 0; dt < kDt; dt += 4)
-                    *reinterpret_cast<float4*>(row_to + r * kDt + dt) =
-                        make_float4(acc[dt][r] * unit, acc[dt + 1][r] * unit, acc[dt + 2][r] * unit, acc[dt + 3][r] * unit);
+            for (int dt = 0; dt < kDt; ++dt)
+                *reinterpret_cast<float4*>(row_to + 16 * dt) = make_float4(acc[dt][0] * unit, acc[dt][1] * unit, acc[dt][2] * unit, acc[dt][3] * unit);
         }
         __syncthreads();
         for (std::uint32_t i = tid; i < heads * kD; i += kThreads) {
@@ -419,7 +442,7 @@ __global__ __launch_bounds__(kThreads, Shape<kD>::kResident) void quant_decode_k
                 const float2 s = stats[w][h];
                 const float f = s.y != s.y ? s.y : merge_weight(s.x, top);
                 sum += s.y * f;
-                o += reduce[(w * kCols + h) * S::kPad + d] * f;
+                o += reinterpret_cast<const float*>(wave_lds[w])[h * S::kPad + d] * f;
             }
             if (ml == nullptr) {
                 to[i] = sum == 0.0f ? 0.0f : o / sum;
@@ -431,7 +454,7 @@ __global__ __launch_bounds__(kThreads, Shape<kD>::kResident) void quant_decode_k
                 }
             }
         }
-        __syncthreads();  // reduce and stats are used again
+        __syncthreads();  // the buffers and stats are used again
     };
     const auto output_of = [&](std::uint32_t row, std::uint32_t kvh, std::uint32_t set) {
         return p.output + ((static_cast<std::uint64_t>(p.row_base) + row) * p.query_heads + kvh * p.group + set * p.set_heads) * kD;
