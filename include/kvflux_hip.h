@@ -544,7 +544,8 @@ int kvflux_quant_gather(const void* key_cache, const void* value_cache, const fl
  * bytes, take a generic kernel (a lane a token, tens of times slower).
  * workspace: kvflux_quant_attention_workspace_size bytes, aligned to 8 (no
  * initialisation needed; calls that share one must be ordered); NULL where that is 0
- * (kv_len of at most 512). */
+ * (short rows). What one call needs is enough for calls of fewer rows and smaller
+ * kv_len. */
 int kvflux_quant_attention_workspace_size(uint64_t num_rows, uint64_t kv_len, uint64_t num_kv_heads,
                                           uint64_t query_heads, uint64_t block_size, uint64_t head_size,
                                           size_t* bytes);

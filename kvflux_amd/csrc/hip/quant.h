@@ -89,6 +89,29 @@ struct QuantInt8 {
     }
 };
 
+// op over a wavefront's 64 values, the same in every lane: lane permutations of the
+// VALU, a few cycles a step where a shuffle through LDS takes some 60.
+template <typename T, typename Op>
+__device__ inline T over_wave(T x, Op op) {
+    static_assert(sizeof(T) == 4, "a register");
+    const auto with = [&](int bits) { x = op(x, __builtin_bit_cast(T, bits)); };
+    const auto bits = [&] { return __builtin_bit_cast(int, x); };
+    with(__builtin_amdgcn_update_dpp(0, bits(), 0xb1, 0xf, 0xf, true));   // quad_perm: lane ^ 1
+    with(__builtin_amdgcn_update_dpp(0, bits(), 0x4e, 0xf, 0xf, true));   // quad_perm: lane ^ 2
+    with(__builtin_amdgcn_update_dpp(0, bits(), 0x141, 0xf, 0xf, true));  // row_half_mirror
+    with(__builtin_amdgcn_update_dpp(0, bits(), 0x140, 0xf, 0xf, true));  // row_mirror
+    // The pair's values are copied out: a bit cast of a vector's element reads the first.
+    const auto a = __builtin_amdgcn_permlane16_swap(static_cast<unsigned>(bits()), static_cast<unsigned>(bits()), false, false);
+    const unsigned a0 = a[0], a1 = a[1];
+    x = op(__builtin_bit_cast(T, a0), __builtin_bit_cast(T, a1));
+    const auto b = __builtin_amdgcn_permlane32_swap(static_cast<unsigned>(bits()), static_cast<unsigned>(bits()), false, false);
+    const unsigned b0 = b[0], b1 = b[1];
+    return op(__builtin_bit_cast(T, b0), __builtin_bit_cast(T, b1));
+}
+__device__ inline float wave_max(float x) {  // of what is no NaN
+    return over_wave(x, [](float a, float b) { return fmaxf(a, b); });
+}
+
 // The scale for values whose largest magnitude has the FP32 bits `largest`; NaN for
 // an infinity or NaN. 2^-110 at least: every value of either format times it is a
 // normal FP32 number (2^-9 * 2^-110 > 2^-126), zeros apart.

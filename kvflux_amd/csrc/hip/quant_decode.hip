@@ -42,12 +42,20 @@ constexpr int kWaves = kThreads / 64;
 constexpr std::uint32_t kTile = 32;       // tokens of a wavefront's step
 constexpr std::uint32_t kCols = 16;       // query heads of a stream
 constexpr std::uint32_t kPlanRows = 2048; // rows of a launch
-// Cost of a part's start and end, in tiles of a workgroup.
-constexpr std::uint32_t kPartCost = 4;
-// The least tiles of a share: fewer workgroups start where there is less to do.
+// Cost of a part's start and end (a chain of loads, 4 us) in tiles of a workgroup. At 4
+// and at 16: 4 rows of <= 1500 tokens 14.7 and 12.3 us, 16 rows of <= 8192 27.5 and 25.3,
+// 256 rows of <= 1024 80 and 67, 128 rows of <= 32768 742 and 722; 28 is behind again.
+constexpr std::uint32_t kPartCost = 16;
+// The least of a share: fewer workgroups start where there is less to do. 4 rows of
+// <= 1500 tokens: 6 16.4 us, 8 12.3, 10 13.2, 16 13.8.
 constexpr std::uint32_t kLeastShare = 8;
-// Rows of at most this many tokens take one workgroup a stream and no merge.
-constexpr std::uint64_t kOneLaunch = 512;
+// Rows of at most this many tokens (half of it with heads of 256) take one workgroup a
+// stream and no merge; twice as many where the streams fill the GPU by themselves.
+// A workgroup a stream, and shares: 1 row of <= 1024 tokens 8.9 and 11.5 us, 8 rows 13.0
+// and 14.2, 256 rows 67.6 and 75.7; 32 rows of <= 2048 21.1 and 24.2, but 8 rows 20.4 and
+// 14.8, and 128 rows of <= 4096 108 and 102.
+constexpr std::uint64_t kOneLaunch = 1024;
+constexpr std::uint64_t kFullStreams = 256;
 // The weights' FP16 parts are of 2^15 times a weight of at most 1: FP16 ends at 2^-24,
 // so two parts miss a weight by at most 2^-40 of the largest, or 2^-23 of itself.
 constexpr float kWeightScale = 32768.0f;
@@ -74,9 +82,9 @@ struct QuantDecodeParams {
     const float* query;
     float* output;
     float scale_log2;             // log2(e) / sqrt(D)
-    // Workspace: for every workgroup the stream that it begins and does not end, with
-    // the last workgroup of it, and two partials.
-    uint2* cuts;                  // [grid] {stream, last workgroup}, {~0, .}: none
+    // Workspace: the streams that are cut, and two partials of every workgroup.
+    std::uint32_t by_stream;      // a cut for every stream, else for every workgroup
+    uint2* cuts;                  // [grid] {stream, or the workgroup that begins it; the last workgroup}, {~0, .}: none
     float* part_acc;              // [2 * grid][set_heads][D]
     float* part_ml;               // [2 * grid][set_heads][2]
 };
@@ -190,10 +198,7 @@ __global__ __launch_bounds__(kThreads, Shape<kD>::kResident) void quant_decode_k
             const auto put_scales = [&](std::uint32_t batch, std::uint64_t id, const Scales& s) {
                 const bool live = id != ~0ull;
                 const float mine = live ? s.v : 0.0f;
-                float top = __builtin_fabsf(mine);
-#pragma unroll
-                for (int d = 1; d < 64; d <<= 1) top = fmaxf(top, __shfl_xor(top, d));
-                next_ref = fmaxf(next_ref, top);
+                next_ref = fmaxf(next_ref, wave_max(__builtin_fabsf(mine)));
                 scales_of[wave][batch & 1][lane] = make_float2(live ? s.k : 0.0f, next_ref > 0.0f ? mine / next_ref * kWeightScale : mine);
                 __builtin_amdgcn_wave_barrier();
             };
@@ -500,23 +505,25 @@ __global__ __launch_bounds__(kThreads, Shape<kD>::kResident) void quant_decode_k
         const std::uint64_t wanted = total / kLeastShare;
         const std::uint32_t shares = wanted == 0 ? 1 : wanted < gridDim.x ? static_cast<std::uint32_t>(wanted) : gridDim.x;
         const std::uint64_t each = total / shares;
-        const std::uint32_t more = static_cast<std::uint32_t>(total % shares);  // the first shares have one more
+        const std::uint32_t more = static_cast<std::uint32_t>(total - each * shares);  // the first shares have one more
         const std::uint32_t w = blockIdx.x;
         // Rows without tokens: zeros.
         for (std::uint32_t r = w; r < p.rows; r += gridDim.x) {
             if (lens_of[r] != 0) continue;
+            if (p.by_stream && tid < streams) p.cuts[r * streams + tid] = make_uint2(~0u, 0);
             float* const out = p.output + (static_cast<std::uint64_t>(p.row_base) + r) * p.query_heads * kD;
             for (std::uint32_t i = tid; i < p.query_heads * kD; i += kThreads) out[i] = 0.0f;
         }
-        if (tid == 0) p.cuts[w] = make_uint2(~0u, 0);
+        if (tid == 0 && !p.by_stream) p.cuts[w] = make_uint2(~0u, 0);
         if (w >= shares) return;
         const std::uint64_t begin = each * w + (w < more ? w : more), end = begin + each + (w < more ? 1 : 0);
-        // The row of the first stream.
-        std::uint32_t row = 0, hi = p.rows;
-        while (hi - row > 1) {
-            const std::uint32_t mid = (row + hi) / 2;
-            if (before[mid] * streams <= begin) row = mid;
-            else hi = mid;
+        // The row of the first stream: the last one that begins at or before it.
+        std::uint32_t row = 0;
+        for (std::uint32_t step = p.rows > 64 ? 64 : 1;; step = 1) {
+            const std::uint32_t r = row + lane * step;
+            const std::uint64_t behind = __builtin_amdgcn_ballot_w64(r < p.rows && before[r < p.rows ? r : 0] * streams <= begin);
+            row += (__builtin_popcountll(behind) - 1) * step;
+            if (step == 1) break;
         }
         std::uint64_t at = begin;
         while (at < end) {
@@ -539,11 +546,16 @@ __global__ __launch_bounds__(kThreads, Shape<kD>::kResident) void quant_decode_k
                 const std::uint32_t slot = 2 * w + (t0 == 0 ? 1 : 0);
                 run_part(row, len, kvh, set, t0, t1, whole ? output_of(row, kvh, set) : p.part_acc + static_cast<std::uint64_t>(slot) * p.set_heads * kD,
                          whole ? nullptr : p.part_ml + static_cast<std::uint64_t>(slot) * p.set_heads * 2);
-                if (t0 == 0 && !whole && tid == 0) {
-                    // The workgroup of the stream's last tile, at cost stop - 1.
-                    const std::uint64_t x = stop - 1, longer = (each + 1) * more;
-                    const std::uint64_t last = x < longer ? x / (each + 1) : more + (x - longer) / each;
-                    p.cuts[w] = make_uint2(row * streams + stream, static_cast<std::uint32_t>(last));
+                if (t0 == 0 && tid == 0) {
+                    const std::uint32_t index = row * streams + stream;
+                    if (!whole) {
+                        // The workgroup of the stream's last tile, at cost stop - 1.
+                        const std::uint64_t x = stop - 1, longer = (each + 1) * more;
+                        const std::uint64_t last = x < longer ? x / (each + 1) : more + (x - longer) / each;
+                        p.cuts[p.by_stream ? index : w] = make_uint2(p.by_stream ? w : index, static_cast<std::uint32_t>(last));
+                    } else if (p.by_stream) {
+                        p.cuts[index] = make_uint2(~0u, 0);
+                    }
                 }
             }
             at = until;
@@ -551,20 +563,21 @@ __global__ __launch_bounds__(kThreads, Shape<kD>::kResident) void quant_decode_k
     }
 }
 
-// Merges the parts of the stream that workgroup blockIdx.x cut: its own second
-// partial and the first ones of the workgroups up to the last, in that order, so
-// results are the same from call to call. A block is one query head; kMergeThreads
+// Merges the parts of a cut stream: the second partial of the workgroup that begins it
+// and the first ones of the workgroups up to the last, in that order, so results are the
+// same from call to call. blockIdx.x is the stream, or the workgroup that begins it. A block is one query head; kMergeThreads
 // hold kD / 4 dims of neighbouring parts each.
 template <int kD, int kMergeThreads>
 __global__ __launch_bounds__(kMergeThreads) void quant_decode_merge_kernel(QuantDecodeParams p) {
     constexpr std::uint32_t kLanes = kD / 4, kGroups = kMergeThreads / kLanes;
     __shared__ float4 sums[kMergeThreads];
     __shared__ float2 ml_of[kGroups];
-    const std::uint32_t w = blockIdx.x, h = blockIdx.y;
-    const uint2 cut = p.cuts[w];
+    const std::uint32_t h = blockIdx.y;
+    const uint2 cut = p.cuts[blockIdx.x];
     if (cut.x == ~0u) return;
+    const std::uint32_t w = p.by_stream ? cut.x : blockIdx.x, index = p.by_stream ? blockIdx.x : cut.x;
     const std::uint32_t streams = p.heads * p.sets;
-    const std::uint32_t row = cut.x / streams, stream = cut.x % streams, kvh = stream / p.sets, set = stream % p.sets;
+    const std::uint32_t row = index / streams, stream = index % streams, kvh = stream / p.sets, set = stream % p.sets;
     const std::uint32_t head = set * p.set_heads + h;
     if (head >= p.group) return;
     const std::uint32_t parts = cut.y - w + 1;
@@ -732,7 +745,8 @@ void head_sets(std::uint64_t group, std::uint32_t* sets, std::uint32_t* heads) {
 
 // Workgroups of a launch over `rows` rows; 0: one for each stream.
 std::uint32_t decode_grid(std::uint64_t rows, std::uint64_t kv_len, std::uint64_t streams, std::uint64_t head_size) {
-    if (kv_len <= kOneLaunch) return 0;
+    const std::uint64_t whole = head_size == 256 ? kOneLaunch / 2 : kOneLaunch;
+    if (kv_len <= whole || (kv_len <= 2 * whole && rows * streams >= kFullStreams)) return 0;
     const std::uint64_t most = head_size == 256 ? Shape<256>::kGrid : Shape<128>::kGrid;
     const std::uint64_t tiles = (kv_len + kTile - 1) / kTile + kPartCost;
     const std::uint64_t shares = tiles > most * kLeastShare ? most : rows * streams * tiles / kLeastShare + 1;
@@ -749,13 +763,18 @@ int launch_decode(QuantDecodeParams& p, std::uint32_t grid, hipStream_t stream) 
         quant_decode_kernel<F, kD, kSub, true><<<dim3(static_cast<unsigned>(p.rows * streams)), dim3(kThreads), 0, stream>>>(p);
         return launch_status("quant_decode_kernel");
     }
+    // The merge takes the shorter list: streams of a few rows, or the workgroups' cuts.
+    // 16 rows of 2 kv heads with 16 query heads each: 40 us by workgroup, 19 by stream.
+    const std::uint32_t cuts = p.rows * streams < grid ? static_cast<std::uint32_t>(p.rows * streams) : grid;
+    p.by_stream = cuts < grid;
     quant_decode_kernel<F, kD, kSub, false><<<dim3(grid), dim3(kThreads), 0, stream>>>(p);
     if (const int s = launch_status("quant_decode_kernel")) return s;
-    // Parts of a stream: many where there are few streams.
-    if (grid > 8 * p.rows * streams)
-        quant_decode_merge_kernel<kD, 1024><<<dim3(grid, p.set_heads), dim3(1024), 0, stream>>>(p);
+    // Parts of a stream: many where there are few streams. With 1024 threads and with 128:
+    // 64 parts 25.3 and 26.6 us (the whole call), 18 parts 16.2 and 13.2.
+    if (grid > 32 * p.rows * streams)
+        quant_decode_merge_kernel<kD, 1024><<<dim3(cuts, p.set_heads), dim3(1024), 0, stream>>>(p);
     else
-        quant_decode_merge_kernel<kD, 128><<<dim3(grid, p.set_heads), dim3(128), 0, stream>>>(p);
+        quant_decode_merge_kernel<kD, 128><<<dim3(cuts, p.set_heads), dim3(128), 0, stream>>>(p);
     return launch_status("quant_decode_merge_kernel");
 }
 template <typename F, int kD>
@@ -810,8 +829,15 @@ extern "C" int kvflux_quant_attention_workspace_size(uint64_t num_rows, uint64_t
     if (num_rows == 0 || !fast_head_size(head_size)) return KVFLUX_OK;
     std::uint32_t sets, set_heads;
     head_sets(query_heads / num_kv_heads, &sets, &set_heads);
-    const std::uint64_t rows = num_rows < kPlanRows ? num_rows : kPlanRows;
-    *bytes = decode_workspace(decode_grid(rows, kv_len, num_kv_heads * sets, head_size), set_heads, head_size);
+    const std::uint64_t streams = num_kv_heads * sets;
+    std::uint64_t rows = num_rows < kPlanRows ? num_rows : kPlanRows;
+    // Enough for fewer rows as well, where those are cut into shares and these not.
+    if (decode_grid(rows, kv_len, streams, head_size) == 0) {
+        const std::uint64_t fewer = (kFullStreams - 1) / streams;
+        if (fewer < rows) rows = fewer;
+    }
+    if (rows == 0) return KVFLUX_OK;
+    *bytes = decode_workspace(decode_grid(rows, kv_len, streams, head_size), set_heads, head_size);
     return KVFLUX_OK;
 }
 

@@ -59,16 +59,6 @@ struct WriteParams {
     std::uint32_t units;
 };
 
-// Largest of an unsigned value over a wavefront.
-__device__ inline std::uint32_t wave_largest(std::uint32_t x) {
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const auto other = static_cast<std::uint32_t>(__shfl_xor(static_cast<int>(x), d));
-        x = other > x ? other : x;
-    }
-    return x;
-}
-
 // kWaves wavefronts for a unit; unit = ((sequence * pages + page) * 2 + cache) *
 // heads + head, so neighbouring wavefronts read neighbouring heads of a token.
 template <typename In, typename F, int kV, int kWaves>
@@ -133,7 +123,7 @@ __global__ __launch_bounds__(kThreads) void quant_write_kernel(WriteParams p) {
 #pragma unroll
     for (int i = 0; i < kHeld; ++i) weigh(held[i]);  // past the end: the last group again
     for (std::uint32_t c = begin + tid + kHeld * kT; c < end; c += kT) weigh(*input(c));
-    largest = wave_largest(largest);
+    largest = over_wave(largest, [](std::uint32_t a, std::uint32_t b) { return a > b ? a : b; });
     if constexpr (kWaves > 1) {
         if (tid % 64 == 0) largest_of[tid / 64] = largest;
         __syncthreads();  // every wavefront has read the scale as well

@@ -82,6 +82,17 @@ def run(cache, table, lens, q, **kw):
     return d.result()
 
 
+# A bound of the lengths from which every call is cut into shares.
+SHARES = 2049
+
+
+def check_both(cache, table, lens, q):
+    """With the lengths' own bound, and in shares."""
+    check(cache, table, lens, q, run(cache, table, lens, q))
+    if max(lens) < SHARES:
+        check(cache, table, lens, q, run(cache, table, lens, q, kv_len=SHARES))
+
+
 @pytest.mark.parametrize("fmt", ["e4m3", "int8"])
 @pytest.mark.parametrize("D", [64, 128, 256])
 @pytest.mark.parametrize("bs", [16, 8, 32, 64, 1, 5, 12])
@@ -90,7 +101,7 @@ def test_lengths_and_pages(gpu, fmt, D, bs):
     lens = np.array([0, 1, 7, 8, 9, 31, 32, 33, 127, 128, 129, 300, 511, 512])
     rng, cache, table, q = make(fmt, 2, 4, D, bs, lens, [D, bs])
     check(cache, table, lens, q, run(cache, table, lens, q))
-    check(cache, table, lens, q, run(cache, table, lens, q, kv_len=table.shape[1] * bs + 513))
+    check(cache, table, lens, q, run(cache, table, lens, q, kv_len=table.shape[1] * bs + SHARES))
 
 
 @pytest.mark.parametrize("fmt", ["e4m3", "int8"])
@@ -98,7 +109,7 @@ def test_lengths_and_pages(gpu, fmt, D, bs):
 def test_groups(gpu, fmt, H, G):
     lens = np.array([700, 1, 45, 0, 1300])
     rng, cache, table, q = make(fmt, H, G, 128, 16, lens, [H, G])
-    check(cache, table, lens, q, run(cache, table, lens, q))
+    check_both(cache, table, lens, q)
     short = np.minimum(lens, 200)
     check(cache, table, short, q, run(cache, table, short, q))
 
@@ -113,14 +124,14 @@ def test_many_and_long_rows(gpu, D, bs, H, G, rows, hi):
     if rows > 20:
         lens[[3, 7]] = 0
     rng, cache, table, q = make("e4m3" if rows % 2 else "int8", H, G, D, bs, lens, rows)
-    check(cache, table, lens, q, run(cache, table, lens, q))
+    check_both(cache, table, lens, q)
 
 
 def test_more_rows_than_a_launch_plans(gpu):
     lens = np.random.default_rng(1).integers(0, 40, 4100)
     lens[[5, 2047, 2048, 4099]] = [900, 700, 650, 530]
     rng, cache, table, q = make("e4m3", 1, 2, 64, 16, lens, 3)
-    check(cache, table, lens, q, run(cache, table, lens, q))
+    check_both(cache, table, lens, q)
 
 
 @pytest.mark.parametrize("fmt", ["e4m3", "int8"])
@@ -129,9 +140,10 @@ def test_missing_pages_drop_out(gpu, fmt, bs):
     lens = np.array([600, 90, 33, 20])
     rng, cache, table, q = make(fmt, 2, 4, 128, bs, lens, bs)
     table[0, [0, 3, 7]], table[1, 1], table[3, :] = cache.blocks, 2 ** 64 - 1, 2 ** 63
-    want_zero = run(cache, table, lens, q)
-    check(cache, table, lens, q, want_zero)
-    assert not want_zero[3].any()
+    for bound in (None, SHARES):
+        got = run(cache, table, lens, q, kv_len=bound)
+        check(cache, table, lens, q, got)
+        assert not got[3].any()
     short = table[:, :2].copy()  # rows end before their tokens do
     check(cache, short, np.minimum(lens, 2 * bs), q, run(cache, short, lens, q))
 
@@ -148,7 +160,7 @@ def test_what_lies_behind_a_row_is_not_seen(gpu, bs, D):
         if n % bs:
             cache.bytes[:, int(table[r, n // bs]), :, n % bs:] = 0x7f
     cache.upload()
-    check(cache, table, lens, q, run(cache, table, lens, q))
+    check_both(cache, table, lens, q)
 
 
 @pytest.mark.parametrize("D", [128, 96])
@@ -159,10 +171,11 @@ def test_a_scale_or_byte_that_is_nan_is_seen(gpu, D):
     cache.scales[1, int(table[1, 30]), 1] = np.nan
     cache.bytes[1, int(table[2, 2]), 1, 0, 5] = 0xff
     cache.upload()
-    got = run(cache, table, lens, q).reshape(3, 2, 2, D)
-    assert np.isnan(got[0, 0]).all() and np.isfinite(got[0, 1]).all()
-    assert np.isnan(got[1, 1]).all() and np.isfinite(got[1, 0]).all()
-    assert np.isnan(got[2, 1, :, 5]).all() and np.isfinite(np.delete(got[2], 5, -1)).all()
+    for bound in (None, SHARES):
+        got = run(cache, table, lens, q, kv_len=bound).reshape(3, 2, 2, D)
+        assert np.isnan(got[0, 0]).all() and np.isfinite(got[0, 1]).all()
+        assert np.isnan(got[1, 1]).all() and np.isfinite(got[1, 0]).all()
+        assert np.isnan(got[2, 1, :, 5]).all() and np.isfinite(np.delete(got[2], 5, -1)).all()
 
 
 @pytest.mark.parametrize("fmt", ["e4m3", "int8"])
@@ -170,10 +183,10 @@ def test_scales_of_any_origin(gpu, fmt):
     """Scales that are no powers of two, sizes from 2^-60 to 2^40 in one row."""
     lens = np.array([900, 64])
     rng, cache, table, q = make(fmt, 2, 4, 128, 16, lens, 4, scales=1.37)
-    check(cache, table, lens, q, run(cache, table, lens, q))
+    check_both(cache, table, lens, q)
     cache.scales[1] *= np.exp2(rng.integers(-60, 41, cache.scales[1].shape)).astype(np.float32)
     cache.upload()
-    check(cache, table, lens, q, run(cache, table, lens, q))
+    check_both(cache, table, lens, q)
 
 
 @pytest.mark.parametrize("size", [2.0 ** -40, 2.0 ** 30])
@@ -220,7 +233,7 @@ def test_rows_of_equal_keys_give_the_mean(gpu):
     cache.bytes[0] = 5
     cache.scales[0] = 1.0
     cache.upload()
-    check(cache, table, lens, q, run(cache, table, lens, q))
+    check_both(cache, table, lens, q)
 
 
 def test_the_same_bits_again(gpu):
@@ -245,7 +258,7 @@ def test_generic_head_sizes_and_alignments(gpu, D, shift):
         cache.fill(rng)
         table = random_table(rng, lens, 6, blocks)
         q = rng.standard_normal((len(lens), 6, D)).astype(np.float32)
-        check(cache, table, lens, q, run(cache, table, lens, q))
+        check_both(cache, table, lens, q)
 
 
 def test_two_streams_with_workspaces_of_their_own(gpu):
@@ -263,9 +276,28 @@ def test_two_streams_with_workspaces_of_their_own(gpu):
 
 
 def test_an_undersized_workspace_is_refused(gpu):
-    lens = np.array([600, 2000])
+    lens = np.array([600, 2100])
     rng, cache, table, q = make("e4m3", 2, 4, 128, 16, lens, 1)
     d = Decode(cache, table, lens, q)
     with pytest.raises(capi.KvfluxError) as e:
         capi.call("kvflux_quant_attention", *d.args[:-1], d.size - 1, None)
     assert e.value.status == capi.ERR_INVALID
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("H,G", [(8, 4), (1, 1), (4, 40), (300, 1)])
+def test_a_workspace_for_the_largest_call_does_for_smaller_ones(gpu, H, G, D):
+    rows = [1, 2, 7, 31, 32, 33, 63, 64, 128, 255, 256, 300, 2048, 5000]
+    bounds = [1, 512, 513, 1024, 1025, 2048, 2049, 4096, 100000]
+    sizes = np.array([[workspace_size(r, n, H, H * G, 16, D) for n in bounds] for r in rows])
+    assert (np.diff(sizes, axis=0) >= 0).all() and (np.diff(sizes, axis=1) >= 0).all()
+    assert sizes[0, -1] > 0 and not sizes[:, :2].any()
+
+
+@pytest.mark.parametrize("H", [8, 1])
+def test_a_bound_at_which_many_rows_take_one_launch_and_few_are_cut(gpu, H):
+    lens = np.random.default_rng(H).integers(0, 1500, 260)
+    lens[[0, 100]] = 1500
+    rng, cache, table, q = make("e4m3", H, 2, 128, 16, lens, 7)
+    check(cache, table, lens, q, run(cache, table, lens, q))
+    check(cache, table[:9], lens[:9], q[:9], run(cache, table[:9].copy(), lens[:9], q[:9].copy()))
