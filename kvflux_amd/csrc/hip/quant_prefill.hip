@@ -34,7 +34,8 @@ typedef __attribute__((ext_vector_type(16))) float qp_f32x16_t;
 
 constexpr std::uint32_t kTile = 64;     // keys of a tile
 constexpr std::uint32_t kWindow = 1024; // pages whose ids and scales are in LDS at a time
-constexpr std::uint32_t kMissing = 0x80000000u;
+constexpr std::uint32_t kUnread = 0x80000000u;  // a page whose bytes are not read, in place of its id
+constexpr std::uint32_t kMissing = ~0u;         // one that is not there
 constexpr float kWeightScale = 32768.0f;  // as in the decode: parts of 2^15 times a weight of at most 1
 
 // kWaves wavefronts hold 32 rows each; kPair tiles are staged, and waited for, at a time.
@@ -174,18 +175,20 @@ __global__ __launch_bounds__(64 * kWaves, (Shape<kD, kWaves>::kPerSimd)) void qu
             const bool live = in_row && id < p.num_blocks;
             const std::uint64_t at = (live ? id : 0) * p.heads + kvh;
             float ks = live ? p.key_scales[at] : 0.0f, vs = live ? p.value_scales[at] : 0.0f;
-            if (vs != vs) {  // what sees these values is NaN by its score, what does not is left alone
+            page_id[i] = live ? static_cast<std::uint32_t>(id) : kMissing;
+            // What sees these values is NaN by its score. What does not is left alone: their
+            // bytes may be NaN as well, and a weight of 0 times that is.
+            if (vs != vs) {
                 ks = vs;
                 vs = 0.0f;
+                page_id[i] = kUnread;
             }
-            page_id[i] = live ? static_cast<std::uint32_t>(id) : kMissing;
             page_ks[i] = ks;
             page_vs[i] = vs;
             top = fmaxf(top, __builtin_fabsf(vs));
             lost |= !live && page * p.block_size.divisor < kv_len;  // behind that no query sees
         }
-#pragma unroll
-        for (int d = 1; d < 64; d <<= 1) top = fmaxf(top, __shfl_xor(top, d));
+        top = wave_max(top);
         const bool any_lost = __builtin_amdgcn_ballot_w64(lost) != 0;
         if (lane == 0) {
             wave_top[wave] = top;
@@ -213,9 +216,9 @@ __global__ __launch_bounds__(64 * kWaves, (Shape<kD, kWaves>::kPerSimd)) void qu
     const auto fetch = [&](std::uint32_t tile) {
         const std::uint32_t key = tile * kTile + my_row, page = p.block_size.div(key);
         const std::uint32_t id = page_id[page - window_page];
-        held_live = !(id & kMissing) && key < kv_len;
-        // Missing pages: the pool's first row.
-        const std::uint64_t at = (id & kMissing ? 0 : (static_cast<std::uint64_t>(id) * p.heads + kvh) * head_bytes +
+        held_live = !(id & kUnread) && key < kv_len;
+        // In place of a page that is not read: the pool's first row.
+        const std::uint64_t at = (id & kUnread ? 0 : (static_cast<std::uint64_t>(id) * p.heads + kvh) * head_bytes +
                                                           (key - page * p.block_size.divisor) * kD) + my_col;
         constexpr int kAlign = kBytes < 16 ? kBytes : 16;
         __builtin_memcpy(held[0], __builtin_assume_aligned(p.key_cache + at, kAlign), kBytes);
@@ -309,7 +312,7 @@ __global__ __launch_bounds__(64 * kWaves, (Shape<kD, kWaves>::kPerSimd)) void qu
             }
         }
         m.live = ~0ull;
-        if (missing) m.live = __builtin_amdgcn_ballot_w64(!(page_id[p.block_size.div(tile * kTile + lane) - window_page] & kMissing));
+        if (missing) m.live = __builtin_amdgcn_ballot_w64(page_id[p.block_size.div(tile * kTile + lane) - window_page] != kMissing);
         return m;
     };
 
@@ -711,7 +714,7 @@ extern "C" int kvflux_quant_prefill(const void* key_cache, const void* value_cac
     if (max_blocks_per_seq == 0) return fail(KVFLUX_ERR_INVALID_ARGUMENT, "quant prefill: empty table rows");
     if (const int s = check_prefill("quant prefill", num_seqs, max_query_tokens, max_kv_len, num_kv_heads, query_heads, block_size, head_size))
         return s;
-    if (num_blocks >= kMissing) return fail(KVFLUX_ERR_UNSUPPORTED, "quant prefill: too many pages");
+    if (num_blocks >= kUnread) return fail(KVFLUX_ERR_UNSUPPORTED, "quant prefill: too many pages");
     if (!aligned(4, {query, output}) || !aligned(8, {block_table, kv_lens, query_lens, query_offsets}))
         return fail(KVFLUX_ERR_INVALID_ARGUMENT, "quant prefill: misaligned array");
     const std::uint64_t group = query_heads / num_kv_heads;

@@ -139,6 +139,24 @@ def test_rows_that_end_before_their_tokens(gpu):
     check(cache, short, call, got)
 
 
+@pytest.mark.parametrize("bs,D,n,m", [(16, 128, 100, 100), (32, 64, 200, 200), (5, 128, 70, 40), (16, 256, 100, 64), (16, 128, 3000, 40)])
+def test_bytes_of_a_page_without_numbers_reach_what_sees_them_alone(gpu, bs, D, n, m):
+    """A NaN that was written makes a page's V NaN bytes under a NaN scale: queries before it share its tile."""
+    rng, cache, table, q = make("e4m3", 2, 2, D, bs, [n], [m], 1)
+    first = (n - m // 2) // bs * bs  # of the last page that begins by the middle query
+    page = int(table[0, first // bs])
+    cache.scales[1, page, 1] = np.nan
+    cache.bytes[1, page, 1] = 0xff
+    cache.upload()
+    call, got = run(cache, table, [n], [m], q)
+    before = first - (n - m)
+    assert 0 < before < m
+    assert np.isnan(got[before:, 2:]).all() and np.isfinite(got[:before]).all() and np.isfinite(got[:, :2]).all()
+    cache.scales[1, page, 1], cache.bytes[1, page, 1] = 1.0, 0
+    want = attention(cache, table[0], n, q[:before], visible=np.arange(n - m + 1, n - m + 1 + before))
+    assert np.abs(got[:before] - want).max() <= 1e-5 * biggest(cache, table[0], n)
+
+
 @pytest.mark.parametrize("bs,D", [(16, 128), (64, 64), (5, 128), (16, 256)])
 def test_what_lies_behind_a_sequence_is_not_seen(gpu, bs, D):
     lens, new = np.array([1, 37, 70, 530]), np.array([1, 30, 70, 100])
