@@ -9,9 +9,10 @@
 // 16x16x32's for the same bytes from LDS.
 //  * A workgroup owns one kv head and 32 rows a wavefront, a row being a (query token,
 //    query head) pair of the heads of that kv head.
-//  * Keys go through LDS in tiles of 64: a thread loads 16 bytes of the next tile's K
+//  * Keys go through LDS in tiles of 64: a thread loads its bytes of the next tile's K
 //    and V into registers while this one is computed, widens them to FP16 once for all
-//    wavefronts and stores them to the other buffer; one barrier a tile.
+//    wavefronts and stores them to the other buffer; one barrier a tile with four
+//    wavefronts, one for two tiles with eight.
 //  * S^T = K Q^T leaves lane (row, half) with keys 8 i + 4 half .. + 3 of the row:
 //    O^T += V^T P^T takes them as they are when V's tokens are read in that order
 //    (ds_read_b64_tr_b16, four tokens of a dim a lane).
@@ -21,6 +22,12 @@
 //    MFMA on a large accumulator drops bits of small weights, always in one direction.
 // A call whose workgroups would leave CUs idle (a short chunk behind a long prefix)
 // spreads each one's keys over several, merged by a second kernel.
+//
+// 32 query heads, 8 kv heads of 128: 512 tokens behind 32768 505 us, 1100 TFLOP/s of the
+// two parts' products, where a large library product in FP16 reaches 1174; 8 prompts of
+// 4096 2.16 ms, 1030 TFLOP/s, the diagonal tiles' masked half counted out. What is left is
+// the arithmetic beside the matrix instructions (330 instructions of a tile and wavefront,
+// each of which a running MFMA lets through, but shares its issue slots with).
 #include "mfma_parts.h"
 #include "quant.h"
 
@@ -43,7 +50,7 @@ template <int kD, int kWaves>
 struct Shape {
     static constexpr int kThreads = 64 * kWaves;
     static constexpr std::uint32_t kRows = 32 * kWaves;
-    static constexpr int kPair = kD <= 128 && kWaves == 8 ? 2 : 1;
+    static constexpr int kPair = kWaves == 8 ? 2 : 1;
     // Wavefronts of a SIMD: the registers of two hold Q and the sums of 32 rows up to D = 128.
     static constexpr int kPerSimd = kD == 256 ? 1 : 2;
 };
@@ -615,13 +622,13 @@ PrefillPlan prefill_plan(std::uint64_t num_seqs, std::uint64_t max_query, std::u
         return num_seqs * plan.blocks * heads;
     };
     // Eight wavefronts share a tile's loads and conversions, two workgroups of four a CU
-    // that waits less at barriers and is filled by fewer rows. Head size 128: 512 tokens
-    // behind 32768 528 us with eight, 563 with four; 8 x 4096 2312 and 2337; one prompt of
-    // 2000 118 and 102; 64 tokens behind 2000 40 and 30; 16 sequences' 4 tokens behind up to
-    // 9000 164 and 104. Head size 64: 8 x 4096 702 and 676, three prompts of up to 3000 85
-    // and 68. At 256 the registers are those of four.
+    // that waits less at barriers and is filled by fewer rows. Head size 128, eight and four:
+    // 512 tokens behind 32768 528 and 563 us; 8 x 4096 2312 and 2337; 8 x 2048 618 and 617;
+    // 16 prompts of up to 1000 200 and 170; one prompt of 2000 118 and 102; 64 tokens behind
+    // 2000 40 and 30; 16 sequences' 4 tokens behind up to 9000 164 and 104. Head size 64:
+    // 8 x 4096 702 and 676. At 256 the registers are those of four.
     std::uint64_t workgroups = shape(head_size == 128 ? 8 : 4);
-    if (plan.waves == 8 && (max_query * group <= 128 || (workgroups < 512 && max_kv < 4096))) workgroups = shape(4);
+    if (plan.waves == 8 && (max_query * group <= 128 || max_kv < 4096)) workgroups = shape(4);
     // Splits: where the heaviest block of queries would run on alone, its keys go to several
     // workgroups, none with more tiles than its share of all (bounds standing for lengths).
     // Two workgroups of a CU take 3.1 us a tile each, one by itself 1.7 (head size 128), so
@@ -659,7 +666,7 @@ int launch_prefill(QuantPrefillParams& p, hipStream_t stream) {
 template <typename F>
 int launch_prefill_head_size(QuantPrefillParams& p, std::uint64_t head_size, std::uint32_t waves, hipStream_t s) {
     switch (head_size) {
-    case 64: return waves == 4 ? launch_prefill<F, 64, 4>(p, s) : launch_prefill<F, 64, 8>(p, s);
+    case 64: return launch_prefill<F, 64, 4>(p, s);
     case 128: return waves == 4 ? launch_prefill<F, 128, 4>(p, s) : launch_prefill<F, 128, 8>(p, s);
     default: return launch_prefill<F, 256, 4>(p, s);
     }
