@@ -91,6 +91,19 @@ def test_whole_prompts(gpu, fmt, D, bs):
     check(cache, table, call, got)
 
 
+@pytest.mark.parametrize("fmt", ["e4m3", "int8"])
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("bs,H,G", [(16, 2, 4), (8, 2, 4), (64, 1, 7), (1, 2, 1), (5, 1, 17), (48, 1, 300)])
+def test_bounds_past_the_lengths(gpu, fmt, D, bs, H, G):
+    """What is chosen by the bounds (wavefronts, splits) on short sequences, with a page missing."""
+    lens, new = np.array([1, 63, 0, 64, 65, 130, 200]), np.array([1, 63, 0, 2, 65, 1, 190])
+    rng, cache, table, q = make(fmt, H, G, D, bs, lens, new, [D, bs])
+    for bound in (4096, 20000):
+        call, got = run(cache, table, lens, new, q, most=max(200, 129 // G + 1), kv_len=bound)
+        check(cache, table, call, got, some=20)
+        table[6, 1] = cache.blocks
+
+
 @pytest.mark.parametrize("D,bs,H,G", [(128, 16, 8, 4), (64, 32, 4, 7), (256, 16, 2, 8), (128, 3, 1, 12), (128, 16, 1, 17),
                                       (64, 16, 1, 71), (128, 16, 8, 1), (128, 16, 1, 300)])
 def test_chunks_behind_a_prefix(gpu, D, bs, H, G):
@@ -148,13 +161,14 @@ def test_bytes_of_a_page_without_numbers_reach_what_sees_them_alone(gpu, bs, D, 
     cache.scales[1, page, 1] = np.nan
     cache.bytes[1, page, 1] = 0xff
     cache.upload()
-    call, got = run(cache, table, [n], [m], q)
+    results = [run(cache, table, [n], [m], q, kv_len=bound)[1] for bound in (n, 5000)]
     before = first - (n - m)
     assert 0 < before < m
-    assert np.isnan(got[before:, 2:]).all() and np.isfinite(got[:before]).all() and np.isfinite(got[:, :2]).all()
     cache.scales[1, page, 1], cache.bytes[1, page, 1] = 1.0, 0
     want = attention(cache, table[0], n, q[:before], visible=np.arange(n - m + 1, n - m + 1 + before))
-    assert np.abs(got[:before] - want).max() <= 1e-5 * biggest(cache, table[0], n)
+    for got in results:
+        assert np.isnan(got[before:, 2:]).all() and np.isfinite(got[:before]).all() and np.isfinite(got[:, :2]).all()
+        assert np.abs(got[:before] - want).max() <= 1e-5 * biggest(cache, table[0], n)
 
 
 @pytest.mark.parametrize("bs,D", [(16, 128), (64, 64), (5, 128), (16, 256)])
