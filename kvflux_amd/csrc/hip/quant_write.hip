@@ -289,6 +289,9 @@ constexpr int kReadGroups = 4;  // groups of a thread
 // A workgroup takes one part of one (page, cache): groups of kV values numbered as
 // they lie in the output, so every store of a wavefront is one run of memory and a
 // page's missing tokens are its last groups.
+// 64 sequences of up to 16384 tokens, 8 kv heads of 128, to BF16 (3.55 GB): 613 us, 5.8
+// TB/s; with the streaming hint on the loads too 621, without it on the stores 635, with
+// 2 and 8 groups a thread 640 and 649, a whole page a workgroup 613.
 template <typename F, typename Out, int kV>
 __global__ __launch_bounds__(kThreads) void quant_gather_kernel(ReadParams p) {
     using Raw = typename std::conditional<kV == 8, V8, std::uint8_t>::type;
@@ -319,7 +322,7 @@ __global__ __launch_bounds__(kThreads) void quant_gather_kernel(ReadParams p) {
         const std::uint32_t token = p.token_groups.div(j), in_token = j - token * p.token_groups.divisor;
         const std::uint32_t head = p.row_groups.div(in_token);
         const std::uint64_t c = (static_cast<std::uint64_t>(head) * p.block_size + token) * cpr + (in_token - head * cpr);
-        raw[u] = stream_load(reinterpret_cast<const Raw*>(src) + c);
+        raw[u] = reinterpret_cast<const Raw*>(src)[c];
         scale[u] = scales[head];
     }
 #pragma unroll
