@@ -26,8 +26,8 @@
 // 32 query heads, 8 kv heads of 128: 512 tokens behind 32768 505 us, 1100 TFLOP/s of the
 // two parts' products, where a large library product in FP16 reaches 1174; 8 prompts of
 // 4096 2.16 ms, 1030 TFLOP/s, the diagonal tiles' masked half counted out. What is left is
-// the arithmetic beside the matrix instructions (330 instructions of a tile and wavefront,
-// each of which a running MFMA lets through, but shares its issue slots with).
+// the arithmetic beside the matrix instructions: some 400 VALU instructions of a tile and
+// wavefront to 64 MFMAs, which a running MFMA lets through only in part.
 #include "mfma_parts.h"
 #include "quant.h"
 
