@@ -11,8 +11,10 @@
 //    query head) pair of the heads of that kv head.
 //  * Keys go through LDS in tiles of 64: a thread loads its bytes of the next tile's K
 //    and V into registers while this one is computed, widens them to FP16 once for all
-//    wavefronts and stores them to the other buffer; one barrier a tile with four
-//    wavefronts, one for two tiles with eight.
+//    wavefronts and stores them to the other buffer.
+//  * Eight wavefronts work in phases: of a SIMD's two, one multiplies while the other works
+//    out weights (512 tokens behind 32768 506 us without the phases, 490 with them: 14 %
+//    fewer cycles, of which the lower clock under that load gives most back).
 //  * S^T = K Q^T leaves lane (row, half) with keys 8 i + 4 half .. + 3 of the row:
 //    O^T += V^T P^T takes them as they are when V's tokens are read in that order
 //    (ds_read_b64_tr_b16, four tokens of a dim a lane).
@@ -23,11 +25,11 @@
 // A call whose workgroups would leave CUs idle (a short chunk behind a long prefix)
 // spreads each one's keys over several, merged by a second kernel.
 //
-// 32 query heads, 8 kv heads of 128: 512 tokens behind 32768 505 us, 1100 TFLOP/s of the
+// 32 query heads, 8 kv heads of 128: 512 tokens behind 32768 490 us, 1130 TFLOP/s of the
 // two parts' products, where a large library product in FP16 reaches 1174; 8 prompts of
-// 4096 2.16 ms, 1030 TFLOP/s, the diagonal tiles' masked half counted out. What is left is
-// the arithmetic beside the matrix instructions: some 400 VALU instructions of a tile and
-// wavefront to 64 MFMAs, which a running MFMA lets through only in part.
+// 4096 2.06 ms, 1070 TFLOP/s, the diagonal tiles' masked half counted out. What is left is
+// the arithmetic beside the matrix instructions, some 400 VALU instructions of a tile and
+// wavefront to 64 MFMAs, and the power that both draw.
 #include "mfma_parts.h"
 #include "quant.h"
 
@@ -45,14 +47,15 @@ constexpr std::uint32_t kUnread = 0x80000000u;  // a page whose bytes are not re
 constexpr std::uint32_t kMissing = ~0u;         // one that is not there
 constexpr float kWeightScale = 32768.0f;  // as in the decode: parts of 2^15 times a weight of at most 1
 
-// kWaves wavefronts hold 32 rows each; kPair tiles are staged, and waited for, at a time.
-template <int kD, int kWaves>
+// kWaves wavefronts hold 32 rows each.
+template <int kD, int kWaves, bool kUniform>
 struct Shape {
     static constexpr int kThreads = 64 * kWaves;
     static constexpr std::uint32_t kRows = 32 * kWaves;
-    static constexpr int kPair = kWaves == 8 ? 2 : 1;
-    // Wavefronts of a SIMD: the registers of two hold Q and the sums of 32 rows up to D = 128.
-    static constexpr int kPerSimd = kD == 256 ? 1 : 2;
+    // Wavefronts of a SIMD: the registers of two hold Q and the sums of 32 rows up to D = 128,
+    // of three at 64 (8 prompts of 2048: two 181 us, three 167), but not with scales that
+    // differ within 16 keys.
+    static constexpr int kPerSimd = kD == 256 ? 1 : kD == 64 && kUniform ? 3 : 2;
 };
 
 struct QuantPrefillParams {
@@ -85,22 +88,22 @@ struct QuantPrefillParams {
 };
 
 // How many workgroups share a block of queries whose last sees `tile_count` tiles, at
-// most `most` each, and the tiles of one: an even number (whole steps).
+// most `most` each, and the tiles of one.
 struct Split {
     std::uint32_t count, tiles;
 };
 __device__ inline Split split_of(std::uint32_t tile_count, std::uint32_t most) {
     const std::uint32_t count = (tile_count - 1) / most + 1;
-    return {count, ((tile_count - 1) / count + 2) & ~1u};
+    return {count, (tile_count - 1) / count + 1};
 }
 
 // kUniform: pages are multiples of 16 tokens, so 16 neighbouring keys of a tile share
 // their scales, which are then one value for a wavefront.
 template <typename F, int kD, int kWaves, bool kUniform>
-__global__ __launch_bounds__(64 * kWaves, (Shape<kD, kWaves>::kPerSimd)) void quant_prefill_kernel(QuantPrefillParams p) {
-    using S = Shape<kD, kWaves>;
+__global__ __launch_bounds__(64 * kWaves, (Shape<kD, kWaves, kUniform>::kPerSimd)) void quant_prefill_kernel(QuantPrefillParams p) {
+    using S = Shape<kD, kWaves, kUniform>;
     using Vec = pf_f16x8_t;
-    constexpr int kThreads = S::kThreads, kPair = S::kPair;
+    constexpr int kThreads = S::kThreads;
     constexpr int kSteps = kD / 16;            // MFMAs of a 32-key block of S^T for one part of Q
     constexpr int kDb = kD / 32;               // dim blocks of O^T
     constexpr int kRowBytes = kD * 2;          // a key's row in LDS
@@ -111,13 +114,13 @@ __global__ __launch_bounds__(64 * kWaves, (Shape<kD, kWaves>::kPerSimd)) void qu
     constexpr int kKeyThreads = kD / kBytes;   // threads of a key
     constexpr int kWords = kBytes / 4;
     static_assert(kBytes >= 8 && kD % kBytes == 0, "tile split");
-    // [buffer][tile][K, V]
-    __shared__ __attribute__((aligned(16))) unsigned char tiles_lds[2][kPair][2][kTileBytes];
+    // [buffer][K, V]
+    __shared__ __attribute__((aligned(16))) unsigned char tiles_lds[2][2][kTileBytes];
     __shared__ std::uint32_t page_id[kWindow];
     __shared__ float page_ks[kWindow], page_vs[kWindow];  // vs over the reference, times kWeightScale
     // Where the scales differ within 16 keys: those of a buffer's keys.
-    __shared__ __attribute__((aligned(16))) float key_ks[kUniform ? 1 : 2][kUniform ? 4 : kPair * kTile];
-    __shared__ __attribute__((aligned(16))) float key_vs[kUniform ? 1 : 2][kUniform ? 4 : kPair * kTile];
+    __shared__ __attribute__((aligned(16))) float key_ks[kUniform ? 1 : 2][kUniform ? 4 : kTile];
+    __shared__ __attribute__((aligned(16))) float key_vs[kUniform ? 1 : 2][kUniform ? 4 : kTile];
     __shared__ float wave_top[kWaves];
     __shared__ std::uint32_t wave_missing[kWaves];
 
@@ -219,30 +222,28 @@ __global__ __launch_bounds__(64 * kWaves, (Shape<kD, kWaves>::kPerSimd)) void qu
     const std::uint32_t my_row = static_cast<std::uint32_t>(tid) / kKeyThreads, my_col = static_cast<std::uint32_t>(tid) % kKeyThreads * kBytes;
     const std::uint64_t head_bytes = static_cast<std::uint64_t>(p.block_size.divisor) * kD;
     std::uint32_t held[2][kWords];
-    bool held_live = false;
-    const auto fetch = [&](std::uint32_t tile) {
+    bool held_live = false;  // V's
+    const auto fetch_one = [&](int which, std::uint32_t tile) {
         const std::uint32_t key = tile * kTile + my_row, page = p.block_size.div(key);
         const std::uint32_t id = page_id[page - window_page];
-        held_live = !(id & kUnread) && key < kv_len;
+        if (which) held_live = !(id & kUnread) && key < kv_len;
         // In place of a page that is not read: the pool's first row.
         const std::uint64_t at = (id & kUnread ? 0 : (static_cast<std::uint64_t>(id) * p.heads + kvh) * head_bytes +
-                                                          (key - page * p.block_size.divisor) * kD) + my_col;
+                                                         (key - page * p.block_size.divisor) * kD) + my_col;
         constexpr int kAlign = kBytes < 16 ? kBytes : 16;
-        __builtin_memcpy(held[0], __builtin_assume_aligned(p.key_cache + at, kAlign), kBytes);
-        __builtin_memcpy(held[1], __builtin_assume_aligned(p.value_cache + at, kAlign), kBytes);
+        __builtin_memcpy(held[which], __builtin_assume_aligned((which ? p.value_cache : p.key_cache) + at, kAlign), kBytes);
     };
     // Swizzled slots of a row's 16-byte chunks (LDS repeats its banks every 128 bytes). K is
     // read 16 rows of one chunk at a time, V 4 rows of 32 bytes.
     const auto k_slot = [](std::uint32_t row, std::uint32_t c) { return c ^ (row & (kCpr >= 16 ? 15 : 7)); };
     const auto v_slot = [](std::uint32_t row, std::uint32_t c) { return c ^ (2 * (row & 3)); };
-    const auto put = [&](std::uint32_t tile, unsigned char* buf) {  // buf: K's tile, V's behind it
+    const auto put_one = [&](int which, unsigned char* buf) {  // buf: K's tile, V's behind it
 #pragma unroll
-        for (int i = 0; i < 2 * kWords; i += 2) {  // eight values: one chunk of K or V
-            const bool value = i >= kWords;
-            std::uint32_t w0 = held[value][i % kWords], w1 = held[value][i % kWords + 1];
-            if (value && !held_live) w0 = w1 = 0;  // 0 * NaN would stay
-            const std::uint32_t c = my_col / 8 + i % kWords / 2;
-            *reinterpret_cast<uint4*>(buf + (value ? kTileBytes : 0) + my_row * kRowBytes + 16 * (value ? v_slot(my_row, c) : k_slot(my_row, c))) =
+        for (int i = 0; i < kWords; i += 2) {  // eight values: one chunk of K or V
+            std::uint32_t w0 = held[which][i], w1 = held[which][i + 1];
+            if (which && !held_live) w0 = w1 = 0;  // 0 * NaN would stay
+            const std::uint32_t c = my_col / 8 + i / 2;
+            *reinterpret_cast<uint4*>(buf + which * kTileBytes + my_row * kRowBytes + 16 * (which ? v_slot(my_row, c) : k_slot(my_row, c))) =
                 make_uint4(F::template pair16<0>(w0), F::template pair16<1>(w0), F::template pair16<0>(w1), F::template pair16<1>(w1));
         }
     };
@@ -324,17 +325,15 @@ __global__ __launch_bounds__(64 * kWaves, (Shape<kD, kWaves>::kPerSimd)) void qu
     };
 
     // Score i of a lane in block kb is key 32 kb + 8 (i / 4) + 4 half + i % 4 of the tile.
-    const auto compute = [&](std::uint32_t tile, const unsigned char* buf, const Marks& marks, float now, const float* key_k, const float* key_v) {
-        if (now != unit) {  // uniform: the reference of the weights moved up
-            const float f = unit / now;
-#pragma unroll
-            for (int db = 0; db < kDb; ++db) acc[db] *= f;
-            unit = now;
-        }
-        const std::uint64_t live = marks.live;
-        const std::uint32_t key0 = tile * kTile;
-        const bool masked = live != ~0ull || key0 + kTile - 1 > least_limit;  // uniform; keys past the sequence are past every limit
-        qp_f32x16_t s[2];
+    struct Scores {
+        qp_f32x16_t of[2];
+    };
+    struct Weights {  // operand j of block kb holds those of scores 8 j .. 8 j + 7, in two parts
+        Vec hi[2][2], lo[2][2];
+    };
+    const auto scores = [&](const unsigned char* buf) {
+        Scores out;
+        auto& s = out.of;
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb) {
             s[kb] = qp_f32x16_t{};
@@ -355,6 +354,19 @@ __global__ __launch_bounds__(64 * kWaves, (Shape<kD, kWaves>::kPerSimd)) void qu
             __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
         }
         __builtin_amdgcn_sched_group_barrier(0x008, 2 * 3, 0);
+        return out;
+    };
+    const auto weights = [&](Scores scores_of, std::uint32_t tile, const Marks& marks, float now, const float* key_k, const float* key_v) {
+        auto& s = scores_of.of;
+        if (now != unit) {  // uniform: the reference of the weights moved up
+            const float f = unit / now;
+#pragma unroll
+            for (int db = 0; db < kDb; ++db) acc[db] *= f;
+            unit = now;
+        }
+        const std::uint64_t live = marks.live;
+        const std::uint32_t key0 = tile * kTile;
+        const bool masked = live != ~0ull || key0 + kTile - 1 > least_limit;  // uniform; keys past the sequence are past every limit
         // Scores to s ks - ref in place: ks times the row's factor, finite (a product of
         // 0 stays 0; NaN stays).
         const auto finite = [](float y) { return y > 3.0e38f ? 3.0e38f : y; };
@@ -413,8 +425,7 @@ __global__ __launch_bounds__(64 * kWaves, (Shape<kD, kWaves>::kPerSimd)) void qu
 #pragma unroll
                 for (int i = 0; i < 16; ++i) s[kb][i] -= shift;
         }
-        // Weights, and their two parts: operand j of block kb holds scores 8 j .. 8 j + 7.
-        Vec p_hi[2][2], p_lo[2][2];
+        Weights out;
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb) {
             float part = 0.0f;
@@ -449,10 +460,13 @@ __global__ __launch_bounds__(64 * kWaves, (Shape<kD, kWaves>::kPerSimd)) void qu
                     const pf_f32x2_t rest = y - __builtin_convertvector(h, pf_f32x2_t);
                     lo[i] = __builtin_bit_cast(std::uint32_t, __builtin_convertvector(rest, pf_f16x2_t));
                 }
-                p_hi[kb][j] = __builtin_bit_cast(Vec, make_uint4(hi[0], hi[1], hi[2], hi[3]));
-                p_lo[kb][j] = __builtin_bit_cast(Vec, make_uint4(lo[0], lo[1], lo[2], lo[3]));
+                out.hi[kb][j] = __builtin_bit_cast(Vec, make_uint4(hi[0], hi[1], hi[2], hi[3]));
+                out.lo[kb][j] = __builtin_bit_cast(Vec, make_uint4(lo[0], lo[1], lo[2], lo[3]));
             }
         }
+        return out;
+    };
+    const auto weigh = [&](const Weights& w, const unsigned char* buf) {
         // V^T: a group of 16 lanes transposes 4 tokens of 16 dims.
         const std::uint32_t in16 = lane % 16, token_in = 4 * half + in16 / 4;
         const std::uint32_t dim_chunk = 2 * (lane / 16 % 2) + in16 % 4 / 2;  // 16-byte chunk within a dim block's 64 bytes
@@ -471,8 +485,8 @@ __global__ __launch_bounds__(64 * kWaves, (Shape<kD, kWaves>::kPerSimd)) void qu
                     };
                     const pf_i16x4_t a0 = read(0), a1 = read(8);
                     const Vec a = __builtin_bit_cast(Vec, __builtin_shufflevector(a0, a1, 0, 1, 2, 3, 4, 5, 6, 7));
-                    o = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, p_lo[kb][j], o, 0, 0, 0);
-                    o = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, p_hi[kb][j], o, 0, 0, 0);
+                    o = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, w.lo[kb][j], o, 0, 0, 0);
+                    o = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, w.hi[kb][j], o, 0, 0, 0);
                 }
             acc[db] += o;
         }
@@ -487,43 +501,85 @@ __global__ __launch_bounds__(64 * kWaves, (Shape<kD, kWaves>::kPerSimd)) void qu
 
     if (tile_begin < tile_end) {  // uniform
         const auto unit_now = [&] { return reference > 0.0f ? reference : 1.0f; };
-        stage();
-#pragma unroll
-        for (int i = 0; i < kPair; ++i) {
-            if (tile_begin + i >= tile_end) break;
-            fetch(tile_begin + i);
-            put(tile_begin + i, tiles_lds[0][i][0]);
-            put_scales(tile_begin + i, key_ks[0] + i * kTile, key_vs[0] + i * kTile);
-        }
-        __syncthreads();
-        int buf = 0;
-        for (std::uint32_t first = tile_begin; first < tile_end; first += kPair) {
-            // What this step's tiles need of their window, before the next step's takes its place.
-            Marks marks[kPair];
+        const auto key_ks_of = [&](std::uint32_t tile) { return key_ks[kUniform ? 0 : tile & 1]; };
+        const auto key_vs_of = [&](std::uint32_t tile) { return key_vs[kUniform ? 0 : tile & 1]; };
+        const auto buffer = [&](std::uint32_t tile) { return tiles_lds[tile & 1][0]; };
+        for (std::uint32_t first = tile_begin;;) {
+            stage();
             const float now = unit_now();
-            const std::uint32_t next = first + kPair;
-#pragma unroll
-            for (int i = 0; i < kPair; ++i)
-                if (first + i < tile_end) marks[i] = marks_of(first + i);
-            if (next < tile_end && next / p.window_tiles != window) {  // uniform (windows are whole steps)
-                __syncthreads();  // all have read the old pages
-                window = next / p.window_tiles;
-                stage();
-            }
-#pragma unroll
-            for (int i = 0; i < kPair; ++i) {
-                const bool more = next + i < tile_end;
-                if (more) fetch(next + i);
-                if (wave_live && first + i < tile_end)
-                    compute(first + i, tiles_lds[buf][i][0], marks[i], now, key_ks[kUniform ? 0 : buf] + (kUniform ? 0 : i * kTile),
-                            key_vs[kUniform ? 0 : buf] + (kUniform ? 0 : i * kTile));
-                if (more) {
-                    put(next + i, tiles_lds[buf ^ 1][i][0]);
-                    if constexpr (!kUniform) put_scales(next + i, key_ks[buf ^ 1] + i * kTile, key_vs[buf ^ 1] + i * kTile);
+            const std::uint32_t behind = (window + 1) * p.window_tiles, last = behind < tile_end ? behind : tile_end;
+            fetch_one(0, first);
+            if constexpr (kWaves == 8) {
+                // Two wavefronts a SIMD take turns: one multiplies (a tile's weighted values and
+                // the next one's scores) while the other works out weights, for whole phases. The
+                // second half's is a phase behind, and fills the buffers a tile ahead.
+                const std::uint32_t ahead = wave / 4;  // uniform
+                // V of `tile` and K of the next one; behind the last tile that one again, into
+                // buffers that nothing reads any more.
+                const auto fill = [&](std::uint32_t tile) {
+                    put_one(0, buffer(tile + 1));
+                    put_one(1, buffer(tile));
+                    fetch_one(0, tile + 2 < last ? tile + 2 : last - 1);
+                    fetch_one(1, tile + 1 < last ? tile + 1 : last - 1);
+                };
+                const auto phase = [&] {
+                    __builtin_amdgcn_sched_barrier(0);
+                    wait_lgkm0();
+                    lds_barrier();
+                    __builtin_amdgcn_sched_barrier(0);
+                };
+                put_one(0, buffer(first));
+                put_scales(first, key_ks_of(first), key_vs_of(first));
+                fetch_one(1, first);
+                fetch_one(0, first + 1 < last ? first + 1 : first);
+                phase();
+                if (ahead) {
+                    fill(first);
+                    phase();
+                }
+                const auto fill_step = [&](std::uint32_t tile) {
+                    fill(tile + ahead);
+                    if constexpr (!kUniform)
+                        if (tile + 1 < last) put_scales(tile + 1, key_ks_of(tile + 1), key_vs_of(tile + 1));
+                };
+                for (std::uint32_t tile = first; tile < last; ++tile) {
+                    const Scores of = scores(buffer(tile));
+                    set_priority<0>();
+                    phase();
+                    fill_step(tile);
+                    const Weights w = weights(of, tile, marks_of(tile), now, key_ks_of(tile), key_vs_of(tile));
+                    phase();
+                    set_priority<1>();
+                    weigh(w, buffer(tile));
+                }
+                if (!ahead) phase();
+                phase();
+            } else {
+                fetch_one(1, first);
+                const auto put = [&](std::uint32_t tile) {
+                    put_one(0, buffer(tile));
+                    put_one(1, buffer(tile));
+                    put_scales(tile, key_ks_of(tile), key_vs_of(tile));
+                };
+                put(first);
+                __syncthreads();
+                for (std::uint32_t tile = first; tile < last; ++tile) {
+                    const bool more = tile + 1 < last;
+                    if (more) {
+                        fetch_one(0, tile + 1);
+                        fetch_one(1, tile + 1);
+                    }
+                    if (wave_live) {
+                        const Scores of = scores(buffer(tile));
+                        weigh(weights(of, tile, marks_of(tile), now, key_ks_of(tile), key_vs_of(tile)), buffer(tile));
+                    }
+                    if (more) put(tile + 1);
+                    __syncthreads();
                 }
             }
-            __syncthreads();
-            buf ^= 1;
+            if (last == tile_end) break;
+            first = last;
+            ++window;
         }
     }
 
@@ -621,12 +677,13 @@ PrefillPlan prefill_plan(std::uint64_t num_seqs, std::uint64_t max_query, std::u
         plan.blocks = static_cast<std::uint32_t>((max_query + plan.tokens - 1) / plan.tokens);
         return num_seqs * plan.blocks * heads;
     };
-    // Eight wavefronts share a tile's loads and conversions, two workgroups of four a CU
-    // that waits less at barriers and is filled by fewer rows. Head size 128, eight and four:
-    // 512 tokens behind 32768 528 and 563 us; 8 x 4096 2312 and 2337; 8 x 2048 618 and 617;
-    // 16 prompts of up to 1000 200 and 170; one prompt of 2000 118 and 102; 64 tokens behind
-    // 2000 40 and 30; 16 sequences' 4 tokens behind up to 9000 164 and 104. Head size 64:
-    // 8 x 4096 702 and 676. At 256 the registers are those of four.
+    // Eight wavefronts share a tile's loads and conversions and take turns; two workgroups
+    // of four a CU are filled by fewer rows and wait less at barriers. Head size 128, eight
+    // and four: 512 tokens behind 32768 490 and 541 us; 8 x 4096 2060 and 2189; 16 prompts
+    // of up to 4096 2000 and 2108, of up to 2048 675 and 656, of up to 1000 191 and 169; 8 x
+    // 2048 573 and 606; one prompt of 2000 116 and 94; 64 tokens behind 2000 40 and 30; 16
+    // sequences' 4 tokens behind up to 9000 164 and 104. Head size 64: prompts of up to 700
+    // 40 and 23, 8 x 2048 199 and 167. At 256 the registers are those of four.
     std::uint64_t workgroups = shape(head_size == 128 ? 8 : 4);
     if (plan.waves == 8 && (max_query * group <= 128 || max_kv < 4096)) workgroups = shape(4);
     // Splits: where the heaviest block of queries would run on alone, its keys go to several
@@ -639,7 +696,6 @@ PrefillPlan prefill_plan(std::uint64_t num_seqs, std::uint64_t max_query, std::u
     const std::uint64_t of_cu = plan.waves == 8 || head_size == 256 ? 1 : 2, slots = of_cu * kCus;
     std::uint64_t share = (workgroups * (tiles + lightest) / 2 + slots - 1) / slots;
     if (share < kLeastTiles) share = kLeastTiles;
-    share = (share + 1) & ~std::uint64_t{1};
     plan.split_tiles = static_cast<std::uint32_t>(of_cu * share + share / 4 < tiles ? share : tiles);
     plan.splits = static_cast<std::uint32_t>((tiles + plan.split_tiles - 1) / plan.split_tiles);
     return plan;
@@ -775,8 +831,8 @@ extern "C" int kvflux_quant_prefill(const void* key_cache, const void* value_cac
     p.blocks = plan.blocks;
     p.splits = plan.splits;
     p.split_tiles = plan.split_tiles;
-    // A window of n tiles, an even number, has at most n * kTile / block_size + 2 pages.
-    const std::uint64_t window = (kWindow - 2) * block_size / kTile & ~std::uint64_t{1};
+    // A window of n tiles has at most n * kTile / block_size + 2 pages.
+    const std::uint64_t window = (kWindow - 2) * block_size / kTile;
     const std::uint64_t of_head = static_cast<std::uint64_t>(plan.splits) * num_seqs * plan.blocks;  // workgroups
     const bool pairs = plan.waves == 4 && head_size != 256 && kCus % num_kv_heads == 0 && of_head * num_kv_heads > kCus &&
                        of_head * num_kv_heads <= 2 * kCus;
