@@ -510,7 +510,9 @@ int kvflux_norm_rope_write_tail(void* key_cache, void* value_cache, uint64_t num
  *   [num_kv_heads][head_size] of `output_dtype`, each value rounded once; its
  *   other arguments as for kvflux_gather_paged_kv_live.
  * Any head_size; block_size and head_size such that a page has fewer than 2^31
- * values, heads below 2^16. Caches need no alignment; with 8 bytes (and inputs and
+ * values, heads below 2^16. KVFLUX_ERR_UNSUPPORTED: writes that may touch 2^24 pages
+ * and more, counted for each head of K and V; reads of 2^24 and more of 1024 groups
+ * (a page and more each). Caches need no alignment; with 8 bytes (and inputs and
  * outputs with 16, head_size and strides multiples of 8) the fast kernels run. All
  * calls are safe under graph capture.
  * ------------------------------------------------------------------------- */
@@ -567,7 +569,8 @@ int kvflux_quant_attention(const void* key_cache, const void* value_cache, const
  * for calls of few queries behind many tokens, whose keys are split over workgroups
  * (0: NULL will do; no initialisation; calls that share one must be ordered).
  * KVFLUX_ERR_UNSUPPORTED: more than 65535 sequences, 2^31 pages or max_kv_len, or
- * num_seqs * max_query_tokens * query_heads of 2^31 and more. */
+ * num_seqs * max_query_tokens * query_heads of 2^31 and more; 2^23 and more
+ * workgroups (of 128 or 256 query rows of a kv head). */
 int kvflux_quant_prefill_workspace_size(uint64_t num_seqs, uint64_t max_query_tokens, uint64_t max_kv_len,
                                         uint64_t num_kv_heads, uint64_t query_heads, uint64_t block_size,
                                         uint64_t head_size, size_t* bytes);

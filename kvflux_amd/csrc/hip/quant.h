@@ -123,6 +123,9 @@ __device__ inline float quant_scale(std::uint32_t largest) {
     return __uint_as_float(largest >= 0x7f800000u ? 0x7fc00000u : static_cast<std::uint32_t>(k + 127) << 23);
 }
 
+// Workgroups of a launch: HIP counts the threads of a grid, 256 a workgroup here, in 32 bits.
+constexpr std::uint64_t kMostWorkgroups = 0xffffffffULL / 256;
+
 inline bool aligned(std::uint64_t bytes, std::initializer_list<const void*> pointers) {
     for (const void* x : pointers)
         if (reinterpret_cast<std::uintptr_t>(x) % bytes != 0) return false;

@@ -752,6 +752,11 @@ std::uint32_t decode_grid(std::uint64_t rows, std::uint64_t kv_len, std::uint64_
     const std::uint64_t shares = tiles > most * kLeastShare ? most : rows * streams * tiles / kLeastShare + 1;
     return static_cast<std::uint32_t>(shares < most ? shares : most);
 }
+// Rows of a launch: what the plan holds, and what a grid counts (query_heads < 2^20).
+std::uint64_t decode_slice(std::uint64_t rows, std::uint64_t streams) {
+    const std::uint64_t most = kMostWorkgroups / streams < kPlanRows ? kMostWorkgroups / streams : kPlanRows;
+    return rows < most ? rows : most;
+}
 std::size_t decode_workspace(std::uint32_t grid, std::uint32_t set_heads, std::uint64_t head_size) {
     return 2ull * grid * set_heads * (head_size + 2) * sizeof(float) + grid * sizeof(uint2);
 }
@@ -803,7 +808,7 @@ int check_shape(const char* op, std::uint64_t num_rows, std::uint64_t kv_len, st
 } // namespace
 
 int launch_quant_rows(const QuantRows& p, std::uint64_t rows, int format, hipStream_t stream) {
-    const std::uint64_t at_once = 0x7fffffffULL / p.query_heads;
+    const std::uint64_t at_once = kMostWorkgroups / p.query_heads;
     for (std::uint64_t first = 0; first < rows; first += at_once) {
         const dim3 grid(static_cast<unsigned>((rows - first < at_once ? rows - first : at_once) * p.query_heads));
         if (format == KVFLUX_QUANT_E4M3)
@@ -830,7 +835,7 @@ extern "C" int kvflux_quant_attention_workspace_size(uint64_t num_rows, uint64_t
     std::uint32_t sets, set_heads;
     head_sets(query_heads / num_kv_heads, &sets, &set_heads);
     const std::uint64_t streams = num_kv_heads * sets;
-    std::uint64_t rows = num_rows < kPlanRows ? num_rows : kPlanRows;
+    std::uint64_t rows = decode_slice(num_rows, streams);
     // Enough for fewer rows as well, where those are cut into shares and these not.
     if (decode_grid(rows, kv_len, streams, head_size) == 0) {
         const std::uint64_t fewer = (kFullStreams - 1) / streams;
@@ -899,7 +904,7 @@ extern "C" int kvflux_quant_attention(const void* key_cache, const void* value_c
     p.output = output;
     p.scale_log2 = scale_log2;
     const std::uint64_t streams = num_kv_heads * p.sets;
-    const std::uint64_t slice = num_rows < kPlanRows ? num_rows : kPlanRows;
+    const std::uint64_t slice = decode_slice(num_rows, streams);
     const std::uint32_t grid = decode_grid(slice, kv_len, streams, head_size);
     if (grid != 0) {
         if (!workspace || workspace_bytes < decode_workspace(grid, p.set_heads, head_size))

@@ -841,7 +841,7 @@ extern "C" int kvflux_quant_prefill(const void* key_cache, const void* value_cac
     p.query = query;
     p.output = output;
     p.scale_log2 = scale_log2;
-    if (static_cast<std::uint64_t>(p.heads) * p.splits * p.num_seqs * p.blocks > 0x7fffffffULL)
+    if (static_cast<std::uint64_t>(p.heads) * p.splits * p.num_seqs * p.blocks > kMostWorkgroups / 2)
         return fail(KVFLUX_ERR_UNSUPPORTED, "quant prefill: shape too large");
     if (plan.splits > 1) {
         if (!workspace || workspace_bytes < prefill_workspace(plan, num_seqs, max_query_tokens, query_heads, head_size))

@@ -55,6 +55,7 @@ struct WriteParams {
     const std::uint64_t* kv_lens;
     const std::uint64_t* new_lens;  // null: one token a sequence, input row = sequence
     const std::uint64_t* offsets;
+    std::uint32_t max_new;    // bound of new_lens
     FastDiv pages;            // pages a sequence may touch
     std::uint32_t units;
 };
@@ -80,12 +81,12 @@ __global__ __launch_bounds__(kThreads) void quant_write_kernel(WriteParams p) {
     const std::uint32_t seq = p.pages.div(rest);
     const std::uint32_t page_of_new = rest - seq * p.pages.divisor;
 
-    const std::uint64_t len = p.kv_lens[seq];
+    const std::uint64_t full = p.kv_lens[seq];
     std::uint64_t fresh = p.new_lens ? p.new_lens[seq] : 1;
     const std::uint64_t offset = p.offsets ? p.offsets[seq] : seq;
-    if (fresh > len) fresh = len;
+    if (fresh > full) fresh = full;
     if (fresh == 0) return;
-    const std::uint64_t start = len - fresh;
+    const std::uint64_t start = full - fresh, len = fresh < p.max_new ? full : start + p.max_new;
     const std::uint64_t page = (p.bs_shift >= 0 ? start >> p.bs_shift : start / p.block_size) + page_of_new;
     const std::uint64_t at = page * p.block_size;  // position of the page's first token
     if (at >= len || page >= p.width) return;
@@ -218,7 +219,7 @@ int write(const char* op, void* key_cache, void* value_cache, float* key_scales,
     }
     // A run of n tokens touches at most (n + block_size - 2) / block_size + 1 pages.
     const std::uint64_t pages = max_new > 0x7fffffffULL ? ~0ULL : (max_new + block_size - 2) / block_size + 1;
-    if (num_seqs > 0x7fffffffULL || pages > 0x7fffffffULL || pages * num_seqs > 0x7fffffffULL / (2 * heads))
+    if (num_seqs > 0x7fffffffULL || pages > 0x7fffffffULL || pages * num_seqs > kMostWorkgroups / (2 * heads))
         return fail(KVFLUX_ERR_UNSUPPORTED, "%s: too many new tokens", op);
     WriteParams p{};
     p.cache[0] = static_cast<std::uint8_t*>(key_cache);
@@ -240,6 +241,7 @@ int write(const char* op, void* key_cache, void* value_cache, float* key_scales,
     p.kv_lens = kv_lens;
     p.new_lens = new_lens;
     p.offsets = offsets;
+    p.max_new = static_cast<std::uint32_t>(max_new);
     p.pages = FastDiv(static_cast<std::uint32_t>(pages));
     p.units = static_cast<std::uint32_t>(pages * num_seqs * 2 * heads);
     const bool wide = head_size % 8 == 0 && key_stride % 8 == 0 && value_stride % 8 == 0 &&
@@ -357,7 +359,7 @@ int launch_gather(ReadParams& p, std::uint64_t pages, hipStream_t stream) {
     const std::uint64_t row_groups = p.head_size / kV, token_groups = row_groups * p.heads;
     const std::uint64_t page_groups = token_groups * p.block_size;
     const std::uint64_t parts = (page_groups - 1) / (kThreads * kReadGroups) + 1;
-    if (page_groups > 0xffffffffULL || parts > 0x7fffffffULL / pages)
+    if (page_groups > 0xffffffffULL || parts > kMostWorkgroups / pages)
         return fail(KVFLUX_ERR_UNSUPPORTED, "quant gather: too many pages");
     p.row_groups = FastDiv(static_cast<std::uint32_t>(row_groups));
     p.token_groups = FastDiv(static_cast<std::uint32_t>(token_groups));

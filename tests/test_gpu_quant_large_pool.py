@@ -75,3 +75,25 @@ def test_pages_past_32_bits(gpu, fmt, D, shift, bound):
     assert int(large[large < blocks].max()) * H * BS * D > 1 << 32
     for a, b in zip(got, want):
         assert np.isfinite(b).all() and np.array_equal(a, b)
+
+
+@pytest.mark.parametrize("call", ["decode", "prompts"])
+def test_more_rows_than_a_grid_holds(gpu, call):
+    """20000 rows of 1024 heads, a workgroup each: past 2^32 threads. One token a row: its values come back."""
+    rows, heads, D, blocks = 20000, 1024, 8, 50
+    rng = np.random.default_rng(3)
+    v = rng.integers(0, 0x7f, (blocks, heads, 1, D)).astype(np.uint8)
+    cache, scales = [device.to_device(v), device.to_device(v)], device.to_device(np.full((blocks, heads), 0.5, np.float32))
+    pages = rng.integers(0, blocks, rows)
+    table, ones, offsets = u64(pages[:, None]), u64(np.ones(rows)), u64(np.arange(rows))
+    q, out = device.DeviceBuffer(rows * heads * D * 4), device.DeviceBuffer(rows * heads * D * 4)
+    q.fill(0)
+    out.fill(0xa5)
+    head = (cache[0].ptr, cache[1].ptr, scales.ptr, scales.ptr, blocks, heads, 1, D, capi.QUANT_INT8, table.ptr, 1)
+    if call == "decode":
+        capi.call("kvflux_quant_attention", *head, ones.ptr, 1, rows, heads, q.ptr, out.ptr, None, 0, None)
+    else:
+        capi.call("kvflux_quant_prefill", *head, ones.ptr, ones.ptr, offsets.ptr, rows, 1, 1, heads, q.ptr, out.ptr, None, 0, None)
+    for r in (0, 1, 9999, 16382, 16383, 16384, 19999):
+        got = out.download(np.float32, heads * D, offset=r * heads * D * 4).reshape(heads, D)
+        assert np.array_equal(got, v[pages[r], :, 0].astype(np.float32) * 0.5), r

@@ -192,11 +192,12 @@ def test_bad_pages_short_tables_and_bounds(gpu):
     for i in range(2):
         cache.write(i, table, [64, 10], [64, 10], [0, 0], rows.x[i])
     same(cache)
-    held += write(cache, rows, table, [64, 10], [64, 10], [0, 0], most=17)  # two pages of each at most
-    device.synchronize()
-    for i in range(2):
-        cache.write(i, table, [32, 10], [32, 10], [0, 0], rows.x[i])
-    same(cache)
+    for most in (17, 1, 16):  # the first of them
+        held += write(cache, rows, table, [64, 10], [64, 10], [0, 0], most=most)
+        device.synchronize()
+        for i in range(2):
+            cache.write(i, table, [most, min(most, 10)], [most, min(most, 10)], [0, 0], rows.x[i])
+        same(cache)
     del held
 
 

@@ -77,6 +77,7 @@ def test_writes(change, want):
 def test_sizes_of_writes():
     assert write(new=None) == capi.ERR_INVALID and write(off=None) == capi.ERR_INVALID
     assert write(seqs=1 << 31) == capi.ERR_UNSUPPORTED and write(most=1 << 40) == capi.ERR_UNSUPPORTED
+    assert write(seqs=1 << 23, most=1) == capi.ERR_UNSUPPORTED and gather(pages=1 << 24) == capi.ERR_UNSUPPORTED
     assert write(most=2 ** 64 - 1) == capi.ERR_UNSUPPORTED and tail(rows=1 << 31) == capi.ERR_UNSUPPORTED
     assert write(seqs=0, kn=None) == capi.OK and write(most=0, kn=None) == capi.OK and tail(rows=0, kn=None) == capi.OK
 
