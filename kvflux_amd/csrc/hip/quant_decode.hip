@@ -49,8 +49,9 @@ constexpr std::uint32_t kPartCost = 16;
 // The least of a share: fewer workgroups start where there is less to do. 4 rows of
 // <= 1500 tokens: 6 16.4 us, 8 12.3, 10 13.2, 16 13.8.
 constexpr std::uint32_t kLeastShare = 8;
-// Rows of at most this many tokens (half of it with heads of 256) take one workgroup a
-// stream and no merge; twice as many where the streams fill the GPU by themselves.
+// Rows of at most this many tokens (half of it with heads of 256, or where tokens have a
+// record each: 8 rows of <= 1000 tokens on 5-token pages 14.9 and 12.0 us) take one workgroup
+// a stream and no merge; twice as many where the streams fill the GPU by themselves.
 // A workgroup a stream, and shares: 1 row of <= 1024 tokens 8.9 and 11.5 us, 8 rows 13.0
 // and 14.2, 256 rows 67.6 and 75.7; 32 rows of <= 2048 21.1 and 24.2, but 8 rows 20.4 and
 // 14.8, and 128 rows of <= 4096 108 and 102.
@@ -121,20 +122,21 @@ struct Shape {
 // kSub: tokens that share a record. 8 where pages are multiples of 8 tokens, so that
 // every 8 tokens of a tile lie in one; 1 for pages of any other size.
 // kWhole: a workgroup takes one whole stream (no shares, no partials).
-template <typename F, int kD, int kSub, bool kWhole>
-__global__ __launch_bounds__(kThreads, Shape<kD>::kResident) void quant_decode_kernel(QuantDecodeParams p) {
+template <typename F, int kD, int kSub, bool kWhole, int kW>
+__global__ __launch_bounds__(64 * kW, Shape<kD>::kResident) void quant_decode_kernel(QuantDecodeParams p) {
     using S = Shape<kD>;
+    constexpr int kT = 64 * kW;
     using Vec = pf_f16x8_t;
     constexpr int kSteps = S::kSteps, kDt = S::kDt, kCpr = S::kCpr, kLoads = S::kLoads, kRowsOf = S::kRowsOf;
     constexpr std::uint32_t kPerTile = kTile / kSub;      // records of a tile
     constexpr std::uint32_t kBatch = 64 / kPerTile;       // tiles whose records the lanes make at once
     __shared__ std::uint64_t before[kWhole ? 1 : kPlanRows + 1];  // costs of a stream of each row before
     __shared__ std::uint32_t lens_of[kWhole ? 1 : kPlanRows];
-    __shared__ std::uint64_t wave_cost[kWaves];
-    __shared__ std::uint64_t places[kWaves][2][64];
-    __shared__ float2 scales_of[kWaves][2][64];
-    __shared__ __attribute__((aligned(16))) unsigned char wave_lds[kWaves][S::kWaveBytes];
-    __shared__ float2 stats[kWaves][kCols];
+    __shared__ std::uint64_t wave_cost[kW];
+    __shared__ std::uint64_t places[kW][2][64];
+    __shared__ float2 scales_of[kW][2][64];
+    __shared__ __attribute__((aligned(16))) unsigned char wave_lds[kW][S::kWaveBytes];
+    __shared__ float2 stats[kW][kCols];
 
     const int tid = threadIdx.x, lane = tid % 64;
     const auto uniform = [](std::uint32_t x) {
@@ -154,7 +156,7 @@ __global__ __launch_bounds__(kThreads, Shape<kD>::kResident) void quant_decode_k
     // in `ml`.
     const auto run_part = [&](std::uint32_t row, std::uint32_t len, std::uint32_t kvh, std::uint32_t set, std::uint32_t t0,
                               std::uint32_t t1, float* to, float* ml) {
-        const std::uint32_t tiles = t1 - t0 > wave ? (t1 - t0 - wave + kWaves - 1) / kWaves : 0;  // of this wavefront
+        const std::uint32_t tiles = t1 - t0 > wave ? (t1 - t0 - wave + kW - 1) / kW : 0;  // of this wavefront
         const std::uint32_t first_head = set * p.set_heads;
         const std::uint32_t heads = p.group - first_head < p.set_heads ? p.group - first_head : p.set_heads;
         const std::uint64_t* const table_row = p.table + (static_cast<std::uint64_t>(p.row_base) + row) * p.width;
@@ -170,7 +172,7 @@ __global__ __launch_bounds__(kThreads, Shape<kD>::kResident) void quant_decode_k
             const auto token_of = [&](std::uint32_t batch) {
                 const std::uint32_t j = batch * kBatch + lane / kPerTile;
                 // Past the wavefront's tiles: at or behind the row's end.
-                return j < tiles ? (t0 + wave + kWaves * j) * kTile + lane % kPerTile * kSub : ~0u;
+                return j < tiles ? (t0 + wave + kW * j) * kTile + lane % kPerTile * kSub : ~0u;
             };
             const auto fetch_page = [&](std::uint32_t batch) {
                 const std::uint32_t token = token_of(batch);
@@ -436,14 +438,14 @@ __global__ __launch_bounds__(kThreads, Shape<kD>::kResident) void quant_decode_k
                 *reinterpret_cast<float4*>(row_to + 16 * dt) = make_float4(acc[dt][0] * unit, acc[dt][1] * unit, acc[dt][2] * unit, acc[dt][3] * unit);
         }
         __syncthreads();
-        for (std::uint32_t i = tid; i < heads * kD; i += kThreads) {
+        for (std::uint32_t i = tid; i < heads * kD; i += kT) {
             const std::uint32_t h = i / kD, d = i % kD;
             float top = -INFINITY;
 #pragma unroll
-            for (int w = 0; w < kWaves; ++w) top = fmaxf(top, stats[w][h].x);
+            for (int w = 0; w < kW; ++w) top = fmaxf(top, stats[w][h].x);
             float sum = 0.0f, o = 0.0f;
 #pragma unroll
-            for (int w = 0; w < kWaves; ++w) {
+            for (int w = 0; w < kW; ++w) {
                 const float2 s = stats[w][h];
                 const float f = s.y != s.y ? s.y : merge_weight(s.x, top);
                 sum += s.y * f;
@@ -473,7 +475,7 @@ __global__ __launch_bounds__(kThreads, Shape<kD>::kResident) void quant_decode_k
         run_part(row, len, kvh, set, 0, tiles_of(len), output_of(row, kvh, set), nullptr);
     } else {
         // ---- plan: the cost of a stream of every row, and the sums of those before.
-        const std::uint32_t per = (p.rows + kThreads - 1) / kThreads;
+        const std::uint32_t per = (p.rows + kT - 1) / kT;
         std::uint64_t mine = 0;
         for (std::uint32_t i = 0; i < per; ++i) {
             const std::uint32_t r = tid * per + i;
@@ -498,7 +500,7 @@ __global__ __launch_bounds__(kThreads, Shape<kD>::kResident) void quant_decode_k
             before[r] = run;
             run += lens_of[r] != 0 ? tiles_of(lens_of[r]) + kPartCost : 0;
         }
-        if (tid == kThreads - 1) before[p.rows] = run;
+        if (tid == kT - 1) before[p.rows] = run;
         __syncthreads();
         const std::uint32_t streams = p.heads * p.sets;  // of a row
         const std::uint64_t total = before[p.rows] * streams;
@@ -512,7 +514,7 @@ __global__ __launch_bounds__(kThreads, Shape<kD>::kResident) void quant_decode_k
             if (lens_of[r] != 0) continue;
             if (p.by_stream && tid < streams) p.cuts[r * streams + tid] = make_uint2(~0u, 0);
             float* const out = p.output + (static_cast<std::uint64_t>(p.row_base) + r) * p.query_heads * kD;
-            for (std::uint32_t i = tid; i < p.query_heads * kD; i += kThreads) out[i] = 0.0f;
+            for (std::uint32_t i = tid; i < p.query_heads * kD; i += kT) out[i] = 0.0f;
         }
         if (tid == 0 && !p.by_stream) p.cuts[w] = make_uint2(~0u, 0);
         if (w >= shares) return;
@@ -744,8 +746,9 @@ void head_sets(std::uint64_t group, std::uint32_t* sets, std::uint32_t* heads) {
 }
 
 // Workgroups of a launch over `rows` rows; 0: one for each stream.
-std::uint32_t decode_grid(std::uint64_t rows, std::uint64_t kv_len, std::uint64_t streams, std::uint64_t head_size) {
-    const std::uint64_t whole = head_size == 256 ? kOneLaunch / 2 : kOneLaunch;
+std::uint32_t decode_grid(std::uint64_t rows, std::uint64_t kv_len, std::uint64_t streams, std::uint64_t block_size,
+                          std::uint64_t head_size) {
+    const std::uint64_t whole = head_size == 256 || block_size % 8 != 0 ? kOneLaunch / 2 : kOneLaunch;
     if (kv_len <= whole || (kv_len <= 2 * whole && rows * streams >= kFullStreams)) return 0;
     const std::uint64_t most = head_size == 256 ? Shape<256>::kGrid : Shape<128>::kGrid;
     const std::uint64_t tiles = (kv_len + kTile - 1) / kTile + kPartCost;
@@ -765,14 +768,24 @@ template <typename F, int kD, int kSub>
 int launch_decode(QuantDecodeParams& p, std::uint32_t grid, hipStream_t stream) {
     const std::uint64_t streams = static_cast<std::uint64_t>(p.heads) * p.sets;
     if (grid == 0) {
-        quant_decode_kernel<F, kD, kSub, true><<<dim3(static_cast<unsigned>(p.rows * streams)), dim3(kThreads), 0, stream>>>(p);
+        const dim3 workgroups(static_cast<unsigned>(p.rows * streams));
+        // Eight wavefronts where a CU has a stream at most (at 256 the registers are those of
+        // four), and each more than a tile or two. 8 rows of <= 1000 tokens: 12.7 us with
+        // four, 11.6 with eight; one of <= 300: 6.6 and 7.2.
+        if constexpr (kD <= 128) {
+            if (p.rows * streams <= kFullStreams && p.kv_len > kOneLaunch / 2) {
+                quant_decode_kernel<F, kD, kSub, true, 2 * kWaves><<<workgroups, dim3(2 * kThreads), 0, stream>>>(p);
+                return launch_status("quant_decode_kernel");
+            }
+        }
+        quant_decode_kernel<F, kD, kSub, true, kWaves><<<workgroups, dim3(kThreads), 0, stream>>>(p);
         return launch_status("quant_decode_kernel");
     }
     // The merge takes the shorter list: streams of a few rows, or the workgroups' cuts.
     // 16 rows of 2 kv heads with 16 query heads each: 40 us by workgroup, 19 by stream.
     const std::uint32_t cuts = p.rows * streams < grid ? static_cast<std::uint32_t>(p.rows * streams) : grid;
     p.by_stream = cuts < grid;
-    quant_decode_kernel<F, kD, kSub, false><<<dim3(grid), dim3(kThreads), 0, stream>>>(p);
+    quant_decode_kernel<F, kD, kSub, false, kWaves><<<dim3(grid), dim3(kThreads), 0, stream>>>(p);
     if (const int s = launch_status("quant_decode_kernel")) return s;
     // Parts of a stream: many where there are few streams. With 1024 threads and with 128:
     // 64 parts 25.3 and 26.6 us (the whole call), 18 parts 16.2 and 13.2.
@@ -837,12 +850,12 @@ extern "C" int kvflux_quant_attention_workspace_size(uint64_t num_rows, uint64_t
     const std::uint64_t streams = num_kv_heads * sets;
     std::uint64_t rows = decode_slice(num_rows, streams);
     // Enough for fewer rows as well, where those are cut into shares and these not.
-    if (decode_grid(rows, kv_len, streams, head_size) == 0) {
+    if (decode_grid(rows, kv_len, streams, block_size, head_size) == 0) {
         const std::uint64_t fewer = (kFullStreams - 1) / streams;
         if (fewer < rows) rows = fewer;
     }
     if (rows == 0) return KVFLUX_OK;
-    *bytes = decode_workspace(decode_grid(rows, kv_len, streams, head_size), set_heads, head_size);
+    *bytes = decode_workspace(decode_grid(rows, kv_len, streams, block_size, head_size), set_heads, head_size);
     return KVFLUX_OK;
 }
 
@@ -905,7 +918,7 @@ extern "C" int kvflux_quant_attention(const void* key_cache, const void* value_c
     p.scale_log2 = scale_log2;
     const std::uint64_t streams = num_kv_heads * p.sets;
     const std::uint64_t slice = decode_slice(num_rows, streams);
-    const std::uint32_t grid = decode_grid(slice, kv_len, streams, head_size);
+    const std::uint32_t grid = decode_grid(slice, kv_len, streams, block_size, head_size);
     if (grid != 0) {
         if (!workspace || workspace_bytes < decode_workspace(grid, p.set_heads, head_size))
             return fail(KVFLUX_ERR_INVALID_ARGUMENT, "quant attention: workspace too small");
