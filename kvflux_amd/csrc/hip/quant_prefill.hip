@@ -22,8 +22,9 @@
 //    multiplies the weight.
 //  * The tile's weighted values are summed from zero and added with one rounding: an
 //    MFMA on a large accumulator drops bits of small weights, always in one direction.
-// A call whose workgroups would leave CUs idle (a short chunk behind a long prefix)
-// spreads each one's keys over several, merged by a second kernel.
+//  * Where workgroups are few, two sets of four wavefronts on the same rows take every other
+//    tile and are merged in LDS; where CUs would be left idle (a short chunk behind a long
+//    prefix) a block's keys go to several workgroups, merged by a second kernel.
 //
 // 32 query heads, 8 kv heads of 128: 512 tokens behind 32768 490 us, 1130 TFLOP/s of the
 // two parts' products, where a large library product in FP16 reaches 1174; 8 prompts of
@@ -47,15 +48,21 @@ constexpr std::uint32_t kUnread = 0x80000000u;  // a page whose bytes are not re
 constexpr std::uint32_t kMissing = ~0u;         // one that is not there
 constexpr float kWeightScale = 32768.0f;  // as in the decode: parts of 2^15 times a weight of at most 1
 
-// kWaves wavefronts hold 32 rows each.
-template <int kD, int kWaves, bool kUniform>
+// How a workgroup's wavefronts share its work: four of 32 rows each; eight that take turns;
+// or two sets of four on the same 128 rows, which take every other tile and are merged.
+enum class Order { Four, Turns, Halves };
+
+template <int kD, Order kOrder, bool kUniform>
 struct Shape {
+    static constexpr int kWaves = kOrder == Order::Four ? 4 : 8;
+    static constexpr int kSets = kOrder == Order::Halves ? 2 : 1;
     static constexpr int kThreads = 64 * kWaves;
-    static constexpr std::uint32_t kRows = 32 * kWaves;
+    static constexpr int kLoaders = kThreads / kSets;  // threads that load a tile
+    static constexpr std::uint32_t kRows = 32 * kWaves / kSets;
     // Wavefronts of a SIMD: the registers of two hold Q and the sums of 32 rows up to D = 128,
     // of three at 64 (8 prompts of 2048: two 181 us, three 167), but not with scales that
     // differ within 16 keys.
-    static constexpr int kPerSimd = kD == 256 ? 1 : kD == 64 && kUniform ? 3 : 2;
+    static constexpr int kPerSimd = kD == 256 ? 1 : kD == 64 && kUniform && kOrder == Order::Four ? 3 : 2;
 };
 
 struct QuantPrefillParams {
@@ -79,7 +86,6 @@ struct QuantPrefillParams {
     std::uint32_t blocks;              // workgroups along max_query
     std::uint32_t splits, split_tiles; // workgroups of a block of queries at most, tiles of each
     std::uint32_t window_tiles;        // tiles whose pages fit kWindow
-    std::uint32_t paired_from;         // see the kernel's order of workgroups
     const float* query;
     float* output;
     float scale_log2;
@@ -99,43 +105,47 @@ __device__ inline Split split_of(std::uint32_t tile_count, std::uint32_t most) {
 
 // kUniform: pages are multiples of 16 tokens, so 16 neighbouring keys of a tile share
 // their scales, which are then one value for a wavefront.
-template <typename F, int kD, int kWaves, bool kUniform>
-__global__ __launch_bounds__(64 * kWaves, (Shape<kD, kWaves, kUniform>::kPerSimd)) void quant_prefill_kernel(QuantPrefillParams p) {
-    using S = Shape<kD, kWaves, kUniform>;
+template <typename F, int kD, Order kOrder, bool kUniform>
+__global__ __launch_bounds__((Shape<kD, kOrder, kUniform>::kThreads), (Shape<kD, kOrder, kUniform>::kPerSimd)) void quant_prefill_kernel(QuantPrefillParams p) {
+    using S = Shape<kD, kOrder, kUniform>;
     using Vec = pf_f16x8_t;
-    constexpr int kThreads = S::kThreads;
+    constexpr int kThreads = S::kThreads, kWaves = S::kWaves, kSets = S::kSets, kLoaders = S::kLoaders;
     constexpr int kSteps = kD / 16;            // MFMAs of a 32-key block of S^T for one part of Q
     constexpr int kDb = kD / 32;               // dim blocks of O^T
     constexpr int kRowBytes = kD * 2;          // a key's row in LDS
     constexpr int kCpr = kRowBytes / 16;
     constexpr int kTileBytes = static_cast<int>(kTile) * kRowBytes;
     // Bytes of K, and as many of V, that a thread loads of a tile: of one key.
-    constexpr int kBytes = static_cast<int>(kTile) * kD / kThreads;
+    constexpr int kBytes = static_cast<int>(kTile) * kD / kLoaders;
     constexpr int kKeyThreads = kD / kBytes;   // threads of a key
     constexpr int kWords = kBytes / 4;
     static_assert(kBytes >= 8 && kD % kBytes == 0, "tile split");
-    // [buffer][K, V]
-    __shared__ __attribute__((aligned(16))) unsigned char tiles_lds[2][2][kTileBytes];
+    // [set][buffer][K, V]; at the end of two sets the second one's sums.
+    constexpr int kPad = kD + 4;
+    __shared__ __attribute__((aligned(16))) unsigned char tiles_lds[kSets][2][2][kTileBytes];
+    static_assert(kSets == 1 || sizeof(tiles_lds) >= S::kRows * kPad * sizeof(float), "merge buffer");
+    __shared__ float2 stats[kSets == 1 ? 1 : S::kRows];
     __shared__ std::uint32_t page_id[kWindow];
     __shared__ float page_ks[kWindow], page_vs[kWindow];  // vs over the reference, times kWeightScale
     // Where the scales differ within 16 keys: those of a buffer's keys.
-    __shared__ __attribute__((aligned(16))) float key_ks[kUniform ? 1 : 2][kUniform ? 4 : kTile];
-    __shared__ __attribute__((aligned(16))) float key_vs[kUniform ? 1 : 2][kUniform ? 4 : kTile];
+    __shared__ __attribute__((aligned(16))) float key_ks[kSets][kUniform ? 1 : 2][kUniform ? 4 : kTile];
+    __shared__ __attribute__((aligned(16))) float key_vs[kSets][kUniform ? 1 : 2][kUniform ? 4 : kTile];
     __shared__ float wave_top[kWaves];
     __shared__ std::uint32_t wave_missing[kWaves];
 
     const int tid = threadIdx.x, lane = tid % 64;
     const std::uint32_t wave = static_cast<std::uint32_t>(__builtin_amdgcn_readfirstlane(tid / 64));
     const int col = lane % 32, half = lane / 32;
-    // Heaviest query blocks first; neighbouring workgroups take the kv heads in turn. Where
-    // all workgroups are resident, two a CU, the heaviest share one with the lightest.
+    // Heaviest query blocks first; neighbouring workgroups take the kv heads in turn, then the
+    // sequences, at every block from another one on: workgroups go to the shader engines in
+    // turn, and the longest sequence's are not to meet on one (16 prompts of up to 2048 tokens,
+    // 8 kv heads: 658 us without, 473 with).
     std::uint32_t x = blockIdx.x;
     const std::uint32_t kvh = x % p.heads;
     x /= p.heads;
-    if (x >= p.paired_from) x = gridDim.x / p.heads - 1 - (x - p.paired_from);
     const std::uint32_t split = x % p.splits;
     x /= p.splits;
-    const std::uint32_t seq = x % p.num_seqs, qb = p.blocks - 1 - x / p.num_seqs;
+    const std::uint32_t level = x / p.num_seqs, qb = p.blocks - 1 - level, seq = (x + level) % p.num_seqs;
     const std::uint64_t full_len = p.kv_lens[seq], full_q = p.query_lens[seq];
     const std::uint32_t kv_len = full_len < p.max_kv ? static_cast<std::uint32_t>(full_len) : p.max_kv;
     std::uint32_t tq = full_q < kv_len ? static_cast<std::uint32_t>(full_q) : kv_len;
@@ -152,7 +162,8 @@ __global__ __launch_bounds__(64 * kWaves, (Shape<kD, kWaves, kUniform>::kPerSimd
     const std::uint64_t* const table = p.table + seq * p.width;
 
     // This lane's row.
-    const std::uint32_t r = 32 * wave + static_cast<std::uint32_t>(col);
+    const std::uint32_t set = kSets == 1 ? 0 : wave / 4;  // uniform
+    const std::uint32_t r = 32 * (kSets == 1 ? wave : wave % 4) + static_cast<std::uint32_t>(col);
     const std::uint32_t token = t0 + p.heads_div.div(r), head = p.first + p.heads_div.mod(r);
     const bool row_live = r < p.tokens * p.heads_of && token < t_end;
     const bool wave_live = __builtin_amdgcn_ballot_w64(row_live) != 0;
@@ -219,7 +230,8 @@ __global__ __launch_bounds__(64 * kWaves, (Shape<kD, kWaves, kUniform>::kPerSimd
     };
 
     // ---- loads: a thread's kBytes of K and of V of one key of a tile, at the same place.
-    const std::uint32_t my_row = static_cast<std::uint32_t>(tid) / kKeyThreads, my_col = static_cast<std::uint32_t>(tid) % kKeyThreads * kBytes;
+    const std::uint32_t loader = static_cast<std::uint32_t>(tid) % kLoaders;
+    const std::uint32_t my_row = loader / kKeyThreads, my_col = loader % kKeyThreads * kBytes;
     const std::uint64_t head_bytes = static_cast<std::uint64_t>(p.block_size.divisor) * kD;
     std::uint32_t held[2][kWords];
     bool held_live = false;  // V's
@@ -249,10 +261,10 @@ __global__ __launch_bounds__(64 * kWaves, (Shape<kD, kWaves, kUniform>::kPerSimd
     };
     // Scales of a tile's keys where those of 16 neighbours differ; missing pages' are 0.
     const auto put_scales = [&](std::uint32_t tile, float* ks, float* vs) {
-        if (kUniform || tid >= static_cast<int>(kTile)) return;
-        const std::uint32_t i = p.block_size.div(tile * kTile + tid) - window_page;
-        ks[tid] = page_ks[i];
-        vs[tid] = page_vs[i];
+        if (kUniform || loader >= kTile) return;
+        const std::uint32_t i = p.block_size.div(tile * kTile + loader) - window_page;
+        ks[loader] = page_ks[i];
+        vs[loader] = page_vs[i];
     };
 
     qp_f32x16_t acc[kDb];
@@ -501,15 +513,15 @@ __global__ __launch_bounds__(64 * kWaves, (Shape<kD, kWaves, kUniform>::kPerSimd
 
     if (tile_begin < tile_end) {  // uniform
         const auto unit_now = [&] { return reference > 0.0f ? reference : 1.0f; };
-        const auto key_ks_of = [&](std::uint32_t tile) { return key_ks[kUniform ? 0 : tile & 1]; };
-        const auto key_vs_of = [&](std::uint32_t tile) { return key_vs[kUniform ? 0 : tile & 1]; };
-        const auto buffer = [&](std::uint32_t tile) { return tiles_lds[tile & 1][0]; };
+        const auto key_ks_of = [&](std::uint32_t tile) { return key_ks[set][kUniform ? 0 : tile / kSets & 1]; };
+        const auto key_vs_of = [&](std::uint32_t tile) { return key_vs[set][kUniform ? 0 : tile / kSets & 1]; };
+        const auto buffer = [&](std::uint32_t tile) { return tiles_lds[set][tile / kSets & 1][0]; };
         for (std::uint32_t first = tile_begin;;) {
             stage();
             const float now = unit_now();
             const std::uint32_t behind = (window + 1) * p.window_tiles, last = behind < tile_end ? behind : tile_end;
-            fetch_one(0, first);
-            if constexpr (kWaves == 8) {
+            if constexpr (kOrder == Order::Turns) {
+                fetch_one(0, first);
                 // Two wavefronts a SIMD take turns: one multiplies (a tile's weighted values and
                 // the next one's scores) while the other works out weights, for whole phases. The
                 // second half's is a phase behind, and fills the buffers a tile ahead.
@@ -555,25 +567,29 @@ __global__ __launch_bounds__(64 * kWaves, (Shape<kD, kWaves, kUniform>::kPerSimd
                 if (!ahead) phase();
                 phase();
             } else {
-                fetch_one(1, first);
+                const auto fetch = [&](std::uint32_t tile) {
+                    fetch_one(0, tile);
+                    fetch_one(1, tile);
+                };
                 const auto put = [&](std::uint32_t tile) {
                     put_one(0, buffer(tile));
                     put_one(1, buffer(tile));
                     put_scales(tile, key_ks_of(tile), key_vs_of(tile));
                 };
-                put(first);
+                if (first + set < last) {
+                    fetch(first + set);
+                    put(first + set);
+                }
                 __syncthreads();
-                for (std::uint32_t tile = first; tile < last; ++tile) {
-                    const bool more = tile + 1 < last;
-                    if (more) {
-                        fetch_one(0, tile + 1);
-                        fetch_one(1, tile + 1);
-                    }
-                    if (wave_live) {
+                for (std::uint32_t step = first; step < last; step += kSets) {
+                    const std::uint32_t tile = step + set;
+                    const bool more = tile + kSets < last;
+                    if (more) fetch(tile + kSets);
+                    if (wave_live && (kSets == 1 || tile < last)) {
                         const Scores of = scores(buffer(tile));
                         weigh(weights(of, tile, marks_of(tile), now, key_ks_of(tile), key_vs_of(tile)), buffer(tile));
                     }
-                    if (more) put(tile + 1);
+                    if (more) put(tile + kSets);
                     __syncthreads();
                 }
             }
@@ -587,12 +603,49 @@ __global__ __launch_bounds__(64 * kWaves, (Shape<kD, kWaves, kUniform>::kPerSimd
     sum += low;
     const auto swapped = __builtin_amdgcn_permlane32_swap(__float_as_uint(sum), __float_as_uint(sum), false, false);
     sum = __uint_as_float(swapped[0]) + __uint_as_float(swapped[1]);
+    float in_ones = unit * (1.0f / kWeightScale);
+    if constexpr (kSets == 2) {
+        float m = threshold == 0.0f ? ref : -INFINITY;  // -INFINITY: no key seen
+        if (set == 1) {
+            if (half == 0) stats[r] = make_float2(m, sum);
+            float* const to = reinterpret_cast<float*>(tiles_lds) + r * kPad + 4 * half;
+#pragma unroll
+            for (int db = 0; db < kDb; ++db)
+#pragma unroll
+                for (int g = 0; g < 4; ++g)
+                    *reinterpret_cast<float4*>(to + 32 * db + 8 * g) =
+                        make_float4(acc[db][4 * g] * in_ones, acc[db][4 * g + 1] * in_ones, acc[db][4 * g + 2] * in_ones, acc[db][4 * g + 3] * in_ones);
+        }
+        __syncthreads();
+        if (set == 1) return;
+        const float2 other = stats[r];
+        const float top = fmaxf(m, other.x);
+        // NaN sums stay NaN.
+        const auto share = [&](float of, float total) {
+            return total != total ? total : of == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(of - top);
+        };
+        const float f0 = share(m, sum), f1 = share(other.x, other.y);
+        const float* const from = reinterpret_cast<const float*>(tiles_lds) + r * kPad + 4 * half;
+#pragma unroll
+        for (int db = 0; db < kDb; ++db)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const float4 v = *reinterpret_cast<const float4*>(from + 32 * db + 8 * g);
+                acc[db][4 * g] = acc[db][4 * g] * in_ones * f0 + v.x * f1;
+                acc[db][4 * g + 1] = acc[db][4 * g + 1] * in_ones * f0 + v.y * f1;
+                acc[db][4 * g + 2] = acc[db][4 * g + 2] * in_ones * f0 + v.z * f1;
+                acc[db][4 * g + 3] = acc[db][4 * g + 3] * in_ones * f0 + v.w * f1;
+            }
+        sum = sum * f0 + other.y * f1;
+        ref = top == -INFINITY ? 0.0f : top;
+        in_ones = 1.0f;
+    }
     if (!row_live) return;
     const bool whole = mine.count == 1;
     const std::uint32_t head_at = kvh * p.group + head;
     const std::uint64_t part_row = ((static_cast<std::uint64_t>(split) * p.num_seqs + seq) * p.max_query + token) * p.query_heads + head_at;
     float* const to = whole ? p.output + ((p.query_offsets[seq] + token) * p.query_heads + head_at) * kD : p.part_acc + part_row * kD;
-    const float inv = whole && sum != 0.0f ? 1.0f / sum : 1.0f, in_ones = unit * (1.0f / kWeightScale);
+    const float inv = whole && sum != 0.0f ? 1.0f / sum : 1.0f;
 #pragma unroll
     for (int db = 0; db < kDb; ++db)
 #pragma unroll
@@ -658,7 +711,7 @@ __global__ __launch_bounds__(256) void quant_prefill_merge_kernel(QuantPrefillPa
 
 // ---------------------------------------------------------------- dispatch
 struct PrefillPlan {
-    std::uint32_t waves;     // of a workgroup
+    Order order;
     std::uint32_t heads_of;  // query heads of a launch: the largest divisor of the group that fits
     std::uint32_t tokens, blocks, splits, split_tiles;
 };
@@ -668,35 +721,50 @@ constexpr std::uint64_t kLeastTiles = 4;  // of a split
 PrefillPlan prefill_plan(std::uint64_t num_seqs, std::uint64_t max_query, std::uint64_t max_kv, std::uint64_t heads,
                          std::uint64_t group, std::uint64_t head_size) {
     PrefillPlan plan{};
-    const auto shape = [&](std::uint32_t waves) {
-        plan.waves = waves;
-        const std::uint64_t rows = 32 * waves;
+    const auto shape = [&](Order order) {
+        plan.order = order;
+        const std::uint64_t rows = order == Order::Turns ? 256 : 128;
         plan.heads_of = static_cast<std::uint32_t>(group < rows ? group : rows);
         while (group % plan.heads_of != 0) --plan.heads_of;
         plan.tokens = static_cast<std::uint32_t>(rows / plan.heads_of);
         plan.blocks = static_cast<std::uint32_t>((max_query + plan.tokens - 1) / plan.tokens);
         return num_seqs * plan.blocks * heads;
     };
-    // Eight wavefronts share a tile's loads and conversions and take turns; two workgroups
-    // of four a CU are filled by fewer rows and wait less at barriers. Head size 128, eight
-    // and four: 512 tokens behind 32768 490 and 541 us; 8 x 4096 2060 and 2189; 16 prompts
-    // of up to 4096 2000 and 2108, of up to 2048 675 and 656, of up to 1000 191 and 169; 8 x
-    // 2048 573 and 606; one prompt of 2000 116 and 94; 64 tokens behind 2000 40 and 30; 16
-    // sequences' 4 tokens behind up to 9000 164 and 104. Head size 64: prompts of up to 700
-    // 40 and 23, 8 x 2048 199 and 167. At 256 the registers are those of four.
-    std::uint64_t workgroups = shape(head_size == 128 ? 8 : 4);
-    if (plan.waves == 8 && (max_query * group <= 128 || max_kv < 4096)) workgroups = shape(4);
-    // Splits: where the heaviest block of queries would run on alone, its keys go to several
-    // workgroups, none with more tiles than its share of all (bounds standing for lengths).
-    // Two workgroups of a CU take 3.1 us a tile each, one by itself 1.7 (head size 128), so
-    // there a block may have twice the share.
+    // Turns: eight wavefronts share a tile's loads and conversions; two workgroups of four a
+    // CU are filled by fewer rows and wait less at barriers. Head size 128, eight and four:
+    // 512 tokens behind 32768 490 and 541 us; 8 x 4096 2060 and 2189; 16 prompts of up to
+    // 4096 2000 and 2108, of up to 2048 675 and 656, of up to 1000 191 and 169; 8 x 2048 573
+    // and 606; 64 tokens behind 2000 34 and 27. Head size 64: 8 x 2048 199 and 167. At 256
+    // the registers are those of four.
+    std::uint64_t workgroups = shape(head_size == 128 ? Order::Turns : Order::Four);
+    if (plan.order == Order::Turns && (max_query * group <= 128 || max_kv < 4096)) workgroups = shape(Order::Four);
+    // Halves: half as many steps for the longest workgroups where there are few, one a CU.
+    // Halves and four: 7 prompts of up to 700, heads of 64, 20.6 and 24.3 us; one prompt of
+    // 1000 45.7 and 53.5, of 2000 86 and 93; 8 x 128 tokens behind up to 3000 104 and 134; but
+    // 16 prompts of up to 700, heads of 64, 37 and 30. A workgroup of one wavefront's rows
+    // leaves the CU to others: 16 x 4 tokens behind up to 9000 127 and 96.
+    if (plan.order == Order::Four && head_size != 256 && workgroups <= 2 * kCus && max_kv > 4 * kTile &&
+        (max_query * group > 32 || max_kv <= 32 * kTile))
+        plan.order = Order::Halves;
     const std::uint64_t tiles = (max_kv + kTile - 1) / kTile;
-    const std::uint64_t first = max_query < plan.tokens ? max_query : plan.tokens;
-    const std::uint64_t lightest = (max_kv - max_query + first + kTile - 1) / kTile;
-    const std::uint64_t of_cu = plan.waves == 8 || head_size == 256 ? 1 : 2, slots = of_cu * kCus;
-    std::uint64_t share = (workgroups * (tiles + lightest) / 2 + slots - 1) / slots;
-    if (share < kLeastTiles) share = kLeastTiles;
-    plan.split_tiles = static_cast<std::uint32_t>(of_cu * share + share / 4 < tiles ? share : tiles);
+    if (plan.order != Order::Four || head_size == 256) {
+        // One workgroup a CU: the keys of each go to as many as fill the CUs once (1024 tokens
+        // behind 16384: 504 us, in shares of the mean 701).
+        std::uint64_t most = workgroups < kCus ? kCus / workgroups : 1;
+        if (tiles <= 2 * kLeastTiles) most = 1;
+        if (most > (tiles + kLeastTiles - 1) / kLeastTiles) most = (tiles + kLeastTiles - 1) / kLeastTiles;
+        plan.split_tiles = static_cast<std::uint32_t>((tiles + most - 1) / most);
+    } else {
+        // Where the heaviest block of queries would run on alone, its keys go to several
+        // workgroups, none with more tiles than its share of all (bounds standing for
+        // lengths). Two workgroups of a CU take 3.1 us a tile each, one by itself 1.7 (head
+        // size 128), so a block may have twice the share.
+        const std::uint64_t first = max_query < plan.tokens ? max_query : plan.tokens;
+        const std::uint64_t lightest = (max_kv - max_query + first + kTile - 1) / kTile;
+        std::uint64_t share = (workgroups * (tiles + lightest) / 2 + 2 * kCus - 1) / (2 * kCus);
+        if (share < kLeastTiles) share = kLeastTiles;
+        plan.split_tiles = static_cast<std::uint32_t>(2 * share + share / 4 < tiles ? share : tiles);
+    }
     plan.splits = static_cast<std::uint32_t>((tiles + plan.split_tiles - 1) / plan.split_tiles);
     return plan;
 }
@@ -705,12 +773,12 @@ std::uint64_t prefill_workspace(const PrefillPlan& plan, std::uint64_t num_seqs,
     return plan.splits == 1 ? 0 : plan.splits * num_seqs * max_query * query_heads * (head_size + 2) * sizeof(float);
 }
 
-template <typename F, int kD, int kWaves>
+template <typename F, int kD, Order kOrder>
 int launch_prefill(QuantPrefillParams& p, hipStream_t stream) {
-    const dim3 grid(p.heads * p.splits * p.num_seqs * p.blocks), threads(64 * kWaves);
+    const dim3 grid(p.heads * p.splits * p.num_seqs * p.blocks), threads(Shape<kD, kOrder, true>::kThreads);
     for (p.first = 0; p.first < p.group; p.first += p.heads_of) {
-        if (p.block_size.divisor % 16 == 0) quant_prefill_kernel<F, kD, kWaves, true><<<grid, threads, 0, stream>>>(p);
-        else quant_prefill_kernel<F, kD, kWaves, false><<<grid, threads, 0, stream>>>(p);
+        if (p.block_size.divisor % 16 == 0) quant_prefill_kernel<F, kD, kOrder, true><<<grid, threads, 0, stream>>>(p);
+        else quant_prefill_kernel<F, kD, kOrder, false><<<grid, threads, 0, stream>>>(p);
         if (const int s = launch_status("quant_prefill_kernel")) return s;
     }
     if (p.splits == 1) return KVFLUX_OK;
@@ -720,11 +788,16 @@ int launch_prefill(QuantPrefillParams& p, hipStream_t stream) {
     return launch_status("quant_prefill_merge_kernel");
 }
 template <typename F>
-int launch_prefill_head_size(QuantPrefillParams& p, std::uint64_t head_size, std::uint32_t waves, hipStream_t s) {
+int launch_prefill_head_size(QuantPrefillParams& p, std::uint64_t head_size, Order order, hipStream_t s) {
     switch (head_size) {
-    case 64: return launch_prefill<F, 64, 4>(p, s);
-    case 128: return waves == 4 ? launch_prefill<F, 128, 4>(p, s) : launch_prefill<F, 128, 8>(p, s);
-    default: return launch_prefill<F, 256, 4>(p, s);
+    case 64: return order == Order::Four ? launch_prefill<F, 64, Order::Four>(p, s) : launch_prefill<F, 64, Order::Halves>(p, s);
+    case 128:
+        switch (order) {
+        case Order::Four: return launch_prefill<F, 128, Order::Four>(p, s);
+        case Order::Turns: return launch_prefill<F, 128, Order::Turns>(p, s);
+        default: return launch_prefill<F, 128, Order::Halves>(p, s);
+        }
+    default: return launch_prefill<F, 256, Order::Four>(p, s);
     }
 }
 
@@ -833,10 +906,6 @@ extern "C" int kvflux_quant_prefill(const void* key_cache, const void* value_cac
     p.split_tiles = plan.split_tiles;
     // A window of n tiles has at most n * kTile / block_size + 2 pages.
     const std::uint64_t window = (kWindow - 2) * block_size / kTile;
-    const std::uint64_t of_head = static_cast<std::uint64_t>(plan.splits) * num_seqs * plan.blocks;  // workgroups
-    const bool pairs = plan.waves == 4 && head_size != 256 && kCus % num_kv_heads == 0 && of_head * num_kv_heads > kCus &&
-                       of_head * num_kv_heads <= 2 * kCus;
-    p.paired_from = pairs ? static_cast<std::uint32_t>(kCus / num_kv_heads) : 0xffffffffu;
     p.window_tiles = static_cast<std::uint32_t>(window < 0x40000000ULL ? window : 0x40000000ULL);
     p.query = query;
     p.output = output;
@@ -850,6 +919,6 @@ extern "C" int kvflux_quant_prefill(const void* key_cache, const void* value_cac
         p.part_acc = static_cast<float*>(workspace);
         p.part_ml = p.part_acc + static_cast<std::uint64_t>(plan.splits) * num_seqs * max_query_tokens * query_heads * head_size;
     }
-    return format == KVFLUX_QUANT_E4M3 ? launch_prefill_head_size<QuantE4m3>(p, head_size, plan.waves, as_stream(stream))
-                                       : launch_prefill_head_size<QuantInt8>(p, head_size, plan.waves, as_stream(stream));
+    return format == KVFLUX_QUANT_E4M3 ? launch_prefill_head_size<QuantE4m3>(p, head_size, plan.order, as_stream(stream))
+                                       : launch_prefill_head_size<QuantInt8>(p, head_size, plan.order, as_stream(stream));
 }

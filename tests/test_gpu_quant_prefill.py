@@ -98,7 +98,7 @@ def test_bounds_past_the_lengths(gpu, fmt, D, bs, H, G):
     """What is chosen by the bounds (wavefronts, splits) on short sequences, with a page missing."""
     lens, new = np.array([1, 63, 0, 64, 65, 130, 200]), np.array([1, 63, 0, 2, 65, 1, 190])
     rng, cache, table, q = make(fmt, H, G, D, bs, lens, new, [D, bs])
-    for bound in (4096, 20000):
+    for bound in (400, 3000, 4096, 20000):
         call, got = run(cache, table, lens, new, q, most=max(200, 129 // G + 1), kv_len=bound)
         check(cache, table, call, got, some=20)
         table[6, 1] = cache.blocks
@@ -122,6 +122,16 @@ def test_keys_split_over_workgroups(gpu, fmt, D, bs, n, m):
     call, got = run(cache, table, [n, 20], [m, 20], q)
     assert call.size > 0
     check(cache, table, call, got, some=6)
+
+
+@pytest.mark.parametrize("seqs", [1, 3, 17])
+def test_every_sequence_and_block_is_reached(gpu, seqs):
+    """The order of workgroups is a permutation: outputs of prompts of many lengths, whole ones at that."""
+    lens = np.random.default_rng(seqs).integers(1, 420, seqs)
+    rng, cache, table, q = make("int8", 4, 2, 64, 16, lens, lens, seqs)
+    call, got = run(cache, table, lens, lens, q)
+    check(cache, table, call, got, some=24)
+    assert (got.view(np.uint32) != 0xa5a5a5a5).all()
 
 
 def test_long_prompts(gpu):
@@ -161,7 +171,7 @@ def test_bytes_of_a_page_without_numbers_reach_what_sees_them_alone(gpu, bs, D, 
     cache.scales[1, page, 1] = np.nan
     cache.bytes[1, page, 1] = 0xff
     cache.upload()
-    results = [run(cache, table, [n], [m], q, kv_len=bound)[1] for bound in (n, 5000)]
+    results = [run(cache, table, [n], [m], q, kv_len=bound)[1] for bound in (n, max(n, 400), 5000)]
     before = first - (n - m)
     assert 0 < before < m
     cache.scales[1, page, 1], cache.bytes[1, page, 1] = 1.0, 0
