@@ -512,7 +512,8 @@ __global__ __launch_bounds__(64 * kW, Shape<kD>::kResident) void quant_decode_ke
         // Rows without tokens: zeros.
         for (std::uint32_t r = w; r < p.rows; r += gridDim.x) {
             if (lens_of[r] != 0) continue;
-            if (p.by_stream && tid < streams) p.cuts[r * streams + tid] = make_uint2(~0u, 0);
+            if (p.by_stream)
+                for (std::uint32_t i = tid; i < streams; i += kT) p.cuts[r * streams + i] = make_uint2(~0u, 0);
             float* const out = p.output + (static_cast<std::uint64_t>(p.row_base) + r) * p.query_heads * kD;
             for (std::uint32_t i = tid; i < p.query_heads * kD; i += kT) out[i] = 0.0f;
         }

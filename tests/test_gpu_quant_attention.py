@@ -261,6 +261,18 @@ def test_generic_head_sizes_and_alignments(gpu, D, shift):
         check_both(cache, table, lens, q)
 
 
+@pytest.mark.parametrize("H,G", [(300, 1), (255, 2), (100, 17)])
+def test_more_heads_than_a_workgroup_has_threads(gpu, H, G):
+    """A row without tokens beside a long one, or alone: whatever the workspace held, it gives zeros."""
+    for lens in ([0], [2100], [0, 70]):
+        lens = np.array(lens)
+        rng, cache, table, q = make("int8", H, G, 64, 16, lens, [H, G])
+        for fill in (0, 0xff):
+            got = run(cache, table, lens, q, kv_len=max(SHARES, lens.max()), fill=fill)
+            check(cache, table, lens, q, got)
+            assert not got[lens == 0].any()
+
+
 def test_two_streams_with_workspaces_of_their_own(gpu):
     lens = np.random.default_rng(3).integers(1, 3000, 30)
     rng, cache, table, q = make("int8", 4, 4, 128, 32, lens, 5)
