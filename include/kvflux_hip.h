@@ -541,9 +541,11 @@ int kvflux_quant_gather(const void* key_cache, const void* value_cache, const fl
  * E4M3 byte that is NaN makes the rows that see it NaN. Scales of any size and
  * origin. Results are the same bits from call to call; a row's may differ between
  * batches.
- * head_size 64, 128 and 256, pages of any size, any group of query heads (16 to a
- * launch's item); other head sizes up to 512, and caches that are not aligned to 16
- * bytes, take a generic kernel (a lane a token, tens of times slower).
+ * head_size of any multiple of 16 up to 256 (64, 128 and 256 are the kernels' own
+ * sizes; others take the next one's arithmetic and their own bytes), pages of any
+ * size, any group of query heads (up to 16 work on one reading of the keys); other
+ * head sizes up to 512, and caches that are not aligned to 16 bytes, take a generic
+ * kernel (a lane a token, tens of times slower).
  * workspace: kvflux_quant_attention_workspace_size bytes, aligned to 8 (no
  * initialisation needed; calls that share one must be ordered); NULL where that is 0
  * (short rows). What one call needs is enough for calls of fewer rows and smaller

@@ -123,6 +123,13 @@ __device__ inline float quant_scale(std::uint32_t largest) {
     return __uint_as_float(largest >= 0x7f800000u ? 0x7fc00000u : static_cast<std::uint32_t>(k + 127) << 23);
 }
 
+// Head size of the attention kernels that a head size runs on, the least that holds it; 0:
+// the generic kernel's.
+inline std::uint64_t padded_head_size(std::uint64_t head_size) {
+    if (head_size % 16 != 0 || head_size > 256) return 0;
+    return head_size <= 64 ? 64 : head_size <= 128 ? 128 : 256;
+}
+
 // Workgroups of a launch: HIP counts the threads of a grid, 256 a workgroup here, in 32 bits.
 constexpr std::uint64_t kMostWorkgroups = 0xffffffffULL / 256;
 

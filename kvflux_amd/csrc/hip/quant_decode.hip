@@ -71,6 +71,7 @@ struct QuantDecodeParams {
     const float* value_scales;
     std::uint64_t num_blocks;
     std::uint32_t heads;          // kv heads
+    std::uint32_t head_size;      // a multiple of 16, at most kD
     FastDiv block_size;
     const std::uint64_t* table;   // [rows][width]
     std::uint64_t width;
@@ -82,11 +83,11 @@ struct QuantDecodeParams {
     std::uint32_t sets, set_heads;  // streams of a (row, kv head), query heads of each but the last
     const float* query;
     float* output;
-    float scale_log2;             // log2(e) / sqrt(D)
+    float scale_log2;             // log2(e) / sqrt(head_size)
     // Workspace: the streams that are cut, and two partials of every workgroup.
     std::uint32_t by_stream;      // a cut for every stream, else for every workgroup
     uint2* cuts;                  // [grid] {stream, or the workgroup that begins it; the last workgroup}, {~0, .}: none
-    float* part_acc;              // [2 * grid][set_heads][D]
+    float* part_acc;              // [2 * grid][set_heads][kD]
     float* part_ml;               // [2 * grid][set_heads][2]
 };
 
@@ -144,7 +145,7 @@ __global__ __launch_bounds__(64 * kW, Shape<kD>::kResident) void quant_decode_ke
     };
     const std::uint32_t wave = uniform(tid / 64);
     const int col = lane % 16, quad = lane / 16;
-    const std::uint32_t bs = p.block_size.divisor;
+    const std::uint32_t bs = p.block_size.divisor, D = p.head_size;
     const auto length = [&](std::uint32_t row) {
         const std::uint64_t n = p.lens[p.row_base + row];
         return n < p.kv_len ? static_cast<std::uint32_t>(n) : p.kv_len;
@@ -191,7 +192,7 @@ __global__ __launch_bounds__(64 * kW, Shape<kD>::kResident) void quant_decode_ke
                 std::uint64_t at = 0;
                 if (id != ~0ull) {
                     const std::uint32_t count = len - token < kSub ? len - token : kSub;
-                    at = ((id * p.heads + kvh) * bs + p.block_size.mod(token)) * kD | static_cast<std::uint64_t>(count) << kCountShift;
+                    at = ((id * p.heads + kvh) * bs + p.block_size.mod(token)) * D | static_cast<std::uint64_t>(count) << kCountShift;
                 }
                 places[wave][batch & 1][lane] = at;
                 __builtin_amdgcn_wave_barrier();  // a wavefront's LDS accesses are in order
@@ -211,7 +212,10 @@ __global__ __launch_bounds__(64 * kW, Shape<kD>::kResident) void quant_decode_ke
             // Load i of a tile: kRowsOf whole rows, 16 bytes a lane; every 128-byte line is
             // read by one instruction, so both caches are streamed past the others. Every
             // load is unconditional: places past the last tile lead to the pool's first rows.
+            // A lane past the head's end reads its first chunk: what is made of it meets queries
+            // of 0, or is an output that is not stored.
             const std::uint32_t my_row = static_cast<std::uint32_t>(lane) / kCpr, my_chunk = static_cast<std::uint32_t>(lane) % kCpr;
+            const std::uint32_t my_byte = my_chunk * 16 < D ? my_chunk * 16 : 0;
             const auto load = [&](std::uint32_t j, Tile& b) {
                 const std::uint64_t* const r = places[wave][j / kBatch & 1] + j % kBatch * kPerTile;
 #pragma unroll
@@ -220,10 +224,10 @@ __global__ __launch_bounds__(64 * kW, Shape<kD>::kResident) void quant_decode_ke
                     if constexpr (kSub == 8 && kRowsOf <= 8) {  // one place for all lanes
                         const std::uint64_t x = r[i * kRowsOf / 8];
                         const std::uint32_t lo = uniform(static_cast<std::uint32_t>(x)), hi = uniform(static_cast<std::uint32_t>(x >> 32));
-                        at = ((static_cast<std::uint64_t>(hi) << 32 | lo) & kOffsetMask) + i * kRowsOf % 8 * kD + (my_row * kD + my_chunk * 16);
+                        at = ((static_cast<std::uint64_t>(hi) << 32 | lo) & kOffsetMask) + i * kRowsOf % 8 * D + (my_row * D + my_byte);
                     } else {
                         const std::uint32_t token = i * kRowsOf + my_row;
-                        at = (r[token / kSub] & kOffsetMask) + token % kSub * kD + my_chunk * 16;
+                        at = (r[token / kSub] & kOffsetMask) + token % kSub * D + my_byte;
                     }
                     b.k[i] = __builtin_bit_cast(uint4, stream_load(reinterpret_cast<const V16*>(p.key_cache + at)));
                     b.v[i] = __builtin_bit_cast(uint4, stream_load(reinterpret_cast<const V16*>(p.value_cache + at)));
@@ -243,13 +247,16 @@ __global__ __launch_bounds__(64 * kW, Shape<kD>::kResident) void quant_decode_ke
             Tile b0, b1;
             {
                 const std::uint32_t head = kvh * p.group + first_head + (static_cast<std::uint32_t>(col) < heads ? col : heads - 1);
-                const float* const src = p.query + ((static_cast<std::uint64_t>(p.row_base) + row) * p.query_heads + head) * kD + 16 * quad;
+                const float* const src = p.query + ((static_cast<std::uint64_t>(p.row_base) + row) * p.query_heads + head) * D;
                 Float4 raw[kSteps][2];
 #pragma unroll
                 for (int kk = 0; kk < kSteps; ++kk)
 #pragma unroll
-                    for (int i = 0; i < 2; ++i)
-                        raw[kk][i] = *reinterpret_cast<const Float4*>(src + 64 * (kk / 2) + 8 * (kk % 2) + 4 * i);
+                    for (int i = 0; i < 2; ++i) {
+                        const std::uint32_t d = 64 * (kk / 2) + 16 * quad + 8 * (kk % 2) + 4 * i;
+                        raw[kk][i] = *reinterpret_cast<const Float4*>(src + (d < D ? d : 0));
+                        if (d >= D) raw[kk][i] = Float4{0.0f, 0.0f, 0.0f, 0.0f};
+                    }
                 load(0, b0);
                 load(1, b1);
                 float largest = 0.0f;
@@ -452,7 +459,7 @@ __global__ __launch_bounds__(64 * kW, Shape<kD>::kResident) void quant_decode_ke
                 o += reinterpret_cast<const float*>(wave_lds[w])[h * S::kPad + d] * f;
             }
             if (ml == nullptr) {
-                to[i] = sum == 0.0f ? 0.0f : o / sum;
+                if (d < D) to[h * D + d] = sum == 0.0f ? 0.0f : o / sum;
             } else {
                 to[i] = o;
                 if (d == 0) {
@@ -464,7 +471,7 @@ __global__ __launch_bounds__(64 * kW, Shape<kD>::kResident) void quant_decode_ke
         __syncthreads();  // the buffers and stats are used again
     };
     const auto output_of = [&](std::uint32_t row, std::uint32_t kvh, std::uint32_t set) {
-        return p.output + ((static_cast<std::uint64_t>(p.row_base) + row) * p.query_heads + kvh * p.group + set * p.set_heads) * kD;
+        return p.output + ((static_cast<std::uint64_t>(p.row_base) + row) * p.query_heads + kvh * p.group + set * p.set_heads) * D;
     };
 
     if constexpr (kWhole) {
@@ -514,8 +521,8 @@ __global__ __launch_bounds__(64 * kW, Shape<kD>::kResident) void quant_decode_ke
             if (lens_of[r] != 0) continue;
             if (p.by_stream)
                 for (std::uint32_t i = tid; i < streams; i += kT) p.cuts[r * streams + i] = make_uint2(~0u, 0);
-            float* const out = p.output + (static_cast<std::uint64_t>(p.row_base) + r) * p.query_heads * kD;
-            for (std::uint32_t i = tid; i < p.query_heads * kD; i += kT) out[i] = 0.0f;
+            float* const out = p.output + (static_cast<std::uint64_t>(p.row_base) + r) * p.query_heads * D;
+            for (std::uint32_t i = tid; i < p.query_heads * D; i += kT) out[i] = 0.0f;
         }
         if (tid == 0 && !p.by_stream) p.cuts[w] = make_uint2(~0u, 0);
         if (w >= shares) return;
@@ -634,12 +641,13 @@ __global__ __launch_bounds__(kMergeThreads) void quant_decode_merge_kernel(Quant
         o.z += v.z * f;
         o.w += v.w * f;
     }
+    if (4 * d4 >= p.head_size) return;
     const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-    *reinterpret_cast<Float4*>(p.output + ((static_cast<std::uint64_t>(p.row_base) + row) * p.query_heads + kvh * p.group + head) * kD + 4 * d4) =
+    *reinterpret_cast<Float4*>(p.output + ((static_cast<std::uint64_t>(p.row_base) + row) * p.query_heads + kvh * p.group + head) * p.head_size + 4 * d4) =
         Float4{o.x * inv, o.y * inv, o.z * inv, o.w * inv};
 }
 
-// Any head_size up to 512, and caches at any byte: a workgroup for each (query row, query
+// Any other head_size up to 512, and caches at any byte: a workgroup for each (query row, query
 // head), a lane for each of 64 tokens of a wavefront's step, FP32 products and sums.
 constexpr std::uint32_t kGenericD = 512;
 template <typename F>
@@ -738,8 +746,6 @@ __global__ __launch_bounds__(kThreads) void quant_rows_kernel(QuantRows p, std::
 }
 
 // ---------------------------------------------------------------- dispatch
-bool fast_head_size(std::uint64_t head_size) { return head_size == 64 || head_size == 128 || head_size == 256; }
-
 // Streams of a (row, kv head), and query heads of each.
 void head_sets(std::uint64_t group, std::uint32_t* sets, std::uint32_t* heads) {
     *sets = static_cast<std::uint32_t>((group + kCols - 1) / kCols);
@@ -845,7 +851,8 @@ extern "C" int kvflux_quant_attention_workspace_size(uint64_t num_rows, uint64_t
     *bytes = 0;
     if (const int s = check_shape("quant attention workspace", num_rows, kv_len, num_kv_heads, query_heads, block_size, head_size))
         return s;
-    if (num_rows == 0 || !fast_head_size(head_size)) return KVFLUX_OK;
+    head_size = padded_head_size(head_size);
+    if (num_rows == 0 || head_size == 0) return KVFLUX_OK;
     std::uint32_t sets, set_heads;
     head_sets(query_heads / num_kv_heads, &sets, &set_heads);
     const std::uint64_t streams = num_kv_heads * sets;
@@ -878,7 +885,8 @@ extern "C" int kvflux_quant_attention(const void* key_cache, const void* value_c
     if (!aligned(4, {query, output}) || !aligned(8, {block_table, seq_lens}))
         return fail(KVFLUX_ERR_INVALID_ARGUMENT, "quant attention: misaligned array");
     const float scale_log2 = static_cast<float>(1.4426950408889634 / std::sqrt(static_cast<double>(head_size)));
-    if (!fast_head_size(head_size) || !aligned(16, {key_cache, value_cache})) {
+    const std::uint64_t padded = padded_head_size(head_size);
+    if (padded == 0 || !aligned(16, {key_cache, value_cache})) {
         QuantRows rows{};
         rows.key_cache = static_cast<const std::uint8_t*>(key_cache);
         rows.value_cache = static_cast<const std::uint8_t*>(value_cache);
@@ -906,6 +914,7 @@ extern "C" int kvflux_quant_attention(const void* key_cache, const void* value_c
     p.value_scales = value_scales;
     p.num_blocks = num_blocks;
     p.heads = static_cast<std::uint32_t>(num_kv_heads);
+    p.head_size = static_cast<std::uint32_t>(head_size);
     p.block_size = FastDiv(static_cast<std::uint32_t>(block_size));
     p.table = block_table;
     p.width = max_blocks_per_seq;
@@ -919,21 +928,21 @@ extern "C" int kvflux_quant_attention(const void* key_cache, const void* value_c
     p.scale_log2 = scale_log2;
     const std::uint64_t streams = num_kv_heads * p.sets;
     const std::uint64_t slice = decode_slice(num_rows, streams);
-    const std::uint32_t grid = decode_grid(slice, kv_len, streams, block_size, head_size);
+    const std::uint32_t grid = decode_grid(slice, kv_len, streams, block_size, padded);
     if (grid != 0) {
-        if (!workspace || workspace_bytes < decode_workspace(grid, p.set_heads, head_size))
+        if (!workspace || workspace_bytes < decode_workspace(grid, p.set_heads, padded))
             return fail(KVFLUX_ERR_INVALID_ARGUMENT, "quant attention: workspace too small");
         if (!aligned(8, {workspace})) return fail(KVFLUX_ERR_INVALID_ARGUMENT, "quant attention: misaligned workspace");
         p.cuts = static_cast<uint2*>(workspace);
         p.part_acc = reinterpret_cast<float*>(p.cuts + grid);
-        p.part_ml = p.part_acc + 2ull * grid * p.set_heads * head_size;
+        p.part_ml = p.part_acc + 2ull * grid * p.set_heads * padded;
     }
     for (std::uint64_t base = 0; base < num_rows; base += slice) {
         p.row_base = static_cast<std::uint32_t>(base);
         p.rows = static_cast<std::uint32_t>(num_rows - base < slice ? num_rows - base : slice);
         const int s = format == KVFLUX_QUANT_E4M3
-                          ? launch_decode_format<QuantE4m3>(p, head_size, grid, as_stream(stream))
-                          : launch_decode_format<QuantInt8>(p, head_size, grid, as_stream(stream));
+                          ? launch_decode_format<QuantE4m3>(p, padded, grid, as_stream(stream))
+                          : launch_decode_format<QuantInt8>(p, padded, grid, as_stream(stream));
         if (s != KVFLUX_OK) return s;
     }
     return KVFLUX_OK;

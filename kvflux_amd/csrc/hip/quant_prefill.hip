@@ -71,7 +71,7 @@ struct QuantPrefillParams {
     const float* key_scales;
     const float* value_scales;
     std::uint64_t num_blocks;
-    std::uint32_t heads;
+    std::uint32_t heads, head_size;    // a multiple of 16, at most kD
     FastDiv block_size;
     const std::uint64_t* table;
     std::uint64_t width;
@@ -89,7 +89,7 @@ struct QuantPrefillParams {
     const float* query;
     float* output;
     float scale_log2;
-    float* part_acc;  // [splits][num_seqs * max_query][query_heads][D]
+    float* part_acc;  // [splits][num_seqs * max_query][query_heads][kD]
     float* part_ml;   // [splits][num_seqs * max_query][query_heads][2]
 };
 
@@ -119,7 +119,7 @@ __global__ __launch_bounds__((Shape<kD, kOrder, kUniform>::kThreads), (Shape<kD,
     constexpr int kBytes = static_cast<int>(kTile) * kD / kLoaders;
     constexpr int kKeyThreads = kD / kBytes;   // threads of a key
     constexpr int kWords = kBytes / 4;
-    static_assert(kBytes >= 8 && kD % kBytes == 0, "tile split");
+    static_assert(kBytes % 16 == 0 && kD % kBytes == 0, "tile split");
     // [set][buffer][K, V]; at the end of two sets the second one's sums.
     constexpr int kPad = kD + 4;
     __shared__ __attribute__((aligned(16))) unsigned char tiles_lds[kSets][2][2][kTileBytes];
@@ -168,13 +168,18 @@ __global__ __launch_bounds__((Shape<kD, kOrder, kUniform>::kThreads), (Shape<kD,
     const bool row_live = r < p.tokens * p.heads_of && token < t_end;
     const bool wave_live = __builtin_amdgcn_ballot_w64(row_live) != 0;
     const std::uint64_t q_row = (p.query_offsets[seq] + (row_live ? token : t0)) * p.query_heads + kvh * p.group + (row_live ? head : p.first);
-    const float* const q_src = p.query + q_row * kD + 8 * half;
+    const std::uint32_t D = p.head_size;
+    const float* const q_src = p.query + q_row * D;
     struct Float4 { float x, y, z, w; };  // float-aligned
     Float4 raw[kSteps][2];
 #pragma unroll
     for (int kk = 0; kk < kSteps; ++kk)
 #pragma unroll
-        for (int i = 0; i < 2; ++i) raw[kk][i] = *reinterpret_cast<const Float4*>(q_src + 16 * kk + 4 * i);
+        for (int i = 0; i < 2; ++i) {
+            const std::uint32_t d = 16 * kk + 8 * half + 4 * i;
+            raw[kk][i] = *reinterpret_cast<const Float4*>(q_src + (d < D ? d : 0));
+            if (d >= D) raw[kk][i] = Float4{0.0f, 0.0f, 0.0f, 0.0f};
+        }
 
     // ---- the window's pages: ids, scales, the largest |vs| so far (the weights' reference).
     std::uint32_t window = tile_begin / p.window_tiles;  // tiles [window * window_tiles, + window_tiles)
@@ -232,7 +237,7 @@ __global__ __launch_bounds__((Shape<kD, kOrder, kUniform>::kThreads), (Shape<kD,
     // ---- loads: a thread's kBytes of K and of V of one key of a tile, at the same place.
     const std::uint32_t loader = static_cast<std::uint32_t>(tid) % kLoaders;
     const std::uint32_t my_row = loader / kKeyThreads, my_col = loader % kKeyThreads * kBytes;
-    const std::uint64_t head_bytes = static_cast<std::uint64_t>(p.block_size.divisor) * kD;
+    const std::uint64_t head_bytes = static_cast<std::uint64_t>(p.block_size.divisor) * D;
     std::uint32_t held[2][kWords];
     bool held_live = false;  // V's
     const auto fetch_one = [&](int which, std::uint32_t tile) {
@@ -240,10 +245,16 @@ __global__ __launch_bounds__((Shape<kD, kOrder, kUniform>::kThreads), (Shape<kD,
         const std::uint32_t id = page_id[page - window_page];
         if (which) held_live = !(id & kUnread) && key < kv_len;
         // In place of a page that is not read: the pool's first row.
-        const std::uint64_t at = (id & kUnread ? 0 : (static_cast<std::uint64_t>(id) * p.heads + kvh) * head_bytes +
-                                                         (key - page * p.block_size.divisor) * kD) + my_col;
-        constexpr int kAlign = kBytes < 16 ? kBytes : 16;
-        __builtin_memcpy(held[which], __builtin_assume_aligned((which ? p.value_cache : p.key_cache) + at, kAlign), kBytes);
+        const std::uint64_t at = id & kUnread ? 0 : (static_cast<std::uint64_t>(id) * p.heads + kvh) * head_bytes +
+                                                        (key - page * p.block_size.divisor) * D;
+        const std::uint8_t* const row = (which ? p.value_cache : p.key_cache) + at;
+#pragma unroll
+        for (int i = 0; i < kBytes / 16; ++i) {
+            // Past the head's end its first bytes: they meet queries of 0, or make outputs that
+            // are not stored.
+            const std::uint32_t c = my_col + 16 * i;
+            __builtin_memcpy(held[which] + 4 * i, __builtin_assume_aligned(row + (c < D ? c : 0), 16), 16);
+        }
     };
     // Swizzled slots of a row's 16-byte chunks (LDS repeats its banks every 128 bytes). K is
     // read 16 rows of one chunk at a time, V 4 rows of 32 bytes.
@@ -644,15 +655,17 @@ __global__ __launch_bounds__((Shape<kD, kOrder, kUniform>::kThreads), (Shape<kD,
     const bool whole = mine.count == 1;
     const std::uint32_t head_at = kvh * p.group + head;
     const std::uint64_t part_row = ((static_cast<std::uint64_t>(split) * p.num_seqs + seq) * p.max_query + token) * p.query_heads + head_at;
-    float* const to = whole ? p.output + ((p.query_offsets[seq] + token) * p.query_heads + head_at) * kD : p.part_acc + part_row * kD;
+    float* const to = whole ? p.output + ((p.query_offsets[seq] + token) * p.query_heads + head_at) * D : p.part_acc + part_row * kD;
     const float inv = whole && sum != 0.0f ? 1.0f / sum : 1.0f;
 #pragma unroll
     for (int db = 0; db < kDb; ++db)
 #pragma unroll
-        for (int g = 0; g < 4; ++g)
+        for (int g = 0; g < 4; ++g) {
+            if (32 * db + 8 * g >= static_cast<int>(D)) break;  // uniform; parts: not read
             *reinterpret_cast<Float4*>(to + 32 * db + 8 * g + 4 * half) =
                 Float4{acc[db][4 * g] * inv * in_ones, acc[db][4 * g + 1] * inv * in_ones, acc[db][4 * g + 2] * inv * in_ones,
                        acc[db][4 * g + 3] * inv * in_ones};
+        }
     if (!whole && half == 0) {
         p.part_ml[2 * part_row] = ref;
         p.part_ml[2 * part_row + 1] = sum;
@@ -678,6 +691,7 @@ __global__ __launch_bounds__(256) void quant_prefill_merge_kernel(QuantPrefillPa
     const std::uint32_t splits = split_of(last / kTile + 1, p.split_tiles).count;
     if (splits == 1) return;
     const std::uint32_t d4 = threadIdx.x % kLanes;
+    if (4 * d4 >= p.head_size) return;
     const std::uint64_t stride = static_cast<std::uint64_t>(p.num_seqs) * p.max_query * p.query_heads;
     const std::uint64_t at = static_cast<std::uint64_t>(seq) * p.max_query * p.query_heads + i;
     float top = -INFINITY, sum = 0.0f;
@@ -705,7 +719,7 @@ __global__ __launch_bounds__(256) void quant_prefill_merge_kernel(QuantPrefillPa
         }
     }
     const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-    *reinterpret_cast<Float4*>(p.output + (p.query_offsets[seq] * p.query_heads + i) * kD + 4 * d4) =
+    *reinterpret_cast<Float4*>(p.output + (p.query_offsets[seq] * p.query_heads + i) * p.head_size + 4 * d4) =
         Float4{o.x * inv, o.y * inv, o.z * inv, o.w * inv};
 }
 
@@ -801,8 +815,6 @@ int launch_prefill_head_size(QuantPrefillParams& p, std::uint64_t head_size, Ord
     }
 }
 
-bool fast_head_size(std::uint64_t head_size) { return head_size == 64 || head_size == 128 || head_size == 256; }
-
 int check_prefill(const char* op, std::uint64_t num_seqs, std::uint64_t max_query, std::uint64_t max_kv,
                   std::uint64_t heads, std::uint64_t query_heads, std::uint64_t block_size, std::uint64_t head_size) {
     if (heads == 0 || block_size == 0 || head_size == 0 || query_heads == 0 || query_heads % heads != 0)
@@ -828,7 +840,8 @@ extern "C" int kvflux_quant_prefill_workspace_size(uint64_t num_seqs, uint64_t m
     if (const int s = check_prefill("quant prefill workspace", num_seqs, max_query_tokens, max_kv_len, num_kv_heads,
                                     query_heads, block_size, head_size))
         return s;
-    if (num_seqs == 0 || max_query_tokens == 0 || !fast_head_size(head_size)) return KVFLUX_OK;
+    head_size = padded_head_size(head_size);
+    if (num_seqs == 0 || max_query_tokens == 0 || head_size == 0) return KVFLUX_OK;
     const PrefillPlan plan = prefill_plan(num_seqs, max_query_tokens, max_kv_len, num_kv_heads, query_heads / num_kv_heads, head_size);
     *bytes = prefill_workspace(plan, num_seqs, max_query_tokens, query_heads, head_size);
     return KVFLUX_OK;
@@ -855,7 +868,8 @@ extern "C" int kvflux_quant_prefill(const void* key_cache, const void* value_cac
         return fail(KVFLUX_ERR_INVALID_ARGUMENT, "quant prefill: misaligned array");
     const std::uint64_t group = query_heads / num_kv_heads;
     const float scale_log2 = static_cast<float>(1.4426950408889634 / std::sqrt(static_cast<double>(head_size)));
-    if (!fast_head_size(head_size) || !aligned(16, {key_cache, value_cache})) {
+    const std::uint64_t padded = padded_head_size(head_size);
+    if (padded == 0 || !aligned(16, {key_cache, value_cache})) {
         QuantRows rows{};
         rows.key_cache = static_cast<const std::uint8_t*>(key_cache);
         rows.value_cache = static_cast<const std::uint8_t*>(value_cache);
@@ -879,13 +893,14 @@ extern "C" int kvflux_quant_prefill(const void* key_cache, const void* value_cac
         rows.scale_log2 = scale_log2;
         return launch_quant_rows(rows, num_seqs * max_query_tokens, format, as_stream(stream));
     }
-    const PrefillPlan plan = prefill_plan(num_seqs, max_query_tokens, max_kv_len, num_kv_heads, group, head_size);
+    const PrefillPlan plan = prefill_plan(num_seqs, max_query_tokens, max_kv_len, num_kv_heads, group, padded);
     QuantPrefillParams p{};
     p.key_cache = static_cast<const std::uint8_t*>(key_cache);
     p.value_cache = static_cast<const std::uint8_t*>(value_cache);
     p.key_scales = key_scales;
     p.value_scales = value_scales;
     p.num_blocks = num_blocks;
+    p.head_size = static_cast<std::uint32_t>(head_size);
     p.heads = static_cast<std::uint32_t>(num_kv_heads);
     p.block_size = FastDiv(static_cast<std::uint32_t>(block_size));
     p.table = block_table;
@@ -913,12 +928,12 @@ extern "C" int kvflux_quant_prefill(const void* key_cache, const void* value_cac
     if (static_cast<std::uint64_t>(p.heads) * p.splits * p.num_seqs * p.blocks > kMostWorkgroups / 2)
         return fail(KVFLUX_ERR_UNSUPPORTED, "quant prefill: shape too large");
     if (plan.splits > 1) {
-        if (!workspace || workspace_bytes < prefill_workspace(plan, num_seqs, max_query_tokens, query_heads, head_size))
+        if (!workspace || workspace_bytes < prefill_workspace(plan, num_seqs, max_query_tokens, query_heads, padded))
             return fail(KVFLUX_ERR_INVALID_ARGUMENT, "quant prefill: workspace too small");
         if (!aligned(4, {workspace})) return fail(KVFLUX_ERR_INVALID_ARGUMENT, "quant prefill: misaligned workspace");
         p.part_acc = static_cast<float*>(workspace);
-        p.part_ml = p.part_acc + static_cast<std::uint64_t>(plan.splits) * num_seqs * max_query_tokens * query_heads * head_size;
+        p.part_ml = p.part_acc + static_cast<std::uint64_t>(plan.splits) * num_seqs * max_query_tokens * query_heads * padded;
     }
-    return format == KVFLUX_QUANT_E4M3 ? launch_prefill_head_size<QuantE4m3>(p, head_size, plan.order, as_stream(stream))
-                                       : launch_prefill_head_size<QuantInt8>(p, head_size, plan.order, as_stream(stream));
+    return format == KVFLUX_QUANT_E4M3 ? launch_prefill_head_size<QuantE4m3>(p, padded, plan.order, as_stream(stream))
+                                       : launch_prefill_head_size<QuantInt8>(p, padded, plan.order, as_stream(stream));
 }

@@ -105,6 +105,16 @@ def test_lengths_and_pages(gpu, fmt, D, bs):
 
 
 @pytest.mark.parametrize("fmt", ["e4m3", "int8"])
+@pytest.mark.parametrize("D", [16, 32, 48, 80, 96, 112, 144, 192, 240])
+@pytest.mark.parametrize("bs", [16, 5])
+def test_head_sizes_that_fill_part_of_a_kernel(gpu, fmt, D, bs):
+    lens = np.array([0, 1, 33, 300, 512])
+    rng, cache, table, q = make(fmt, 3, 5, D, bs, lens, [D, bs], spare=0)
+    for bound in (None, 1000, SHARES):
+        check(cache, table, lens, q, run(cache, table, lens, q, kv_len=bound))
+
+
+@pytest.mark.parametrize("fmt", ["e4m3", "int8"])
 @pytest.mark.parametrize("H,G", [(8, 4), (4, 7), (1, 12), (8, 1), (2, 16), (1, 17), (2, 33), (3, 5), (1, 71)])
 def test_groups(gpu, fmt, H, G):
     lens = np.array([700, 1, 45, 0, 1300])
@@ -148,7 +158,7 @@ def test_missing_pages_drop_out(gpu, fmt, bs):
     check(cache, short, np.minimum(lens, 2 * bs), q, run(cache, short, lens, q))
 
 
-@pytest.mark.parametrize("bs,D", [(16, 128), (64, 64), (5, 128), (16, 256), (16, 96)])
+@pytest.mark.parametrize("bs,D", [(16, 128), (64, 64), (5, 128), (16, 256), (16, 96), (16, 100)])
 def test_what_lies_behind_a_row_is_not_seen(gpu, bs, D):
     """NaN bytes and scales behind a row's end, in its last page and in pages it does not use."""
     lens = np.array([1, 37, 70, 530])
@@ -163,7 +173,7 @@ def test_what_lies_behind_a_row_is_not_seen(gpu, bs, D):
     check_both(cache, table, lens, q)
 
 
-@pytest.mark.parametrize("D", [128, 96])
+@pytest.mark.parametrize("D", [128, 96, 100])
 def test_a_scale_or_byte_that_is_nan_is_seen(gpu, D):
     lens = np.array([40, 600, 33])
     rng, cache, table, q = make("e4m3", 2, 2, D, 16, lens, 1)
@@ -248,7 +258,7 @@ def test_the_same_bits_again(gpu):
         assert np.array_equal(d.result(), first)
 
 
-@pytest.mark.parametrize("D,shift", [(80, 0), (96, 0), (512, 0), (20, 0), (128, 1), (64, 8)])
+@pytest.mark.parametrize("D,shift", [(84, 0), (100, 0), (512, 0), (20, 0), (128, 1), (64, 8)])
 def test_generic_head_sizes_and_alignments(gpu, D, shift):
     rng = np.random.default_rng(D)
     lens = np.array([0, 1, 63, 64, 65, 400, 700])

@@ -60,7 +60,7 @@ def everything(pool, fmt, D, table, rows, q, bound):
 
 
 @pytest.mark.parametrize("fmt", ["e4m3", "int8"])
-@pytest.mark.parametrize("D,shift,bound", [(128, 0, 700), (128, 0, 5000), (64, 0, 2049), (96, 0, 700), (128, 4, 700)])
+@pytest.mark.parametrize("D,shift,bound", [(128, 0, 700), (128, 0, 5000), (64, 0, 2049), (96, 0, 700), (100, 0, 700), (128, 4, 700)])
 def test_pages_past_32_bits(gpu, fmt, D, shift, bound):
     rng = np.random.default_rng(D + shift)
     used = int((-(-LENS // BS)).sum())

@@ -92,6 +92,20 @@ def test_whole_prompts(gpu, fmt, D, bs):
 
 
 @pytest.mark.parametrize("fmt", ["e4m3", "int8"])
+@pytest.mark.parametrize("D", [16, 32, 48, 80, 96, 112, 144, 192, 240])
+@pytest.mark.parametrize("bs", [16, 5])
+def test_head_sizes_that_fill_part_of_a_kernel(gpu, fmt, D, bs):
+    lens, new = np.array([1, 0, 65, 130, 300]), np.array([1, 0, 65, 3, 290])
+    rng, cache, table, q = make(fmt, 2, 5, D, bs, lens, new, [D, bs], spare=0)
+    for most, bound in ((290, 300), (290, 3000), (290, 6000), (1000, 200000)):
+        call, got = run(cache, table, lens, new, q, most=most, kv_len=bound)
+        check(cache, table, call, got, some=10)
+    few = np.minimum(lens, 200)
+    call, got = run(cache, table, few, np.minimum(new, few), q[:int(np.minimum(new, few).sum())])
+    check(cache, table, call, got, some=10)
+
+
+@pytest.mark.parametrize("fmt", ["e4m3", "int8"])
 @pytest.mark.parametrize("D", [64, 128, 256])
 @pytest.mark.parametrize("bs,H,G", [(16, 2, 4), (8, 2, 4), (64, 1, 7), (1, 2, 1), (5, 1, 17), (48, 1, 300)])
 def test_bounds_past_the_lengths(gpu, fmt, D, bs, H, G):
@@ -294,7 +308,7 @@ def test_the_same_bits_again(gpu):
         assert np.array_equal(call.result(), first)
 
 
-@pytest.mark.parametrize("D,shift", [(80, 0), (96, 0), (512, 0), (20, 0), (128, 1), (64, 8)])
+@pytest.mark.parametrize("D,shift", [(84, 0), (100, 0), (512, 0), (20, 0), (128, 1), (64, 8)])
 def test_generic_head_sizes_and_alignments(gpu, D, shift):
     rng = np.random.default_rng(D)
     lens, new = np.array([0, 1, 63, 70, 200]), np.array([0, 1, 63, 3, 10])

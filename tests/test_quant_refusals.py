@@ -121,7 +121,8 @@ def test_workspace_sizes_of_attention():
     assert ask() == capi.OK and size.value > 0
     assert ask(kv_len=512) == capi.OK and size.value == 0
     assert ask(rows=0) == capi.OK and size.value == 0
-    assert ask(D=96) == capi.OK and size.value == 0
+    assert ask(D=96) == capi.OK and size.value > 0
+    assert ask(D=100) == capi.OK and size.value == 0 and ask(D=272) == capi.OK and size.value == 0
     assert ask(Hq=7) == capi.ERR_INVALID and ask(H=0) == capi.ERR_INVALID and ask(kv_len=1 << 32) == capi.ERR_UNSUPPORTED
     assert status("kvflux_quant_attention_workspace_size", 1, 1, 1, 1, 1, 64, None) == capi.ERR_INVALID
 
@@ -149,7 +150,8 @@ def test_shapes_of_prefill():
 
     assert ask() == capi.OK and size.value > 0
     assert ask(seqs=64, most=4096, kv_len=4096, H=8, Hq=32) == capi.OK and size.value == 0
-    assert ask(D=80) == capi.OK and size.value == 0
+    assert ask(D=80) == capi.OK and size.value > 0
+    assert ask(D=84) == capi.OK and size.value == 0
     assert ask(seqs=0) == capi.OK and size.value == 0
     assert ask(most=50001) == capi.ERR_INVALID and ask(Hq=3) == capi.ERR_INVALID and ask(kv_len=1 << 31) == capi.ERR_UNSUPPORTED
     assert status("kvflux_quant_prefill_workspace_size", 1, 1, 1, 1, 1, 1, 64, None) == capi.ERR_INVALID
