@@ -7,9 +7,9 @@
 // 16-bit cache is left for the same arithmetic. So
 //  * K and V are read past the caches, whole 128-byte lines by one instruction, two
 //    tiles ahead, and reach the matrix instructions through a wavefront's own LDS
-//    (no barrier). 128 rows of <= 32768 tokens, 8 kv heads of 128: 747 us, 6.3 TB/s;
-//    with loads in the operands' own layout, which split lines, 805 us. Loads alone
-//    take 705 us. The same loads without the streaming hint took 1611 us;
+//    (no barrier). 128 rows of <= 32768 tokens, 8 kv heads of 128: 730 us, 6.4 TB/s,
+//    where loads alone take 705. The step to it (805 to 747) was from loads in the
+//    operands' own layout, which split lines; without the streaming hint it took 1611 us;
 //  * bytes are widened in registers, one conversion for two values; both formats are
 //    exact in FP16;
 //  * the products are FP16 MFMAs with FP32 sums, on Q and the weights in two FP16

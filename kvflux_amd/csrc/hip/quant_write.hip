@@ -10,7 +10,9 @@
 // registers (their largest magnitude is needed before the first of them can be
 // rounded) and written once. A wavefront takes a unit of up to 2048 values (16
 // tokens of 128), so nothing waits at a barrier; a workgroup takes a larger one
-// (8192 in registers, what is behind them is read again from the L2).
+// (8192 in registers, what is behind them is read again from the L2). 4096 tokens of
+// BF16, 8 kv heads of 128 (25 MB): 6.6 us a call, 5.7 to 6.9 in the kernel (7.2 with
+// shuffles through LDS); one token each of 8 rows 3.4 in the kernel, 6.0 a call.
 #include "quant.h"
 
 #include <type_traits>
