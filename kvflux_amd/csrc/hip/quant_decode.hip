@@ -123,7 +123,8 @@ struct Shape {
 // kSub: tokens that share a record. 8 where pages are multiples of 8 tokens, so that
 // every 8 tokens of a tile lie in one; 1 for pages of any other size.
 // kWhole: a workgroup takes one whole stream (no shares, no partials).
-template <typename F, int kD, int kSub, bool kWhole, int kW>
+// kFull: head_size is kD (as a value of the launch it cost 4 rows of <= 1500 tokens 0.5 us of 12.4).
+template <typename F, int kD, int kSub, bool kWhole, int kW, bool kFull>
 __global__ __launch_bounds__(64 * kW, Shape<kD>::kResident) void quant_decode_kernel(QuantDecodeParams p) {
     using S = Shape<kD>;
     constexpr int kT = 64 * kW;
@@ -145,7 +146,7 @@ __global__ __launch_bounds__(64 * kW, Shape<kD>::kResident) void quant_decode_ke
     };
     const std::uint32_t wave = uniform(tid / 64);
     const int col = lane % 16, quad = lane / 16;
-    const std::uint32_t bs = p.block_size.divisor, D = p.head_size;
+    const std::uint32_t bs = p.block_size.divisor, D = kFull ? kD : p.head_size;
     const auto length = [&](std::uint32_t row) {
         const std::uint64_t n = p.lens[p.row_base + row];
         return n < p.kv_len ? static_cast<std::uint32_t>(n) : p.kv_len;
@@ -253,9 +254,9 @@ __global__ __launch_bounds__(64 * kW, Shape<kD>::kResident) void quant_decode_ke
                 for (int kk = 0; kk < kSteps; ++kk)
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
-                        const std::uint32_t d = 64 * (kk / 2) + 16 * quad + 8 * (kk % 2) + 4 * i;
-                        raw[kk][i] = *reinterpret_cast<const Float4*>(src + (d < D ? d : 0));
-                        if (d >= D) raw[kk][i] = Float4{0.0f, 0.0f, 0.0f, 0.0f};
+                        const std::uint32_t at = 64 * (kk / 2) + 8 * (kk % 2) + 4 * i;
+                        raw[kk][i] = Float4{0.0f, 0.0f, 0.0f, 0.0f};
+                        if (kFull || at + 16 * quad < D) raw[kk][i] = *reinterpret_cast<const Float4*>(src + 16 * quad + at);
                     }
                 load(0, b0);
                 load(1, b1);
@@ -515,7 +516,10 @@ __global__ __launch_bounds__(64 * kW, Shape<kD>::kResident) void quant_decode_ke
         const std::uint32_t shares = wanted == 0 ? 1 : wanted < gridDim.x ? static_cast<std::uint32_t>(wanted) : gridDim.x;
         const std::uint64_t each = total / shares;
         const std::uint32_t more = static_cast<std::uint32_t>(total - each * shares);  // the first shares have one more
-        const std::uint32_t w = blockIdx.x;
+        // Neighbouring shares, whose streams are often heads of one row, go to one XCD: the
+        // scales of a page's heads share lines in its L2 (128 rows of <= 32768 tokens: 730 us
+        // without, 724 with; but one row of 32768 24.9 and 25.7).
+        const std::uint32_t w = p.rows > 1 && gridDim.x % 8 == 0 ? blockIdx.x % 8 * (gridDim.x / 8) + blockIdx.x / 8 : blockIdx.x;
         // Rows without tokens: zeros.
         for (std::uint32_t r = w; r < p.rows; r += gridDim.x) {
             if (lens_of[r] != 0) continue;
@@ -771,7 +775,7 @@ std::size_t decode_workspace(std::uint32_t grid, std::uint32_t set_heads, std::u
     return 2ull * grid * set_heads * (head_size + 2) * sizeof(float) + grid * sizeof(uint2);
 }
 
-template <typename F, int kD, int kSub>
+template <typename F, int kD, int kSub, bool kFull>
 int launch_decode(QuantDecodeParams& p, std::uint32_t grid, hipStream_t stream) {
     const std::uint64_t streams = static_cast<std::uint64_t>(p.heads) * p.sets;
     if (grid == 0) {
@@ -779,20 +783,20 @@ int launch_decode(QuantDecodeParams& p, std::uint32_t grid, hipStream_t stream) 
         // Eight wavefronts where a CU has a stream at most (at 256 the registers are those of
         // four), and each more than a tile or two. 8 rows of <= 1000 tokens: 12.7 us with
         // four, 11.6 with eight; one of <= 300: 6.6 and 7.2.
-        if constexpr (kD <= 128) {
+        if constexpr (kD <= 128 && kFull) {
             if (p.rows * streams <= kFullStreams && p.kv_len > kOneLaunch / 2) {
-                quant_decode_kernel<F, kD, kSub, true, 2 * kWaves><<<workgroups, dim3(2 * kThreads), 0, stream>>>(p);
+                quant_decode_kernel<F, kD, kSub, true, 2 * kWaves, kFull><<<workgroups, dim3(2 * kThreads), 0, stream>>>(p);
                 return launch_status("quant_decode_kernel");
             }
         }
-        quant_decode_kernel<F, kD, kSub, true, kWaves><<<workgroups, dim3(kThreads), 0, stream>>>(p);
+        quant_decode_kernel<F, kD, kSub, true, kWaves, kFull><<<workgroups, dim3(kThreads), 0, stream>>>(p);
         return launch_status("quant_decode_kernel");
     }
     // The merge takes the shorter list: streams of a few rows, or the workgroups' cuts.
     // 16 rows of 2 kv heads with 16 query heads each: 40 us by workgroup, 19 by stream.
     const std::uint32_t cuts = p.rows * streams < grid ? static_cast<std::uint32_t>(p.rows * streams) : grid;
     p.by_stream = cuts < grid;
-    quant_decode_kernel<F, kD, kSub, false, kWaves><<<dim3(grid), dim3(kThreads), 0, stream>>>(p);
+    quant_decode_kernel<F, kD, kSub, false, kWaves, kFull><<<dim3(grid), dim3(kThreads), 0, stream>>>(p);
     if (const int s = launch_status("quant_decode_kernel")) return s;
     // Parts of a stream: many where there are few streams. With 1024 threads and with 128:
     // 64 parts 25.3 and 26.6 us (the whole call), 18 parts 16.2 and 13.2.
@@ -804,7 +808,9 @@ int launch_decode(QuantDecodeParams& p, std::uint32_t grid, hipStream_t stream) 
 }
 template <typename F, int kD>
 int launch_decode_pages(QuantDecodeParams& p, std::uint32_t grid, hipStream_t s) {
-    return p.block_size.divisor % 8 == 0 ? launch_decode<F, kD, 8>(p, grid, s) : launch_decode<F, kD, 1>(p, grid, s);
+    if (p.head_size == kD)
+        return p.block_size.divisor % 8 == 0 ? launch_decode<F, kD, 8, true>(p, grid, s) : launch_decode<F, kD, 1, true>(p, grid, s);
+    return p.block_size.divisor % 8 == 0 ? launch_decode<F, kD, 8, false>(p, grid, s) : launch_decode<F, kD, 1, false>(p, grid, s);
 }
 template <typename F>
 int launch_decode_format(QuantDecodeParams& p, std::uint64_t head_size, std::uint32_t grid, hipStream_t s) {
