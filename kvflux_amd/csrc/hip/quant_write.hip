@@ -11,7 +11,7 @@
 // rounded) and written once. A wavefront takes a unit of up to 2048 values (16
 // tokens of 128), so nothing waits at a barrier; a workgroup takes a larger one
 // (8192 in registers, what is behind them is read again from the L2). 4096 tokens of
-// BF16, 8 kv heads of 128 (25 MB): 6.6 us a call, 5.7 to 6.9 in the kernel (7.2 with
+// BF16, 8 kv heads of 128 (25 MB): 6.4 us a call, 5.7 to 6.9 in the kernel (7.2 with
 // shuffles through LDS); one token each of 8 rows 3.4 in the kernel, 6.0 a call.
 #include "quant.h"
 
@@ -92,8 +92,7 @@ __global__ __launch_bounds__(kThreads) void quant_write_kernel(WriteParams p) {
     const std::uint64_t page = (p.bs_shift >= 0 ? start >> p.bs_shift : start / p.block_size) + page_of_new;
     const std::uint64_t at = page * p.block_size;  // position of the page's first token
     if (at >= len || page >= p.width) return;
-    const std::uint64_t id = p.table[seq * p.width + page];
-    if (id >= p.num_blocks) return;
+    const std::uint64_t entry = p.table[seq * p.width + page];
     const std::uint32_t first = start > at ? static_cast<std::uint32_t>(start - at) : 0;
     const std::uint32_t last = len - at < p.block_size ? static_cast<std::uint32_t>(len - at) : p.block_size;
 
@@ -121,6 +120,10 @@ __global__ __launch_bounds__(kThreads) void quant_write_kernel(WriteParams p) {
         const std::uint32_t c = begin + tid + i * kT;
         held[i] = *input(c < end ? c : end - 1);
     }
+    // The input needs no page: it is on its way while the table is read. (A page that is
+    // not there: the first one's scale, and no store.)
+    const bool there = entry < p.num_blocks;
+    const std::uint64_t id = there ? entry : 0;
     float* const scale_at = p.scales[kv] + (id * p.heads.divisor + head);
     const float before = *scale_at;
 #pragma unroll
@@ -133,6 +136,7 @@ __global__ __launch_bounds__(kThreads) void quant_write_kernel(WriteParams p) {
 #pragma unroll
         for (int w = 0; w < kWaves; ++w) largest = largest_of[w] > largest ? largest_of[w] : largest;
     }
+    if (!there) return;  // uniform in the unit
     float scale = quant_scale<F>(largest);
     if (first != 0 && !(scale >= before)) scale = before != before || scale == scale ? before : scale;
     const float inverse = 1.0f / scale;
