@@ -46,6 +46,8 @@ constexpr std::uint32_t kTile = 64;     // keys of a tile
 constexpr std::uint32_t kWindow = 1024; // pages whose ids and scales are in LDS at a time
 constexpr std::uint32_t kUnread = 0x80000000u;  // a page whose bytes are not read, in place of its id
 constexpr std::uint32_t kMissing = ~0u;         // one that is not there
+constexpr std::uint32_t kBand = 16;       // powers of two of |vs| worked on at once, see `bands`
+constexpr std::uint32_t kMostBands = 8;   // behind them FP32 ends
 constexpr float kWeightScale = 32768.0f;  // as in the decode: parts of 2^15 times a weight of at most 1
 
 // How a workgroup's wavefronts share its work: four of 32 rows each; eight that take turns;
@@ -130,7 +132,7 @@ __global__ __launch_bounds__((Shape<kD, kOrder, kUniform>::kThreads), (Shape<kD,
     // Where the scales differ within 16 keys: those of a buffer's keys.
     __shared__ __attribute__((aligned(16))) float key_ks[kSets][kUniform ? 1 : 2][kUniform ? 4 : kTile];
     __shared__ __attribute__((aligned(16))) float key_vs[kSets][kUniform ? 1 : 2][kUniform ? 4 : kTile];
-    __shared__ float wave_top[kWaves];
+    __shared__ float wave_top[kWaves], wave_least[kWaves];
     __shared__ std::uint32_t wave_missing[kWaves];
 
     const int tid = threadIdx.x, lane = tid % 64;
@@ -186,13 +188,19 @@ __global__ __launch_bounds__((Shape<kD, kOrder, kUniform>::kThreads), (Shape<kD,
     std::uint32_t window_page = 0;                       // page of page_id[0]
     float reference = 0.0f;
     bool missing = false;                                // a page of the window is
-    const auto stage = [&] {
+    // A query need not see the window's largest |vs|: a weight's parts, relative to that, would
+    // lose bits of what it sees (2^15 times a weight over 2^16 is 2^-1, and FP16 ends at
+    // 2^-24). So pages whose |vs| is under 2^-16 of the largest are worked on in a pass of
+    // their own, and so on: nearly always there is one.
+    std::uint32_t bands = 1;
+    float band_down = 1.0f, counted = 1.0f;  // of the pass: what its sums are scaled by; 1 in the first
+    const auto stage = [&](std::uint32_t band) {
         const std::uint32_t from = window * p.window_tiles;  // its part of this workgroup's tiles
         const std::uint32_t tile0 = from > tile_begin ? from : tile_begin;
         const std::uint32_t tile1 = from + p.window_tiles < tile_end ? from + p.window_tiles : tile_end;
         window_page = p.block_size.div(tile0 * kTile);
         const std::uint32_t pages = p.block_size.div(tile1 * kTile - 1) - window_page + 1;
-        float top = 0.0f;
+        float top = 0.0f, least = INFINITY;
         bool lost = false;
         for (std::uint32_t i = tid; i < pages; i += kThreads) {
             const std::uint64_t page = window_page + i;
@@ -204,33 +212,50 @@ __global__ __launch_bounds__((Shape<kD, kOrder, kUniform>::kThreads), (Shape<kD,
             page_id[i] = live ? static_cast<std::uint32_t>(id) : kMissing;
             // What sees these values is NaN by its score. What does not is left alone: their
             // bytes may be NaN as well, and a weight of 0 times that is.
-            if (vs != vs) {
-                ks = vs;
+            if (!(__builtin_fabsf(vs) < INFINITY)) {
+                ks = __builtin_nanf("");
                 vs = 0.0f;
                 page_id[i] = kUnread;
             }
             page_ks[i] = ks;
             page_vs[i] = vs;
             top = fmaxf(top, __builtin_fabsf(vs));
+            if (vs != 0.0f) least = fminf(least, __builtin_fabsf(vs));
             lost |= !live && page * p.block_size.divisor < kv_len;  // behind that no query sees
         }
         top = wave_max(top);
+        least = -wave_max(-least);
         const bool any_lost = __builtin_amdgcn_ballot_w64(lost) != 0;
         if (lane == 0) {
             wave_top[wave] = top;
+            wave_least[wave] = least;
             wave_missing[wave] = any_lost;
         }
         __syncthreads();
         std::uint32_t lost_all = 0;
 #pragma unroll
         for (int w = 0; w < kWaves; ++w) {
-            reference = fmaxf(reference, wave_top[w]);
+            top = fmaxf(top, wave_top[w]);
+            least = fminf(least, wave_least[w]);
             lost_all |= wave_missing[w];
         }
-        reference = __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(reference)));
+        reference = __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(fmaxf(reference, top))));
+        const int tallest = __builtin_amdgcn_frexp_expf(top);
+        bands = top > 0.0f ? static_cast<std::uint32_t>(tallest - __builtin_amdgcn_frexp_expf(least)) / kBand + 1 : 1;
+        bands = static_cast<std::uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(bands < kMostBands ? bands : kMostBands)));
+        // A band's |vs| are under 2^(1 - kBand * band) of the largest.
+        const int up = band == 0 ? 0 : static_cast<int>(kBand * band) - 1;
+        band_down = __uint_as_float(static_cast<std::uint32_t>(127 - up) << 23);
+        counted = __uint_as_float(band == 0 ? 0x3f800000u : 0u);
         missing = __builtin_amdgcn_readfirstlane(static_cast<int>(lost_all)) != 0;
         if (reference > 0.0f)
-            for (std::uint32_t i = tid; i < pages; i += kThreads) page_vs[i] = page_vs[i] / reference * kWeightScale;
+            for (std::uint32_t i = tid; i < pages; i += kThreads) {
+                const float vs = page_vs[i];
+                std::uint32_t its = static_cast<std::uint32_t>(tallest - __builtin_amdgcn_frexp_expf(vs)) / kBand;
+                if (its >= bands) its = bands - 1;
+                const bool of_band = bands == 1 || its == band;
+                page_vs[i] = of_band ? __builtin_amdgcn_ldexpf(vs / reference, up) * kWeightScale : 0.0f;
+            }
         __syncthreads();
     };
 
@@ -456,7 +481,7 @@ __global__ __launch_bounds__((Shape<kD, kOrder, kUniform>::kThreads), (Shape<kD,
             for (int i = 0; i < 16; ++i) s[kb][i] = __builtin_amdgcn_exp2f(s[kb][i]);
 #pragma unroll
             for (int i = 0; i < 16; i += 4) part += (s[kb][i] + s[kb][i + 1]) + (s[kb][i + 2] + s[kb][i + 3]);
-            two_sum_add(sum, low, part);
+            two_sum_add(sum, low, part * counted);
 #pragma unroll
             for (int g = 0; g < (kUniform ? 2 : 4); ++g) {
                 if constexpr (kUniform) {
@@ -511,7 +536,8 @@ __global__ __launch_bounds__((Shape<kD, kOrder, kUniform>::kThreads), (Shape<kD,
                     o = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, w.lo[kb][j], o, 0, 0, 0);
                     o = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, w.hi[kb][j], o, 0, 0, 0);
                 }
-            acc[db] += o;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) acc[db][i] = fmaf(o[i], band_down, acc[db][i]);
         }
         __builtin_amdgcn_sched_group_barrier(0x100, 2 * 2, 0);
 #pragma unroll
@@ -527,8 +553,9 @@ __global__ __launch_bounds__((Shape<kD, kOrder, kUniform>::kThreads), (Shape<kD,
         const auto key_ks_of = [&](std::uint32_t tile) { return key_ks[set][kUniform ? 0 : tile / kSets & 1]; };
         const auto key_vs_of = [&](std::uint32_t tile) { return key_vs[set][kUniform ? 0 : tile / kSets & 1]; };
         const auto buffer = [&](std::uint32_t tile) { return tiles_lds[set][tile / kSets & 1][0]; };
+        std::uint32_t band = 0;
         for (std::uint32_t first = tile_begin;;) {
-            stage();
+            stage(band);
             const float now = unit_now();
             const std::uint32_t behind = (window + 1) * p.window_tiles, last = behind < tile_end ? behind : tile_end;
             if constexpr (kOrder == Order::Turns) {
@@ -604,6 +631,8 @@ __global__ __launch_bounds__((Shape<kD, kOrder, kUniform>::kThreads), (Shape<kD,
                     __syncthreads();
                 }
             }
+            if (++band < bands) continue;  // the window again
+            band = 0;
             if (last == tile_end) break;
             first = last;
             ++window;

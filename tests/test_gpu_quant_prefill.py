@@ -138,6 +138,30 @@ def test_keys_split_over_workgroups(gpu, fmt, D, bs, n, m):
     check(cache, table, call, got, some=6)
 
 
+@pytest.mark.parametrize("fmt", ["e4m3", "int8"])
+@pytest.mark.parametrize("bs,D,bound", [(16, 128, 300), (16, 128, 900), (16, 128, 5000), (5, 128, 900), (32, 64, 900), (3, 64, 300),
+                                        (16, 256, 900)])
+@pytest.mark.parametrize("order", ["rising", "mixed", "falling"])
+def test_scales_that_a_query_does_not_see(gpu, fmt, bs, D, bound, order):
+    """Scales of V from 2^-60 to 2^60 along a sequence: each query is as exact as the values that it sees are
+    large, whatever the pages behind it hold."""
+    n, m = 280, 200
+    rng, cache, table, q = make(fmt, 2, 4, D, bs, [n], [m], [D, bs])
+    pages = table[0].astype(np.int64)
+    sizes = np.linspace(-60, 60, len(pages)).round()
+    sizes = {"rising": sizes, "falling": sizes[::-1], "mixed": rng.permutation(sizes)}[order]
+    cache.scales[1, pages] *= np.exp2(sizes).astype(np.float32)[:, None]
+    cache.upload()
+    q *= 0.1  # weights of one size: the seen values, not the scores, decide
+    call, got = run(cache, table, [n], [m], q, kv_len=bound)
+    for i in range(m):
+        see = n - m + i + 1
+        want = attention(cache, table[0], see, q[i:i + 1])[0]
+        values = np.abs(VALUES[fmt][cache.bytes[1, pages]] * cache.scales[1, pages, :, None, None].astype(np.float64))
+        top = values.transpose(0, 2, 1, 3).reshape(-1, 2 * D)[:see].max()
+        assert np.abs(got[i] - want).max() <= 1e-5 * top, i
+
+
 @pytest.mark.parametrize("seqs", [1, 3, 17])
 def test_every_sequence_and_block_is_reached(gpu, seqs):
     """The order of workgroups is a permutation: outputs of prompts of many lengths, whole ones at that."""
