@@ -549,6 +549,10 @@ std::vector<TokenLocation> decode_step(QuantizedKVStorage& storage, DeviceBatchT
     validate_batch_attention(storage, batch, query_device, output_device, query_heads);
     if (batch.rows() == 0) return {};
     const auto strides = detail::check_new_rows(storage, rows, batch.rows());
+    // The attention's own limits and its workspace, while nothing has changed yet.
+    std::size_t longest = 0;
+    for (const auto* s : batch.sequences()) longest = std::max(longest, s->num_tokens());
+    (void)detail::quantized_decode_workspace(storage, longest + 1, batch.rows(), query_heads);
     return append_and_run(storage, batch, [&] {
         check(kvflux_quant_write_tail(storage.key_base(), storage.value_base(), storage.key_scales(),
                                       storage.value_scales(), layout.num_blocks(), layout.num_kv_heads(),

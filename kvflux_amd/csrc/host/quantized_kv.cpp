@@ -145,15 +145,21 @@ void copy_quantized_pages(const QuantizedKVStorage& storage, const std::uint64_t
           "copy KV scales");
 }
 
-void enqueue_quantized_decode(const QuantizedKVStorage& storage, const std::uint64_t* table, std::size_t width,
-                              const std::uint64_t* lengths, std::size_t max_len, std::size_t rows, const float* query,
-                              float* output, std::size_t query_heads) {
+std::pair<void*, std::size_t> quantized_decode_workspace(const QuantizedKVStorage& storage, std::size_t max_len,
+                                                         std::size_t rows, std::size_t query_heads) {
     const auto& layout = storage.layout();
     std::size_t bytes = 0;
     check(kvflux_quant_attention_workspace_size(rows, max_len, layout.num_kv_heads(), query_heads, layout.block_size(),
                                                 layout.head_size(), &bytes),
           "attention workspace size");
-    void* const workspace = bytes ? storage.scratch().workspace.reserve(bytes) : nullptr;
+    return {bytes ? storage.scratch().workspace.reserve(bytes) : nullptr, bytes};
+}
+
+void enqueue_quantized_decode(const QuantizedKVStorage& storage, const std::uint64_t* table, std::size_t width,
+                              const std::uint64_t* lengths, std::size_t max_len, std::size_t rows, const float* query,
+                              float* output, std::size_t query_heads) {
+    const auto& layout = storage.layout();
+    const auto [workspace, bytes] = quantized_decode_workspace(storage, max_len, rows, query_heads);
     check(kvflux_quant_attention(storage.key_base(), storage.value_base(), storage.key_scales(), storage.value_scales(),
                                  layout.num_blocks(), layout.num_kv_heads(), layout.block_size(), layout.head_size(),
                                  abi_format(layout.format()), table, width, lengths, max_len, rows, query_heads, query,

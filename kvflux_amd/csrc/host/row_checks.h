@@ -54,6 +54,11 @@ std::pair<std::size_t, std::size_t> check_new_rows(const QuantizedKVStorage& sto
 // Enqueues the copies of {source, destination} pages (a device array) and of their scales.
 void copy_quantized_pages(const QuantizedKVStorage& storage, const std::uint64_t* pairs, std::size_t count);
 
+// Workspace of the decode attention of `rows` rows of at most max_len tokens, and its bytes;
+// null where none is needed. Throws for shapes that the attention refuses.
+std::pair<void*, std::size_t> quantized_decode_workspace(const QuantizedKVStorage& storage, std::size_t max_len,
+                                                         std::size_t rows, std::size_t query_heads);
+
 // Enqueues the decode attention of `rows` rows of a device table.
 void enqueue_quantized_decode(const QuantizedKVStorage& storage, const std::uint64_t* table, std::size_t width,
                               const std::uint64_t* lengths, std::size_t max_len, std::size_t rows, const float* query,
