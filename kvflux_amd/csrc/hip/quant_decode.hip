@@ -652,7 +652,10 @@ __global__ __launch_bounds__(kMergeThreads) void quant_decode_merge_kernel(Quant
 }
 
 // Any other head_size up to 512, and caches at any byte: a workgroup for each (query row, query
-// head), a lane for each of 64 tokens of a wavefront's step, FP32 products and sums.
+// head), a lane for each of 64 tokens of a wavefront's step, FP32 products and sums. A step's
+// weighted values are summed from zero and added with the addition's rounding error kept: one
+// by one beside a dominant key's value, thousands of small ones are lost (16384 tokens of
+// 2^-24 each: 2.4e-4 of the row).
 constexpr std::uint32_t kGenericD = 512;
 template <typename F>
 __global__ __launch_bounds__(kThreads) void quant_rows_kernel(QuantRows p, std::uint32_t first_row) {
@@ -680,8 +683,8 @@ __global__ __launch_bounds__(kThreads) void quant_rows_kernel(QuantRows p, std::
     out_row = out_row * p.query_heads + head;
     for (std::uint32_t d = tid; d < D; d += kThreads) q[d] = p.query[out_row * D + d] * p.scale_log2;
     __syncthreads();
-    float top = -INFINITY, sum = 0.0f;
-    float acc[kGenericD / 64] = {};
+    float top = -INFINITY, sum = 0.0f, sum_low = 0.0f;
+    float acc[kGenericD / 64] = {}, low[kGenericD / 64] = {};
     for (std::uint64_t base = wave * 64; base < len; base += kThreads) {
         const std::uint32_t token = static_cast<std::uint32_t>(base) + lane;
         const std::uint64_t page = p.block_size.div(token);
@@ -705,13 +708,19 @@ __global__ __launch_bounds__(kThreads) void quant_rows_kernel(QuantRows p, std::
         const float f = top == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(top - ref);
         const float w = live ? __builtin_amdgcn_exp2f(s - ref) : 0.0f;
         top = next;
-        sum = sum * f + w;
+        sum *= f;
+        sum_low *= f;
+        two_sum_add(sum, sum_low, w);
         // A missing token's row is read from the pool's first page, and dropped.
         weight[wave][lane] = live ? w * p.value_scales[scale_at] : 0.0f;
         at_of[wave][lane] = live ? at : ~0ull;
         __builtin_amdgcn_wave_barrier();
 #pragma unroll
-        for (std::uint32_t i = 0; i < kGenericD / 64; ++i) acc[i] *= f;
+        for (std::uint32_t i = 0; i < kGenericD / 64; ++i) {
+            acc[i] *= f;
+            low[i] *= f;
+        }
+        float step[kGenericD / 64] = {};
         for (int t = 0; t < 64; ++t) {
             const std::uint64_t from = at_of[wave][t];
             if (from == ~0ull) continue;  // uniform
@@ -720,17 +729,24 @@ __global__ __launch_bounds__(kThreads) void quant_rows_kernel(QuantRows p, std::
             for (std::uint32_t i = 0; i < kGenericD / 64; ++i) {
                 if (lane + 64 * i >= D) break;
                 F::values4(p.value_cache[from + lane + 64 * i], v4);
-                acc[i] = fmaf(wt, v4[0], acc[i]);
+                step[i] = fmaf(wt, v4[0], step[i]);
             }
         }
+#pragma unroll
+        for (std::uint32_t i = 0; i < kGenericD / 64; ++i) two_sum_add(acc[i], low[i], step[i]);
         __builtin_amdgcn_wave_barrier();
     }
 #pragma unroll
-    for (int d = 1; d < 64; d <<= 1) sum += __shfl_xor(sum, d);
+    for (int d = 1; d < 64; d <<= 1) {
+        const float other = __shfl_xor(sum, d);
+        sum_low += __shfl_xor(sum_low, d);
+        two_sum_add(sum, sum_low, other);
+    }
+    sum += sum_low;
     if (lane == 0) stats[wave] = make_float2(top, sum);
 #pragma unroll
     for (std::uint32_t i = 0; i < kGenericD / 64; ++i)
-        if (lane + 64 * i < D) reduce[wave][lane + 64 * i] = acc[i];
+        if (lane + 64 * i < D) reduce[wave][lane + 64 * i] = acc[i] + low[i];
     __syncthreads();
     float all = -INFINITY, total = 0.0f;
 #pragma unroll
