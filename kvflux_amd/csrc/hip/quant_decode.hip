@@ -717,23 +717,35 @@ __global__ __launch_bounds__(kThreads) void quant_rows_kernel(QuantRows p, std::
         __builtin_amdgcn_wave_barrier();
 #pragma unroll
         for (std::uint32_t i = 0; i < kGenericD / 64; ++i) {
+            if (64 * i >= D) break;  // uniform
             acc[i] *= f;
             low[i] *= f;
         }
         float step[kGenericD / 64] = {};
-        for (int t = 0; t < 64; ++t) {
-            const std::uint64_t from = at_of[wave][t];
-            if (from == ~0ull) continue;  // uniform
-            const float wt = weight[wave][t];
+        constexpr int kAtOnce = 8;  // tokens whose bytes are on their way together
+        for (int t = 0; t < 64; t += kAtOnce) {
 #pragma unroll
             for (std::uint32_t i = 0; i < kGenericD / 64; ++i) {
-                if (lane + 64 * i >= D) break;
-                F::values4(p.value_cache[from + lane + 64 * i], v4);
-                step[i] = fmaf(wt, v4[0], step[i]);
+                if (64 * i >= D) break;  // uniform
+                const std::uint32_t d = lane + 64 * i < D ? lane + 64 * i : 0;  // past the head's end its first, not stored
+                std::uint8_t raw[kAtOnce];
+#pragma unroll
+                for (int u = 0; u < kAtOnce; ++u) {
+                    const std::uint64_t from = at_of[wave][t + u];
+                    raw[u] = p.value_cache[(from == ~0ull ? 0 : from) + d];
+                }
+#pragma unroll
+                for (int u = 0; u < kAtOnce; ++u) {
+                    F::values4(raw[u], v4);
+                    step[i] = fmaf(weight[wave][t + u], at_of[wave][t + u] == ~0ull ? 0.0f : v4[0], step[i]);
+                }
             }
         }
 #pragma unroll
-        for (std::uint32_t i = 0; i < kGenericD / 64; ++i) two_sum_add(acc[i], low[i], step[i]);
+        for (std::uint32_t i = 0; i < kGenericD / 64; ++i) {
+            if (64 * i >= D) break;  // uniform
+            two_sum_add(acc[i], low[i], step[i]);
+        }
         __builtin_amdgcn_wave_barrier();
     }
 #pragma unroll
