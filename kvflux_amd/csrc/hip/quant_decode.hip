@@ -60,6 +60,12 @@ constexpr std::uint64_t kFullStreams = 256;
 // The weights' FP16 parts are of 2^15 times a weight of at most 1: FP16 ends at 2^-24,
 // so two parts miss a weight by at most 2^-40 of the largest, or 2^-23 of itself.
 constexpr float kWeightScale = 32768.0f;
+// Tiles of a wavefront after which its sums are folded into a second set, with the addition's
+// rounding error kept. A tile's sum is added to the accumulator in FP32: beside a dominant key's
+// value one that is under half a step is lost, 2^-24 a tile at most, so 4e-6 of a row for 64
+// (rows of 65536 tokens without: 3e-5). Parts that are never longer do without the registers:
+// 16 rows of <= 8192 tokens 23.0 us, with the second set 24.0; 128 rows of <= 32768 722 and 723.
+constexpr std::uint32_t kFold = 64;
 
 typedef __attribute__((ext_vector_type(2))) int qd_i32x2_t;
 typedef __attribute__((address_space(3))) qd_i32x2_t qd_lds_i32x2_t;
@@ -123,8 +129,9 @@ struct Shape {
 // kSub: tokens that share a record. 8 where pages are multiples of 8 tokens, so that
 // every 8 tokens of a tile lie in one; 1 for pages of any other size.
 // kWhole: a workgroup takes one whole stream (no shares, no partials).
+// kFolds: a wavefront may have more than kFold tiles of a part.
 // kFull: head_size is kD (as a value of the launch it cost 4 rows of <= 1500 tokens 0.5 us of 12.4).
-template <typename F, int kD, int kSub, bool kWhole, int kW, bool kFull>
+template <typename F, int kD, int kSub, bool kWhole, int kW, bool kFolds, bool kFull>
 __global__ __launch_bounds__(64 * kW, Shape<kD>::kResident) void quant_decode_kernel(QuantDecodeParams p) {
     using S = Shape<kD>;
     constexpr int kT = 64 * kW;
@@ -166,6 +173,11 @@ __global__ __launch_bounds__(64 * kW, Shape<kD>::kResident) void quant_decode_ke
         pf_f32x4_t acc[kDt];
 #pragma unroll
         for (int dt = 0; dt < kDt; ++dt) acc[dt] = pf_f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+        // The sums of the tiles folded so far; acc goes on from what that rounding left.
+        constexpr int kFolded = kFolds ? kDt : 0;
+        pf_f32x4_t base[kFolds ? kDt : 1];
+#pragma unroll
+        for (int dt = 0; dt < kFolded; ++dt) base[dt] = pf_f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
         float run_max = -INFINITY, run_sum = 0.0f, run_low = 0.0f;
         float value_ref = 1.0f;  // acc is in units of this over kWeightScale
 
@@ -323,6 +335,8 @@ __global__ __launch_bounds__(64 * kW, Shape<kD>::kResident) void quant_decode_ke
                     const float f = value_ref / next_ref;
 #pragma unroll
                     for (int dt = 0; dt < kDt; ++dt) acc[dt] *= f;
+#pragma unroll
+                    for (int dt = 0; dt < kFolded; ++dt) base[dt] *= f;
                     value_ref = next_ref;
                 }
                 // Per token of the lane's eight, or one for all of them.
@@ -388,6 +402,8 @@ __global__ __launch_bounds__(64 * kW, Shape<kD>::kResident) void quant_decode_ke
                     run_low *= f;
 #pragma unroll
                     for (int dt = 0; dt < kDt; ++dt) acc[dt] *= f;
+#pragma unroll
+                    for (int dt = 0; dt < kFolded; ++dt) base[dt] *= f;
                 }
                 const float ref = run_max == -INFINITY ? 0.0f : run_max;
                 std::uint32_t hi[4], lo[4];
@@ -431,7 +447,20 @@ __global__ __launch_bounds__(64 * kW, Shape<kD>::kResident) void quant_decode_ke
                 load(j + 2, b0);
                 if (j + 1 < tiles) compute(j + 1, b1);
                 load(j + 3, b1);
+                if (kFolds && j % kFold == kFold - 2) {  // uniform
+#pragma unroll
+                    for (int dt = 0; dt < kFolded; ++dt)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) {
+                            float sum = base[dt][r], rest = 0.0f;
+                            two_sum_add(sum, rest, acc[dt][r]);
+                            base[dt][r] = sum;
+                            acc[dt][r] = rest;
+                        }
+                }
             }
+#pragma unroll
+            for (int dt = 0; dt < kFolded; ++dt) acc[dt] += base[dt];
         }
 
         // The wavefronts' sums: in units of 1, then merged. acc[dt][r] is dim 16 dt + 4 quad + r
@@ -813,18 +842,24 @@ int launch_decode(QuantDecodeParams& p, std::uint32_t grid, hipStream_t stream) 
         // four, 11.6 with eight; one of <= 300: 6.6 and 7.2.
         if constexpr (kD <= 128 && kFull) {
             if (p.rows * streams <= kFullStreams && p.kv_len > kOneLaunch / 2) {
-                quant_decode_kernel<F, kD, kSub, true, 2 * kWaves, kFull><<<workgroups, dim3(2 * kThreads), 0, stream>>>(p);
+                quant_decode_kernel<F, kD, kSub, true, 2 * kWaves, false, kFull><<<workgroups, dim3(2 * kThreads), 0, stream>>>(p);
                 return launch_status("quant_decode_kernel");
             }
         }
-        quant_decode_kernel<F, kD, kSub, true, kWaves, kFull><<<workgroups, dim3(kThreads), 0, stream>>>(p);
+        quant_decode_kernel<F, kD, kSub, true, kWaves, false, kFull><<<workgroups, dim3(kThreads), 0, stream>>>(p);
         return launch_status("quant_decode_kernel");
     }
     // The merge takes the shorter list: streams of a few rows, or the workgroups' cuts.
     // 16 rows of 2 kv heads with 16 query heads each: 40 us by workgroup, 19 by stream.
     const std::uint32_t cuts = p.rows * streams < grid ? static_cast<std::uint32_t>(p.rows * streams) : grid;
     p.by_stream = cuts < grid;
-    quant_decode_kernel<F, kD, kSub, false, kWaves, kFull><<<dim3(grid), dim3(kThreads), 0, stream>>>(p);
+    // The longest part's tiles: a row's, or a share's.
+    const std::uint64_t tiles = (static_cast<std::uint64_t>(p.kv_len) + kTile - 1) / kTile;
+    const std::uint64_t share = p.rows * streams * (tiles + kPartCost) / grid + 1;
+    if ((tiles < share ? tiles : share) > kFold * kWaves)
+        quant_decode_kernel<F, kD, kSub, false, kWaves, true, kFull><<<dim3(grid), dim3(kThreads), 0, stream>>>(p);
+    else
+        quant_decode_kernel<F, kD, kSub, false, kWaves, false, kFull><<<dim3(grid), dim3(kThreads), 0, stream>>>(p);
     if (const int s = launch_status("quant_decode_kernel")) return s;
     // Parts of a stream: many where there are few streams. With 1024 threads and with 128:
     // 64 parts 25.3 and 26.6 us (the whole call), 18 parts 16.2 and 13.2.

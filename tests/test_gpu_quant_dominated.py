@@ -39,6 +39,17 @@ def dominated(fmt, H, D, bs, n, weight, value):
 
 
 @pytest.mark.parametrize("fmt", ["e4m3", "int8"])
+@pytest.mark.parametrize("D,bs", [(128, 16), (64, 16), (256, 16), (128, 5)])
+@pytest.mark.parametrize("value", [1.0, 1.5])
+def test_long_rows(gpu, fmt, D, bs, value):
+    """As many streams as workgroups, so that each goes through a whole row."""
+    n, rows, H, G = 65536, 256, 2, 4
+    cache, table, q, want = dominated(fmt, H, D, bs, n, 0.98 * 2.0 ** -29, value)
+    got = decode(cache, np.repeat(table, rows, 0), [n] * rows, np.full((rows, H * G, D), q, np.float32))
+    assert np.abs(got - want).max() <= 1e-5 * value
+
+
+@pytest.mark.parametrize("fmt", ["e4m3", "int8"])
 @pytest.mark.parametrize("D", [100, 272])
 @pytest.mark.parametrize("call", ["decode", "prompts"])
 def test_other_head_sizes(gpu, fmt, D, call):
