@@ -46,8 +46,7 @@ constexpr std::uint32_t kTile = 64;     // keys of a tile
 constexpr std::uint32_t kWindow = 1024; // pages whose ids and scales are in LDS at a time
 constexpr std::uint32_t kUnread = 0x80000000u;  // a page whose bytes are not read, in place of its id
 constexpr std::uint32_t kMissing = ~0u;         // one that is not there
-constexpr std::uint32_t kBand = 16;       // powers of two of |vs| worked on at once, see `bands`
-constexpr std::uint32_t kMostBands = 8;   // behind them FP32 ends
+constexpr std::uint32_t kBand = 16;       // powers of two of |vs| worked on at once, see `present`
 constexpr float kWeightScale = 32768.0f;  // as in the decode: parts of 2^15 times a weight of at most 1
 
 // How a workgroup's wavefronts share its work: four of 32 rows each; eight that take turns;
@@ -133,7 +132,7 @@ __global__ __launch_bounds__((Shape<kD, kOrder, kUniform>::kThreads), (Shape<kD,
     __shared__ __attribute__((aligned(16))) float key_ks[kSets][kUniform ? 1 : 2][kUniform ? 4 : kTile];
     __shared__ __attribute__((aligned(16))) float key_vs[kSets][kUniform ? 1 : 2][kUniform ? 4 : kTile];
     __shared__ float wave_top[kWaves], wave_least[kWaves];
-    __shared__ std::uint32_t wave_missing[kWaves];
+    __shared__ std::uint32_t wave_missing[kWaves], wave_bands[kWaves];
 
     const int tid = threadIdx.x, lane = tid % 64;
     const std::uint32_t wave = static_cast<std::uint32_t>(__builtin_amdgcn_readfirstlane(tid / 64));
@@ -183,18 +182,24 @@ __global__ __launch_bounds__((Shape<kD, kOrder, kUniform>::kThreads), (Shape<kD,
             if (d >= D) raw[kk][i] = Float4{0.0f, 0.0f, 0.0f, 0.0f};
         }
 
+    const auto one = [](float y) { return __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(y))); };
+
     // ---- the window's pages: ids, scales, the largest |vs| so far (the weights' reference).
     std::uint32_t window = tile_begin / p.window_tiles;  // tiles [window * window_tiles, + window_tiles)
     std::uint32_t window_page = 0;                       // page of page_id[0]
-    float reference = 0.0f;
+    float reference = 0.0f, floor = 0.0f;                // floor: of the windows before
     bool missing = false;                                // a page of the window is
     // A query need not see the window's largest |vs|: a weight's parts, relative to that, would
     // lose bits of what it sees (2^15 times a weight over 2^16 is 2^-1, and FP16 ends at
-    // 2^-24). So pages whose |vs| is under 2^-16 of the largest are worked on in a pass of
-    // their own, and so on: nearly always there is one.
-    std::uint32_t bands = 1;
-    float band_down = 1.0f, counted = 1.0f;  // of the pass: what its sums are scaled by; 1 in the first
-    const auto stage = [&](std::uint32_t band) {
+    // 2^-24). So pages whose |vs| is under 2^-16 of the largest are worked on in a pass of their
+    // own, in a smaller unit, and so on from the smallest up: the sums' unit only grows. Such a pass
+    // takes the tiles that have a page of its band, run by run; the last one takes all, and counts
+    // the weights. (512 tokens behind 16384 302 us; with 2 pages of zeros, whose scale is the least
+    // there is, 304; with 20 339.) What sees a page of this window sees all of the windows before,
+    // so no unit need be smaller than `floor`.
+    std::uint32_t present = 1;                    // bits of the bands that have a page, and of the last pass's, 0
+    float now = 1.0f, counted = 1.0f;             // the pass's unit; whether its weights count (1 or 0)
+    const auto stage = [&](std::uint32_t band) {  // ~0: of the window's first pass. Returns the pass's band
         const std::uint32_t from = window * p.window_tiles;  // its part of this workgroup's tiles
         const std::uint32_t tile0 = from > tile_begin ? from : tile_begin;
         const std::uint32_t tile1 = from + p.window_tiles < tile_end ? from + p.window_tiles : tile_end;
@@ -239,24 +244,44 @@ __global__ __launch_bounds__((Shape<kD, kOrder, kUniform>::kThreads), (Shape<kD,
             least = fminf(least, wave_least[w]);
             lost_all |= wave_missing[w];
         }
-        reference = __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(fmaxf(reference, top))));
-        const int tallest = __builtin_amdgcn_frexp_expf(top);
-        bands = top > 0.0f ? static_cast<std::uint32_t>(tallest - __builtin_amdgcn_frexp_expf(least)) / kBand + 1 : 1;
-        bands = static_cast<std::uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(bands < kMostBands ? bands : kMostBands)));
-        // A band's |vs| are under 2^(1 - kBand * band) of the largest.
-        const int up = band == 0 ? 0 : static_cast<int>(kBand * band) - 1;
-        band_down = __uint_as_float(static_cast<std::uint32_t>(127 - up) << 23);
-        counted = __uint_as_float(band == 0 ? 0x3f800000u : 0u);
+        reference = one(fmaxf(reference, top));
         missing = __builtin_amdgcn_readfirstlane(static_cast<int>(lost_all)) != 0;
-        if (reference > 0.0f)
-            for (std::uint32_t i = tid; i < pages; i += kThreads) {
-                const float vs = page_vs[i];
-                std::uint32_t its = static_cast<std::uint32_t>(tallest - __builtin_amdgcn_frexp_expf(vs)) / kBand;
-                if (its >= bands) its = bands - 1;
-                const bool of_band = bands == 1 || its == band;
-                page_vs[i] = of_band ? __builtin_amdgcn_ldexpf(vs / reference, up) * kWeightScale : 0.0f;
-            }
+        now = reference > 0.0f ? reference : 1.0f;
+        // Exponents of a float that is not 0 lie between -148 and 128.
+        const int tallest = __builtin_amdgcn_frexp_expf(now), lowest = floor > 0.0f ? __builtin_amdgcn_frexp_expf(floor) : -1024;
+        const auto band_of = [&](float vs) {
+            const int e = __builtin_amdgcn_frexp_expf(vs);
+            return static_cast<std::uint32_t>(tallest - (e > lowest ? e : lowest)) / kBand;
+        };
+        const bool one_band = __builtin_amdgcn_readfirstlane(top == 0.0f || band_of(least) == 0);
+        if (__builtin_expect(one_band, 1)) {
+            present = 1;
+            band = 0;
+        } else {
+            std::uint32_t seen = 0;
+            for (std::uint32_t i = tid; i < pages; i += kThreads)
+                if (page_vs[i] != 0.0f) seen |= 1u << band_of(page_vs[i]);
+            seen = over_wave(seen, [](std::uint32_t a, std::uint32_t b) { return a | b; });
+            if (lane == 0) wave_bands[wave] = seen;
+            __syncthreads();
+            present = 1;
+#pragma unroll 1
+            for (int w = 0; w < kWaves; ++w) present |= wave_bands[w];
+            present = static_cast<std::uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(present)));
+            if (band == ~0u) band = 31 - __builtin_clz(present);
+            // |vs| of a band are under 2^(1 - kBand * band) of the largest.
+            if (band != 0) now = one(__builtin_amdgcn_ldexpf(now, 1 - static_cast<int>(kBand * band)));
+            for (std::uint32_t i = tid; i < pages; i += kThreads)
+                if (band_of(page_vs[i]) != band) page_vs[i] = 0.0f;
+        }
+        counted = band == 0 ? 1.0f : 0.0f;
+        for (std::uint32_t i = tid; i < pages; i += kThreads) page_vs[i] = page_vs[i] / now * kWeightScale;
         __syncthreads();
+        return band;
+    };
+    // Whether a tile has a page of the pass's band; the same in every wavefront.
+    const auto band_tile = [&](std::uint32_t tile) {
+        return __builtin_amdgcn_ballot_w64(page_vs[p.block_size.div(tile * kTile + lane) - window_page] != 0.0f) != 0;
     };
 
     // ---- loads: a thread's kBytes of K and of V of one key of a tile, at the same place.
@@ -356,7 +381,6 @@ __global__ __launch_bounds__((Shape<kD, kOrder, kUniform>::kThreads), (Shape<kD,
         float ks[4], vs[4];
         std::uint64_t live;
     };
-    const auto one = [](float y) { return __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(y))); };
     const auto marks_of = [&](std::uint32_t tile) {
         Marks m;
         if constexpr (kUniform) {
@@ -404,7 +428,7 @@ __global__ __launch_bounds__((Shape<kD, kOrder, kUniform>::kThreads), (Shape<kD,
         __builtin_amdgcn_sched_group_barrier(0x008, 2 * 3, 0);
         return out;
     };
-    const auto weights = [&](Scores scores_of, std::uint32_t tile, const Marks& marks, float now, const float* key_k, const float* key_v) {
+    const auto weights = [&](Scores scores_of, std::uint32_t tile, const Marks& marks, const float* key_k, const float* key_v) {
         auto& s = scores_of.of;
         if (now != unit) {  // uniform: the reference of the weights moved up
             const float f = unit / now;
@@ -537,7 +561,7 @@ __global__ __launch_bounds__((Shape<kD, kOrder, kUniform>::kThreads), (Shape<kD,
                     o = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, w.hi[kb][j], o, 0, 0, 0);
                 }
 #pragma unroll
-            for (int i = 0; i < 16; ++i) acc[db][i] = fmaf(o[i], band_down, acc[db][i]);
+            for (int i = 0; i < 16; ++i) acc[db][i] += o[i];
         }
         __builtin_amdgcn_sched_group_barrier(0x100, 2 * 2, 0);
 #pragma unroll
@@ -549,17 +573,12 @@ __global__ __launch_bounds__((Shape<kD, kOrder, kUniform>::kThreads), (Shape<kD,
     };
 
     if (tile_begin < tile_end) {  // uniform
-        const auto unit_now = [&] { return reference > 0.0f ? reference : 1.0f; };
         const auto key_ks_of = [&](std::uint32_t tile) { return key_ks[set][kUniform ? 0 : tile / kSets & 1]; };
         const auto key_vs_of = [&](std::uint32_t tile) { return key_vs[set][kUniform ? 0 : tile / kSets & 1]; };
         const auto buffer = [&](std::uint32_t tile) { return tiles_lds[set][tile / kSets & 1][0]; };
-        std::uint32_t band = 0;
-        for (std::uint32_t first = tile_begin;;) {
-            stage(band);
-            const float now = unit_now();
-            const std::uint32_t behind = (window + 1) * p.window_tiles, last = behind < tile_end ? behind : tile_end;
+        const auto work = [&](std::uint32_t from, std::uint32_t to) {  // tiles [from, to), from < to
             if constexpr (kOrder == Order::Turns) {
-                fetch_one(0, first);
+                fetch_one(0, from);
                 // Two wavefronts a SIMD take turns: one multiplies (a tile's weighted values and
                 // the next one's scores) while the other works out weights, for whole phases. The
                 // second half's is a phase behind, and fills the buffers a tile ahead.
@@ -569,8 +588,8 @@ __global__ __launch_bounds__((Shape<kD, kOrder, kUniform>::kThreads), (Shape<kD,
                 const auto fill = [&](std::uint32_t tile) {
                     put_one(0, buffer(tile + 1));
                     put_one(1, buffer(tile));
-                    fetch_one(0, tile + 2 < last ? tile + 2 : last - 1);
-                    fetch_one(1, tile + 1 < last ? tile + 1 : last - 1);
+                    fetch_one(0, tile + 2 < to ? tile + 2 : to - 1);
+                    fetch_one(1, tile + 1 < to ? tile + 1 : to - 1);
                 };
                 const auto phase = [&] {
                     __builtin_amdgcn_sched_barrier(0);
@@ -578,26 +597,26 @@ __global__ __launch_bounds__((Shape<kD, kOrder, kUniform>::kThreads), (Shape<kD,
                     lds_barrier();
                     __builtin_amdgcn_sched_barrier(0);
                 };
-                put_one(0, buffer(first));
-                put_scales(first, key_ks_of(first), key_vs_of(first));
-                fetch_one(1, first);
-                fetch_one(0, first + 1 < last ? first + 1 : first);
+                put_one(0, buffer(from));
+                put_scales(from, key_ks_of(from), key_vs_of(from));
+                fetch_one(1, from);
+                fetch_one(0, from + 1 < to ? from + 1 : from);
                 phase();
                 if (ahead) {
-                    fill(first);
+                    fill(from);
                     phase();
                 }
                 const auto fill_step = [&](std::uint32_t tile) {
                     fill(tile + ahead);
                     if constexpr (!kUniform)
-                        if (tile + 1 < last) put_scales(tile + 1, key_ks_of(tile + 1), key_vs_of(tile + 1));
+                        if (tile + 1 < to) put_scales(tile + 1, key_ks_of(tile + 1), key_vs_of(tile + 1));
                 };
-                for (std::uint32_t tile = first; tile < last; ++tile) {
+                for (std::uint32_t tile = from; tile < to; ++tile) {
                     const Scores of = scores(buffer(tile));
                     set_priority<0>();
                     phase();
                     fill_step(tile);
-                    const Weights w = weights(of, tile, marks_of(tile), now, key_ks_of(tile), key_vs_of(tile));
+                    const Weights w = weights(of, tile, marks_of(tile), key_ks_of(tile), key_vs_of(tile));
                     phase();
                     set_priority<1>();
                     weigh(w, buffer(tile));
@@ -614,27 +633,60 @@ __global__ __launch_bounds__((Shape<kD, kOrder, kUniform>::kThreads), (Shape<kD,
                     put_one(1, buffer(tile));
                     put_scales(tile, key_ks_of(tile), key_vs_of(tile));
                 };
-                if (first + set < last) {
-                    fetch(first + set);
-                    put(first + set);
+                if (from + set < to) {
+                    fetch(from + set);
+                    put(from + set);
                 }
                 __syncthreads();
-                for (std::uint32_t step = first; step < last; step += kSets) {
+                for (std::uint32_t step = from; step < to; step += kSets) {
                     const std::uint32_t tile = step + set;
-                    const bool more = tile + kSets < last;
+                    const bool more = tile + kSets < to;
                     if (more) fetch(tile + kSets);
-                    if (wave_live && (kSets == 1 || tile < last)) {
-                        const Scores of = scores(buffer(tile));
-                        weigh(weights(of, tile, marks_of(tile), now, key_ks_of(tile), key_vs_of(tile)), buffer(tile));
+                    if (wave_live && (kSets == 1 || tile < to)) {
+                        const auto finish = [&](const Scores& of, const Marks& marks) {
+                            weigh(weights(of, tile, marks, key_ks_of(tile), key_vs_of(tile)), buffer(tile));
+                        };
+                        if constexpr (kSets == 2) {
+                            // Marks before the products, whose reads of LDS would wait for each of
+                            // theirs in turn (one prompt of 1000 tokens 42.2 us and 41.0).
+                            const Marks marks = marks_of(tile);
+                            __builtin_amdgcn_sched_barrier(0);
+                            finish(scores(buffer(tile)), marks);
+                        } else {
+                            const Scores of = scores(buffer(tile));
+                            finish(of, marks_of(tile));
+                        }
                     }
                     if (more) put(tile + kSets);
                     __syncthreads();
                 }
             }
-            if (++band < bands) continue;  // the window again
-            band = 0;
-            if (last == tile_end) break;
-            first = last;
+        };
+        std::uint32_t band = ~0u;
+        for (std::uint32_t from = tile_begin;;) {
+            band = stage(band);
+            const std::uint32_t behind = (window + 1) * p.window_tiles, last = behind < tile_end ? behind : tile_end;
+            std::uint32_t to = last;
+            if (__builtin_expect(band != 0, 0)) {
+                // The next run of the pass's tiles, over gaps of two: a run's start costs as much.
+                while (from < last && !band_tile(from)) ++from;
+                to = from;
+                for (std::uint32_t next = from; next < last && next < to + 3; ++next)
+                    if (band_tile(next)) to = next + 1;
+                __syncthreads();  // every wavefront has looked for them
+            }
+            if (__builtin_expect(from < to, 1)) work(from, to);
+            from = to;
+            if (__builtin_expect(band != 0, 0)) {
+                if (to == last) {  // the window's next pass
+                    band = 31 - __builtin_clz(present & ((1u << band) - 1));
+                    from = window * p.window_tiles > tile_begin ? window * p.window_tiles : tile_begin;
+                }
+                continue;
+            }
+            if (to == tile_end) break;
+            band = ~0u;
+            floor = reference;
             ++window;
         }
     }

@@ -1,0 +1,101 @@
+"""An 8-bit cache whose scales are not the writes' own, or lie far apart.
+
+Attention: within 1e-5 of the largest value that a query itself sees, of its kv head
+(test_gpu_quant_attention.py says where that comes from).
+"""
+from __future__ import annotations
+
+import numpy as np
+import pytest
+
+from kvflux_amd import device
+from quant_util import VALUES, attention
+from test_gpu_quant_prefill import Prefill
+from test_gpu_quant_prefill import make as make_prompts
+from test_gpu_quant_prefill import run as prefill
+
+pytestmark = pytest.mark.gpu
+
+
+def check_visible(cache, table, call, got, some=None):
+    """Every query, or `some` of each sequence, within 1e-5 of the largest value that it sees."""
+    G = got.shape[1] // cache.H
+    for r, (n, m) in enumerate(zip(call.lens, call.new)):
+        n, m, at = int(n), int(m), int(call.offsets[r])
+        rows = np.arange(m) if some is None or m <= some else np.unique(np.r_[0, m - 1, np.random.default_rng(r).integers(0, m, some)])
+        pages = table[r, :-(-n // cache.bs)].astype(np.int64)
+        sizes = np.abs(VALUES[cache.fmt][cache.bytes[1, pages]]).max(-1) * cache.scales[1, pages][..., None].astype(np.float64)
+        sizes = sizes.transpose(1, 0, 2).reshape(cache.H, -1)  # of every token's V
+        want = attention(cache, table[r], n, call.q[at + rows], visible=n - m + rows + 1)
+        for i, row in enumerate(rows):
+            top = np.repeat(sizes[:, :n - m + row + 1].max(1), G)[:, None]
+            err = np.abs(got[at + row] - want[i])
+            assert (err <= 1e-5 * top).all(), (r, row, (err / top).max())
+
+
+# ------------------------------------------------- what each query sees
+@pytest.mark.parametrize("fmt", ["e4m3", "int8"])
+@pytest.mark.parametrize("bs,D,bound", [(16, 128, None), (16, 128, 900), (16, 128, 5000), (16, 64, 900), (16, 256, None), (5, 128, 900),
+                                        (3, 64, None), (5, 128, 5000), (64, 128, 5000)])
+def test_each_query_by_what_it_sees(gpu, fmt, bs, D, bound):
+    """Scales of V from 2^-60 to 2^40 at random by page and head, ordinary queries."""
+    lens, new = np.array([300, 64, 700]), np.array([100, 64, 300])
+    rng, cache, table, q = make_prompts(fmt, 2, 4, D, bs, lens, new, [D, bs], scales=1.37)
+    cache.scales[1] *= np.exp2(rng.integers(-60, 41, cache.scales[1].shape)).astype(np.float32)
+    cache.upload()
+    call, got = prefill(cache, table, lens, new, q, kv_len=bound)
+    check_visible(cache, table, call, got)
+
+
+@pytest.mark.parametrize("fmt,D,bs,n,m", [("e4m3", 128, 16, 9000, 40), ("int8", 64, 16, 40000, 70), ("int8", 128, 1, 5000, 300),
+                                          ("e4m3", 128, 16, 33000, 130)])
+def test_each_query_of_split_keys(gpu, fmt, D, bs, n, m):
+    """A chunk behind a long prefix, its keys split over workgroups and windows, scales far apart in its last pages."""
+    rng, cache, table, q = make_prompts(fmt, 2, 4, D, bs, [n], [m], [n, m])
+    last = table[0, -(-m // bs) - 3:].astype(np.int64)
+    cache.scales[1, last] *= np.exp2(rng.integers(0, 60, (len(last), 2))).astype(np.float32)
+    cache.upload()
+    call, got = prefill(cache, table, [n], [m], q)
+    check_visible(cache, table, call, got, some=12)
+
+
+def zero_pages(rng, cache, table, count):
+    """V of `count` pages all zeros, as the writes leave them: with the least scale."""
+    pages = rng.choice(table[table < cache.blocks].astype(np.int64), count, replace=False)
+    cache.bytes[1, pages] = 0
+    cache.scales[1, pages] = 2.0 ** -110
+    cache.upload()
+
+
+@pytest.mark.parametrize("fmt", ["e4m3", "int8"])
+@pytest.mark.parametrize("bs,D,bound", [(16, 128, None), (16, 128, 5000), (16, 64, None), (16, 64, 2000), (16, 256, None), (5, 128, None),
+                                        (5, 128, 5000), (3, 64, 2000), (128, 128, 5000), (200, 64, None)])
+def test_pages_of_zeros_among_others(gpu, fmt, bs, D, bound):
+    lens, new = np.array([300, 64, 700, 1600]), np.array([100, 64, 300, 40])
+    rng, cache, table, q = make_prompts(fmt, 2, 4, D, bs, lens, new, [D, bs])
+    zero_pages(rng, cache, table, 5)
+    call, got = prefill(cache, table, lens, new, q, kv_len=bound)
+    check_visible(cache, table, call, got)
+
+
+def test_a_page_of_zeros_costs_no_pass_over_the_others(gpu):
+    """512 tokens behind 16384 with two pages of zeros among them: the time without, and half of it more at most (seven
+    times as long where every power of two between the scales had its pass)."""
+    rng, cache, table, q = make_prompts("e4m3", 8, 4, 128, 16, [16896], [512], 1)
+    call = Prefill(cache, table, [16896], [512], q)
+
+    def time():
+        best = np.inf
+        for _ in range(5):
+            a, b = device.Event(), device.Event()
+            a.record()
+            call.run()
+            b.record()
+            device.synchronize()
+            best = min(best, a.elapsed_ms(b))
+        return best
+
+    time()
+    without = time()
+    zero_pages(rng, cache, table, 2)
+    assert time() < 1.5 * without
