@@ -695,7 +695,10 @@ __global__ __launch_bounds__((Shape<kD, kOrder, kUniform>::kThreads), (Shape<kD,
     sum += low;
     const auto swapped = __builtin_amdgcn_permlane32_swap(__float_as_uint(sum), __float_as_uint(sum), false, false);
     sum = __uint_as_float(swapped[0]) + __uint_as_float(swapped[1]);
-    float in_ones = unit * (1.0f / kWeightScale);
+    // One after the other: a unit of 2^-126 over 2^15 would lose bits.
+#pragma unroll
+    for (int db = 0; db < kDb; ++db) acc[db] *= 1.0f / kWeightScale;
+    float in_ones = unit;
     if constexpr (kSets == 2) {
         float m = threshold == 0.0f ? ref : -INFINITY;  // -INFINITY: no key seen
         if (set == 1) {

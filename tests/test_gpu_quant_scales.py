@@ -10,6 +10,9 @@ import pytest
 
 from kvflux_amd import device
 from quant_util import VALUES, attention
+from test_gpu_quant_attention import SHARES
+from test_gpu_quant_attention import check as check_decode
+from test_gpu_quant_attention import run as decode
 from test_gpu_quant_prefill import Prefill
 from test_gpu_quant_prefill import make as make_prompts
 from test_gpu_quant_prefill import run as prefill
@@ -99,3 +102,21 @@ def test_a_page_of_zeros_costs_no_pass_over_the_others(gpu):
     without = time()
     zero_pages(rng, cache, table, 2)
     assert time() < 1.5 * without
+
+
+# ------------------------------------------------- scales of any size
+@pytest.mark.parametrize("fmt", ["e4m3", "int8"])
+@pytest.mark.parametrize("bs", [16, 3])
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_scales_near_the_end_of_fp32(gpu, fmt, bs, D):
+    """Scales of V of 2^-125 that are no powers of two: values of 2^-125 to 2^-116, outputs that FP32 holds in full."""
+    lens, new = np.array([900, 64]), np.array([100, 64])
+    rng, cache, table, q = make_prompts(fmt, 2, 4, D, bs, lens, new, 4)
+    cache.scales[1] = (rng.uniform(1, 2, cache.scales[1].shape) * 2.0 ** -125).astype(np.float32)
+    cache.upload()
+    for bound in (None, 5000):
+        call, got = prefill(cache, table, lens, new, q, kv_len=bound)
+        check_visible(cache, table, call, got)
+    rows = q[[0, -1]]
+    for bound in (None, SHARES):
+        check_decode(cache, table, lens, rows, decode(cache, table, lens, rows, kv_len=bound))
