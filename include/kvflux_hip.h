@@ -501,7 +501,9 @@ int kvflux_norm_rope_write_tail(void* key_cache, void* value_cache, uint64_t num
  *   page's scale if that is larger. Values are divided by it (exactly) and rounded
  *   to nearest, ties to even. Where it grows, the earlier tokens are rounded again
  *   to it: exactly for E4M3 except for what falls below 2^-6 of the scale. Scales of
- *   another origin stay as they are until they grow. An infinity or NaN makes the
+ *   another origin stay as they are until they grow (the quotient by one that is no
+ *   power of two is rounded to FP32 first, as are the earlier tokens' by the scale
+ *   that replaces it). An infinity or NaN makes the
  *   scale of its page and head NaN, and with it all that is read there, until a
  *   write that starts the page anew. Places behind the new tokens keep their
  *   bytes. Nothing is written for lengths of zero, pages past table_width and page

@@ -2,6 +2,7 @@
 // page and kv head:
 //   write  s' = max(s if the page has earlier tokens, 2^ceil(log2(max|x| / top)))
 //          q = round(x / s'), and q' = round(q s / s') of those earlier tokens
+//          (the quotients in FP32: exact, unless a scale of another origin is no power of two)
 //   read   x = q s
 //
 // Both are bound by memory, and small calls by the chain of dependent loads: a
@@ -154,6 +155,11 @@ __global__ __launch_bounds__(kThreads) void quant_write_kernel(WriteParams p) {
         float y[kV];
 #pragma unroll
         for (int i = 0; i < kV; ++i) y[i] = In::value(g.x[i]) * inverse;
+        // A kept scale of another origin may be no power of two: its reciprocal is rounded.
+        if (__builtin_expect((__float_as_uint(scale) & 0x7fffffu) != 0, 0)) {  // uniform in the unit
+#pragma unroll
+            for (int i = 0; i < kV; ++i) y[i] = In::value(g.x[i]) / scale;
+        }
         put(c, y);
     };
 #pragma unroll

@@ -1,7 +1,8 @@
 """An 8-bit cache whose scales are not the writes' own, or lie far apart.
 
 Attention: within 1e-5 of the largest value that a query itself sees, of its kv head
-(test_gpu_quant_attention.py says where that comes from).
+(test_gpu_quant_attention.py says where that comes from). Writes: bytes and scales bit for
+bit with the definition, a value over a scale that is no power of two by way of FP32.
 """
 from __future__ import annotations
 
@@ -9,13 +10,14 @@ import numpy as np
 import pytest
 
 from kvflux_amd import device
-from quant_util import VALUES, attention
+from quant_util import VALUES, Cache, attention, hold, scale_of
 from test_gpu_quant_attention import SHARES
 from test_gpu_quant_attention import check as check_decode
 from test_gpu_quant_attention import run as decode
 from test_gpu_quant_prefill import Prefill
 from test_gpu_quant_prefill import make as make_prompts
 from test_gpu_quant_prefill import run as prefill
+from test_gpu_quant_write import Rows, same, write
 
 pytestmark = pytest.mark.gpu
 
@@ -120,3 +122,48 @@ def test_scales_near_the_end_of_fp32(gpu, fmt, bs, D):
     rows = q[[0, -1]]
     for bound in (None, SHARES):
         check_decode(cache, table, lens, rows, decode(cache, table, lens, rows, kv_len=bound))
+
+
+# ------------------------------------------------- writes behind scales of another origin
+def half_page(fmt, scale, D=128, bs=16):
+    """One page and head with 8 tokens of bytes at a scale of another origin, and its table."""
+    rng = np.random.default_rng(3)
+    cache = Cache(fmt, 1, 1, bs, D)
+    cache.bytes[:] = hold(np.rint(rng.uniform(-100, 100, cache.bytes.shape)), fmt)
+    cache.scales[:] = np.float32(scale)
+    cache.upload()
+    return rng, cache, np.zeros((1, 1), np.uint64)
+
+
+def append(cache, table, x, name="f32"):
+    """Tokens behind the first 8; the model's bytes and scales by the definition, divided in FP32."""
+    n = x[0].shape[0]
+    rows = Rows(x, name)
+    held = write(cache, rows, table, [8 + n], [n], [0])
+    device.synchronize()
+    del held
+    for i in range(2):
+        before = cache.scales[i, 0, 0]
+        s = np.float32(scale_of(np.abs(rows.x[i]).max(), cache.fmt))
+        if abs(before) >= s:
+            s = before
+        else:
+            cache.bytes[i, 0, 0, :8] = hold(VALUES[cache.fmt][cache.bytes[i, 0, 0, :8]] * (float(before) / float(s)), cache.fmt)
+        cache.bytes[i, 0, 0, 8:8 + n] = hold((rows.x[i][:, 0].astype(np.float32) / s).astype(np.float64), cache.fmt)
+        cache.scales[i, 0, 0] = s
+    same(cache)
+
+
+@pytest.mark.parametrize("fmt", ["e4m3", "int8"])
+@pytest.mark.parametrize("D", [128, 100])
+def test_a_kept_scale_that_is_no_power_of_two(gpu, fmt, D):
+    """Values half way between two bytes, whose quotient by the scale is exact where their product with
+    its rounded reciprocal is a step beside it."""
+    for scale in np.random.default_rng(1).uniform(1, 2, 40).astype(np.float32):
+        rng, cache, table = half_page(fmt, scale, D)
+        steps = np.arange(8 * D) % 63 + 0.5  # of at most half the top, so that the scale is large enough
+        if fmt == "e4m3":
+            steps = np.exp2(steps // 8) * (8 + steps % 8) / 8  # between two of the eight of a power of two
+            steps = np.where(steps <= 224, steps, 1.0)
+        x = (steps * float(scale)).astype(np.float32).reshape(8, 1, D)
+        append(cache, table, [x, -x])
