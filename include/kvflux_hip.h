@@ -498,16 +498,16 @@ int kvflux_norm_rope_write_tail(void* key_cache, void* value_cache, uint64_t num
  *   The scale of a page and head is the smallest power of two, 2^-110 at least,
  *   that brings the largest magnitude among the new values to 448 or 127, or, if
  *   the page has earlier tokens (of positions before the first new one), the
- *   page's scale if that is larger. Values are divided by it (exactly) and rounded
- *   to nearest, ties to even. Where it grows, the earlier tokens are rounded again
- *   to it: exactly for E4M3 except for what falls below 2^-6 of the scale. Scales of
- *   another origin stay as they are until they grow (the quotient by one that is no
- *   power of two is rounded to FP32 first, as are the earlier tokens' by the scale
- *   that replaces it). An infinity or NaN makes the
- *   scale of its page and head NaN, and with it all that is read there, until a
- *   write that starts the page anew. Places behind the new tokens keep their
- *   bytes. Nothing is written for lengths of zero, pages past table_width and page
- *   ids >= num_blocks.
+ *   page's scale if that is larger (in size: it may be negative). Values are
+ *   divided by it (exactly) and rounded to nearest, ties to even. Where it grows,
+ *   the earlier tokens are rounded again to it: exactly for E4M3 except for what
+ *   falls below 2^-6 of the scale. Scales of another origin stay as they are until
+ *   they grow (the quotient by one that is no power of two is rounded to FP32
+ *   first, as are the earlier tokens' by the scale that replaces it). An infinity
+ *   or NaN makes the scale of its page and head NaN, and with it all that is read
+ *   there, until a write that starts the page anew. Places behind the new tokens
+ *   keep their bytes. Nothing is written for lengths of zero, pages past
+ *   table_width and page ids >= num_blocks.
  * kvflux_quant_gather: K and V of every sequence as [sum of lengths]
  *   [num_kv_heads][head_size] of `output_dtype`, each value rounded once; its
  *   other arguments as for kvflux_gather_paged_kv_live.

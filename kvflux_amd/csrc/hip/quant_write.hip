@@ -139,7 +139,8 @@ __global__ __launch_bounds__(kThreads) void quant_write_kernel(WriteParams p) {
     }
     if (!there) return;  // uniform in the unit
     float scale = quant_scale<F>(largest);
-    if (first != 0 && !(scale >= before)) scale = before != before || scale == scale ? before : scale;
+    // A scale of another origin may be negative: it is its size that has to do.
+    if (first != 0 && !(scale > __builtin_fabsf(before))) scale = before != before || scale == scale ? before : scale;
     const float inverse = 1.0f / scale;
 
     std::uint8_t* const held_at = p.cache[kv] + (id * p.heads.divisor + head) * p.block_size * static_cast<std::uint64_t>(p.head_size);

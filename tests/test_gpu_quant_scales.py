@@ -167,3 +167,12 @@ def test_a_kept_scale_that_is_no_power_of_two(gpu, fmt, D):
             steps = np.where(steps <= 224, steps, 1.0)
         x = (steps * float(scale)).astype(np.float32).reshape(8, 1, D)
         append(cache, table, [x, -x])
+
+
+@pytest.mark.parametrize("fmt", ["e4m3", "int8"])
+@pytest.mark.parametrize("scale", [-4.0, -0.37])
+@pytest.mark.parametrize("size", [1.0, 1e4])
+def test_a_negative_scale(gpu, fmt, scale, size):
+    """It stays while its size is enough for the new values, and is replaced by a positive one where it is not."""
+    rng, cache, table = half_page(fmt, scale)
+    append(cache, table, [(rng.standard_normal((5, 1, 128)) * size).astype(np.float32) for _ in range(2)])
