@@ -97,7 +97,8 @@ struct NewRows {
 // another pool, more new tokens than tokens, as many counts as sequences not given, two
 // sequences writing to the same page (fork_shared before append_tokens_cow), null, host,
 // foreign or misaligned rows, a stride below a token's heads, rows overlapping the cache.
-// No new tokens: no-op. Returns after completion.
+// std::length_error: a sequence whose new tokens touch 2^24 pages and more, counted for each
+// head of K and V. No new tokens: no-op. Returns after completion.
 void write_quantized_kv(QuantizedKVStorage& storage, const std::vector<const SequenceState*>& sequences,
                         const std::vector<std::size_t>& new_tokens, const NewRows& rows);
 

@@ -544,7 +544,6 @@ void paged_attention_batch(const QuantizedKVStorage& storage, const DeviceBatchT
 
 std::vector<TokenLocation> decode_step(QuantizedKVStorage& storage, DeviceBatchTable& batch, const NewRows& rows,
                                        const float* query_device, float* output_device, std::size_t query_heads) {
-    const auto& layout = storage.layout();
     detail::DeviceGuard guard(storage.device());
     validate_batch_attention(storage, batch, query_device, output_device, query_heads);
     if (batch.rows() == 0) return {};
@@ -554,13 +553,8 @@ std::vector<TokenLocation> decode_step(QuantizedKVStorage& storage, DeviceBatchT
     for (const auto* s : batch.sequences()) longest = std::max(longest, s->num_tokens());
     (void)detail::quantized_decode_workspace(storage, longest + 1, batch.rows(), query_heads);
     return append_and_run(storage, batch, [&] {
-        check(kvflux_quant_write_tail(storage.key_base(), storage.value_base(), storage.key_scales(),
-                                      storage.value_scales(), layout.num_blocks(), layout.num_kv_heads(),
-                                      layout.block_size(), layout.head_size(), detail::abi_format(layout.format()),
-                                      rows.key, rows.value, detail::abi_dtype(rows.dtype), strides.first,
-                                      strides.second, batch.device_table(), batch.capacity_blocks(),
-                                      batch.device_lengths(), batch.rows(), nullptr),
-              "decode step quantised KV write");
+        detail::enqueue_quantized_tails(storage, rows, strides, batch.device_table(), batch.capacity_blocks(),
+                                        batch.device_lengths(), batch.rows());
         enqueue_batch_attention(storage, batch, query_device, output_device, query_heads);
     });
 }

@@ -145,6 +145,30 @@ void copy_quantized_pages(const QuantizedKVStorage& storage, const std::uint64_t
           "copy KV scales");
 }
 
+// What a write counts in 24 bits: pages that a launch's sequences may touch, for each head of K and V.
+std::size_t pages_of_a_launch(const QuantizedKVStorage& storage) {
+    constexpr std::size_t most = (std::size_t{1} << 24) - 1;
+    return most / (2 * storage.layout().num_kv_heads());
+}
+
+void enqueue_quantized_tails(const QuantizedKVStorage& storage, const NewRows& rows,
+                             const std::pair<std::size_t, std::size_t>& strides, const std::uint64_t* table,
+                             std::size_t width, const std::uint64_t* lengths, std::size_t count) {
+    const auto& layout = storage.layout();
+    const std::size_t element = abi_dtype(rows.dtype) == KVFLUX_DTYPE_F32 ? 4 : 2;
+    const std::size_t at_once = std::max<std::size_t>(1, pages_of_a_launch(storage));  // none: refused below
+    for (std::size_t first = 0; first < count; first += at_once) {
+        check(kvflux_quant_write_tail(storage.key_base(), storage.value_base(), storage.key_scales(),
+                                      storage.value_scales(), layout.num_blocks(), layout.num_kv_heads(),
+                                      layout.block_size(), layout.head_size(), abi_format(layout.format()),
+                                      static_cast<const unsigned char*>(rows.key) + first * strides.first * element,
+                                      static_cast<const unsigned char*>(rows.value) + first * strides.second * element,
+                                      abi_dtype(rows.dtype), strides.first, strides.second, table + first * width,
+                                      width, lengths + first, std::min(count - first, at_once), nullptr),
+              "quantised KV tail write kernel launch");
+    }
+}
+
 std::pair<void*, std::size_t> quantized_decode_workspace(const QuantizedKVStorage& storage, std::size_t max_len,
                                                          std::size_t rows, std::size_t query_heads) {
     const auto& layout = storage.layout();
@@ -240,18 +264,42 @@ void write_quantized_kv(QuantizedKVStorage& storage, const std::vector<const Seq
             }
         }
     }
+    // A launch has room for as many pages of each of its sequences as the longest may touch: runs of
+    // sequences that fit one, so that a long prompt beside many single tokens does not count for each.
+    struct Run {
+        std::size_t first, count, most;
+    };
+    std::vector<Run> runs;
+    const auto room = detail::pages_of_a_launch(storage);
+    const auto pages = [&](std::size_t tokens) { return (tokens + layout.block_size() - 2) / layout.block_size() + 1; };
+    for (std::size_t r = 0; r < sequences.size(); ++r) {
+        if (b.counts[r] == 0) continue;
+        if (pages(b.counts[r]) > room) throw std::length_error("too many new tokens of a sequence");
+        if (!runs.empty()) {
+            auto& last = runs.back();
+            const std::size_t most = std::max<std::size_t>(last.most, b.counts[r]), count = r + 1 - last.first;
+            if (pages(most) <= room / count) {
+                last.count = count;
+                last.most = most;
+                continue;
+            }
+        }
+        runs.push_back({r, 1, b.counts[r]});
+    }
     detail::DeviceGuard guard(storage.device());
     const auto strides = detail::check_new_rows(storage, rows, b.total);
     const auto dev = storage.scratch().upload({{b.table.block_table().data(), b.table.block_table().size() * 8},
                                                {b.lengths.data(), b.lengths.size() * 8},
                                                {b.counts.data(), b.counts.size() * 8},
                                                {b.offsets.data(), b.offsets.size() * 8}});
-    check(kvflux_quant_write(storage.key_base(), storage.value_base(), storage.key_scales(), storage.value_scales(),
-                             layout.num_blocks(), layout.num_kv_heads(), layout.block_size(), layout.head_size(),
-                             detail::abi_format(layout.format()), rows.key, rows.value, detail::abi_dtype(rows.dtype),
-                             strides.first, strides.second, dev[0], width, dev[1], dev[2], dev[3], sequences.size(),
-                             b.most, nullptr),
-          "quantised KV write kernel launch");
+    for (const auto& run : runs) {
+        check(kvflux_quant_write(storage.key_base(), storage.value_base(), storage.key_scales(), storage.value_scales(),
+                                 layout.num_blocks(), layout.num_kv_heads(), layout.block_size(), layout.head_size(),
+                                 detail::abi_format(layout.format()), rows.key, rows.value, detail::abi_dtype(rows.dtype),
+                                 strides.first, strides.second, dev[0] + run.first * width, width, dev[1] + run.first,
+                                 dev[2] + run.first, dev[3] + run.first, run.count, run.most, nullptr),
+              "quantised KV write kernel launch");
+    }
     check(kvflux_stream_synchronize(nullptr), "quantised KV write synchronize");
 }
 

@@ -54,6 +54,11 @@ std::pair<std::size_t, std::size_t> check_new_rows(const QuantizedKVStorage& sto
 // Enqueues the copies of {source, destination} pages (a device array) and of their scales.
 void copy_quantized_pages(const QuantizedKVStorage& storage, const std::uint64_t* pairs, std::size_t count);
 
+// Enqueues the writes of one new token for each of `count` rows of a device table.
+void enqueue_quantized_tails(const QuantizedKVStorage& storage, const NewRows& rows,
+                             const std::pair<std::size_t, std::size_t>& strides, const std::uint64_t* table,
+                             std::size_t width, const std::uint64_t* lengths, std::size_t count);
+
 // Workspace of the decode attention of `rows` rows of at most max_len tokens, and its bytes;
 // null where none is needed. Throws for shapes that the attention refuses.
 std::pair<void*, std::size_t> quantized_decode_workspace(const QuantizedKVStorage& storage, std::size_t max_len,
