@@ -574,7 +574,8 @@ int kvflux_quant_attention(const void* key_cache, const void* value_cache, const
  * (0: NULL will do; no initialisation; calls that share one must be ordered).
  * KVFLUX_ERR_UNSUPPORTED: more than 65535 sequences, 2^31 pages or max_kv_len, or
  * num_seqs * max_query_tokens * query_heads of 2^31 and more; 2^23 and more
- * workgroups (of 128 or 256 query rows of a kv head). */
+ * workgroups (of 128 or 256 query rows of a kv head); split keys of 2^26 query rows and
+ * more (of 2^28 at head sizes up to 64, 2^27 up to 128). */
 int kvflux_quant_prefill_workspace_size(uint64_t num_seqs, uint64_t max_query_tokens, uint64_t max_kv_len,
                                         uint64_t num_kv_heads, uint64_t query_heads, uint64_t block_size,
                                         uint64_t head_size, size_t* bytes);

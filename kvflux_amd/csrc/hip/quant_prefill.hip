@@ -871,6 +871,11 @@ std::uint64_t prefill_workspace(const PrefillPlan& plan, std::uint64_t num_seqs,
     return plan.splits == 1 ? 0 : plan.splits * num_seqs * max_query * query_heads * (head_size + 2) * sizeof(float);
 }
 
+// Whether the merge's threads, four dims each, fit a grid.
+bool merge_fits(const PrefillPlan& plan, std::uint64_t max_query, std::uint64_t query_heads, std::uint64_t head_size) {
+    return plan.splits == 1 || max_query * query_heads <= kMostWorkgroups * (256 / (head_size / 4));
+}
+
 template <typename F, int kD, Order kOrder>
 int launch_prefill(QuantPrefillParams& p, hipStream_t stream) {
     const dim3 grid(p.heads * p.splits * p.num_seqs * p.blocks), threads(Shape<kD, kOrder, true>::kThreads);
@@ -927,6 +932,8 @@ extern "C" int kvflux_quant_prefill_workspace_size(uint64_t num_seqs, uint64_t m
     head_size = padded_head_size(head_size);
     if (num_seqs == 0 || max_query_tokens == 0 || head_size == 0) return KVFLUX_OK;
     const PrefillPlan plan = prefill_plan(num_seqs, max_query_tokens, max_kv_len, num_kv_heads, query_heads / num_kv_heads, head_size);
+    if (!merge_fits(plan, max_query_tokens, query_heads, head_size))
+        return fail(KVFLUX_ERR_UNSUPPORTED, "quant prefill workspace: shape too large");
     *bytes = prefill_workspace(plan, num_seqs, max_query_tokens, query_heads, head_size);
     return KVFLUX_OK;
 }
@@ -1009,7 +1016,8 @@ extern "C" int kvflux_quant_prefill(const void* key_cache, const void* value_cac
     p.query = query;
     p.output = output;
     p.scale_log2 = scale_log2;
-    if (static_cast<std::uint64_t>(p.heads) * p.splits * p.num_seqs * p.blocks > kMostWorkgroups / 2)
+    if (static_cast<std::uint64_t>(p.heads) * p.splits * p.num_seqs * p.blocks > kMostWorkgroups / 2 ||
+        !merge_fits(plan, max_query_tokens, query_heads, padded))
         return fail(KVFLUX_ERR_UNSUPPORTED, "quant prefill: shape too large");
     if (plan.splits > 1) {
         if (!workspace || workspace_bytes < prefill_workspace(plan, num_seqs, max_query_tokens, query_heads, padded))
