@@ -47,6 +47,11 @@ constexpr std::uint32_t kWindow = 1024; // pages whose ids and scales are in LDS
 constexpr std::uint32_t kUnread = 0x80000000u;  // a page whose bytes are not read, in place of its id
 constexpr std::uint32_t kMissing = ~0u;         // one that is not there
 constexpr std::uint32_t kBand = 16;       // powers of two of |vs| worked on at once, see `present`
+// Tiles after which a row's sums are folded into its place in the output, with the addition's
+// rounding error kept. A tile's sum is added to the accumulator in FP32: beside a dominant key's
+// value one that is under half a step is lost, 2^-24 a tile at most, so 9e-6 of a row for 144
+// (rows of 32768 tokens without: 3e-5; the contract is 1e-5).
+constexpr std::uint32_t kFold = 144;
 constexpr float kWeightScale = 32768.0f;  // as in the decode: parts of 2^15 times a weight of at most 1
 
 // How a workgroup's wavefronts share its work: four of 32 rows each; eight that take turns;
@@ -86,7 +91,8 @@ struct QuantPrefillParams {
     std::uint32_t tokens;              // query tokens of a workgroup
     std::uint32_t blocks;              // workgroups along max_query
     std::uint32_t splits, split_tiles; // workgroups of a block of queries at most, tiles of each
-    std::uint32_t window_tiles;        // tiles whose pages fit kWindow
+    std::uint32_t window_tiles;        // tiles whose pages fit kWindow; at most kFold where sums are folded
+    std::uint32_t fold_windows;        // windows that are folded together
     const float* query;
     float* output;
     float scale_log2;
@@ -106,7 +112,8 @@ __device__ inline Split split_of(std::uint32_t tile_count, std::uint32_t most) {
 
 // kUniform: pages are multiples of 16 tokens, so 16 neighbouring keys of a tile share
 // their scales, which are then one value for a wavefront.
-template <typename F, int kD, Order kOrder, bool kUniform>
+// kFolds: a workgroup may have more than kFold tiles (and is not in two sets).
+template <typename F, int kD, Order kOrder, bool kUniform, bool kFolds>
 __global__ __launch_bounds__((Shape<kD, kOrder, kUniform>::kThreads), (Shape<kD, kOrder, kUniform>::kPerSimd)) void quant_prefill_kernel(QuantPrefillParams p) {
     using S = Shape<kD, kOrder, kUniform>;
     using Vec = pf_f16x8_t;
@@ -133,6 +140,9 @@ __global__ __launch_bounds__((Shape<kD, kOrder, kUniform>::kThreads), (Shape<kD,
     __shared__ __attribute__((aligned(16))) float key_vs[kSets][kUniform ? 1 : 2][kUniform ? 4 : kTile];
     __shared__ float wave_top[kWaves], wave_least[kWaves];
     __shared__ std::uint32_t wave_missing[kWaves], wave_bands[kWaves];
+    static_assert(!kFolds || kSets == 1, "a set has no place to fold into");
+    __shared__ float* place_of[kFolds ? kThreads : 1];
+    __shared__ float fold_ref[kFolds ? S::kRows : 1], fold_unit;  // of the sums folded so far: ref, -INFINITY for none, and unit
 
     const int tid = threadIdx.x, lane = tid % 64;
     const std::uint32_t wave = static_cast<std::uint32_t>(__builtin_amdgcn_readfirstlane(tid / 64));
@@ -169,7 +179,12 @@ __global__ __launch_bounds__((Shape<kD, kOrder, kUniform>::kThreads), (Shape<kD,
     const bool row_live = r < p.tokens * p.heads_of && token < t_end;
     const bool wave_live = __builtin_amdgcn_ballot_w64(row_live) != 0;
     const std::uint64_t q_row = (p.query_offsets[seq] + (row_live ? token : t0)) * p.query_heads + kvh * p.group + (row_live ? head : p.first);
-    const std::uint32_t D = p.head_size;
+    const std::uint32_t D = p.head_size, head_at = kvh * p.group + head;
+    // A live row's place: in the output where one workgroup sees all its keys, else a partial.
+    const auto row_place = [&] {
+        const std::uint64_t part = ((static_cast<std::uint64_t>(split) * p.num_seqs + seq) * p.max_query + token) * p.query_heads + head_at;
+        return mine.count == 1 ? p.output + ((p.query_offsets[seq] + token) * p.query_heads + head_at) * D : p.part_acc + part * kD;
+    };
     const float* const q_src = p.query + q_row * D;
     struct Float4 { float x, y, z, w; };  // float-aligned
     Float4 raw[kSteps][2];
@@ -185,10 +200,10 @@ __global__ __launch_bounds__((Shape<kD, kOrder, kUniform>::kThreads), (Shape<kD,
     const auto one = [](float y) { return __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(y))); };
 
     // ---- the window's pages: ids, scales, the largest |vs| so far (the weights' reference).
-    std::uint32_t window = tile_begin / p.window_tiles;  // tiles [window * window_tiles, + window_tiles)
-    std::uint32_t window_page = 0;                       // page of page_id[0]
-    float reference = 0.0f, floor = 0.0f;                // floor: of the windows before
-    bool missing = false;                                // a page of the window is
+    std::uint32_t window = 0;              // window_tiles tiles each, from tile_begin on
+    std::uint32_t window_page = 0;         // page of page_id[0]
+    float reference = 0.0f, floor = 0.0f;  // floor: of the windows before
+    bool missing = false;                  // a page of the window is
     // A query need not see the window's largest |vs|: a weight's parts, relative to that, would
     // lose bits of what it sees (2^15 times a weight over 2^16 is 2^-1, and FP16 ends at
     // 2^-24). So pages whose |vs| is under 2^-16 of the largest are worked on in a pass of their
@@ -200,9 +215,8 @@ __global__ __launch_bounds__((Shape<kD, kOrder, kUniform>::kThreads), (Shape<kD,
     std::uint32_t present = 1;                    // bits of the bands that have a page, and of the last pass's, 0
     float now = 1.0f, counted = 1.0f;             // the pass's unit; whether its weights count (1 or 0)
     const auto stage = [&](std::uint32_t band) {  // ~0: of the window's first pass. Returns the pass's band
-        const std::uint32_t from = window * p.window_tiles;  // its part of this workgroup's tiles
-        const std::uint32_t tile0 = from > tile_begin ? from : tile_begin;
-        const std::uint32_t tile1 = from + p.window_tiles < tile_end ? from + p.window_tiles : tile_end;
+        const std::uint32_t tile0 = tile_begin + window * p.window_tiles;
+        const std::uint32_t tile1 = tile0 + p.window_tiles < tile_end ? tile0 + p.window_tiles : tile_end;
         window_page = p.block_size.div(tile0 * kTile);
         const std::uint32_t pages = p.block_size.div(tile1 * kTile - 1) - window_page + 1;
         float top = 0.0f, least = INFINITY;
@@ -572,6 +586,40 @@ __global__ __launch_bounds__((Shape<kD, kOrder, kUniform>::kThreads), (Shape<kD,
         __builtin_amdgcn_sched_group_barrier(0x008, 2 * 2, 0);
     };
 
+    if constexpr (kFolds) place_of[tid] = row_live ? row_place() + 4 * half : nullptr;
+    // What fold needs of a lane comes from LDS and the lane's number: registers held over the
+    // loop for it undo the order of the products' reads (4 x 512 tokens behind 32768 5 %).
+    const auto this_lane = [] { return __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0u)); };
+    // What the sums folded so far count now.
+    const auto folded = [&] { return __builtin_amdgcn_exp2f(fold_ref[32 * wave + this_lane() % 32] - ref) * (fold_unit / unit); };
+    const auto fold = [&] {
+        const bool begun = window >= p.fold_windows;
+        if (float* const at = place_of[64 * wave + this_lane()]) {
+            const float f = begun ? folded() : 0.0f;
+#pragma unroll
+            for (int db = 0; db < kDb; ++db)
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                    if (32 * db + 8 * g >= static_cast<int>(D)) break;  // uniform
+                    Float4* const held = reinterpret_cast<Float4*>(at + 32 * db + 8 * g);
+                    Float4 v{0.0f, 0.0f, 0.0f, 0.0f};
+                    if (begun) v = *held;
+                    float sums[4] = {v.x * f, v.y * f, v.z * f, v.w * f};
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        float rest = 0.0f;
+                        two_sum_add(sums[i], rest, acc[db][4 * g + i]);
+                        acc[db][4 * g + i] = rest;
+                    }
+                    *held = Float4{sums[0], sums[1], sums[2], sums[3]};
+                }
+        }
+        __builtin_amdgcn_wave_barrier();  // a row's two lanes have read the ones before
+        fold_ref[32 * wave + this_lane() % 32] = threshold == 0.0f ? ref : -INFINITY;
+        __syncthreads();  // every wavefront has read the unit before
+        fold_unit = now;  // what `unit` is where a wavefront has rows
+    };
+
     if (tile_begin < tile_end) {  // uniform
         const auto key_ks_of = [&](std::uint32_t tile) { return key_ks[set][kUniform ? 0 : tile / kSets & 1]; };
         const auto key_vs_of = [&](std::uint32_t tile) { return key_vs[set][kUniform ? 0 : tile / kSets & 1]; };
@@ -665,7 +713,7 @@ __global__ __launch_bounds__((Shape<kD, kOrder, kUniform>::kThreads), (Shape<kD,
         std::uint32_t band = ~0u;
         for (std::uint32_t from = tile_begin;;) {
             band = stage(band);
-            const std::uint32_t behind = (window + 1) * p.window_tiles, last = behind < tile_end ? behind : tile_end;
+            const std::uint32_t behind = tile_begin + (window + 1) * p.window_tiles, last = behind < tile_end ? behind : tile_end;
             std::uint32_t to = last;
             if (__builtin_expect(band != 0, 0)) {
                 // The next run of the pass's tiles, over gaps of two: a run's start costs as much.
@@ -680,11 +728,13 @@ __global__ __launch_bounds__((Shape<kD, kOrder, kUniform>::kThreads), (Shape<kD,
             if (__builtin_expect(band != 0, 0)) {
                 if (to == last) {  // the window's next pass
                     band = 31 - __builtin_clz(present & ((1u << band) - 1));
-                    from = window * p.window_tiles > tile_begin ? window * p.window_tiles : tile_begin;
+                    from = tile_begin + window * p.window_tiles;
                 }
                 continue;
             }
             if (to == tile_end) break;
+            if constexpr (kFolds)
+                if ((window + 1) % p.fold_windows == 0) fold();
             band = ~0u;
             floor = reference;
             ++window;
@@ -695,6 +745,22 @@ __global__ __launch_bounds__((Shape<kD, kOrder, kUniform>::kThreads), (Shape<kD,
     sum += low;
     const auto swapped = __builtin_amdgcn_permlane32_swap(__float_as_uint(sum), __float_as_uint(sum), false, false);
     sum = __uint_as_float(swapped[0]) + __uint_as_float(swapped[1]);
+    float* place = nullptr;  // of a live row
+    if constexpr (kFolds) place = place_of[64 * wave + this_lane()];
+    if (kFolds && window >= p.fold_windows && place) {
+        const float f = folded();
+#pragma unroll
+        for (int db = 0; db < kDb; ++db)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                if (32 * db + 8 * g >= static_cast<int>(D)) break;  // uniform
+                const Float4 v = *reinterpret_cast<const Float4*>(place + 32 * db + 8 * g);
+                acc[db][4 * g] += v.x * f;
+                acc[db][4 * g + 1] += v.y * f;
+                acc[db][4 * g + 2] += v.z * f;
+                acc[db][4 * g + 3] += v.w * f;
+            }
+    }
     // One after the other: a unit of 2^-126 over 2^15 would lose bits.
 #pragma unroll
     for (int db = 0; db < kDb; ++db) acc[db] *= 1.0f / kWeightScale;
@@ -735,24 +801,23 @@ __global__ __launch_bounds__((Shape<kD, kOrder, kUniform>::kThreads), (Shape<kD,
         ref = top == -INFINITY ? 0.0f : top;
         in_ones = 1.0f;
     }
-    if (!row_live) return;
+    if constexpr (!kFolds) place = row_live ? row_place() + 4 * half : nullptr;
+    if (!place) return;
     const bool whole = mine.count == 1;
-    const std::uint32_t head_at = kvh * p.group + head;
-    const std::uint64_t part_row = ((static_cast<std::uint64_t>(split) * p.num_seqs + seq) * p.max_query + token) * p.query_heads + head_at;
-    float* const to = whole ? p.output + ((p.query_offsets[seq] + token) * p.query_heads + head_at) * D : p.part_acc + part_row * kD;
     const float inv = whole && sum != 0.0f ? 1.0f / sum : 1.0f;
 #pragma unroll
     for (int db = 0; db < kDb; ++db)
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
             if (32 * db + 8 * g >= static_cast<int>(D)) break;  // uniform; parts: not read
-            *reinterpret_cast<Float4*>(to + 32 * db + 8 * g + 4 * half) =
+            *reinterpret_cast<Float4*>(place + 32 * db + 8 * g) =
                 Float4{acc[db][4 * g] * inv * in_ones, acc[db][4 * g + 1] * inv * in_ones, acc[db][4 * g + 2] * inv * in_ones,
                        acc[db][4 * g + 3] * inv * in_ones};
         }
-    if (!whole && half == 0) {
-        p.part_ml[2 * part_row] = ref;
-        p.part_ml[2 * part_row + 1] = sum;
+    const std::uint64_t part = static_cast<std::uint64_t>(place - p.part_acc) / kD;  // half 0's
+    if (!whole && (kFolds ? this_lane() < 32 : half == 0)) {
+        p.part_ml[2 * part] = ref;
+        p.part_ml[2 * part + 1] = sum;
     }
 }
 
@@ -851,6 +916,8 @@ PrefillPlan prefill_plan(std::uint64_t num_seqs, std::uint64_t max_query, std::u
         std::uint64_t most = workgroups < kCus ? kCus / workgroups : 1;
         if (tiles <= 2 * kLeastTiles) most = 1;
         if (most > (tiles + kLeastTiles - 1) / kLeastTiles) most = (tiles + kLeastTiles - 1) / kLeastTiles;
+        // Two sets have no place to fold sums into: kFold tiles each.
+        if (plan.order == Order::Halves && most * 2 * kFold < tiles) most = (tiles + 2 * kFold - 1) / (2 * kFold);
         plan.split_tiles = static_cast<std::uint32_t>((tiles + most - 1) / most);
     } else {
         // Where the heaviest block of queries would run on alone, its keys go to several
@@ -880,8 +947,19 @@ template <typename F, int kD, Order kOrder>
 int launch_prefill(QuantPrefillParams& p, hipStream_t stream) {
     const dim3 grid(p.heads * p.splits * p.num_seqs * p.blocks), threads(Shape<kD, kOrder, true>::kThreads);
     for (p.first = 0; p.first < p.group; p.first += p.heads_of) {
-        if (p.block_size.divisor % 16 == 0) quant_prefill_kernel<F, kD, kOrder, true><<<grid, threads, 0, stream>>>(p);
-        else quant_prefill_kernel<F, kD, kOrder, false><<<grid, threads, 0, stream>>>(p);
+        const bool uniform = p.block_size.divisor % 16 == 0;
+        bool folds = false;
+        if constexpr (kOrder != Order::Halves) {
+            folds = p.split_tiles > kFold;
+            if (folds) {
+                if (uniform) quant_prefill_kernel<F, kD, kOrder, true, true><<<grid, threads, 0, stream>>>(p);
+                else quant_prefill_kernel<F, kD, kOrder, false, true><<<grid, threads, 0, stream>>>(p);
+            }
+        }
+        if (!folds) {
+            if (uniform) quant_prefill_kernel<F, kD, kOrder, true, false><<<grid, threads, 0, stream>>>(p);
+            else quant_prefill_kernel<F, kD, kOrder, false, false><<<grid, threads, 0, stream>>>(p);
+        }
         if (const int s = launch_status("quant_prefill_kernel")) return s;
     }
     if (p.splits == 1) return KVFLUX_OK;
@@ -1011,8 +1089,9 @@ extern "C" int kvflux_quant_prefill(const void* key_cache, const void* value_cac
     p.splits = plan.splits;
     p.split_tiles = plan.split_tiles;
     // A window of n tiles has at most n * kTile / block_size + 2 pages.
-    const std::uint64_t window = (kWindow - 2) * block_size / kTile;
-    p.window_tiles = static_cast<std::uint32_t>(window < 0x40000000ULL ? window : 0x40000000ULL);
+    const std::uint64_t window = (kWindow - 2) * block_size / kTile, longest = plan.order == Order::Halves ? 2 * kFold : kFold;
+    p.window_tiles = static_cast<std::uint32_t>(window < longest ? window : longest);
+    p.fold_windows = kFold / p.window_tiles;  // read where sums are folded
     p.query = query;
     p.output = output;
     p.scale_log2 = scale_log2;

@@ -5,8 +5,8 @@ tile of 32, or one token) lies just under half a step of a sum that holds the fi
 value in FP32: added to that one by one, all of them would be lost, up to (tokens a sum
 runs over) * 2^-k of the value.
 
-Tolerance: the contract of 1e-5 of the largest value. What the kernels may leave out of it:
-32 additions beside the dominant value of at most 2^-24 each (2e-6), a few merges, and the
+Tolerance: the contract of 1e-5 of the largest value. What the decode may leave out of it:
+64 additions beside the dominant value of at most 2^-24 each (4e-6), a few merges, and the
 weights' own error, 2^-20 of them, which are 1e-3 of the row.
 """
 from __future__ import annotations
@@ -61,3 +61,19 @@ def test_other_head_sizes(gpu, fmt, D, call):
     else:
         _, got = prefill(cache, table, [n], [2], np.full((2, H * G, D), q, np.float32))
     assert np.abs(got - want).max() <= 1e-5
+
+
+@pytest.mark.parametrize("fmt", ["e4m3", "int8"])
+@pytest.mark.parametrize("D,bs,seqs,m", [(128, 16, 128, 8), (128, 5, 128, 8), (64, 16, 128, 8), (256, 16, 128, 8), (128, 1, 128, 8),
+                                         (128, 16, 64, 64), (128, 5, 64, 64), (128, 16, 64, 32), (64, 16, 64, 32)])
+@pytest.mark.parametrize("value", [1.0, 1.5])
+def test_long_prompts(gpu, fmt, D, bs, seqs, m, value):
+    """Chunks behind 32768 tokens, as many as fill the GPU, so that each workgroup goes through all keys, in every
+    order of work. At most 144 additions of 2^-24 beside the dominant value here: 8.6e-6."""
+    n, H, G = 32768, 4, 4
+    cache, table, q, _ = dominated(fmt, H, D, bs, n, 0.98 * 2.0 ** -30, value)
+    first = 1.0 if fmt == "e4m3" else 2.0
+    _, got = prefill(cache, np.repeat(table, seqs, 0), [n] * seqs, [m] * seqs, np.full((seqs * m, H * G, D), q, np.float32))
+    small = np.exp(-float(q) * first * np.sqrt(D)) * (n - m + np.arange(m))
+    want = (1.0 + value * small) / (1.0 + small)
+    assert np.abs(got.reshape(seqs, m, -1) - want[None, :, None]).max() <= 1e-5 * value
