@@ -467,12 +467,17 @@ __global__ __launch_bounds__(64 * kW, Shape<kD>::kResident) void quant_decode_ke
         // of head col.
         const float total = sum_across_quads(run_sum + run_low);
         if (quad == 0) stats[wave][col] = make_float2(run_max, total);
+        float unit = value_ref * (1.0f / kWeightScale);
+        if (__builtin_expect(value_ref < 0x1p-111f, 0)) {  // uniform; a subnormal number would lose bits
+#pragma unroll
+            for (int dt = 0; dt < kDt; ++dt) acc[dt] *= 1.0f / kWeightScale;
+            unit = value_ref;
+        }
         if (static_cast<std::uint32_t>(col) < heads) {
             float* const row_to = reinterpret_cast<float*>(wave_lds[wave]) + col * S::kPad + 4 * quad;
 #pragma unroll
             for (int dt = 0; dt < kDt; ++dt) {
-                // One after the other: a reference of 2^-126 over 2^15 would lose bits.
-                const pf_f32x4_t o = acc[dt] * (1.0f / kWeightScale) * value_ref;
+                const pf_f32x4_t o = acc[dt] * unit;
                 *reinterpret_cast<float4*>(row_to + 16 * dt) = make_float4(o[0], o[1], o[2], o[3]);
             }
         }

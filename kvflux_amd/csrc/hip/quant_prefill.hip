@@ -761,10 +761,12 @@ __global__ __launch_bounds__((Shape<kD, kOrder, kUniform>::kThreads), (Shape<kD,
                 acc[db][4 * g + 3] += v.w * f;
             }
     }
-    // One after the other: a unit of 2^-126 over 2^15 would lose bits.
+    float in_ones = unit * (1.0f / kWeightScale);
+    if (__builtin_expect(unit < 0x1p-111f && unit != 0.0f, 0)) {  // uniform; a subnormal number would lose bits
 #pragma unroll
-    for (int db = 0; db < kDb; ++db) acc[db] *= 1.0f / kWeightScale;
-    float in_ones = unit;
+        for (int db = 0; db < kDb; ++db) acc[db] *= 1.0f / kWeightScale;
+        in_ones = unit;
+    }
     if constexpr (kSets == 2) {
         float m = threshold == 0.0f ? ref : -INFINITY;  // -INFINITY: no key seen
         if (set == 1) {
