@@ -497,20 +497,21 @@ int kvflux_norm_rope_write_tail(void* key_cache, void* value_cache, uint64_t num
  *   1 of table row r (as kvflux_write_paged_kv_tail).
  *   The scale of a page and head is the smallest power of two, 2^-110 at least,
  *   that brings the largest magnitude among the new values to 448 or 127, or, if
- *   the page has earlier tokens (of positions before the first new one), the
- *   page's scale if that is larger (in size: it may be negative). Values are
- *   divided by it (exactly) and rounded to nearest, ties to even. Where it grows,
- *   the earlier tokens are rounded again to it: exactly for E4M3 except for what
- *   falls below 2^-6 of the scale. Scales of another origin stay as they are until
- *   they grow (the quotient by one that is no power of two is rounded to FP32
- *   first, as are the earlier tokens' by the scale that replaces it). An infinity
- *   or NaN makes the scale of its page and head NaN, and with it all that is read
- *   there, until a write that starts the page anew. Places behind the new tokens
- *   keep their bytes. Nothing is written for lengths of zero, pages past
+ *   the page has earlier tokens (of positions before the first new one, written
+ *   before), the page's scale if that is larger (in size: it may be negative).
+ *   Values are divided by it (exactly) and rounded to nearest, ties to even. Where
+ *   it grows, the earlier tokens are rounded again to it: exactly for E4M3 except
+ *   for what falls below 2^-6 of the scale. Scales of another origin stay as they
+ *   are until they grow (the quotient by one that is no power of two is rounded to
+ *   FP32 first, as are the earlier tokens' by the scale that replaces it). An
+ *   infinity or NaN makes the scale of its page and head NaN, and with it all that
+ *   is read there, until a write that starts the page anew. Places behind the new
+ *   tokens keep their bytes. Nothing is written for lengths of zero, pages past
  *   table_width and page ids >= num_blocks.
  * kvflux_quant_gather: K and V of every sequence as [sum of lengths]
- *   [num_kv_heads][head_size] of `output_dtype`, each value rounded once; its
- *   other arguments as for kvflux_gather_paged_kv_live.
+ *   [num_kv_heads][head_size] of `output_dtype`, each value rounded once (by way
+ *   of FP32 where its scale is no power of two); its other arguments as for
+ *   kvflux_gather_paged_kv_live.
  * Any head_size; block_size and head_size such that a page has fewer than 2^31
  * values, heads below 2^16. KVFLUX_ERR_UNSUPPORTED: writes that may touch 2^24 pages
  * and more, counted for each head of K and V; reads of 2^24 and more of 1024 groups
@@ -538,16 +539,18 @@ int kvflux_quant_gather(const void* key_cache, const void* value_cache, const fl
 
 /* kvflux_quant_attention: kvflux_paged_attention's batch decode (seq_lens given) on
  * such a cache, with its arguments, FP32 queries and outputs, and the 1e-5 contract
- * against the values that the cache holds. Rows of zero tokens give zeros, missing
- * pages (ids >= num_blocks, entries past the table's rows) drop out, a scale or live
- * E4M3 byte that is NaN makes the rows that see it NaN. Scales of any size and
- * origin. Results are the same bits from call to call; a row's may differ between
+ * against the values that the cache holds: 1e-5 of the largest value of V that a row
+ * sees, a page's taken as its scale times 448 or 127. Rows of zero tokens give zeros,
+ * missing pages (ids >= num_blocks, entries past the table's rows) drop out, a scale or
+ * live E4M3 byte that is NaN makes the rows that see it NaN. Scales of any size and
+ * origin, as long as a row's sum of weights (at most 1 each) times values stays within
+ * FP32. Results are the same bits from call to call; a row's may differ between
  * batches.
  * head_size of any multiple of 16 up to 256 (64, 128 and 256 are the kernels' own
  * sizes; others take the next one's arithmetic and their own bytes), pages of any
  * size, any group of query heads (up to 16 work on one reading of the keys); other
  * head sizes up to 512, and caches that are not aligned to 16 bytes, take a generic
- * kernel (a lane a token, tens of times slower).
+ * kernel (a lane a token, some ten times slower).
  * workspace: kvflux_quant_attention_workspace_size bytes, aligned to 8 (no
  * initialisation needed; calls that share one must be ordered); NULL where that is 0
  * (short rows). What one call needs is enough for calls of fewer rows and smaller
@@ -569,7 +572,8 @@ int kvflux_quant_attention(const void* key_cache, const void* value_cache, const
  * max_kv_len bound them and size the grid. Accuracy, missing pages, NaN and head sizes
  * as kvflux_quant_attention; pages of any size, any group of query heads.
  * A live E4M3 byte of V that is NaN (the writes make none) may reach queries before
- * its token. workspace: kvflux_quant_prefill_workspace_size bytes for the same bounds,
+ * its token. Where V scales of a sequence lie 2^125 and more apart, queries that see
+ * small ones alone may lose bits of them. workspace: kvflux_quant_prefill_workspace_size bytes for the same bounds,
  * for calls of few queries behind many tokens, whose keys are split over workgroups
  * (0: NULL will do; no initialisation; calls that share one must be ordered).
  * KVFLUX_ERR_UNSUPPORTED: more than 65535 sequences, 2^31 pages or max_kv_len, or

@@ -25,10 +25,12 @@
 //  * Where workgroups are few, two sets of four wavefronts on the same rows take every other
 //    tile and are merged in LDS; where CUs would be left idle (a short chunk behind a long
 //    prefix) a block's keys go to several workgroups, merged by a second kernel.
+//  * Every 144 tiles a row's sums are folded into its place in the output, so that a row
+//    which one key dominates loses nothing of the others (kFold).
 //
-// 32 query heads, 8 kv heads of 128: 512 tokens behind 32768 490 us, 1130 TFLOP/s of the
+// 32 query heads, 8 kv heads of 128: 512 tokens behind 32768 479 us, 1157 TFLOP/s of the
 // two parts' products, where a large library product in FP16 reaches 1174; 8 prompts of
-// 4096 2.06 ms, 1070 TFLOP/s, the diagonal tiles' masked half counted out. What is left is
+// 4096 2.00 ms, 1097 TFLOP/s, the diagonal tiles' masked half counted out. What is left is
 // the arithmetic beside the matrix instructions, some 400 VALU instructions of a tile and
 // wavefront to 64 MFMAs, and the power that both draw.
 #include "mfma_parts.h"
