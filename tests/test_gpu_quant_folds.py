@@ -7,7 +7,9 @@ from __future__ import annotations
 import numpy as np
 import pytest
 
+from kvflux_amd import device
 from quant_util import VALUES, Cache, attention
+from test_gpu_projected_step import Graph
 from test_gpu_quant_attention import run as decode
 from test_gpu_quant_prefill import run as prefill
 
@@ -128,3 +130,30 @@ def test_the_same_bits_again(gpu):
     for _ in range(3):
         call.run()
         assert np.array_equal(call.result(), first)
+
+
+@pytest.mark.parametrize("D,seqs,m", [(128, 64, 64), (128, 32, 64), (64, 128, 8)])
+def test_captured_and_replayed_at_other_lengths(gpu, D, seqs, m):
+    """A captured call at a bound of 40000 tokens, lengths from none to that: every replay is the eager call's bits,
+    whatever the output held before."""
+    rng, cache, table, q = long_rows("e4m3", D, 16, 40000, seqs, m)
+    tables = np.repeat(table[None], seqs, 0)
+    call, _ = prefill(cache, tables, [40000] * seqs, [m] * seqs, q)
+    stream = device.Stream()
+    graph = Graph(stream, lambda h: call.run(h))
+    for seed in range(3):
+        r = np.random.default_rng(seed)
+        lens = r.integers(0, 40001, seqs)
+        lens[:4] = 40000, 9216, 9217, 0
+        call.held[1].upload(lens.astype(np.uint64))
+        call.held[2].upload(np.minimum(lens, m).astype(np.uint64))
+        call.out.fill(0xa5)
+        call.run()
+        want = call.result().copy()
+        call.out.fill(0xa5 if seed == 0 else 0xff)
+        call.out.upload(np.full(256, 0xa5, np.uint8), call.q.size * 4)
+        graph.replay()
+        got = call.result()
+        written = (np.arange(m)[None] < np.minimum(lens, m)[:, None]).reshape(-1)
+        assert np.array_equal(got[written], want[written]), seed
+    graph.close()
